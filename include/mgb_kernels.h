@@ -469,6 +469,52 @@ int mgb_metric_sum_async(const float* pred, const float* labels, const float* we
 int mgb_metric_auc_async(const float* pred, const float* labels, const float* weights, uint32_t rows, int pr,
                          double* out, void* workspace, size_t workspace_bytes);
 
+/* ---- leaf encoder: operators on the caller's stream --------------------
+ * What turns a model's leaves (mgb_predict_leaf) into vectors and trains the
+ * matrices behind them.  These entry points take the caller's device buffers
+ * and hipStream_t (`stream`; NULL is the device's default stream), run on the
+ * current device, allocate nothing, wait for nothing and keep nothing between
+ * calls, so a stream capture records them.  Workspaces (256-byte aligned) are
+ * the caller's, of at least the size that the *_workspace_bytes function gives
+ * for the same arguments, and may be reused once the stream has passed the
+ * call.  `dtype` is one of the three below; strides are in elements, between
+ * rows (values of a row follow each other), of any size or sign. */
+enum { MGB_F32 = 0, MGB_F16 = 1, MGB_BF16 = 2 };
+
+/* out[r] = scale * sum of weight[tokens[r * bag + j]] over j < bag (bag 1: a
+ * lookup).  Tokens (int32 or int64 by token_bytes) outside [0, vocabulary)
+ * name no row and add nothing.  Sums in binary32, rounded once. */
+int mgb_embedding_lookup(void* out, const void* weight, const void* tokens, int64_t rows, int64_t bag,
+                         int64_t vocabulary, int64_t dim, int64_t weight_stride, float scale, int dtype,
+                         int token_bytes, void* stream);
+/* out[v] = scale * sum of grad[r] over the tokens (r, j) equal to v, for every
+ * row of the table (rows no token names: 0); fewer than 2^31 tokens
+ * (rows * bag).  The order of each sum is fixed by the arguments. */
+size_t mgb_embedding_gradient_workspace_bytes(int64_t tokens, int64_t vocabulary, int64_t dim, int dtype);
+int mgb_embedding_gradient(void* out, const void* grad, const void* tokens, int64_t rows, int64_t bag,
+                           int64_t vocabulary, int64_t dim, int64_t grad_stride, float scale, int dtype,
+                           int token_bytes, void* workspace, size_t workspace_bytes, void* stream);
+/* Layer norm over rows of `dim` values: y (rows without gaps), and each row's
+ * mean and 1 / sqrt(variance + eps).  weight may be NULL, bias too (a bias
+ * needs a weight); both of weight_dtype, MGB_F32 or dtype. */
+int mgb_layer_norm(void* y, float* mean, float* rstd, const void* x, const void* weight, const void* bias,
+                   int64_t rows, int64_t dim, int64_t x_stride, float eps, int dtype, int weight_dtype, void* stream);
+/* Its gradients: dx (rows without gaps), and where dweight is not NULL the
+ * sums over the rows for dweight and dbias (dbias may be NULL). */
+size_t mgb_layer_norm_gradient_workspace_bytes(int64_t rows, int64_t dim, int dtype);
+int mgb_layer_norm_gradient(void* dx, void* dweight, void* dbias, const void* grad, const void* x, const float* mean,
+                            const float* rstd, const void* weight, int64_t rows, int64_t dim, int64_t grad_stride,
+                            int64_t x_stride, int dtype, int weight_dtype, void* workspace, size_t workspace_bytes,
+                            void* stream);
+/* `batch` matrices' updates by Newton-Schulz products: X = G / (|G|_F + eps),
+ * then `steps` (1 to 100) times X <- (c0 I + c1 A + c2 A^2) X with A = X X^T
+ * (matrices taller than wide transposed before and after).  Coefficients
+ * within -8 and 8; sides up to 2^20.  out: matrices without gaps. */
+size_t mgb_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t columns);
+int mgb_orthogonalize(void* out, const void* update, int64_t batch, int64_t rows, int64_t columns, int64_t row_stride,
+                      int64_t batch_stride, int steps, const float* coefficients, float eps, int dtype,
+                      void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

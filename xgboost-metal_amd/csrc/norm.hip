@@ -1,0 +1,467 @@
+// Layer norm over the last axis and its gradient.
+//
+//   mean = sum x / D,  rstd = (sum (x - mean)^2 / D + eps)^-1/2
+//   y = (x - mean) rstd w + b
+// and, with h = (x - mean) rstd and g = dy w,
+//   dx = rstd (g - sum g / D - h sum(g h) / D),  dw = sum_rows dy h,  db = sum_rows dy.
+//
+// Both passes are bound by memory: a row is read once into registers by the
+// lanes that hold it (a part of a wave, a wave or a workgroup, by its width),
+// the sums go over those lanes, and the row is written from the registers.
+// The variance is the sum of centred squares, not a difference of sums, so
+// rows far from zero lose nothing.  All sums are binary32.
+#include <type_traits>
+
+#include "encoder_common.hpp"
+
+namespace mgb {
+namespace {
+
+constexpr int kNormThreads = 256;
+constexpr int kReduceColumns = 32, kReduceSlices = 32;
+
+// Elements a lane holds at most; beyond kNormThreads * that, 1024 lanes take a
+// row, and rows wider still are read again for each sum.
+constexpr int kWaveElements = 16, kBlockElements = 32;
+
+// Sum over the kLanes that share a row.
+template <int kLanes>
+__device__ __forceinline__ float row_sum(float v, float* shared) {
+  if constexpr (kLanes <= kWave) {
+    return group_sum<kLanes>(v);
+  } else {
+    return block_sum<kLanes>(v, shared);
+  }
+}
+
+template <typename T, typename W, int kLanes, int kPacks>
+__global__ __launch_bounds__(kLanes > kNormThreads ? kLanes : kNormThreads) void k_norm(
+    T* __restrict__ y, float* __restrict__ means, float* __restrict__ rstds, const T* __restrict__ x,
+    const W* __restrict__ weight, const W* __restrict__ bias, int64_t rows, int64_t dim, int64_t stride, float eps) {
+  constexpr int kSize = Pack<T>::kSize;
+  constexpr int kThreads = kLanes > kNormThreads ? kLanes : kNormThreads;
+  __shared__ float shared[kThreads / kWave];
+  const int lane = threadIdx.x % kLanes;
+  const int64_t row = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
+  // Lanes of a row beyond the last only occur where a row is at most a wave's:
+  // no barrier follows.
+  if (row >= rows) return;
+  const T* in = x + row * stride;
+  float v[kPacks][kSize];
+  float sum = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kPacks; ++k) load_pack(in, (int64_t)(k * kLanes + lane) * kSize, dim, v[k]);
+#pragma unroll
+  for (int k = 0; k < kPacks; ++k)
+#pragma unroll
+    for (int e = 0; e < kSize; ++e) sum += v[k][e];
+  const float mean = row_sum<kLanes>(sum, shared) / (float)dim;
+  float squares = 0.0f;
+#pragma unroll
+  for (int k = 0; k < kPacks; ++k)
+#pragma unroll
+    for (int e = 0; e < kSize; ++e) {
+      v[k][e] = (int64_t)(k * kLanes + lane) * kSize + e < dim ? v[k][e] - mean : 0.0f;
+      squares = fmaf(v[k][e], v[k][e], squares);
+    }
+  const float rstd = 1.0f / sqrtf(row_sum<kLanes>(squares, shared) / (float)dim + eps);
+  if (lane == 0) {
+    means[row] = mean;
+    rstds[row] = rstd;
+  }
+  T* out = y + row * dim;
+#pragma unroll
+  for (int k = 0; k < kPacks; ++k) {
+    const int64_t at = (int64_t)(k * kLanes + lane) * kSize;
+    float w[kSize], b[kSize];
+    if (weight) load_some<kSize>(weight, at, dim, w);
+    if (bias) load_some<kSize>(bias, at, dim, b);
+#pragma unroll
+    for (int e = 0; e < kSize; ++e) {
+      const float h = v[k][e] * rstd;
+      v[k][e] = weight ? (bias ? fmaf(h, w[e], b[e]) : h * w[e]) : h;
+    }
+    store_pack(out, at, dim, v[k]);
+  }
+}
+
+// Rows wider than the registers of 1024 lanes: three readings, the later two
+// from cache.
+template <typename T, typename W>
+__global__ __launch_bounds__(1024) void k_norm_wide(T* __restrict__ y, float* __restrict__ means,
+                                                    float* __restrict__ rstds, const T* __restrict__ x,
+                                                    const W* __restrict__ weight, const W* __restrict__ bias,
+                                                    int64_t dim, int64_t stride, float eps) {
+  constexpr int kSize = Pack<T>::kSize;
+  __shared__ float shared[1024 / kWave];
+  const int64_t row = blockIdx.x;
+  const T* in = x + row * stride;
+  float v[kSize], w[kSize], b[kSize];
+  float sum = 0.0f, squares = 0.0f;
+  for (int64_t at = (int64_t)threadIdx.x * kSize; at < dim; at += 1024 * kSize) {
+    load_pack(in, at, dim, v);
+    for (int e = 0; e < kSize; ++e) sum += v[e];
+  }
+  const float mean = block_sum<1024>(sum, shared) / (float)dim;
+  for (int64_t at = (int64_t)threadIdx.x * kSize; at < dim; at += 1024 * kSize) {
+    load_pack(in, at, dim, v);
+    for (int e = 0; e < kSize; ++e) {
+      const float c = at + e < dim ? v[e] - mean : 0.0f;
+      squares = fmaf(c, c, squares);
+    }
+  }
+  const float rstd = 1.0f / sqrtf(block_sum<1024>(squares, shared) / (float)dim + eps);
+  if (threadIdx.x == 0) {
+    means[row] = mean;
+    rstds[row] = rstd;
+  }
+  for (int64_t at = (int64_t)threadIdx.x * kSize; at < dim; at += 1024 * kSize) {
+    load_pack(in, at, dim, v);
+    if (weight) load_some<kSize>(weight, at, dim, w);
+    if (bias) load_some<kSize>(bias, at, dim, b);
+    for (int e = 0; e < kSize; ++e) {
+      const float h = (v[e] - mean) * rstd;
+      v[e] = weight ? (bias ? fmaf(h, w[e], b[e]) : h * w[e]) : h;
+    }
+    store_pack(y + row * dim, at, dim, v);
+  }
+}
+
+// dx row by row; the rows of a workgroup are its column sums' slice, kept in
+// registers (a lane holds the same columns of every row) and joined over the
+// workgroup's row groups at the end.  partial: [workgroup][2][dim], dw then db.
+template <typename T, typename W, int kLanes, int kPacks>
+__global__ __launch_bounds__(kLanes > kNormThreads ? kLanes : kNormThreads) void k_norm_gradient(
+    T* __restrict__ dx, float* __restrict__ partial, const T* __restrict__ grad, const T* __restrict__ x,
+    const float* __restrict__ means, const float* __restrict__ rstds, const W* __restrict__ weight, int64_t rows,
+    int64_t dim, int64_t grad_stride, int64_t stride) {
+  constexpr int kSize = Pack<T>::kSize;
+  constexpr int kThreads = kLanes > kNormThreads ? kLanes : kNormThreads;
+  constexpr int kGroups = kThreads / kLanes;
+  __shared__ float shared[kThreads / kWave];
+  __shared__ float joined[kGroups > 1 ? kThreads * kSize : 1];
+  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  float dw[kPacks][kSize] = {}, db[kPacks][kSize] = {}, w[kPacks][kSize];
+#pragma unroll
+  for (int k = 0; k < kPacks; ++k)
+    if (weight) load_some<kSize>(weight, (int64_t)(k * kLanes + lane) * kSize, dim, w[k]);
+  const float inverse = 1.0f / (float)dim;
+  // Where a row takes the whole workgroup, all its lanes run the same rows.
+  for (int64_t row = (int64_t)blockIdx.x * kGroups + group; row < rows; row += (int64_t)gridDim.x * kGroups) {
+    const T* in = x + row * stride;
+    const T* gin = grad + row * grad_stride;
+    float h[kPacks][kSize], g[kPacks][kSize];
+#pragma unroll
+    for (int k = 0; k < kPacks; ++k) {
+      const int64_t at = (int64_t)(k * kLanes + lane) * kSize;
+      load_pack(in, at, dim, h[k]);
+      load_pack(gin, at, dim, g[k]);
+    }
+    const float mean = means[row], rstd = rstds[row];
+    float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kPacks; ++k)
+#pragma unroll
+      for (int e = 0; e < kSize; ++e) {
+        // Beyond the row g and h are 0 and add nothing.
+        h[k][e] = (int64_t)(k * kLanes + lane) * kSize + e < dim ? (h[k][e] - mean) * rstd : 0.0f;
+        dw[k][e] = fmaf(g[k][e], h[k][e], dw[k][e]);
+        db[k][e] += g[k][e];
+        if (weight) g[k][e] *= w[k][e];
+        s1 += g[k][e];
+        s2 = fmaf(g[k][e], h[k][e], s2);
+      }
+    s1 = row_sum<kLanes>(s1, shared) * inverse;
+    s2 = row_sum<kLanes>(s2, shared) * inverse;
+    T* out = dx + row * dim;
+#pragma unroll
+    for (int k = 0; k < kPacks; ++k) {
+#pragma unroll
+      for (int e = 0; e < kSize; ++e) g[k][e] = rstd * (g[k][e] - fmaf(h[k][e], s2, s1));
+      store_pack(out, (int64_t)(k * kLanes + lane) * kSize, dim, g[k]);
+    }
+  }
+  if (!partial) return;
+  float* slice = partial + (int64_t)blockIdx.x * 2 * dim;
+#pragma unroll
+  for (int part = 0; part < 2; ++part)
+#pragma unroll
+    for (int k = 0; k < kPacks; ++k) {
+      float* mine = part ? db[k] : dw[k];
+      if constexpr (kGroups > 1) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < kSize; ++e) joined[(group * kLanes + lane) * kSize + e] = mine[e];
+        __syncthreads();
+        if (group) continue;
+        for (int other = 1; other < kGroups; ++other)
+#pragma unroll
+          for (int e = 0; e < kSize; ++e) mine[e] += joined[(other * kLanes + lane) * kSize + e];
+      }
+      const int64_t at = (int64_t)(k * kLanes + lane) * kSize;
+#pragma unroll
+      for (int e = 0; e < kSize; ++e)
+        if (at + e < dim) slice[part * dim + at + e] = mine[e];
+    }
+}
+
+// The wide form: a workgroup per strip of rows, as above, with dx in two
+// readings and the column sums added up in its slice of `partial`, which only
+// this workgroup touches.
+template <typename T, typename W>
+__global__ __launch_bounds__(1024) void k_norm_gradient_wide(T* __restrict__ dx, float* __restrict__ partial,
+                                                             const T* __restrict__ grad, const T* __restrict__ x,
+                                                             const float* __restrict__ means,
+                                                             const float* __restrict__ rstds,
+                                                             const W* __restrict__ weight, int64_t rows, int64_t dim,
+                                                             int64_t grad_stride, int64_t stride) {
+  constexpr int kSize = Pack<T>::kSize;
+  __shared__ float shared[1024 / kWave];
+  const float inverse = 1.0f / (float)dim;
+  float* slice = partial ? partial + (int64_t)blockIdx.x * 2 * dim : nullptr;
+  if (slice && blockIdx.x >= rows)
+    for (int64_t at = threadIdx.x; at < 2 * dim; at += 1024) slice[at] = 0.0f;
+  float h[kSize], g[kSize], w[kSize];
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+    const float mean = means[row], rstd = rstds[row];
+    float s1 = 0.0f, s2 = 0.0f;
+    for (int64_t at = (int64_t)threadIdx.x * kSize; at < dim; at += 1024 * kSize) {
+      load_pack(x + row * stride, at, dim, h);
+      load_pack(grad + row * grad_stride, at, dim, g);
+      if (weight) load_some<kSize>(weight, at, dim, w);
+      for (int e = 0; e < kSize; ++e) {
+        if (at + e >= dim) break;
+        h[e] = (h[e] - mean) * rstd;
+        if (slice) {
+          // Columns at .. at + kSize are this lane's in every row.
+          const bool first = row == blockIdx.x;
+          float* pw = slice + at + e;
+          float* pb = pw + dim;
+          *pw = fmaf(g[e], h[e], first ? 0.0f : *pw);
+          *pb = g[e] + (first ? 0.0f : *pb);
+        }
+        if (weight) g[e] *= w[e];
+        s1 += g[e];
+        s2 = fmaf(g[e], h[e], s2);
+      }
+    }
+    s1 = block_sum<1024>(s1, shared) * inverse;
+    s2 = block_sum<1024>(s2, shared) * inverse;
+    for (int64_t at = (int64_t)threadIdx.x * kSize; at < dim; at += 1024 * kSize) {
+      load_pack(x + row * stride, at, dim, h);
+      load_pack(grad + row * grad_stride, at, dim, g);
+      if (weight) load_some<kSize>(weight, at, dim, w);
+      for (int e = 0; e < kSize; ++e) {
+        h[e] = (h[e] - mean) * rstd;
+        if (weight) g[e] *= w[e];
+        g[e] = rstd * (g[e] - fmaf(h[e], s2, s1));
+      }
+      store_pack(dx + row * dim, at, dim, g);
+    }
+  }
+}
+
+// dw and db from the workgroups' slices, in their order: a column to a lane,
+// kReduceSlices lanes share its slices.
+template <typename W>
+__global__ __launch_bounds__(kReduceColumns* kReduceSlices) void k_norm_reduce(W* __restrict__ dweight,
+                                                                               W* __restrict__ dbias,
+                                                                               const float* __restrict__ partial,
+                                                                               int64_t dim, int slices) {
+  __shared__ float sums[kReduceSlices][kReduceColumns + 1];
+  const int column = threadIdx.x % kReduceColumns, part = threadIdx.x / kReduceColumns;
+  const int64_t at = (int64_t)blockIdx.x * kReduceColumns + column;
+  float sum = 0.0f;
+  if (at < 2 * dim)
+    for (int s = part; s < slices; s += kReduceSlices) sum += partial[(int64_t)s * 2 * dim + at];
+  sums[part][column] = sum;
+  __syncthreads();
+  if (part == 0 && at < 2 * dim) {
+    for (int p = 1; p < kReduceSlices; ++p) sum += sums[p][column];
+    if (at < dim) {
+      dweight[at] = (W)sum;
+    } else if (dbias) {
+      dbias[at - dim] = (W)sum;
+    }
+  }
+}
+
+// Lanes and packs for a row: the least of 8 .. 64 lanes with kWaveElements
+// each, then a workgroup's 256 and 1024 with kBlockElements.  Returns 0 where
+// the wide form takes the row.
+struct RowShape {
+  int lanes, packs;
+};
+
+RowShape row_shape(int64_t dim, int size, int block_elements) {
+  const int64_t packs = (dim + size - 1) / size;
+  int lanes = 8;
+  while (lanes < 64 && lanes < packs) lanes *= 2;
+  if (lanes == 64 && packs > 64 * (kWaveElements / size)) lanes = 256;
+  if (lanes == 256 && packs > 256 * (kBlockElements / size)) lanes = 1024;
+  if (lanes == 1024 && packs > 1024 * (block_elements / size)) return {0, 0};
+  int each = 1;
+  while ((int64_t)each * lanes < packs) each *= 2;
+  return {lanes, each};
+}
+
+// Calls fn(lanes, packs) with both as constants; the combinations row_shape gives.
+template <int kMaxPacks, typename F>
+bool with_packs(int packs, F&& fn) {
+  switch (packs) {
+    case 1: fn(std::integral_constant<int, 1>()); return true;
+    case 2: if constexpr (kMaxPacks >= 2) { fn(std::integral_constant<int, 2>()); return true; } break;
+    case 4: if constexpr (kMaxPacks >= 4) { fn(std::integral_constant<int, 4>()); return true; } break;
+    case 8: if constexpr (kMaxPacks >= 8) { fn(std::integral_constant<int, 8>()); return true; } break;
+  }
+  return false;
+}
+
+template <int kSize, int kWideElements, typename F>
+bool with_shape(RowShape shape, F&& fn) {
+  auto lanes = [&](auto l) { return [&, l](auto p) { fn(l, p); }; };
+  switch (shape.lanes) {
+    case 8: return with_packs<1>(shape.packs, lanes(std::integral_constant<int, 8>()));
+    case 16: return with_packs<1>(shape.packs, lanes(std::integral_constant<int, 16>()));
+    case 32: return with_packs<1>(shape.packs, lanes(std::integral_constant<int, 32>()));
+    case 64: return with_packs<kWaveElements / kSize>(shape.packs, lanes(std::integral_constant<int, 64>()));
+    case 256: return with_packs<kBlockElements / kSize>(shape.packs, lanes(std::integral_constant<int, 256>()));
+    case 1024: return with_packs<kWideElements / kSize>(shape.packs, lanes(std::integral_constant<int, 1024>()));
+  }
+  return false;
+}
+
+template <typename T, typename W>
+int norm(T* y, float* mean, float* rstd, const T* x, const W* weight, const W* bias, int64_t rows, int64_t dim,
+         int64_t stride, float eps, hipStream_t stream) {
+  constexpr int kSize = Pack<T>::kSize;
+  const RowShape shape = row_shape(dim, kSize, kBlockElements);
+  // A launch holds fewer than 2^32 lanes: very many narrow rows take several.
+  constexpr int64_t kRowsAtOnce = int64_t(1) << 21;
+  for (int64_t first = 0; first < rows; first += kRowsAtOnce) {
+    const int64_t count = rows - first < kRowsAtOnce ? rows - first : kRowsAtOnce;
+    const T* in = x + first * stride;
+    T* out = y + first * dim;
+    const bool done = with_shape<kSize, kBlockElements>(shape, [&](auto l, auto p) {
+      constexpr int kLanes = decltype(l)::value, kPacks = decltype(p)::value;
+      constexpr int kThreads = kLanes > kNormThreads ? kLanes : kNormThreads;
+      const uint32_t grid = (uint32_t)((count + kThreads / kLanes - 1) / (kThreads / kLanes));
+      hipLaunchKernelGGL((k_norm<T, W, kLanes, kPacks>), dim3(grid), dim3(kThreads), 0, stream, out, mean + first,
+                         rstd + first, in, weight, bias, count, dim, stride, eps);
+    });
+    if (!done)
+      hipLaunchKernelGGL((k_norm_wide<T, W>), dim3((uint32_t)count), dim3(1024), 0, stream, out, mean + first,
+                         rstd + first, in, weight, bias, dim, stride, eps);
+    MGB_LAUNCH_CHECK("layer norm");
+  }
+  return 0;
+}
+
+// Gradient: 1024 lanes hold half as much of a row, for the column sums.
+constexpr int kGradientWideElements = 16;
+// Workgroups of 256: two to a CU keep the memory busy, and their slices of the
+// column sums stay small against the rows.
+constexpr int64_t kGradientGroups = 512;
+
+int64_t gradient_slices(int64_t rows, int64_t dim, int size) {
+  const RowShape shape = row_shape(dim, size, kGradientWideElements);
+  const int64_t at_once = shape.lanes && shape.lanes < kNormThreads ? kNormThreads / shape.lanes : 1;
+  const int64_t most = shape.lanes == 1024 || !shape.lanes ? kGradientGroups / 2 : kGradientGroups;
+  const int64_t wanted = (rows + at_once - 1) / at_once;
+  return wanted < 1 ? 1 : wanted < most ? wanted : most;
+}
+
+template <typename T, typename W>
+int norm_gradient(T* dx, W* dweight, W* dbias, const T* grad, const T* x, const float* mean, const float* rstd,
+                  const W* weight, int64_t rows, int64_t dim, int64_t grad_stride, int64_t stride, float* partial,
+                  hipStream_t stream) {
+  constexpr int kSize = Pack<T>::kSize;
+  const RowShape shape = row_shape(dim, kSize, kGradientWideElements);
+  const int64_t slices = gradient_slices(rows, dim, kSize);
+  if (!dweight) partial = nullptr;
+  if (rows || partial) {
+    const bool done = with_shape<kSize, kGradientWideElements>(shape, [&](auto l, auto p) {
+      constexpr int kLanes = decltype(l)::value, kPacks = decltype(p)::value;
+      constexpr int kThreads = kLanes > kNormThreads ? kLanes : kNormThreads;
+      hipLaunchKernelGGL((k_norm_gradient<T, W, kLanes, kPacks>), dim3((uint32_t)slices), dim3(kThreads), 0, stream, dx,
+                         partial, grad, x, mean, rstd, weight, rows, dim, grad_stride, stride);
+    });
+    if (!done)
+      hipLaunchKernelGGL((k_norm_gradient_wide<T, W>), dim3((uint32_t)slices), dim3(1024), 0, stream, dx, partial, grad,
+                         x, mean, rstd, weight, rows, dim, grad_stride, stride);
+    MGB_LAUNCH_CHECK("layer norm gradient");
+  }
+  if (partial) {
+    hipLaunchKernelGGL((k_norm_reduce<W>), dim3((uint32_t)((2 * dim + kReduceColumns - 1) / kReduceColumns)),
+                       dim3(kReduceColumns * kReduceSlices), 0, stream, dweight, dbias, partial, dim, (int)slices);
+    MGB_LAUNCH_CHECK("layer norm parameter gradients");
+  }
+  return 0;
+}
+
+// fn(data type, parameter type): parameters are binary32 or the data's type.
+template <typename F>
+int with_types(int dtype, int weight_dtype, F&& fn) {
+  if (dtype == MGB_F32 && weight_dtype == MGB_F32) return fn((float*)nullptr, (float*)nullptr);
+  if (dtype == MGB_F16 && weight_dtype == MGB_F16) return fn((_Float16*)nullptr, (_Float16*)nullptr);
+  if (dtype == MGB_F16 && weight_dtype == MGB_F32) return fn((_Float16*)nullptr, (float*)nullptr);
+  if (dtype == MGB_BF16 && weight_dtype == MGB_BF16) return fn((__bf16*)nullptr, (__bf16*)nullptr);
+  if (dtype == MGB_BF16 && weight_dtype == MGB_F32) return fn((__bf16*)nullptr, (float*)nullptr);
+  set_error("layer norm: types must be float32, float16 or bfloat16, parameters float32 or the data's type");
+  return -1;
+}
+
+int check_rows(int64_t rows, int64_t dim, int64_t stride) {
+  MGB_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31), "layer norm: rows must be below 2^31");
+  MGB_REQUIRE(dim >= 1 && dim < (int64_t(1) << 31), "layer norm: a row must have 1 to 2^31 - 1 values");
+  // Row strides of either sign and of 0 (a broadcast row) are addresses like others.
+  MGB_REQUIRE(stride < (int64_t(1) << 40) && stride > -(int64_t(1) << 40), "layer norm: row stride out of range");
+  return 0;
+}
+
+}  // namespace
+}  // namespace mgb
+
+using namespace mgb;
+
+extern "C" {
+
+int mgb_layer_norm(void* y, float* mean, float* rstd, const void* x, const void* weight, const void* bias, int64_t rows,
+                   int64_t dim, int64_t stride, float eps, int dtype, int weight_dtype, void* stream) {
+  if (check_rows(rows, dim, stride)) return -1;
+  MGB_REQUIRE(weight || !bias, "layer norm: a bias needs a weight");
+  if (rows == 0) return 0;
+  MGB_REQUIRE(y && mean && rstd && x, "layer norm: null pointer");
+  return with_types(dtype, weight_dtype, [&](auto* t, auto* w) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    using W = std::remove_pointer_t<decltype(w)>;
+    return norm<T, W>((T*)y, mean, rstd, (const T*)x, (const W*)weight, (const W*)bias, rows, dim, stride, eps,
+                      (hipStream_t)stream);
+  });
+}
+
+size_t mgb_layer_norm_gradient_workspace_bytes(int64_t rows, int64_t dim, int dtype) {
+  if (rows < 0 || dim < 1) return 0;
+  return (size_t)gradient_slices(rows, dim, dtype == MGB_F32 ? 4 : 8) * 2 * dim * sizeof(float);
+}
+
+int mgb_layer_norm_gradient(void* dx, void* dweight, void* dbias, const void* grad, const void* x, const float* mean,
+                            const float* rstd, const void* weight, int64_t rows, int64_t dim, int64_t grad_stride,
+                            int64_t stride, int dtype, int weight_dtype, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+  if (check_rows(rows, dim, stride) || check_rows(rows, dim, grad_stride)) return -1;
+  MGB_REQUIRE(dweight || !dbias, "layer norm gradient: a bias' gradient needs the weight's");
+  MGB_REQUIRE(!dweight || workspace_bytes >= mgb_layer_norm_gradient_workspace_bytes(rows, dim, dtype),
+              "layer norm gradient: workspace too small");
+  MGB_REQUIRE(!dweight || workspace, "layer norm gradient: null workspace");
+  MGB_REQUIRE(rows == 0 || (dx && grad && x && mean && rstd), "layer norm gradient: null pointer");
+  return with_types(dtype, weight_dtype, [&](auto* t, auto* w) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    using W = std::remove_pointer_t<decltype(w)>;
+    return norm_gradient<T, W>((T*)dx, (W*)dweight, (W*)dbias, (const T*)grad, (const T*)x, mean, rstd,
+                               (const W*)weight, rows, dim, grad_stride, stride, (float*)workspace,
+                               (hipStream_t)stream);
+  });
+}
+
+}  // extern "C"
