@@ -490,7 +490,8 @@ int mgb_embedding_lookup(void* out, const void* weight, const void* tokens, int6
 /* out[v] = scale * sum of grad[r] over the tokens (r, j) equal to v, for every
  * row of the table (rows no token names: 0); fewer than 2^31 tokens
  * (rows * bag).  The order of each sum is fixed by the arguments. */
-size_t mgb_embedding_gradient_workspace_bytes(int64_t tokens, int64_t vocabulary, int64_t dim, int dtype);
+size_t mgb_embedding_gradient_workspace_bytes(int64_t rows, int64_t bag, int64_t vocabulary, int64_t dim,
+                                              int dtype);
 int mgb_embedding_gradient(void* out, const void* grad, const void* tokens, int64_t rows, int64_t bag,
                            int64_t vocabulary, int64_t dim, int64_t grad_stride, float scale, int dtype,
                            int token_bytes, void* workspace, size_t workspace_bytes, void* stream);

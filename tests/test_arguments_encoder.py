@@ -59,7 +59,7 @@ def test_c_entries_refuse_bad_sizes_and_pointers():
     _refused(lib, gradient(rows=1 << 31), "below 2^31")
     _refused(lib, gradient(rows=1 << 20, bag=1 << 11), "below 2^31")
     _refused(lib, gradient(workspace=None), "null")
-    need = lib.mgb_embedding_gradient_workspace_bytes(I64(10), I64(4), I64(8), 0)
+    need = lib.mgb_embedding_gradient_workspace_bytes(I64(10), I64(1), I64(4), I64(8), 0)
     _refused(lib, gradient(size=need - 1), "workspace too small")
 
     def norm(rows=1, dim=8, weight=one, bias=one, dtype=0, weight_dtype=0):

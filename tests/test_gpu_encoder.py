@@ -129,6 +129,25 @@ def test_gradient_of_frequent_and_rare_tokens(enc, tokens, table):
     _near(dw, want, size * count * E32)
 
 
+@pytest.mark.parametrize("rows,bag,table,dim,dtype", [
+    (20011, 60, 900, 128, torch.bfloat16),   # windows of 32-bit entries, the last one short
+    (9, 4000, 3, 500000, torch.float32),     # wide rows: more windows than rows
+    (40000, 60, 50, 64, torch.float32),      # long tiles
+    (3_000_000, 1, 2000, 8, torch.float16),  # windows of single tokens
+    (70000, 1, 1 << 21, 4, torch.float32),   # 64-bit entries, three digits
+    (300, 20, 1 << 26, 2, torch.float16),    # 64-bit entries in one workgroup
+])
+def test_gradient_sorts(enc, rows, bag, table, dim, dtype):
+    """Each way the tokens are sorted and the windows summed, with tokens outside the table."""
+    g = _gen(rows)
+    tokens = _tokens(g, (rows, bag), table, torch.int32, 0.05)
+    grad = _randn(g, rows, dim, dtype=dtype)
+    dw = enc.embedding_gradient(grad, tokens, table, scale=0.5, pool=True)
+    want, size, count = _gradient64(grad, tokens, table, 0.5, True)
+    _near(dw, want, size * (count + 1) * E32)
+    assert torch.equal(dw, enc.embedding_gradient(grad, tokens, table, scale=0.5, pool=True))
+
+
 def test_lookup_leaves_unnamed_rows_alone(enc):
     """NaN and infinity in rows that no token names, row 0 among them, stay there."""
     weight = torch.ones(10, 40, device="cuda")

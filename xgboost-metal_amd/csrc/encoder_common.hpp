@@ -5,6 +5,8 @@
 #pragma once
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "device_common.hpp"
 
 namespace mgb {
@@ -78,6 +80,81 @@ __device__ __forceinline__ void store_pack(T* row, int64_t at, int64_t dim, cons
     for (int e = 0; e < kSize; ++e)
       if (at + e < dim) row[at + e] = (T)in[e];
   }
+}
+
+// kSize elements as they lie in memory, 16 bytes or one element: loaded without
+// a branch, so that many are in flight, and converted afterwards.
+template <typename T, int kSize>
+struct Raw {
+  static_assert(kSize == 1 || kSize == Pack<T>::kSize, "a pack or an element");
+  using Bits = std::conditional_t<kSize == 1, std::conditional_t<sizeof(T) == 4, uint32_t, uint16_t>,
+                                  __attribute__((ext_vector_type(4))) uint32_t>;
+  Bits bits;
+  __device__ __forceinline__ void load(const T* from) { __builtin_memcpy(&bits, from, sizeof(bits)); }
+  __device__ __forceinline__ void keep_if(bool keep) {
+    if constexpr (kSize == 1) {
+      bits = keep ? bits : Bits(0);
+    } else {
+#pragma unroll
+      for (int w = 0; w < 4; ++w) bits[w] = keep ? bits[w] : 0u;
+    }
+  }
+  __device__ __forceinline__ void get(float* out) const {
+    T v[kSize];
+    __builtin_memcpy(v, &bits, sizeof(bits));
+#pragma unroll
+    for (int e = 0; e < kSize; ++e) out[e] = (float)v[e];
+  }
+  __device__ __forceinline__ void put(const float* in, T* to) {  // rounds to nearest even
+    T v[kSize];
+#pragma unroll
+    for (int e = 0; e < kSize; ++e) v[e] = (T)in[e];
+    __builtin_memcpy(to, v, sizeof(v));
+  }
+};
+
+// sum += v, and sum += a + b.  The chip adds binary16 to binary32 in one
+// instruction if it is a multiply-add (`one` is 1, from where the compiler does
+// not see it), and two bfloat16 by a dot product with (1, 1): 8 instructions
+// for a pack of two tokens' eight, where conversions and additions take 32.
+template <typename T, int kSize>
+__device__ __forceinline__ void add_one(const Raw<T, kSize>& v, float one, float* sum) {
+  T x[kSize];
+  __builtin_memcpy(x, &v.bits, sizeof(v.bits));
+#pragma unroll
+  for (int e = 0; e < kSize; ++e)
+    if constexpr (std::is_same_v<T, _Float16>) sum[e] = fmaf((float)x[e], one, sum[e]);
+    else sum[e] += (float)x[e];
+}
+
+template <typename T, int kSize>
+__device__ __forceinline__ void add_two(const Raw<T, kSize>& a, const Raw<T, kSize>& b, float one, float* sum) {
+  if constexpr (std::is_same_v<T, __bf16> && kSize > 1) {
+    using Pair = __attribute__((ext_vector_type(2))) __bf16;
+    const uint32_t ones_bits = 0x3f803f80;
+    Pair ones;
+    __builtin_memcpy(&ones, &ones_bits, 4);
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const uint32_t low = __builtin_amdgcn_perm(b.bits[w], a.bits[w], 0x05040100u);
+      const uint32_t high = __builtin_amdgcn_perm(b.bits[w], a.bits[w], 0x07060302u);
+      Pair l, h;
+      __builtin_memcpy(&l, &low, 4);
+      __builtin_memcpy(&h, &high, 4);
+      sum[2 * w] = __builtin_amdgcn_fdot2_f32_bf16(l, ones, sum[2 * w], false);
+      sum[2 * w + 1] = __builtin_amdgcn_fdot2_f32_bf16(h, ones, sum[2 * w + 1], false);
+    }
+  } else {
+    add_one<T, kSize>(a, one, sum);
+    add_one<T, kSize>(b, one, sum);
+  }
+}
+
+// 1, as a value of the run.
+__device__ __forceinline__ float runtime_one() {
+  float one = 1.0f;
+  asm volatile("" : "+v"(one));
+  return one;
 }
 
 // Sum over aligned groups of kLanes (a power of two, at most a wave); every

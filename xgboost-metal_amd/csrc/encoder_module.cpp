@@ -179,7 +179,7 @@ PyObject* lookup_gradient(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const Rows grad = rows_of(given);
   const int64_t dim = given.size(-1);
   const c10::DeviceGuard guard(given.device());
-  const size_t need = mgb_embedding_gradient_workspace_bytes(tokens.t.numel(), table, dim, type);
+  const size_t need = mgb_embedding_gradient_workspace_bytes(count(tokens.rows), tokens.bag, table, dim, type);
   Tensor out = empty({table, dim}, given.scalar_type(), given), space = workspace(need, given);
   check(mgb_embedding_gradient(out.data_ptr(), grad.t.data_ptr(), tokens.t.data_ptr(), count(tokens.rows), tokens.bag,
                                table, dim, grad.stride, (float)real(args[3]), type, tokens.bytes, space.data_ptr(),
