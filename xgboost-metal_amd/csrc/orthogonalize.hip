@@ -17,6 +17,7 @@
 // numbers, 22 bits, and a product takes three matrix instructions (high by
 // high, high by low, low by high; low by low is below binary32's rounding).
 // Sums are binary32.
+#include <type_traits>
 #include <utility>
 
 #include "encoder_common.hpp"
@@ -25,33 +26,59 @@ namespace mgb {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kTile = 64;      // rows and columns of a workgroup's tile, and the padding of every matrix
-constexpr int kDepth = 64;     // depth of a stage in LDS
-constexpr int kSegment = 3;
+constexpr int kPad = 64;       // rows and columns of every matrix in the workspace are padded to whole 64s
 constexpr int kNormGroups = 256;
 constexpr int64_t kMostSide = int64_t(1) << 20;
-// With these a segment's P stays far below binary16's 65,504 while X's singular
-// values are at most about 1.
 constexpr float kMostCoefficient = 8.0f;
 
-// Stored values are scaled so that the low part stays a normal number: entries
-// of X and A are at most about 1, those of Z and P at most a^kSegment.
+// Steps of a segment at most.  Results of 24 bits show what a third step adds
+// (64 x 256: 4.4e-6 of the norm against 1.1e-6 with two), those of 11 and 8 do not.
+constexpr int kSegment32 = 2, kSegment16 = 3;
+
+// Stored values are scaled so that the low part is a normal number: entries of X
+// and A are at most about 1, those of Z and P at most a^kSegment16 = 512.
 constexpr float kScaleX = 4096.0f, kScaleZ = 64.0f;
 
 using half8 = __attribute__((ext_vector_type(8))) _Float16;
+using half4 = __attribute__((ext_vector_type(4))) _Float16;
 using float4v = __attribute__((ext_vector_type(4))) float;
+using float16v = __attribute__((ext_vector_type(16))) float;
 
-// High and low parts of a matrix, rows of `stride` values.
+// A matrix as the matrix instructions take it: blocks of 32 rows and 16 columns,
+// the high parts' 1 KB before the low parts', where lane l's 16 bytes are row
+// l % 32, columns l / 32 * 8 .. + 7.  A wave loads a block whole.
+constexpr int kBlock = 32 * 16;
 struct Split {
-  _Float16 *high, *low;
-  int64_t stride, batch_stride;
+  _Float16* data;
+  int64_t blocks;        // side by side: padded columns / 16
+  int64_t batch_stride;  // elements
 };
 
-__device__ __forceinline__ void split_store(const Split& m, int64_t batch, int64_t row, int64_t column, float v) {
-  const _Float16 high = (_Float16)v;
-  const int64_t at = batch * m.batch_stride + row * m.stride + column;
-  m.high[at] = high;
-  m.low[at] = (_Float16)(v - (float)high);
+__device__ __forceinline__ _Float16* element(const Split& m, int64_t batch, int64_t row, int64_t column) {
+  return m.data + batch * m.batch_stride + (row / 32 * m.blocks + column / 16) * (2 * kBlock) +
+         (row % 32 + column % 16 / 8 * 32) * 8 + column % 8;
+}
+
+// Four values that follow each other in a row, from column 4 k on.
+__device__ __forceinline__ void store_four(const Split& m, int64_t batch, int64_t row, int64_t column, float4v v) {
+  half4 high, low;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    high[e] = (_Float16)v[e];
+    low[e] = (_Float16)(v[e] - (float)high[e]);
+  }
+  _Float16* to = element(m, batch, row, column);
+  *(half4*)to = high;
+  *(half4*)(to + kBlock) = low;
+}
+
+__device__ __forceinline__ float4v load_four(const Split& m, int64_t batch, int64_t row, int64_t column) {
+  const _Float16* from = element(m, batch, row, column);
+  const half4 high = *(const half4*)from, low = *(const half4*)(from + kBlock);
+  float4v v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = (float)high[e] + (float)low[e];
+  return v;
 }
 
 template <typename T>
@@ -73,149 +100,349 @@ __global__ __launch_bounds__(kThreads) void k_square_sums(float* __restrict__ pa
   if (threadIdx.x == 0) partial[blockIdx.y * kNormGroups + blockIdx.x] = sum;
 }
 
-// G scaled, as it lies and transposed, both with zeros up to whole tiles.
+// G as it lies and transposed, split and padded with zeros.  binary32 values are
+// scaled to kScaleX X; those of 11 bits and fewer stay whole numbers of their
+// last place by a power of two alone (their low parts are zero and never read),
+// and factor[batch] is what then takes them to kScaleX X.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void k_normalize(Split straight, Split turned, const T* __restrict__ g,
-                                                        const float* __restrict__ partial, int64_t rows,
-                                                        int64_t columns, int64_t stride, int64_t batch_stride,
-                                                        float eps) {
+__global__ __launch_bounds__(kThreads) void k_normalize(Split straight, Split turned, float* __restrict__ factor,
+                                                        const T* __restrict__ g, const float* __restrict__ partial,
+                                                        int64_t rows, int64_t columns, int64_t stride,
+                                                        int64_t batch_stride, float eps) {
   __shared__ float shared[kThreads / kWave];
-  __shared__ float tile[kTile][kTile + 1];
+  __shared__ float tile[kPad][kPad + 1];
   const int64_t batch = blockIdx.z;
-  const float norm = sqrtf(block_sum<kThreads>(partial[batch * kNormGroups + threadIdx.x], shared));
-  const float factor = kScaleX / (norm + eps);
-  const T* in = g + batch * batch_stride;
-  const int64_t row0 = (int64_t)blockIdx.y * kTile, column0 = (int64_t)blockIdx.x * kTile;
-  const int x = threadIdx.x % kTile;
-  for (int y = threadIdx.x / kTile; y < kTile; y += kThreads / kTile) {
-    const float v = row0 + y < rows && column0 + x < columns
-                        ? (float)in[(row0 + y) * stride + column0 + x] * factor : 0.0f;
-    tile[y][x] = v;
-    split_store(straight, batch, row0 + y, column0 + x, v);
+  const float norm = sqrtf(block_sum<kThreads>(partial[batch * kNormGroups + threadIdx.x], shared)) + eps;
+  float scale = kScaleX / norm;
+  if constexpr (sizeof(T) == 2) {
+    // The power of two at most that; beside it 1 .. 2 remain.
+    const float exact = scale;
+    scale = __uint_as_float(__float_as_uint(scale) & 0x7f800000u);
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) factor[batch] = scale > 0.0f ? exact / scale : exact;
+  } else if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
+    factor[batch] = 1.0f;
   }
+  const T* in = g + batch * batch_stride;
+  const int64_t row0 = (int64_t)blockIdx.y * kPad, column0 = (int64_t)blockIdx.x * kPad;
+  const int x = threadIdx.x % kPad;
+  for (int y = threadIdx.x / kPad; y < kPad; y += kThreads / kPad)
+    tile[y][x] = row0 + y < rows && column0 + x < columns ? (float)in[(row0 + y) * stride + column0 + x] * scale : 0.0f;
   __syncthreads();
-  for (int y = threadIdx.x / kTile; y < kTile; y += kThreads / kTile)
-    split_store(turned, batch, column0 + y, row0 + x, tile[x][y]);
+  // A lane takes four columns of four rows of each.
+  for (int k = threadIdx.x; k < kPad * kPad / 4; k += kThreads) {
+    const int y = k % kPad, from = k / kPad * 4;
+    float4v a, b;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      a[e] = tile[y][from + e];
+      b[e] = tile[from + e][y];
+    }
+    store_four(straight, batch, row0 + y, column0 + from, a);
+    store_four(turned, batch, column0 + y, row0 + from, b);
+  }
 }
 
-// What a product's tile becomes.
+// What a product becomes.
 enum { kSymmetric, kBoth, kFinal };
 
-struct Product {
-  Split left, right;       // result = left right^T, both with rows of `depth` values
+struct Job {
+  Split left, right;       // result = left right^T
   Split out, turned;       // kSymmetric: out; kBoth: out and its transpose
-  Split added;             // kSymmetric with `added.high`: + added_factor added + diagonal I
-  int64_t depth;
-  float factor, added_factor, diagonal;
+  Split added;             // kSymmetric, where added.data: + added_factor added + diagonal I
+  float added_factor, diagonal;
+  float factor;            // of the sums,
+  int powers;              // and this often given[batch]
+};
+
+struct Product {
+  Job job[2];              // blockIdx.y: products of the same sizes
+  const float* given;
+  int64_t row_tiles, column_tiles, depth;  // of 32 rows; depth in blocks of 16
   void* result;            // kFinal: the caller's matrix, element (i, j) at i row_step + j column_step
   int64_t rows, columns, row_step, column_step, result_batch;
 };
 
-// LDS rows of kDepth binary16 values are 128 bytes, as wide as the banks; the
-// 16-byte piece a lane wants of row r lies at piece ^ (r >> 1 & 7), so that 16
-// rows' pieces fall on different banks.
-__device__ __forceinline__ int piece_at(int row, int piece) {
-  return row * (kDepth / 8) + (piece ^ (row >> 1 & 7));
+// Lanes t = 0 .. 3 of a quad hold element [e][t] of a 4 x 4 as v[e]; afterwards [t][e].
+__device__ __forceinline__ float4v turn_quads(float4v v) {
+  auto swap = [&](int a, int b, bool second, auto move) {
+    const float send = second ? v[a] : v[b];
+    const float got = move(send);
+    v[a] = second ? got : v[a];
+    v[b] = second ? v[b] : got;
+  };
+  const bool odd = threadIdx.x & 1, upper = threadIdx.x & 2;
+  auto one = [](float f) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(f), 0xb1, 0xf, 0xf, false));
+  };
+  auto two = [](float f) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(f), 0x4e, 0xf, 0xf, false));
+  };
+  swap(0, 1, odd, one);
+  swap(2, 3, odd, one);
+  swap(0, 2, upper, two);
+  swap(1, 3, upper, two);
+  return v;
 }
 
-template <int kMode, typename T>
-__global__ __launch_bounds__(kThreads) void k_product(Product p) {
-  __shared__ half8 lds[4][kTile * kDepth / 8];
-  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-  const int64_t batch = blockIdx.z;
-  int64_t ti = blockIdx.y, tj = blockIdx.x;
-  if constexpr (kMode == kSymmetric) {
-    // Tiles on and above the diagonal, counted column by column.
-    const uint32_t t = blockIdx.x;
-    uint32_t j = (uint32_t)((sqrtf(8.0f * (float)t + 1.0f) - 1.0f) * 0.5f);
-    while (j * (j + 1) / 2 > t) --j;
-    while ((j + 1) * (j + 2) / 2 <= t) ++j;
-    tj = j;
-    ti = t - j * (j + 1) / 2;
+constexpr uint32_t kBand = 8;
+
+// The tile of a workgroup: bands of kBand rows of tiles, column by column, and a
+// share of that order to each chiplet (blockIdx.x modulo 8), so that what a
+// chiplet works on at one time shares rows and columns in its cache.  Symmetric
+// results have the tiles on and above the diagonal.
+template <int kMode>
+__device__ __forceinline__ bool find_tile(uint32_t row_tiles, uint32_t column_tiles, uint32_t* ti, uint32_t* tj) {
+  uint32_t at = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
+  for (uint32_t first = 0; first < row_tiles; first += kBand) {
+    const uint32_t count = kBand * (kMode == kSymmetric ? column_tiles - first : column_tiles);
+    if (at < count) {
+      *ti = first + at % kBand;
+      *tj = (kMode == kSymmetric ? first : 0) + at / kBand;
+      return *ti < row_tiles && (kMode != kSymmetric || *ti <= *tj);
+    }
+    at -= count;
   }
-  const _Float16* from[4] = {
-      p.left.high + batch * p.left.batch_stride + ti * kTile * p.left.stride,
-      p.left.low + batch * p.left.batch_stride + ti * kTile * p.left.stride,
-      p.right.high + batch * p.right.batch_stride + tj * kTile * p.right.stride,
-      p.right.low + batch * p.right.batch_stride + tj * kTile * p.right.stride};
-  const int64_t stride[4] = {p.left.stride, p.left.stride, p.right.stride, p.right.stride};
-  constexpr int kPieces = kTile * kDepth / 8 / kThreads;  // of each of the four, a lane's
-  half8 held[4][kPieces];
-  auto fetch = [&](int64_t k) {
+  return false;
+}
+
+// A quarter of a 32 x 32 of the result, from row 32 bi and column 32 bj: a lane's
+// g-th four values are rows 8 g + 4 (lane / 32) .. + 3 of column lane % 32.
+template <int kMode, typename T>
+__device__ __forceinline__ void finish(const Product& p, const Job& job, int64_t batch, float factor, int64_t bi,
+                                       int64_t bj, bool mirrored, int g, float4v v) {
+  const int lane = threadIdx.x % kWave;
+  const int64_t i = bi * 32 + g * 8 + lane / 32 * 4, j = bj * 32 + lane % 32;
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+  for (int e = 0; e < 4; ++e) v[e] *= factor;
+  if constexpr (kMode == kFinal) {
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        const int piece = i * kThreads + threadIdx.x;
-        held[m][i] = *(const half8*)(from[m] + piece / (kDepth / 8) * stride[m] + k + piece % (kDepth / 8) * 8);
-      }
+    for (int e = 0; e < 4; ++e)
+      if (i + e < p.rows && j < p.columns)
+        ((T*)p.result)[batch * p.result_batch + (i + e) * p.row_step + j * p.column_step] = (T)v[e];
+  } else {
+    if (kMode == kSymmetric && job.added.data) {
+      const float4v a = load_four(job.added, batch, j, i);  // symmetric
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = fmaf(job.added_factor, a[e], v[e]) + (i + e == j ? job.diagonal : 0.0f);
+    }
+    // As it lies in the registers it is four of a row of the transpose.
+    store_four(kMode == kSymmetric ? job.out : job.turned, batch, j, i, v);
+    if (mirrored) store_four(job.out, batch, i + lane % 4, j - lane % 4, turn_quads(v));
+  }
+}
+
+__device__ __forceinline__ float4v four_of(const float16v& v, int g) {
+  return float4v{v[g * 4], v[g * 4 + 1], v[g * 4 + 2], v[g * 4 + 3]};
+}
+
+// sum += left right^T for a block each.
+template <bool kLeftLow, bool kRightLow>
+__device__ __forceinline__ void multiply_block(const half8* left, const half8* right, float16v& sum) {
+  if constexpr (kRightLow) sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(left[0], right[1], sum, 0, 0, 0);
+  if constexpr (kLeftLow) sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(left[1], right[0], sum, 0, 0, 0);
+  sum = __builtin_amdgcn_mfma_f32_32x32x16_f16(left[0], right[0], sum, 0, 0, 0);
+}
+
+__device__ __forceinline__ float total_factor(const Product& p, const Job& job, int64_t batch) {
+  float factor = job.factor;
+  for (int k = 0; k < job.powers; ++k) factor *= p.given[batch];
+  return factor;
+}
+
+// Small products: a workgroup has a tile of 32 x 32, its kWaves waves a part of the
+// depth each, joined in LDS.  Operands go from memory to registers, a ring of
+// kAhead blocks, without a branch between a load and its use.
+template <int kMode, typename T, int kWaves, bool kLeftLow, bool kRightLow>
+__global__ __launch_bounds__(kWaves* kWave) void k_product_small(Product p) {
+  constexpr int kAhead = 4;
+  __shared__ float4v joined[kWaves > 1 ? kWaves * 4 * kWave : 1];
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int64_t batch = blockIdx.z;
+  const Job& job = p.job[blockIdx.y];
+  uint32_t ti, tj;
+  if (!find_tile<kMode>((uint32_t)p.row_tiles, (uint32_t)p.column_tiles, &ti, &tj)) return;
+  const half8* left = (const half8*)(job.left.data + batch * job.left.batch_stride + ti * job.left.blocks * 2 * kBlock) + lane;
+  const half8* right = (const half8*)(job.right.data + batch * job.right.batch_stride + tj * job.right.blocks * 2 * kBlock) + lane;
+  struct Operands {
+    half8 left[2], right[2];
   };
-  fetch(0);
-  float4v sum[2][2] = {};
-  const int wi = wave / 2 * 32, wj = wave % 2 * 32;
-  for (int64_t k = 0; k < p.depth; k += kDepth) {
-    __syncthreads();
+  auto fetch = [&](Operands& o, int64_t k) {
+    o.left[0] = left[k * 2 * kWave];
+    if constexpr (kLeftLow) o.left[1] = left[k * 2 * kWave + kWave];
+    o.right[0] = right[k * 2 * kWave];
+    if constexpr (kRightLow) o.right[1] = right[k * 2 * kWave + kWave];
+  };
+  float16v sum = {};
+  const int64_t share = (p.depth + kWaves - 1) / kWaves, begin = wave * share;
+  const int64_t steps = (begin + share < p.depth ? begin + share : p.depth) - begin;
+  if (steps > 0) {
+    Operands ring[kAhead];
 #pragma unroll
-    for (int m = 0; m < 4; ++m)
+    for (int q = 0; q < kAhead; ++q) fetch(ring[q], begin + (q < steps ? q : steps - 1));
+    int64_t k = 0;
+    for (; k + kAhead <= steps; k += kAhead)
 #pragma unroll
-      for (int i = 0; i < kPieces; ++i) {
-        const int piece = i * kThreads + threadIdx.x;
-        lds[m][piece_at(piece / (kDepth / 8), piece % (kDepth / 8))] = held[m][i];
+      for (int q = 0; q < kAhead; ++q) {
+        multiply_block<kLeftLow, kRightLow>(ring[q].left, ring[q].right, sum);
+        const int64_t ahead = k + q + kAhead;
+        fetch(ring[q], begin + (ahead < steps ? ahead : steps - 1));
       }
+#pragma unroll
+    for (int q = 0; q < kAhead; ++q)
+      if (k + q < steps) multiply_block<kLeftLow, kRightLow>(ring[q].left, ring[q].right, sum);
+  }
+  const float factor = total_factor(p, job, batch);
+  const bool mirrored = kMode == kBoth || ti != tj;
+  if constexpr (kWaves > 1) {
+    // The first four waves join and finish a quarter each.
+#pragma unroll
+    for (int g = 0; g < 4; ++g) joined[(wave * 4 + g) * kWave + lane] = four_of(sum, g);
     __syncthreads();
-    if (k + kDepth < p.depth) fetch(k + kDepth);
+    if (wave >= 4) return;
+    float4v v = joined[wave * kWave + lane];
 #pragma unroll
-    for (int q = 0; q < kDepth / 32; ++q) {
-      half8 v[4][2];
+    for (int w = 1; w < kWaves; ++w) v += joined[(w * 4 + wave) * kWave + lane];
+    finish<kMode, T>(p, job, batch, factor, ti, tj, mirrored, wave, v);
+  } else {
 #pragma unroll
-      for (int m = 0; m < 4; ++m)
+    for (int g = 0; g < 4; ++g) finish<kMode, T>(p, job, batch, factor, ti, tj, mirrored, g, four_of(sum, g));
+  }
+}
+
+using GlobalBytes = const __attribute__((address_space(1))) void*;
+using SharedBytes = __attribute__((address_space(3))) void*;
+
+// Large products: a tile of 64 kHalf x 64 kHalf, kHalf x kHalf blocks of 32 to each
+// of four waves.  What a compute unit gets from its chiplet's cache bounds
+// products of this kind (34 bytes a clock measured, where registers alone carry
+// them), so the waves share their operands in LDS.  Stages of kDepth blocks of 16
+// are loaded straight into a ring of kRing in LDS, a block as it lies in memory,
+// a lane's 16 bytes at 16 lane; a wave reads a stage into registers while it
+// multiplies the one before.
+template <int kMode, typename T, int kHalf, bool kLeftLow, bool kRightLow>
+__global__ __launch_bounds__(4 * kWave, 1) void k_product(Product p) {
+  constexpr int kRing = 4, kDepth = 4 / kHalf;
+  constexpr int kSide = 2 * kHalf;  // blocks of the tile on either side
+  constexpr int kLeft = kSide * (1 + kLeftLow), kRight = kSide * (1 + kRightLow);  // blocks of one depth
+  constexpr int kLoads = (kLeft + kRight) * kDepth / 4;  // of a wave and stage
+  constexpr int kStage = (kLeft + kRight) * kDepth * kBlock;
+  __shared__ __attribute__((aligned(1024))) _Float16 stages[kRing][kStage];
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int64_t batch = blockIdx.z;
+  const Job& job = p.job[blockIdx.y];
+  uint32_t ti, tj;
+  if (!find_tile<kMode>((uint32_t)(p.row_tiles / kSide), (uint32_t)(p.column_tiles / kSide), &ti, &tj)) return;
+  // The blocks this wave loads of every stage.
+  const _Float16* from[kLoads];
 #pragma unroll
-        for (int s = 0; s < 2; ++s) v[m][s] = lds[m][piece_at((m < 2 ? wi : wj) + s * 16 + lane % 16, q * 4 + lane / 16)];
+  for (int q = 0; q < kLoads; ++q) {
+    const int b = q * 4 + wave, d = b / (kLeft + kRight), in = b % (kLeft + kRight);
+    const bool is_left = in < kLeft;
+    const int c = is_left ? in : in - kLeft;
+    const Split& m = is_left ? job.left : job.right;
+    from[q] = m.data + batch * m.batch_stride + ((int64_t)((is_left ? ti : tj) * kSide + c % kSide) * m.blocks + d) * (2 * kBlock) +
+              c / kSide * kBlock + lane * 8;
+  }
+  const int64_t steps = p.depth / kDepth;
+  // Steps beyond the last are loaded (again) and not multiplied: the count of
+  // loads in flight stays what the waits below take it for.
+  auto load = [&](int64_t step, int q) {
+    const int64_t at = (step < steps ? step : steps - 1) * (kDepth * 2 * kBlock);
+    __builtin_amdgcn_global_load_lds((GlobalBytes)(from[q] + at),
+                                     (SharedBytes)(stages[step % kRing] + (q * 4 + wave) * kBlock), 16, 0, 0);
+  };
+  // Until this wave's loads of the oldest of three stages in flight are there and
+  // its reads of LDS done; then until the other waves' are.
+  auto arrived = [&] {
+    constexpr int kFlight = 2 * kLoads;
+    static_assert(kFlight < 64, "vmcnt");
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x70 | (kFlight & 15) | (kFlight >> 4) << 14);  // vmcnt(kFlight) lgkmcnt(0)
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  // A stage's operands in registers: [side][depth][block][high, low].
+  struct Operands {
+    half8 v[2][kDepth][kHalf][2];
+  };
+  const int wi = wave / 2 * kHalf, wj = wave % 2 * kHalf;
+  constexpr int kEach = kDepth * kHalf, kReads = kEach * (2 + kLeftLow + kRightLow);
+  auto read = [&](Operands& o, int64_t step, int r) {
+    const int high = r < 2 * kEach, side = high ? r / kEach : kLeftLow && r < 3 * kEach ? 0 : 1;
+    const int d = r % kEach / kHalf, i = r % kHalf;
+    const half8* blocks = (const half8*)stages[step % kRing] + lane;
+    o.v[side][d][i][1 - high] = blocks[(d * (kLeft + kRight) + (side ? kLeft + wj : wi) + i + (high ? 0 : kSide)) * kWave];
+  };
+  // The instructions of a stage, those on one sum far apart.
+  constexpr int kSums = kHalf * kHalf, kProducts = 1 + kLeftLow + kRightLow, kCalls = kProducts * kDepth * kSums;
+  constexpr int kChains = kSums < 4 ? 2 : 1;  // sums of a block, where the blocks are few
+  float16v sum[kSums][kChains] = {};
+  auto multiply = [&](const Operands& o, int t) {
+    const int s = t % kSums, d = t / kSums % kDepth, product = t / (kSums * kDepth);
+    const int low_left = kLeftLow && product == 1, low_right = kRightLow && product == 1 + kLeftLow;
+    sum[s][t / kSums % kChains] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+        o.v[0][d][s / kHalf][low_left], o.v[1][d][s % kHalf][low_right], sum[s][t / kSums % kChains], 0, 0, 0);
+  };
+  for (int q = 0; q < kRing; ++q)
 #pragma unroll
-      for (int a = 0; a < 2; ++a)
+    for (int l = 0; l < kLoads; ++l) load(q, l);
+  Operands ring[2];
+  __builtin_amdgcn_s_waitcnt(0x70 | (3 * kLoads & 15) | (3 * kLoads >> 4) << 14);
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 #pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          sum[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0][a], v[3][b], sum[a][b], 0, 0, 0);
-          sum[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[1][a], v[2][b], sum[a][b], 0, 0, 0);
-          sum[a][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[0][a], v[2][b], sum[a][b], 0, 0, 0);
+  for (int r = 0; r < kReads; ++r) read(ring[0], 0, r);
+  // A step: its operands are in registers; the next one's are read from LDS and the
+  // stage it was read from itself is loaded anew (every wave has reached the
+  // barrier with its reads of that stage done) between the multiplications, as
+  // many of these after each load as keep a wave from waiting to issue it.
+  constexpr int kPer = kCalls / kLoads;
+  for (int64_t step = 0; step < steps; step += 2) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const int64_t here = step + q;
+      if (q == 1 && here >= steps) break;
+      arrived();
+#pragma unroll
+      for (int t = 0; t < kCalls; ++t) {
+        if (t % kPer == 0) {
+          __builtin_amdgcn_sched_barrier(0);
+          if (t / kPer < kLoads) load(here + kRing, t / kPer);
+#pragma unroll
+          for (int more = 0; more < (kReads + kLoads - 1) / kLoads; ++more)
+            if (t / kPer * ((kReads + kLoads - 1) / kLoads) + more < kReads)
+              read(ring[1 - q], here + 1, t / kPer * ((kReads + kLoads - 1) / kLoads) + more);
+          __builtin_amdgcn_sched_barrier(0);
         }
+        multiply(ring[q], t);
+      }
     }
   }
-  // A lane has rows 4 (lane / 16) .. + 3 of column lane % 16 of each 16 x 16.
+  // Nothing may land in LDS after the workgroup has ended.
+  __builtin_amdgcn_s_waitcnt(0x70);  // vmcnt(0) lgkmcnt(0)
+  const float factor = total_factor(p, job, batch);
 #pragma unroll
-  for (int a = 0; a < 2; ++a)
+  for (int s = 0; s < kSums; ++s) {
+    if constexpr (kChains > 1) sum[s][0] += sum[s][1];
 #pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int64_t i = ti * kTile + wi + a * 16 + lane / 16 * 4 + r, j = tj * kTile + wj + b * 16 + lane % 16;
-        float v = sum[a][b][r] * p.factor;
-        if constexpr (kMode == kSymmetric) {
-          if (p.added.high) {
-            const int64_t at = batch * p.added.batch_stride + i * p.added.stride + j;
-            v = fmaf(p.added_factor, (float)p.added.high[at] + (float)p.added.low[at], v);
-            if (i == j) v += p.diagonal;
-          }
-          split_store(p.out, batch, i, j, v);
-          if (ti != tj) split_store(p.out, batch, j, i, v);
-        } else if constexpr (kMode == kBoth) {
-          split_store(p.out, batch, i, j, v);
-          split_store(p.turned, batch, j, i, v);
-        } else {
-          if (i < p.rows && j < p.columns)
-            ((T*)p.result)[batch * p.result_batch + i * p.row_step + j * p.column_step] = (T)v;
-        }
-      }
+    for (int g = 0; g < 4; ++g)
+      finish<kMode, T>(p, job, batch, factor, (int64_t)ti * kSide + wi + s / kHalf, (int64_t)tj * kSide + wj + s % kHalf,
+                       kMode == kBoth || ti != tj, g, four_of(sum[s][0], g));
+  }
 }
 
 // ---- host -------------------------------------------------------------------
 
-int64_t padded(int64_t v) { return (v + kTile - 1) / kTile * kTile; }
+// Whole tiles of 64, of 128 where those are taken.
+int64_t padded(int64_t v) {
+  const int64_t to = v > 1024 ? 2 * kPad : kPad;
+  return (v + to - 1) / to * to;
+}
 
 // Where the matrices lie in the workspace.
 struct Plan {
   int64_t m, n, mp, np;
-  size_t partial, x, xt, xt_next, square[5], bytes;
+  size_t partial, factor, x, xt, xt_next, square[5], bytes;
 };
 
 Plan plan(int64_t batch, int64_t rows, int64_t columns) {
@@ -231,6 +458,7 @@ Plan plan(int64_t batch, int64_t rows, int64_t columns) {
     return from;
   };
   p.partial = take((size_t)batch * kNormGroups * sizeof(float));
+  p.factor = take((size_t)batch * sizeof(float));
   const size_t wide = (size_t)batch * p.mp * p.np * 2 * sizeof(_Float16);
   p.x = take(wide);
   p.xt = take(wide);
@@ -240,17 +468,50 @@ Plan plan(int64_t batch, int64_t rows, int64_t columns) {
   return p;
 }
 
+// Workgroups for tiles of `side` blocks: whole eights, so that every chiplet's
+// share of find_tile's order has the same length.
+template <int kMode>
+dim3 product_grid(const Product& p, int side, int jobs, int64_t batch) {
+  const int64_t rows = p.row_tiles / side, columns = p.column_tiles / side;
+  int64_t tiles = 0;
+  for (int64_t first = 0; first < rows; first += kBand) tiles += kBand * (kMode == kSymmetric ? columns - first : columns);
+  return dim3((uint32_t)((tiles + 7) / 8 * 8), (uint32_t)jobs, (uint32_t)batch);
+}
+
+// Tiles of 128 where they are enough for half the compute units, of 64 where those
+// are enough for a quarter, else of 32 with the depth cut into as many parts as
+// help.
+template <int kMode, typename T, bool kLeftLow, bool kRightLow>
+void product(const Product& p, int jobs, int64_t batch, hipStream_t stream) {
+  auto tiles = [&](int side) {
+    const int64_t rows = p.row_tiles / side, columns = p.column_tiles / side;
+    return (kMode == kSymmetric ? rows * (rows + 1) / 2 : rows * columns) * jobs * batch;
+  };
+  auto small = [&](auto waves) {
+    constexpr int kWaves = decltype(waves)::value;
+    hipLaunchKernelGGL((k_product_small<kMode, T, kWaves, kLeftLow, kRightLow>), product_grid<kMode>(p, 1, jobs, batch),
+                       dim3(kWaves * kWave), 0, stream, p);
+  };
+  if (p.row_tiles % 4 == 0 && p.column_tiles % 4 == 0 && tiles(4) >= 128)
+    hipLaunchKernelGGL((k_product<kMode, T, 2, kLeftLow, kRightLow>), product_grid<kMode>(p, 4, jobs, batch),
+                       dim3(4 * kWave), 0, stream, p);
+  else if (tiles(2) >= 64 && p.depth >= 16)
+    hipLaunchKernelGGL((k_product<kMode, T, 1, kLeftLow, kRightLow>), product_grid<kMode>(p, 2, jobs, batch),
+                       dim3(4 * kWave), 0, stream, p);
+  else if (p.depth < 16) small(std::integral_constant<int, 1>());
+  else if (p.depth < 64) small(std::integral_constant<int, 4>());
+  else small(std::integral_constant<int, 16>());
+}
+
 template <typename T>
 int orthogonalize(T* out, const T* g, int64_t batch, int64_t rows, int64_t columns, int64_t stride,
                   int64_t batch_stride, int steps, float a, float b, float c, float eps, uint8_t* ws,
                   hipStream_t stream) {
+  constexpr bool kExact = sizeof(T) == 2;  // X0 has no low parts
   const Plan pl = plan(batch, rows, columns);
   const bool tall = rows > columns;
-  float* partial = (float*)(ws + pl.partial);
-  auto matrix = [&](size_t at, int64_t r, int64_t s) {
-    _Float16* high = (_Float16*)(ws + at);
-    return Split{high, high + batch * r * s, s, r * s};
-  };
+  float *partial = (float*)(ws + pl.partial), *factor = (float*)(ws + pl.factor);
+  auto matrix = [&](size_t at, int64_t r, int64_t s) { return Split{(_Float16*)(ws + at), s / 16, r * s * 2}; };
   const Split x = matrix(pl.x, pl.mp, pl.np);
   Split xt = matrix(pl.xt, pl.np, pl.mp), xt_next = matrix(pl.xt_next, pl.np, pl.mp);
   Split A = matrix(pl.square[0], pl.mp, pl.mp), Z = matrix(pl.square[1], pl.mp, pl.mp),
@@ -258,65 +519,74 @@ int orthogonalize(T* out, const T* g, int64_t batch, int64_t rows, int64_t colum
         Q = matrix(pl.square[4], pl.mp, pl.mp);
   hipLaunchKernelGGL((k_square_sums<T>), dim3(kNormGroups, (uint32_t)batch), dim3(kThreads), 0, stream, partial, g, rows,
                      columns, stride, batch_stride);
-  hipLaunchKernelGGL((k_normalize<T>), dim3((uint32_t)(padded(columns) / kTile), (uint32_t)(padded(rows) / kTile), (uint32_t)batch),
-                     dim3(kThreads), 0, stream, tall ? xt : x, tall ? x : xt, g, partial, rows, columns, stride,
+  hipLaunchKernelGGL((k_normalize<T>),
+                     dim3((uint32_t)(padded(columns) / kPad), (uint32_t)(padded(rows) / kPad), (uint32_t)batch),
+                     dim3(kThreads), 0, stream, tall ? xt : x, tall ? x : xt, factor, g, partial, rows, columns, stride,
                      batch_stride, eps);
   MGB_LAUNCH_CHECK("orthogonalize: scaling");
-  const uint32_t mt = (uint32_t)(pl.mp / kTile), nt = (uint32_t)(pl.np / kTile);
-  auto square = [&](Split left, Split right, Split to, int64_t depth, float factor, const Split* added = nullptr) {
-    Product p = {};
-    p.left = left;
-    p.right = right;
-    p.out = to;
-    p.depth = depth;
-    p.factor = factor;
-    if (added) {
-      p.added = *added;
-      p.added_factor = b * kScaleZ / kScaleX;
-      p.diagonal = a * kScaleZ;
-    }
-    hipLaunchKernelGGL((k_product<kSymmetric, float>), dim3(mt * (mt + 1) / 2, 1, (uint32_t)batch), dim3(kThreads), 0,
-                       stream, p);
+  Product square = {};  // m x m results
+  square.given = factor;
+  square.row_tiles = square.column_tiles = pl.mp / 32;
+  square.depth = pl.mp / 16;
+  auto job = [&](Split left, Split right, Split to, float scale) {
+    Job j = {};
+    j.left = left;
+    j.right = right;
+    j.out = to;
+    j.factor = scale;
+    return j;
   };
-  const int segments = (steps + kSegment - 1) / kSegment;
+  const int most = kExact ? kSegment16 : kSegment32, segments = (steps + most - 1) / most;
   for (int s = 0; s < segments; ++s) {
     const int length = steps / segments + (s < steps % segments ? 1 : 0);
-    square(x, x, A, pl.np, 1.0f / kScaleX);
+    Product gram = square;
+    gram.job[0] = job(x, x, A, 1.0f / kScaleX);
+    gram.depth = pl.np / 16;
+    if (kExact && s == 0) {
+      gram.job[0].powers = 2;
+      product<kSymmetric, float, false, false>(gram, 1, batch, stream);
+    } else {
+      product<kSymmetric, float, true, true>(gram, 1, batch, stream);
+    }
     for (int k = 0; k < length; ++k) {
-      square(A, A, Z, pl.mp, c * kScaleZ / (kScaleX * kScaleX), &A);
-      if (k == 0) {
-        std::swap(P, Z);
-      } else {
-        square(Z, P, Q, pl.mp, 1.0f / kScaleZ);
-        std::swap(P, Q);
-      }
+      square.job[0] = job(A, A, Z, c * kScaleZ / (kScaleX * kScaleX));
+      square.job[0].added = A;
+      square.job[0].added_factor = b * kScaleZ / kScaleX;
+      square.job[0].diagonal = a * kScaleZ;
+      product<kSymmetric, float, true, true>(square, 1, batch, stream);
+      // P <- Z P (Z itself at first) and U <- Z A side by side, then A <- U Z.
+      int jobs = 0;
+      if (k > 0) square.job[jobs++] = job(Z, P, Q, 1.0f / kScaleZ);
+      if (k + 1 < length) square.job[jobs++] = job(Z, A, U, 1.0f / kScaleZ);
+      if (jobs) product<kSymmetric, float, true, true>(square, jobs, batch, stream);
       if (k + 1 < length) {
-        const Split z = k == 0 ? P : Z;
-        square(z, A, U, pl.mp, 1.0f / kScaleZ);
-        square(U, z, A, pl.mp, 1.0f / kScaleZ);
+        square.job[0] = job(U, Z, A, 1.0f / kScaleZ);
+        product<kSymmetric, float, true, true>(square, 1, batch, stream);
       }
+      if (k == 0) std::swap(P, Z);
+      else std::swap(P, Q);
     }
-    Product p = {};
-    p.left = P;
-    p.right = xt;
-    p.depth = pl.mp;
-    if (s + 1 < segments) {
-      // X^T is read whole while the new one is written: two buffers in turn.
-      p.out = x;
-      p.turned = xt_next;
-      p.factor = 1.0f / kScaleZ;
-      hipLaunchKernelGGL((k_product<kBoth, float>), dim3(nt, mt, (uint32_t)batch), dim3(kThreads), 0, stream, p);
-      std::swap(xt, xt_next);
-      continue;
-    }
-    p.factor = 1.0f / (kScaleZ * kScaleX);
-    p.result = out;
-    p.rows = pl.m;
-    p.columns = pl.n;
-    p.row_step = tall ? 1 : columns;
-    p.column_step = tall ? columns : 1;
-    p.result_batch = rows * columns;
-    hipLaunchKernelGGL((k_product<kFinal, T>), dim3(nt, mt, (uint32_t)batch), dim3(kThreads), 0, stream, p);
+    Product wide = {};
+    wide.given = factor;
+    wide.row_tiles = pl.mp / 32;
+    wide.column_tiles = pl.np / 32;
+    wide.depth = pl.mp / 16;
+    const bool first = kExact && s == 0, last = s + 1 == segments;
+    wide.job[0] = job(P, xt, x, last ? 1.0f / (kScaleZ * kScaleX) : 1.0f / kScaleZ);
+    wide.job[0].powers = first ? 1 : 0;
+    // X^T is read whole while the new one is written: two buffers in turn.
+    wide.job[0].turned = xt_next;
+    wide.result = out;
+    wide.rows = pl.m;
+    wide.columns = pl.n;
+    wide.row_step = tall ? 1 : columns;
+    wide.column_step = tall ? columns : 1;
+    wide.result_batch = rows * columns;
+    if (last && first) product<kFinal, T, true, false>(wide, 1, batch, stream);
+    else if (last) product<kFinal, T, true, true>(wide, 1, batch, stream);
+    else if (first) product<kBoth, float, true, false>(wide, 1, batch, stream);
+    else product<kBoth, float, true, true>(wide, 1, batch, stream);
+    std::swap(xt, xt_next);
   }
   MGB_LAUNCH_CHECK("orthogonalize: products");
   return 0;
