@@ -54,31 +54,78 @@ struct Split {
   int64_t batch_stride;  // elements
 };
 
-__device__ __forceinline__ _Float16* element(const Split& m, int64_t batch, int64_t row, int64_t column) {
+__device__ __forceinline__ _Float16* element(const Split& m, int64_t batch, uint32_t row, uint32_t column) {
   return m.data + batch * m.batch_stride + (row / 32 * m.blocks + column / 16) * (2 * kBlock) +
          (row % 32 + column % 16 / 8 * 32) * 8 + column % 8;
 }
 
-// Four values that follow each other in a row, from column 4 k on.
-__device__ __forceinline__ void store_four(const Split& m, int64_t batch, int64_t row, int64_t column, float4v v) {
+// Four values as high and low parts.
+struct Parts {
   half4 high, low;
+};
+
+__device__ __forceinline__ Parts parts_of(float4v v) {
+  Parts p;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    high[e] = (_Float16)v[e];
-    low[e] = (_Float16)(v[e] - (float)high[e]);
+    p.high[e] = (_Float16)v[e];
+    p.low[e] = (_Float16)(v[e] - (float)p.high[e]);
   }
-  _Float16* to = element(m, batch, row, column);
-  *(half4*)to = high;
-  *(half4*)(to + kBlock) = low;
+  return p;
 }
 
-__device__ __forceinline__ float4v load_four(const Split& m, int64_t batch, int64_t row, int64_t column) {
-  const _Float16* from = element(m, batch, row, column);
+// Where four that follow each other in a row go, from a column 4 k on.
+__device__ __forceinline__ void store_parts(_Float16* to, const Parts& p) {
+  *(half4*)to = p.high;
+  *(half4*)(to + kBlock) = p.low;
+}
+
+__device__ __forceinline__ void store_four(_Float16* to, float4v v) { store_parts(to, parts_of(v)); }
+
+// Lanes t = 0 .. 3 of a quad hold element [e][t] of a 4 x 4 as v[e]; afterwards
+// [t][e]: pairs of lanes exchange halves of words, then pairs of pairs words.
+__device__ __forceinline__ half4 turn_quads(half4 v) {
+  uint32_t w[2];
+  __builtin_memcpy(w, &v, sizeof(w));
+  const bool odd = threadIdx.x & 1, upper = threadIdx.x & 2;
+  const uint32_t halves = odd ? 0x03020706u : 0x05040100u;  // of (other, own): the upper ones, or the lower
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const uint32_t other = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w[k], 0xb1, 0xf, 0xf, false);
+    w[k] = __builtin_amdgcn_perm(other, w[k], halves);
+  }
+  const uint32_t got =
+      (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(upper ? w[0] : w[1]), 0x4e, 0xf, 0xf, false);
+  w[0] = upper ? got : w[0];
+  w[1] = upper ? w[1] : got;
+  __builtin_memcpy(&v, w, sizeof(w));
+  return v;
+}
+
+__device__ __forceinline__ Parts turn_quads(const Parts& p) { return {turn_quads(p.high), turn_quads(p.low)}; }
+
+__device__ __forceinline__ float4v load_four(const _Float16* from) {
   const half4 high = *(const half4*)from, low = *(const half4*)(from + kBlock);
   float4v v;
 #pragma unroll
   for (int e = 0; e < 4; ++e) v[e] = (float)high[e] + (float)low[e];
   return v;
+}
+
+// A 32 x 32 of a product in registers: a lane's q-th four values are rows
+// 8 q + 4 (lane / 32) .. + 3 of column lane % 32.  As it lies there it is four of a
+// row of the transpose, row lane % 32; after an exchange among quads of lanes
+// (turn_quads) four of row 8 q + 4 (lane / 32) + lane % 4 from column
+// lane % 32 / 4 * 4 on.  The two places in a 32 x 32 in memory, from its first
+// block on:
+__device__ __forceinline__ int turned_place(int lane, int q) {
+  return lane % 32 * 8 + lane / 32 * 4 + q / 2 * (2 * kBlock) + q % 2 * 256;
+}
+__device__ __forceinline__ int straight_place(int lane, int q) {
+  return lane % 32 / 16 * (2 * kBlock) + (lane / 32 * 4 + lane % 4) * 8 + lane % 16 / 8 * 256 + lane % 8 / 4 * 4 + q * 64;
+}
+__device__ __forceinline__ _Float16* tile_of(const Split& m, int64_t batch, uint32_t row_tile, uint32_t column_tile) {
+  return m.data + batch * m.batch_stride + ((int64_t)row_tile * m.blocks + 2 * column_tile) * (2 * kBlock);
 }
 
 template <typename T>
@@ -100,10 +147,22 @@ __global__ __launch_bounds__(kThreads) void k_square_sums(float* __restrict__ pa
   if (threadIdx.x == 0) partial[blockIdx.y * kNormGroups + blockIdx.x] = sum;
 }
 
-// G as it lies and transposed, split and padded with zeros.  binary32 values are
-// scaled to kScaleX X; those of 11 bits and fewer stay whole numbers of their
-// last place by a power of two alone (their low parts are zero and never read),
-// and factor[batch] is what then takes them to kScaleX X.
+// binary32 values are scaled to kScaleX X.  Those of 11 bits and fewer are scaled
+// by a power of two alone, which leaves them what they are (their low parts are
+// zero and never read); `rest`, 1 to 2, is what then takes them to kScaleX X.
+struct Scaling {
+  float scale, rest;
+};
+
+template <typename T>
+__device__ __forceinline__ Scaling scale_for(float norm) {
+  const float exact = kScaleX / norm;
+  if constexpr (sizeof(T) == 4) return {exact, 1.0f};
+  const float power = __uint_as_float(__float_as_uint(exact) & 0x7f800000u);
+  return {power, power > 0.0f ? exact / power : exact};
+}
+
+// G as it lies and transposed, split and padded with zeros.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_normalize(Split straight, Split turned, float* __restrict__ factor,
                                                         const T* __restrict__ g, const float* __restrict__ partial,
@@ -113,20 +172,13 @@ __global__ __launch_bounds__(kThreads) void k_normalize(Split straight, Split tu
   __shared__ float tile[kPad][kPad + 1];
   const int64_t batch = blockIdx.z;
   const float norm = sqrtf(block_sum<kThreads>(partial[batch * kNormGroups + threadIdx.x], shared)) + eps;
-  float scale = kScaleX / norm;
-  if constexpr (sizeof(T) == 2) {
-    // The power of two at most that; beside it 1 .. 2 remain.
-    const float exact = scale;
-    scale = __uint_as_float(__float_as_uint(scale) & 0x7f800000u);
-    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) factor[batch] = scale > 0.0f ? exact / scale : exact;
-  } else if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
-    factor[batch] = 1.0f;
-  }
+  const Scaling scaling = scale_for<T>(norm);
+  if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) factor[batch] = scaling.rest;
   const T* in = g + batch * batch_stride;
   const int64_t row0 = (int64_t)blockIdx.y * kPad, column0 = (int64_t)blockIdx.x * kPad;
   const int x = threadIdx.x % kPad;
   for (int y = threadIdx.x / kPad; y < kPad; y += kThreads / kPad)
-    tile[y][x] = row0 + y < rows && column0 + x < columns ? (float)in[(row0 + y) * stride + column0 + x] * scale : 0.0f;
+    tile[y][x] = row0 + y < rows && column0 + x < columns ? (float)in[(row0 + y) * stride + column0 + x] * scaling.scale : 0.0f;
   __syncthreads();
   // A lane takes four columns of four rows of each.
   for (int k = threadIdx.x; k < kPad * kPad / 4; k += kThreads) {
@@ -137,18 +189,21 @@ __global__ __launch_bounds__(kThreads) void k_normalize(Split straight, Split tu
       a[e] = tile[y][from + e];
       b[e] = tile[from + e][y];
     }
-    store_four(straight, batch, row0 + y, column0 + from, a);
-    store_four(turned, batch, column0 + y, row0 + from, b);
+    store_four(element(straight, batch, (uint32_t)row0 + y, (uint32_t)column0 + from), a);
+    store_four(element(turned, batch, (uint32_t)column0 + y, (uint32_t)row0 + from), b);
   }
 }
 
-// What a product becomes.
-enum { kSymmetric, kBoth, kFinal };
+// What a product becomes: symmetric results, of which only tiles on and above the
+// diagonal are computed, alone or with the rest of a polynomial; a matrix and its
+// transpose; the caller's result.
+enum { kSymmetric, kPolynomial, kBoth, kFinal };
+constexpr bool symmetric(int mode) { return mode == kSymmetric || mode == kPolynomial; }
 
 struct Job {
   Split left, right;       // result = left right^T
-  Split out, turned;       // kSymmetric: out; kBoth: out and its transpose
-  Split added;             // kSymmetric, where added.data: + added_factor added + diagonal I
+  Split out, turned;       // symmetric: out; kBoth: out and its transpose
+  Split added;             // kPolynomial: + added_factor added + diagonal I
   float added_factor, diagonal;
   float factor;            // of the sums,
   int powers;              // and this often given[batch]
@@ -162,28 +217,6 @@ struct Product {
   int64_t rows, columns, row_step, column_step, result_batch;
 };
 
-// Lanes t = 0 .. 3 of a quad hold element [e][t] of a 4 x 4 as v[e]; afterwards [t][e].
-__device__ __forceinline__ float4v turn_quads(float4v v) {
-  auto swap = [&](int a, int b, bool second, auto move) {
-    const float send = second ? v[a] : v[b];
-    const float got = move(send);
-    v[a] = second ? got : v[a];
-    v[b] = second ? v[b] : got;
-  };
-  const bool odd = threadIdx.x & 1, upper = threadIdx.x & 2;
-  auto one = [](float f) {
-    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(f), 0xb1, 0xf, 0xf, false));
-  };
-  auto two = [](float f) {
-    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(f), 0x4e, 0xf, 0xf, false));
-  };
-  swap(0, 1, odd, one);
-  swap(2, 3, odd, one);
-  swap(0, 2, upper, two);
-  swap(1, 3, upper, two);
-  return v;
-}
-
 constexpr uint32_t kBand = 8;
 
 // The tile of a workgroup: bands of kBand rows of tiles, column by column, and a
@@ -194,42 +227,77 @@ template <int kMode>
 __device__ __forceinline__ bool find_tile(uint32_t row_tiles, uint32_t column_tiles, uint32_t* ti, uint32_t* tj) {
   uint32_t at = blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8;
   for (uint32_t first = 0; first < row_tiles; first += kBand) {
-    const uint32_t count = kBand * (kMode == kSymmetric ? column_tiles - first : column_tiles);
+    const uint32_t count = kBand * (symmetric(kMode) ? column_tiles - first : column_tiles);
     if (at < count) {
       *ti = first + at % kBand;
-      *tj = (kMode == kSymmetric ? first : 0) + at / kBand;
-      return *ti < row_tiles && (kMode != kSymmetric || *ti <= *tj);
+      *tj = (symmetric(kMode) ? first : 0) + at / kBand;
+      return *ti < row_tiles && (!symmetric(kMode) || *ti <= *tj);
     }
     at -= count;
   }
   return false;
 }
 
-// A quarter of a 32 x 32 of the result, from row 32 bi and column 32 bj: a lane's
-// g-th four values are rows 8 g + 4 (lane / 32) .. + 3 of column lane % 32.
+// Where the four values of a lane belong in a tile's 32 x 32 (of tile (ti, tj)),
+// and what they take.
 template <int kMode, typename T>
-__device__ __forceinline__ void finish(const Product& p, const Job& job, int64_t batch, float factor, int64_t bi,
-                                       int64_t bj, bool mirrored, int g, float4v v) {
-  const int lane = threadIdx.x % kWave;
-  const int64_t i = bi * 32 + g * 8 + lane / 32 * 4, j = bj * 32 + lane % 32;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] *= factor;
-  if constexpr (kMode == kFinal) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (i + e < p.rows && j < p.columns)
-        ((T*)p.result)[batch * p.result_batch + (i + e) * p.row_step + j * p.column_step] = (T)v[e];
-  } else {
-    if (kMode == kSymmetric && job.added.data) {
-      const float4v a = load_four(job.added, batch, j, i);  // symmetric
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = fmaf(job.added_factor, a[e], v[e]) + (i + e == j ? job.diagonal : 0.0f);
+struct Finish {
+  const Product& p;
+  _Float16 *turned, *straight;  // of the transposed tile, and of the tile
+  const _Float16* old;
+  T* final_to;
+  float factor, added_factor, diagonal;
+  bool mirrored, diagonal_tile;
+  int64_t rows_left, columns_left;
+
+  __device__ __forceinline__ Finish(const Product& product, const Job& job, int64_t batch, float total, uint32_t ti,
+                                    uint32_t tj, bool off_diagonal)
+      : p(product), factor(total), added_factor(job.added_factor), diagonal(job.diagonal),
+        mirrored(kMode == kBoth || off_diagonal), diagonal_tile(ti == tj) {
+    const int lane = threadIdx.x % kWave;
+    if constexpr (kMode == kFinal) {
+      const int64_t i = (int64_t)ti * 32 + lane / 32 * 4, j = (int64_t)tj * 32 + lane % 32;
+      final_to = (T*)p.result + batch * p.result_batch + i * p.row_step + j * p.column_step;
+      rows_left = p.rows - i;
+      columns_left = p.columns - j;
+    } else {
+      turned = tile_of(kMode == kBoth ? job.turned : job.out, batch, tj, ti);
+      straight = tile_of(job.out, batch, ti, tj);
+      if constexpr (kMode == kPolynomial) old = tile_of(job.added, batch, tj, ti);  // symmetric
     }
-    // As it lies in the registers it is four of a row of the transpose.
-    store_four(kMode == kSymmetric ? job.out : job.turned, batch, j, i, v);
-    if (mirrored) store_four(job.out, batch, i + lane % 4, j - lane % 4, turn_quads(v));
   }
-}
+  // The added matrix' four, fetched before they are needed.
+  __device__ __forceinline__ Parts fetch(int q) const {
+    Parts parts = {};
+    if constexpr (kMode == kPolynomial) {
+      const _Float16* from = old + turned_place(threadIdx.x % kWave, q);
+      parts.high = *(const half4*)from;
+      parts.low = *(const half4*)(from + kBlock);
+    }
+    return parts;
+  }
+  __device__ __forceinline__ void operator()(int q, float4v v, const Parts& added) const {
+    const int lane = threadIdx.x % kWave;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= factor;
+    if constexpr (kMode == kFinal) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (q * 8 + e < rows_left && columns_left > 0) final_to[(q * 8 + e) * p.row_step] = (T)v[e];
+    } else {
+      if constexpr (kMode == kPolynomial) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          v[e] = fmaf(added_factor, (float)added.high[e] + (float)added.low[e], v[e]);
+          v[e] += diagonal_tile && q * 8 + lane / 32 * 4 + e == lane % 32 ? diagonal : 0.0f;
+        }
+      }
+      const Parts parts = parts_of(v);
+      store_parts(turned + turned_place(lane, q), parts);
+      if (mirrored) store_parts(straight + straight_place(lane, q), turn_quads(parts));
+    }
+  }
+};
 
 __device__ __forceinline__ float4v four_of(const float16v& v, int g) {
   return float4v{v[g * 4], v[g * 4 + 1], v[g * 4 + 2], v[g * 4 + 3]};
@@ -291,21 +359,24 @@ __global__ __launch_bounds__(kWaves* kWave) void k_product_small(Product p) {
     for (int q = 0; q < kAhead; ++q)
       if (k + q < steps) multiply_block<kLeftLow, kRightLow>(ring[q].left, ring[q].right, sum);
   }
-  const float factor = total_factor(p, job, batch);
-  const bool mirrored = kMode == kBoth || ti != tj;
+  const Finish<kMode, T> finish(p, job, batch, total_factor(p, job, batch), ti, tj, ti != tj);
   if constexpr (kWaves > 1) {
     // The first four waves join and finish a quarter each.
 #pragma unroll
     for (int g = 0; g < 4; ++g) joined[(wave * 4 + g) * kWave + lane] = four_of(sum, g);
     __syncthreads();
     if (wave >= 4) return;
+    const Parts added = finish.fetch(wave);
     float4v v = joined[wave * kWave + lane];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) v += joined[(w * 4 + wave) * kWave + lane];
-    finish<kMode, T>(p, job, batch, factor, ti, tj, mirrored, wave, v);
+    finish(wave, v, added);
   } else {
+    Parts added[4];
 #pragma unroll
-    for (int g = 0; g < 4; ++g) finish<kMode, T>(p, job, batch, factor, ti, tj, mirrored, g, four_of(sum, g));
+    for (int q = 0; q < 4; ++q) added[q] = finish.fetch(q);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) finish(q, four_of(sum, q), added[q]);
   }
 }
 
@@ -421,13 +492,229 @@ __global__ __launch_bounds__(4 * kWave, 1) void k_product(Product p) {
   // Nothing may land in LDS after the workgroup has ended.
   __builtin_amdgcn_s_waitcnt(0x70);  // vmcnt(0) lgkmcnt(0)
   const float factor = total_factor(p, job, batch);
+  auto finish_of = [&](int s) {
+    return Finish<kMode, T>(p, job, batch, factor, ti * kSide + wi + s / kHalf, tj * kSide + wj + s % kHalf, ti != tj);
+  };
+  Parts added[kSums][4];
+#pragma unroll
+  for (int s = 0; s < kSums; ++s)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) added[s][q] = finish_of(s).fetch(q);
 #pragma unroll
   for (int s = 0; s < kSums; ++s) {
     if constexpr (kChains > 1) sum[s][0] += sum[s][1];
+    const Finish<kMode, T> finish = finish_of(s);
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
-      finish<kMode, T>(p, job, batch, factor, (int64_t)ti * kSide + wi + s / kHalf, (int64_t)tj * kSide + wj + s % kHalf,
-                       kMode == kBoth || ti != tj, g, four_of(sum[s][0], g));
+    for (int q = 0; q < 4; ++q) finish(q, four_of(sum[s][0], q), added[s][q]);
+  }
+}
+
+// One workgroup for a whole matrix of at most 64 rows (after transposition): the
+// m x m matrices stay in LDS, X and its transpose in the workspace, where they
+// are in this compute unit's cache, and nothing waits for a launch.
+constexpr int kOneSide = 64, kOneThreads = 512, kOneWaves = kOneThreads / kWave;
+constexpr int kSquare = kOneSide * kOneSide * 2;      // halves of a matrix in LDS
+constexpr int kJoined = kOneWaves / 2 * 3 * 4 * kWave;  // float4s of the partial sums of A
+
+template <typename T>
+__global__ __launch_bounds__(kOneThreads) void k_one(T* __restrict__ out, const T* __restrict__ g, Split x, Split xt,
+                                                     Split xt_next, int64_t rows, int64_t columns, int64_t stride,
+                                                     int64_t batch_stride, int steps, int most, float a, float b,
+                                                     float c, float eps) {
+  constexpr bool kExact = sizeof(T) == 2;
+  constexpr int kSize = Pack<T>::kSize;
+  // A apart: its partial sums lie where the others will.
+  constexpr int kA = 4 * kSquare;
+  static_assert(kJoined * 8 <= kA, "the partial sums fit the others' place");
+  __shared__ __attribute__((aligned(1024))) _Float16 lds[kA + kSquare];
+  __shared__ float shared[kOneWaves];
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int64_t batch = blockIdx.x;
+  const bool tall = rows > columns;
+  const int64_t m = tall ? columns : rows, n = tall ? rows : columns, np = x.blocks * 16;
+  const T* in = g + batch * batch_stride;
+
+  float squares = 0.0f, v[kSize];
+  const int64_t packs = (columns + kSize - 1) / kSize;
+  for (int64_t i = threadIdx.x; i < rows * packs; i += kOneThreads) {
+    const int64_t row = i / packs;
+    load_pack(in + row * stride, (i - row * packs) * kSize, columns, v);
+#pragma unroll
+    for (int e = 0; e < kSize; ++e) squares = fmaf(v[e], v[e], squares);
+  }
+  const Scaling scaling = scale_for<T>(sqrtf(block_sum<kOneThreads>(squares, shared)) + eps);
+
+  // X and X^T, a 4 x 4 at a time; lanes follow each other along G's rows.
+  const uint32_t quads = (uint32_t)np / 4;
+  for (uint32_t k = threadIdx.x; k < kOneSide / 4 * quads; k += kOneThreads) {
+    const uint32_t i = (tall ? k % (kOneSide / 4) : k / quads) * 4, j = (tall ? k / (kOneSide / 4) : k % quads) * 4;
+    const int64_t down = tall ? 1 : stride, across = tall ? stride : 1;
+    const T* from = in + i * down + j * across;
+    float4v straight[4], turned[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float value = i + r < m && j + e < n ? (float)from[r * down + e * across] * scaling.scale : 0.0f;
+        straight[r][e] = value;
+        turned[e][r] = value;
+      }
+    _Float16 *first = element(x, batch, i, j), *first_turned = element(xt, batch, j, i);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {  // rows of a block follow each other at 8 halves
+      store_four(first + r * 8, straight[r]);
+      store_four(first_turned + r * 8, turned[r]);
+    }
+  }
+  __syncthreads();
+
+  int Z = 0, U = kSquare, P = 2 * kSquare, Q = 3 * kSquare;
+  auto block_at = [&](int matrix, int row_tile, int k) {
+    return (const half8*)(lds + matrix + (row_tile * (kOneSide / 16) + k) * 2 * kBlock) + lane;
+  };
+  auto square_tile = [&](int matrix, int row_tile, int column_tile) {
+    return lds + matrix + (row_tile * (kOneSide / 16) + 2 * column_tile) * (2 * kBlock);
+  };
+  // A tile of left right^T (0: upper left, 1: upper right, 2: lower right) by a wave;
+  // one sum for each kind of product, so that four depths follow each other, not twelve.
+  auto square = [&](int tile, int left, int right, int to, float factor, bool added) {
+    const int ti = tile / 2, tj = (tile + 1) / 2;
+    float16v sum[3] = {};
+#pragma unroll
+    for (int k = 0; k < kOneSide / 16; ++k) {
+      const half8 *l = block_at(left, ti, k), *r = block_at(right, tj, k);
+      sum[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[0], r[0], sum[0], 0, 0, 0);
+      sum[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[kWave], r[0], sum[1], 0, 0, 0);
+      sum[2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[0], r[kWave], sum[2], 0, 0, 0);
+    }
+    sum[0] += sum[1] + sum[2];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      float4v w = four_of(sum[0], q);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] *= factor;
+      if (added) {
+        const float4v old = load_four(square_tile(kA, tj, ti) + turned_place(lane, q));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = fmaf(b * kScaleZ / kScaleX, old[e], w[e]);
+        if (ti == tj)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] += q * 8 + lane / 32 * 4 + e == lane % 32 ? a * kScaleZ : 0.0f;
+      }
+      const Parts parts = parts_of(w);
+      store_parts(square_tile(to, tj, ti) + turned_place(lane, q), parts);
+      if (ti != tj) store_parts(square_tile(to, ti, tj) + straight_place(lane, q), turn_quads(parts));
+    }
+  };
+
+  const int segments = (steps + most - 1) / most;
+  for (int s = 0; s < segments; ++s) {
+    const int length = steps / segments + (s < steps % segments ? 1 : 0);
+    const bool exact = kExact && s == 0, last = s + 1 == segments;
+    // A = X X^T: every wave some depths of all three tiles.
+    {
+      float16v sum[3] = {};
+      const half8* from = (const half8*)(x.data + batch * x.batch_stride) + lane;
+#pragma unroll 2
+      for (int64_t k = wave; k < x.blocks; k += kOneWaves) {
+        half8 top[2], bottom[2];
+#pragma unroll
+        for (int part = 0; part < 2; ++part) {
+          top[part] = from[(k * 2 + part) * kWave];
+          bottom[part] = from[((x.blocks + k) * 2 + part) * kWave];
+        }
+        multiply_block<true, true>(top, top, sum[0]);
+        multiply_block<true, true>(top, bottom, sum[1]);
+        multiply_block<true, true>(bottom, bottom, sum[2]);
+      }
+      float4v* joined = (float4v*)lds;
+      const int slot = wave % (kOneWaves / 2);
+      for (int half = 1; half >= 0; --half) {
+        if (wave / (kOneWaves / 2) == half)
+#pragma unroll
+          for (int t = 0; t < 3; ++t)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              float4v& at = joined[((t * 4 + q) * (kOneWaves / 2) + slot) * kWave + lane];
+              at = half ? four_of(sum[t], q) : at + four_of(sum[t], q);
+            }
+        __syncthreads();
+      }
+      for (int part = wave; part < 12; part += kOneWaves) {
+        const int tile = part / 4, q = part % 4, ti = tile / 2, tj = (tile + 1) / 2;
+        float4v w = joined[part * (kOneWaves / 2) * kWave + lane];
+#pragma unroll
+        for (int k = 1; k < kOneWaves / 2; ++k) w += joined[(part * (kOneWaves / 2) + k) * kWave + lane];
+        const float factor = exact ? scaling.rest * scaling.rest / kScaleX : 1.0f / kScaleX;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] *= factor;
+        const Parts parts = parts_of(w);
+        store_parts(square_tile(kA, tj, ti) + turned_place(lane, q), parts);
+        if (ti != tj) store_parts(square_tile(kA, ti, tj) + straight_place(lane, q), turn_quads(parts));
+      }
+      __syncthreads();
+    }
+    for (int k = 0; k < length; ++k) {
+      // Z; then U <- Z A and (but Z itself is P at first) Q <- Z P side by side; then
+      // A <- U Z.  One copy of the code: what is fetched once only costs more than
+      // it computes.
+      const bool more = k + 1 < length;
+#pragma unroll 1
+      for (int phase = 0; phase < 3; ++phase) {
+        const bool second = wave >= 3;
+        const bool runs = phase == 0 ? !second : phase == 1 ? (second ? k > 0 : more) : !second && more;
+        if (wave < 6 && runs)
+          square(wave % 3, phase == 0 ? kA : phase == 1 ? Z : U, phase == 2 ? Z : second ? P : kA,
+                 phase == 0 ? Z : phase == 1 ? (second ? Q : U) : kA,
+                 phase == 0 ? c * kScaleZ / (kScaleX * kScaleX) : 1.0f / kScaleZ, phase == 0);
+        __syncthreads();
+      }
+      const int next = k == 0 ? Z : Q;
+      (k == 0 ? Z : Q) = P;
+      P = next;
+    }
+    // X = P X, a tile of 32 x 32 a wave.
+    const float factor = (exact ? scaling.rest : 1.0f) / (last ? kScaleZ * kScaleX : kScaleZ);
+    for (uint32_t t = wave; t < 2 * (uint32_t)(np / 32); t += kOneWaves) {
+      const uint32_t ti = t % 2, tj = t / 2;
+      const half8* from = (const half8*)(xt.data + batch * xt.batch_stride + tj * xt.blocks * 2 * kBlock) + lane;
+      float16v sum[3] = {};
+      half8 right[kOneSide / 16][2];
+#pragma unroll
+      for (int k = 0; k < kOneSide / 16; ++k) {
+        right[k][0] = from[k * 2 * kWave];
+        right[k][1] = from[k * 2 * kWave + kWave];
+      }
+#pragma unroll
+      for (int k = 0; k < kOneSide / 16; ++k) {
+        const half8* l = block_at(P, ti, k);
+        sum[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[0], right[k][0], sum[0], 0, 0, 0);
+        sum[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[kWave], right[k][0], sum[1], 0, 0, 0);
+        sum[2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[0], right[k][1], sum[2], 0, 0, 0);
+      }
+      sum[0] += sum[1] + sum[2];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        float4v w = four_of(sum[0], q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] *= factor;
+        if (last) {
+          const int64_t i = ti * 32 + q * 8 + lane / 32 * 4, j = tj * 32 + lane % 32;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (i + e < m && j < n)
+              out[batch * rows * columns + (tall ? j * columns + i + e : (i + e) * columns + j)] = (T)w[e];
+        } else {
+          const Parts parts = parts_of(w);
+          store_parts(tile_of(xt_next, batch, tj, ti) + turned_place(lane, q), parts);
+          store_parts(tile_of(x, batch, ti, tj) + straight_place(lane, q), turn_quads(parts));
+        }
+      }
+    }
+    __syncthreads();
+    const Split now = xt;
+    xt = xt_next;
+    xt_next = now;
   }
 }
 
@@ -438,6 +725,9 @@ int64_t padded(int64_t v) {
   const int64_t to = v > 1024 ? 2 * kPad : kPad;
   return (v + to - 1) / to * to;
 }
+
+// The longer side up to which one workgroup takes a matrix of kOneSide rows.
+constexpr int64_t kOneLength = 1024;
 
 // Where the matrices lie in the workspace.
 struct Plan {
@@ -474,7 +764,7 @@ template <int kMode>
 dim3 product_grid(const Product& p, int side, int jobs, int64_t batch) {
   const int64_t rows = p.row_tiles / side, columns = p.column_tiles / side;
   int64_t tiles = 0;
-  for (int64_t first = 0; first < rows; first += kBand) tiles += kBand * (kMode == kSymmetric ? columns - first : columns);
+  for (int64_t first = 0; first < rows; first += kBand) tiles += kBand * (symmetric(kMode) ? columns - first : columns);
   return dim3((uint32_t)((tiles + 7) / 8 * 8), (uint32_t)jobs, (uint32_t)batch);
 }
 
@@ -485,7 +775,7 @@ template <int kMode, typename T, bool kLeftLow, bool kRightLow>
 void product(const Product& p, int jobs, int64_t batch, hipStream_t stream) {
   auto tiles = [&](int side) {
     const int64_t rows = p.row_tiles / side, columns = p.column_tiles / side;
-    return (kMode == kSymmetric ? rows * (rows + 1) / 2 : rows * columns) * jobs * batch;
+    return (symmetric(kMode) ? rows * (rows + 1) / 2 : rows * columns) * jobs * batch;
   };
   auto small = [&](auto waves) {
     constexpr int kWaves = decltype(waves)::value;
@@ -517,6 +807,13 @@ int orthogonalize(T* out, const T* g, int64_t batch, int64_t rows, int64_t colum
   Split A = matrix(pl.square[0], pl.mp, pl.mp), Z = matrix(pl.square[1], pl.mp, pl.mp),
         U = matrix(pl.square[2], pl.mp, pl.mp), P = matrix(pl.square[3], pl.mp, pl.mp),
         Q = matrix(pl.square[4], pl.mp, pl.mp);
+  constexpr int kMost = kExact ? kSegment16 : kSegment32;
+  if (pl.m <= kOneSide && pl.n <= kOneLength) {
+    hipLaunchKernelGGL((k_one<T>), dim3((uint32_t)batch), dim3(kOneThreads), 0, stream, out, g, x, xt, xt_next, rows,
+                       columns, stride, batch_stride, steps, kMost, a, b, c, eps);
+    MGB_LAUNCH_CHECK("orthogonalize: one workgroup");
+    return 0;
+  }
   hipLaunchKernelGGL((k_square_sums<T>), dim3(kNormGroups, (uint32_t)batch), dim3(kThreads), 0, stream, partial, g, rows,
                      columns, stride, batch_stride);
   hipLaunchKernelGGL((k_normalize<T>),
@@ -536,7 +833,7 @@ int orthogonalize(T* out, const T* g, int64_t batch, int64_t rows, int64_t colum
     j.factor = scale;
     return j;
   };
-  const int most = kExact ? kSegment16 : kSegment32, segments = (steps + most - 1) / most;
+  const int segments = (steps + kMost - 1) / kMost;
   for (int s = 0; s < segments; ++s) {
     const int length = steps / segments + (s < steps % segments ? 1 : 0);
     Product gram = square;
@@ -553,7 +850,7 @@ int orthogonalize(T* out, const T* g, int64_t batch, int64_t rows, int64_t colum
       square.job[0].added = A;
       square.job[0].added_factor = b * kScaleZ / kScaleX;
       square.job[0].diagonal = a * kScaleZ;
-      product<kSymmetric, float, true, true>(square, 1, batch, stream);
+      product<kPolynomial, float, true, true>(square, 1, batch, stream);
       // P <- Z P (Z itself at first) and U <- Z A side by side, then A <- U Z.
       int jobs = 0;
       if (k > 0) square.job[jobs++] = job(Z, P, Q, 1.0f / kScaleZ);
