@@ -178,17 +178,13 @@ __device__ __forceinline__ uint32_t window_tokens(const Sort& s, uint32_t window
   return (rows < s.window ? rows : s.window) * s.bag;
 }
 
-// Workgroups of one chiplet follow each other at distance kChiplets.
+// Workgroups of one chiplet follow each other at distance kChiplets; the windows
+// are a multiple of it or divide it.
 __device__ __forceinline__ void window_of(uint32_t windows, uint32_t parts, uint32_t block, uint32_t* window,
                                           uint32_t* part) {
-  if (windows == 1) {
-    *window = 0;
-    *part = block;
-  } else {
-    const uint32_t turn = block / kChiplets;
-    *window = turn / parts * kChiplets + block % kChiplets;
-    *part = turn % parts;
-  }
+  const uint32_t side_by_side = windows < kChiplets ? windows : kChiplets, turn = block / side_by_side;
+  *window = turn / parts * side_by_side + block % side_by_side;
+  *part = turn % parts;
 }
 
 template <typename E, typename I>
@@ -213,6 +209,18 @@ __device__ __forceinline__ uint32_t digit_of(const Sort& s, E entry, int pass) {
   return (uint32_t)(entry >> (s.row_bits + pass * s.digit_bits)) & ((1u << s.digit_bits) - 1);
 }
 
+// The lanes among `of` whose digit is this lane's, by ballots.
+__device__ __forceinline__ uint64_t equal_digits(uint32_t digit, uint64_t of) {
+  uint64_t same = of;
+#pragma unroll
+  for (int b = 0; b < kDigitBits; ++b) {
+    const uint32_t bit = 0u - (digit >> b & 1);  // all ones, or none
+    const uint64_t ones = __ballot(bit != 0), all = (uint64_t)bit << 32 | bit;
+    same &= ~(ones ^ all);
+  }
+  return same;
+}
+
 // Ranks `kRounds` entries of each lane (a wave's entries follow each other, 64
 // a round) among the workgroup's entries of equal digit, in their order:
 // in a round, lanes of equal digits find each other by ballots; counts[wave][]
@@ -228,14 +236,9 @@ __device__ __forceinline__ void rank_digits(const Sort& s, int pass, const E* en
   for (int k = 0; k < kRounds; ++k) {
     const uint32_t digit = digit_of(s, entry[k], pass);
     const bool valid = first + k * kWave < count;
-    uint64_t same = __ballot(valid);
-    if (same == 0) break;  // the whole wave
-#pragma unroll
-    for (int b = 0; b < kDigitBits; ++b) {
-      const uint32_t bit = 0u - (digit >> b & 1);  // all ones, or none
-      const uint64_t ones = __ballot(bit != 0), all = (uint64_t)bit << 32 | bit;
-      same &= ~(ones ^ all);
-    }
+    const uint64_t valids = __ballot(valid);
+    if (valids == 0) break;  // the whole wave
+    const uint64_t same = equal_digits(digit, valids);
     const int leader = same ? __ffsll((unsigned long long)same) - 1 : (int)lane;
     uint32_t before = 0;
     if (valid && leader == (int)lane) before = atomicAdd(&counts[wave][digit], (uint32_t)__popcll(same));
@@ -288,43 +291,91 @@ __device__ __forceinline__ void clear(const Clear& c, uint32_t block, uint32_t b
   }
 }
 
-constexpr int kSmallThreads = 1024, kSmallWaves = kSmallThreads / kWave;
+constexpr int kRangeThreads = 1024, kRangeWaves = kRangeThreads / kWave;
+constexpr uint32_t kRanges = 256;  // workgroups at most, and table rows of each at most
 
-// One workgroup sorts everything in LDS, all passes; the others clear.
-template <typename E, typename I, int kRounds>
-__global__ __launch_bounds__(kSmallThreads) void k_sort_small(E* __restrict__ out, const I* __restrict__ tokens, Sort s,
-                                                              int passes, Clear zero) {
-  if (blockIdx.x > 0) {
-    clear<kSmallThreads>(zero, blockIdx.x - 1, gridDim.x - 1);
+// Few tokens: workgroup w sorts those of its `range` table rows.  Every workgroup
+// reads all tokens, a wave a sixteenth of them in their order, and so knows
+// without the others how many lie before its own: one launch.  Those beyond the
+// ranges clear.
+template <typename E, typename I>
+__global__ __launch_bounds__(kRangeThreads) void k_sort_ranges(E* __restrict__ out, const I* __restrict__ tokens, Sort s,
+                                                               uint32_t range, uint32_t ranges, uint32_t share,
+                                                               Clear zero) {
+  if (blockIdx.x >= ranges) {
+    clear<kRangeThreads>(zero, blockIdx.x - ranges, gridDim.x - ranges);
     return;
   }
   extern __shared__ __align__(16) uint8_t lds[];
-  uint32_t(*counts)[kDigits] = (uint32_t(*)[kDigits])lds;
-  uint32_t* totals = (uint32_t*)(counts + kSmallWaves);
-  uint32_t* shared = totals + kDigits;
-  E* entries = (E*)(shared + 2 * kSmallWaves);
-  const uint32_t n = (uint32_t)s.tokens;
-  const uint32_t first = threadIdx.x / kWave * (kRounds * kWave) + lane_id();
-  E entry[kRounds];
-  uint32_t rank[kRounds];
-  const TokenEntries<E, I> from = {tokens};
+  uint32_t(*counts)[kDigits] = (uint32_t(*)[kDigits])lds;  // [wave][table row]
+  uint32_t* totals = (uint32_t*)(counts + kRangeWaves);
+  uint32_t* shared = totals + kDigits;                     // a scan's words, then each wave's smaller tokens
+  uint32_t* smaller = shared + 2 * kRangeWaves;
+  E* mine = (E*)(smaller + kRangeWaves) + threadIdx.x / kWave * share;
+  const uint32_t lane = lane_id(), wave = threadIdx.x / kWave, n = (uint32_t)s.tokens;
+  const uint32_t low = blockIdx.x * range, none = ~0u;
+  const bool takes_none = s.vocabulary - low < range;
+  // (The last range may reach beyond the table: none of its tokens do.)
+  range = takes_none ? s.vocabulary - low : range;
+  for (uint32_t d = lane; d < kDigits; d += kWave) counts[wave][d] = 0;
+  const uint32_t begin = wave * share, end = begin + share < n ? begin + share : n;
+  uint32_t found = 0, before = 0;
+  for (uint32_t first = begin; first < end; first += kAhead * kWave) {
+    // What is compared is the token's low word: those outside the table become
+    // `none`, above every row, which only the last range (of the number
+    // `vocabulary`) takes in.
+    uint32_t key[kAhead];
 #pragma unroll
-  for (int k = 0; k < kRounds; ++k) entry[k] = first + k * kWave < n ? from(s, 0, first + k * kWave) : 0;
-  for (int pass = 0; pass < passes; ++pass) {
-    if (pass > 0)
+    for (int j = 0; j < kAhead; ++j) {
+      const uint32_t i = first + j * kWave + lane;
+      const I id = i < end ? tokens[i] : I(-1);
+      if constexpr (sizeof(I) == 8) key[j] = (uint64_t)id >> 31 ? none : (uint32_t)id;
+      else key[j] = (uint32_t)id;
+    }
 #pragma unroll
-      for (int k = 0; k < kRounds; ++k) entry[k] = first + k * kWave < n ? entries[first + k * kWave] : 0;
-    rank_digits<kSmallWaves, kRounds>(s, pass, entry, first, n, counts, totals, rank);
-    scan_digits(totals, shared);
-#pragma unroll
-    for (int k = 0; k < kRounds; ++k)
-      if (first + k * kWave < n) {
-        const uint32_t d = digit_of(s, entry[k], pass);
-        entries[totals[d] + counts[threadIdx.x / kWave][d] + rank[k]] = entry[k];
+    for (int j = 0; j < kAhead; ++j) {
+      const uint32_t i = first + j * kWave + lane;
+      const bool in = key[j] - low < range || (takes_none && key[j] >= s.vocabulary && i < end);
+      const uint64_t all = __ballot(in);
+      before += (uint32_t)__popcll(__ballot(key[j] < low));
+      if (all == 0) continue;
+      if (in) {
+        const uint32_t row = key[j] < s.vocabulary ? key[j] : s.vocabulary;
+        mine[found + (uint32_t)__popcll(all & ((1ull << lane) - 1))] = (E)row << s.row_bits | i / s.bag;
+        atomicAdd(&counts[wave][row - low], 1u);
       }
-    __syncthreads();
+      found += (uint32_t)__popcll(all);
+    }
   }
-  for (uint32_t i = threadIdx.x; i < n; i += kSmallThreads) out[i] = entries[i];
+  if (lane == 0) smaller[wave] = before;
+  __syncthreads();
+  // A table row's tokens wave by wave, after the rows below it and the ranges below.
+  if (threadIdx.x < kDigits) {
+    uint32_t offset = 0;
+#pragma unroll
+    for (int w = 0; w < kRangeWaves; ++w) {
+      const uint32_t c = counts[w][threadIdx.x];
+      counts[w][threadIdx.x] = offset;
+      offset += c;
+    }
+    totals[threadIdx.x] = offset;
+  }
+  __syncthreads();
+  scan_digits(totals, shared);
+  uint32_t start = 0;
+#pragma unroll
+  for (int w = 0; w < kRangeWaves; ++w) start += smaller[w];
+  for (uint32_t first = 0; first < found; first += kWave) {
+    const bool valid = first + lane < found;
+    const E entry = valid ? mine[first + lane] : 0;
+    const uint32_t digit = valid ? (uint32_t)(entry >> s.row_bits) - low : 0;
+    const uint64_t same = equal_digits(digit, __ballot(valid));
+    const int leader = same ? __ffsll((unsigned long long)same) - 1 : (int)lane;
+    uint32_t at = 0;
+    if (valid && leader == (int)lane) at = atomicAdd(&counts[wave][digit], (uint32_t)__popcll(same));
+    at = __shfl(at, leader, kWave);
+    if (valid) out[start + totals[digit] + at + (uint32_t)__popcll(same & ((1ull << lane) - 1))] = entry;
+  }
 }
 
 constexpr int kSortThreads = 512, kSortWaves = kSortThreads / kWave;
@@ -600,68 +651,86 @@ __global__ __launch_bounds__(kThreads) void k_segment_sums(T* __restrict__ out, 
   for (; i < limit; i += kAhead) {
     O offset[kMine];
     uint32_t after_each[kMine];  // the key behind each entry
-    bool ends_here = false;
+    // Where something is to be done behind an entry: its segment ends, or the walk
+    // does.  `mine_ends` has the eight of this lane's group, `any_ends` those of
+    // any group of the wave.
+    bool ends_here[kMine];
 #pragma unroll
     for (int j = 0; j < kMine; ++j) {
       offset[j] = (O)((int64_t)(mine[j] & mask) * stride_bytes);
       after_each[j] = (uint32_t)(behind[j] >> s.row_bits);
-      // Where the segment ends or the walk does.
       const uint32_t p = i + (kMine == 1 ? lane % kAhead : j) + 1;
-      ends_here = ends_here || after_each[j] != (uint32_t)(mine[j] >> s.row_bits) || p >= n || p == end || p >= limit;
+      ends_here[j] = after_each[j] != (uint32_t)(mine[j] >> s.row_bits) || p >= n || p == end || p >= limit;
+    }
+    uint32_t mine_ends = 0, any_ends = 0;
+    if constexpr (kMine == 1) {
+      const uint64_t all = __ballot(ends_here[0]);
+      mine_ends = (uint32_t)(all >> (lane_id() / kAhead * kAhead)) & 0xff;
+      const uint32_t folded = (uint32_t)all | (uint32_t)(all >> 32);
+      any_ends = (folded | folded >> 8 | folded >> 16 | folded >> 24) & 0xff;
+    } else {
+#pragma unroll
+      for (int j = 0; j < kMine; ++j) {
+        mine_ends |= (uint32_t)ends_here[j] << j;
+        any_ends |= (uint32_t)__any(ends_here[j]) << j;
+      }
     }
     fetch(i + kAhead);
     O from[kAhead];
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) from[j] = share_of<kLanes>(offset, j) + column;
     Raw<T, kSize> v[kAhead];
-    if (active) {
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) v[j].load((const T*)(rows + from[j]));
-    }
-    if (!__any(ends_here)) {
-      if (active) {
-#pragma unroll
-        for (int j = 0; j < kAhead; j += 2) add_two<T, kSize>(v[j], v[j + 1], one, sum);
-      }
-      continue;
-    }
-    // The eight keys behind, by their lanes.
-    uint32_t following[kAhead];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) following[j] = share_of<kLanes>(after_each, j);
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
+    for (int j = 0; j < kAhead; ++j) v[j].load((const T*)(rows + from[j]));
+    bool done = false;
+    auto behind_entry = [&](int j) {
+      const uint32_t following = share_of<kLanes>(after_each, j);
       const uint32_t p = i + j + 1;  // the tokens up to here
-      if (p > limit) break;
-      if (active) add_one<T, kSize>(v[j], one, sum);
-      const bool ends = p >= n || following[j] != key;
-      if (!ends && (p != end || follow)) continue;
-      if (active && key < s.vocabulary && !skip) {
-        if (ends && !head) {
-          store_segment<T, kSize>(g, out, s.vocabulary, window, key, at, sum);
-        } else {
-          store_floats<kSize>((head ? g.heads : g.tails) + ((uint64_t)window * g.chunks + c) * g.dim + at, sum);
+      const bool ends = p >= n || following != key;
+      if (mine_ends >> j & 1 && (ends || p != end || !follow)) {
+        if (active && key < s.vocabulary && !skip) {
+          if (ends && !head) {
+            store_segment<T, kSize>(g, out, s.vocabulary, window, key, at, sum);
+          } else {
+            store_floats<kSize>((head ? g.heads : g.tails) + ((uint64_t)window * g.chunks + c) * g.dim + at, sum);
+          }
         }
-      }
-      if (p >= end || following[j] >= s.vocabulary) return;
-      key = following[j];
-      head = skip = false;
+        if (p >= end || following >= s.vocabulary) {
+          done = true;
+          mine_ends = 0;
+        }
+        key = following;
+        head = skip = false;
 #pragma unroll
-      for (int e = 0; e < kSize; ++e) sum[e] = 0.0f;
+        for (int e = 0; e < kSize; ++e) sum[e] = 0.0f;
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < kAhead; j += 2) {
+      if (any_ends >> j & 1) {
+        add_one<T, kSize>(v[j], one, sum);
+        behind_entry(j);
+        add_one<T, kSize>(v[j + 1], one, sum);
+      } else {
+        add_two<T, kSize>(v[j], v[j + 1], one, sum);
+      }
+      if (any_ends >> (j + 1) & 1) behind_entry(j + 1);
     }
+    if (done) break;
   }
 }
 
 // Chunks of a workgroup of k_segment_join, and the heads from which on all its
 // groups share a segment.
 constexpr uint32_t kJoinChunks = 64, kJoinLong = 32;
+constexpr int kJoinThreads = 256;
 
 // Segments left in parts that begin in kJoinChunks chunks.
 template <typename T, typename E, int kLanes, int kSize>
-__global__ __launch_bounds__(kThreads) void k_segment_join(T* __restrict__ out, const E* __restrict__ sorted, Sort s,
+__global__ __launch_bounds__(kJoinThreads) void k_segment_join(T* __restrict__ out, const E* __restrict__ sorted, Sort s,
                                                            Segments g) {
-  constexpr int kGroups = kThreads / kLanes;
-  __shared__ float shared[kThreads * kSize];
+  constexpr int kGroups = kJoinThreads / kLanes;
+  __shared__ float shared[kJoinThreads * kSize];
   __shared__ uint32_t short_chunk[kJoinChunks], short_heads[kJoinChunks], long_chunk[kJoinChunks];
   __shared__ uint32_t shorts, longs, run;
   if (threadIdx.x == 0) shorts = longs = 0;
@@ -680,22 +749,25 @@ __global__ __launch_bounds__(kThreads) void k_segment_join(T* __restrict__ out, 
       const uint32_t front_after = (uint64_t)end + g.chunk < n ? key_at(end + g.chunk) : ~0u;
       if (key_at(end - 1) == key && key < s.vocabulary && !(front == key && before == key) &&
           (front == key || front_after == key)) {
-        // The chunks that begin with its key, eight looked at together.
+        // The chunks that begin with its key: eight looked at together, then the others.
         uint32_t heads = 1;
-        for (bool more = true; more && heads < kJoinLong;) {
-          uint32_t fronts[kAhead];
+        bool more = true;
+        auto probe = [&](auto first, auto last) {
+          uint32_t fronts[kJoinLong];
 #pragma unroll
-          for (int j = 0; j < kAhead; ++j) {
-            const uint64_t i = (uint64_t)end + (uint64_t)(heads + j) * g.chunk;
+          for (uint32_t j = decltype(first)::value; j < decltype(last)::value; ++j) {
+            const uint64_t i = (uint64_t)end + (uint64_t)j * g.chunk;
             fronts[j] = i < n ? key_at((uint32_t)i) : ~0u;
           }
 #pragma unroll
-          for (int j = 0; j < kAhead; ++j) {
+          for (uint32_t j = decltype(first)::value; j < decltype(last)::value; ++j) {
             more = more && fronts[j] == key;
             heads += more;
           }
-        }
-        if (heads < kJoinLong) {  // (a count at kJoinLong or beyond may not be all)
+        };
+        probe(std::integral_constant<uint32_t, 1>(), std::integral_constant<uint32_t, 8>());
+        if (more) probe(std::integral_constant<uint32_t, 8>(), std::integral_constant<uint32_t, kJoinLong>());
+        if (heads < kJoinLong) {  // (kJoinLong may not be all of them)
           const uint32_t k = atomicAdd(&shorts, 1u);
           short_chunk[k] = c;
           short_heads[k] = heads;
@@ -722,7 +794,7 @@ __global__ __launch_bounds__(kThreads) void k_segment_join(T* __restrict__ out, 
     const uint32_t c = long_chunk[k], key = key_at((c + 1) * g.chunk);
     uint32_t heads = kJoinLong;
     for (;;) {
-      if (threadIdx.x == 0) run = kThreads;
+      if (threadIdx.x == 0) run = kJoinThreads;
       __syncthreads();
       const uint64_t i = (uint64_t)(c + 1 + heads + threadIdx.x) * g.chunk;
       if (i >= n || key_at((uint32_t)i) != key) atomicMin(&run, threadIdx.x);
@@ -730,7 +802,7 @@ __global__ __launch_bounds__(kThreads) void k_segment_join(T* __restrict__ out, 
       const uint32_t more = run;
       __syncthreads();
       heads += more;
-      if (more < kThreads) break;
+      if (more < kJoinThreads) break;
     }
     float sum[kSize] = {};
     if (active) add_rows<kSize>(g.heads + (here + c) * g.dim + at, g.dim, 1 + group, 1 + heads, kGroups, sum);
@@ -846,9 +918,9 @@ int lookup(T* out, const T* weight, const I* tokens, int64_t rows, int64_t bag, 
 }
 
 // A chiplet's cache, and the part of it that a window's rows of grad may take.
-constexpr int64_t kCache = int64_t(4) << 20, kWindowBytes = int64_t(2) << 20;
-// Most tokens for the one-workgroup sort.
-constexpr int64_t kSmallTokens = kSmallThreads * 4;
+constexpr int64_t kCache = int64_t(4) << 20, kWindowBytes = int64_t(9) << 18;
+// Most tokens for the sort by ranges (LDS holds them all, were they one row's).
+constexpr int64_t kRangeTokens = 32768, kRangeWideTokens = 16384;
 constexpr int64_t kLongTiles = int64_t(1) << 21;  // tokens from which a tile has 16 rounds, not 4
 
 // How the gradient of rows x bag tokens is computed and laid out in the workspace.
@@ -856,7 +928,7 @@ struct GradientPlan {
   Sort sort;
   Segments segments;
   RowLanes row;
-  bool wide, small, few;  // 64-bit entries; one-workgroup sort; few tiles
+  bool wide, by_range, few;  // 64-bit entries; sort by ranges; few tiles
   int passes, rounds;
   size_t entries[2], counts, totals, heads, tails, parts, named, next_counts, clear_bytes, bytes;
 };
@@ -871,20 +943,19 @@ GradientPlan gradient_plan(int64_t rows, int64_t bag, int64_t vocabulary, int64_
   GradientPlan p = {};
   const int64_t n = rows * bag;
   p.row = row_lanes(dim, size);
-  // Windows, a multiple of the chiplets, where a table row keeps at least 16
+  // Windows that a chiplet's cache holds, where a table row keeps at least 16
   // tokens in each: its partial sums are then few against what they gather.
   int64_t windows = 1;
-  const int64_t bytes = rows * dim * (16 / size), most = n / (16 * vocabulary) / kChiplets * kChiplets;
-  if (bytes > kCache && most >= kChiplets) {
-    windows = ((bytes + kWindowBytes - 1) / kWindowBytes + kChiplets - 1) / kChiplets * kChiplets;
-    if (windows > most) windows = most;
-  }
+  const int64_t bytes = rows * dim * (16 / size), most = n / (16 * vocabulary);
+  if (bytes > kCache)
+    while (windows * kWindowBytes < bytes && (windows < kChiplets ? 2 * windows : windows + kChiplets) <= most)
+      windows = windows < kChiplets ? 2 * windows : windows + kChiplets;
   const int64_t window = (rows + windows - 1) / windows;
   const int key_bits = bits_of(vocabulary), row_bits = bits_of(window - 1);
   p.passes = (key_bits + kDigitBits - 1) / kDigitBits;
   p.wide = key_bits + row_bits > 32;
-  p.small = windows == 1 && n <= kSmallTokens;
-  p.few = !p.small && windows == 1 && n <= (int64_t)kFewTiles * 4 * kSortThreads;
+  p.by_range = windows == 1 && n <= (p.wide ? kRangeWideTokens : kRangeTokens) && vocabulary < kRanges * kRanges;
+  p.few = !p.by_range && windows == 1 && n <= (int64_t)kFewTiles * 4 * kSortThreads;
   p.rounds = p.few ? 1 : n < kLongTiles ? 4 : 16;
   while (p.few && n > (int64_t)kFewTiles * p.rounds * kSortThreads) p.rounds *= 2;
   const int64_t tile = (int64_t)p.rounds * kSortThreads;
@@ -899,7 +970,7 @@ GradientPlan gradient_plan(int64_t rows, int64_t bag, int64_t vocabulary, int64_
   p.sort.tokens = (uint64_t)(window * bag);
   // Sorted tokens of a group: enough groups for the chip, then longer walks,
   // which leave fewer parts to join.
-  int64_t chunk = n * p.row.lanes * p.row.groups / (4 * kBusyLanes);
+  int64_t chunk = n * p.row.lanes * p.row.groups / (2 * kBusyLanes);
   chunk = (chunk + kAhead - 1) / kAhead * kAhead;
   chunk = chunk < kAhead ? kAhead : chunk > 512 ? 512 : chunk;
   p.segments.chunk = (uint32_t)chunk;
@@ -913,8 +984,8 @@ GradientPlan gradient_plan(int64_t rows, int64_t bag, int64_t vocabulary, int64_
   };
   const size_t sorted = (size_t)n * (p.wide ? 8 : 4);
   p.entries[0] = take(sorted);
-  p.entries[1] = p.small ? p.entries[0] : take(sorted);
-  if (!p.small) {
+  p.entries[1] = p.by_range ? p.entries[0] : take(sorted);
+  if (!p.by_range) {
     p.counts = take((size_t)windows * kDigits * p.sort.tiles * sizeof(uint32_t));
     p.totals = take((size_t)windows * kDigits * sizeof(uint32_t));
   }
@@ -958,12 +1029,17 @@ uint32_t clear_blocks(const Clear& c, int threads) {
   return at_most((bytes + 128 * threads - 1) / (128 * threads), 1024);
 }
 
-template <typename E, typename I, int kRounds>
-void sort_small(const GradientPlan& p, E* out, const I* tokens, Clearing& clearing, hipStream_t stream) {
-  const uint32_t lds = kSmallWaves * kDigits * 4 + kDigits * 4 + 2 * kSmallWaves * 4 + (uint32_t)p.sort.tokens * sizeof(E);
+template <typename E, typename I>
+int sort_ranges(const GradientPlan& p, E* out, const I* tokens, Clearing& clearing, hipStream_t stream) {
+  const uint32_t keys = p.sort.vocabulary + 1, range = (keys + kRanges - 1) / kRanges, ranges = (keys + range - 1) / range;
+  const uint32_t n = (uint32_t)p.sort.tokens, share = (n + kRangeThreads - 1) / kRangeThreads * kWave;
+  const uint32_t lds = (kRangeWaves * kDigits + kDigits + 3 * kRangeWaves) * 4 + kRangeWaves * share * (uint32_t)sizeof(E);
+  if (lds > 65536)
+    MGB_CHECK(hipFuncSetAttribute((const void*)k_sort_ranges<E, I>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
   const Clear zero = next_clear(clearing);
-  hipLaunchKernelGGL((k_sort_small<E, I, kRounds>), dim3(1 + clear_blocks(zero, kSmallThreads)), dim3(kSmallThreads),
-                     lds, stream, out, tokens, p.sort, p.passes, zero);
+  hipLaunchKernelGGL((k_sort_ranges<E, I>), dim3(ranges + clear_blocks(zero, kRangeThreads)), dim3(kRangeThreads), lds,
+                     stream, out, tokens, p.sort, range, ranges, share, zero);
+  return 0;
 }
 
 template <typename E, typename F, int kRounds, bool kFew>
@@ -986,16 +1062,12 @@ void sort_pass(const GradientPlan& p, uint8_t* ws, F from, E* out, int pass, Cle
                      kFew && pass + 1 < p.passes ? later + (size_t)pass * each : nullptr, p.sort, pass, zero);
 }
 
-// The sorted entries' place.
+// The sorted entries' place; null after an error.
 template <typename E, typename I>
 E* sort_tokens(const GradientPlan& p, uint8_t* ws, const I* tokens, Clearing clearing, hipStream_t stream) {
   E* entries[2] = {(E*)(ws + p.entries[0]), (E*)(ws + p.entries[1])};
-  clearing.launches = p.small ? 1 : p.few ? p.passes + 1 : 2 * p.passes;
-  if (p.small) {
-    if (p.sort.tokens <= kSmallThreads) sort_small<E, I, 1>(p, entries[0], tokens, clearing, stream);
-    else sort_small<E, I, 4>(p, entries[0], tokens, clearing, stream);
-    return entries[0];
-  }
+  clearing.launches = p.by_range ? 1 : p.few ? p.passes + 1 : 2 * p.passes;
+  if (p.by_range) return sort_ranges<E, I>(p, entries[0], tokens, clearing, stream) ? nullptr : entries[0];
   int now = 0;
   for (int pass = 0; pass < p.passes; ++pass, now ^= 1) {
     auto run = [&](auto from) {
@@ -1026,6 +1098,7 @@ int lookup_gradient(GradientPlan& p, T* out, const T* grad, const I* tokens, uin
     clearing.left = (uint64_t)p.sort.vocabulary * p.segments.dim * sizeof(T);
   }
   const E* sorted = sort_tokens<E, I>(p, ws, tokens, clearing, stream);
+  if (!sorted) return -1;
   MGB_LAUNCH_CHECK("embedding gradient: sort");
   with_lanes<T>(p.row, [&](auto l, auto size) {
     constexpr int kLanes = decltype(l)::value, kSize = decltype(size)::value;
@@ -1041,8 +1114,8 @@ int lookup_gradient(GradientPlan& p, T* out, const T* grad, const I* tokens, uin
                          sorted, p.sort, p.segments);
     if (chunks > 1)
       hipLaunchKernelGGL((k_segment_join<T, E, kLanes, kSize>),
-                         dim3(windows * ((chunks + kJoinChunks - 1) / kJoinChunks), columns), dim3(kThreads), 0, stream,
-                         out, sorted, p.sort, p.segments);
+                         dim3(windows * ((chunks + kJoinChunks - 1) / kJoinChunks), columns), dim3(kJoinThreads), 0,
+                         stream, out, sorted, p.sort, p.segments);
     if (windows > 1)
       hipLaunchKernelGGL((k_segment_windows<T, kLanes, kSize>),
                          dim3(at_most((p.sort.vocabulary + kGroups - 1) / kGroups, 4096), columns), dim3(kThreads), 0,
