@@ -18,6 +18,9 @@ namespace mgb {
 namespace {
 
 constexpr int kNormThreads = 256;
+// Of the gradient's workgroups: several rows where a row is at most a wave's, else
+// one (its sums take the whole workgroup's barriers).
+constexpr int gradient_threads(int lanes) { return lanes > kWave ? lanes : 512; }
 constexpr int kReduceColumns = 32, kReduceSlices = 32;
 
 // Elements a lane holds at most; beyond kNormThreads * that, 1024 lanes take a
@@ -34,11 +37,41 @@ __device__ __forceinline__ float row_sum(float v, float* shared) {
   }
 }
 
-template <typename T, typename W, int kLanes, int kPacks>
+// A lane's columns of a row: kPacks times kSize, a pack or, in rows narrower than
+// a pack, one.  The last pack of a row that is no whole number of packs begins
+// early, so that it ends with the row, and lanes beyond the row take that too:
+// what a lane shares with the one before it counts in no sum, and both store the
+// same values.
+template <int kLanes, int kPacks, int kSize>
+struct Columns {
+  int64_t at[kPacks];
+  int shared_with[kPacks];  // the first values, another lane's
+  __device__ __forceinline__ Columns(int lane, int64_t dim) {
+#pragma unroll
+    for (int k = 0; k < kPacks; ++k) {
+      const int64_t nominal = (int64_t)(k * kLanes + lane) * kSize;
+      at[k] = nominal < dim - kSize ? nominal : dim - kSize;
+      const int64_t common = nominal - at[k];
+      shared_with[k] = common < kSize ? (int)common : kSize;
+    }
+  }
+  // v, or 0 where it counts for another lane.
+  __device__ __forceinline__ float own(int k, int e, float v) const { return e >= shared_with[k] ? v : 0.0f; }
+  __device__ __forceinline__ bool any(int k) const { return shared_with[k] < kSize; }
+};
+
+template <typename W, int kSize>
+__device__ __forceinline__ void load_row_part(const W* from, float* out) {
+  W w[kSize];
+  __builtin_memcpy(w, from, sizeof(w));
+#pragma unroll
+  for (int e = 0; e < kSize; ++e) out[e] = (float)w[e];
+}
+
+template <typename T, typename W, int kLanes, int kPacks, int kSize>
 __global__ __launch_bounds__(kLanes > kNormThreads ? kLanes : kNormThreads) void k_norm(
     T* __restrict__ y, float* __restrict__ means, float* __restrict__ rstds, const T* __restrict__ x,
     const W* __restrict__ weight, const W* __restrict__ bias, int64_t rows, int64_t dim, int64_t stride, float eps) {
-  constexpr int kSize = Pack<T>::kSize;
   constexpr int kThreads = kLanes > kNormThreads ? kLanes : kNormThreads;
   __shared__ float shared[kThreads / kWave];
   const int lane = threadIdx.x % kLanes;
@@ -46,23 +79,27 @@ __global__ __launch_bounds__(kLanes > kNormThreads ? kLanes : kNormThreads) void
   // Lanes of a row beyond the last only occur where a row is at most a wave's:
   // no barrier follows.
   if (row >= rows) return;
+  const Columns<kLanes, kPacks, kSize> columns(lane, dim);
   const T* in = x + row * stride;
+  Raw<T, kSize> raw[kPacks];
+#pragma unroll
+  for (int k = 0; k < kPacks; ++k) raw[k].load(in + columns.at[k]);
   float v[kPacks][kSize];
   float sum = 0.0f;
 #pragma unroll
-  for (int k = 0; k < kPacks; ++k) load_pack(in, (int64_t)(k * kLanes + lane) * kSize, dim, v[k]);
+  for (int k = 0; k < kPacks; ++k) {
+    raw[k].get(v[k]);
 #pragma unroll
-  for (int k = 0; k < kPacks; ++k)
-#pragma unroll
-    for (int e = 0; e < kSize; ++e) sum += v[k][e];
+    for (int e = 0; e < kSize; ++e) sum += columns.own(k, e, v[k][e]);
+  }
   const float mean = row_sum<kLanes>(sum, shared) / (float)dim;
   float squares = 0.0f;
 #pragma unroll
   for (int k = 0; k < kPacks; ++k)
 #pragma unroll
     for (int e = 0; e < kSize; ++e) {
-      v[k][e] = (int64_t)(k * kLanes + lane) * kSize + e < dim ? v[k][e] - mean : 0.0f;
-      squares = fmaf(v[k][e], v[k][e], squares);
+      v[k][e] -= mean;
+      squares = fmaf(columns.own(k, e, v[k][e]), v[k][e], squares);
     }
   const float rstd = 1.0f / sqrtf(row_sum<kLanes>(squares, shared) / (float)dim + eps);
   if (lane == 0) {
@@ -72,16 +109,15 @@ __global__ __launch_bounds__(kLanes > kNormThreads ? kLanes : kNormThreads) void
   T* out = y + row * dim;
 #pragma unroll
   for (int k = 0; k < kPacks; ++k) {
-    const int64_t at = (int64_t)(k * kLanes + lane) * kSize;
     float w[kSize], b[kSize];
-    if (weight) load_some<kSize>(weight, at, dim, w);
-    if (bias) load_some<kSize>(bias, at, dim, b);
+    if (weight) load_row_part<W, kSize>(weight + columns.at[k], w);
+    if (bias) load_row_part<W, kSize>(bias + columns.at[k], b);
 #pragma unroll
     for (int e = 0; e < kSize; ++e) {
       const float h = v[k][e] * rstd;
       v[k][e] = weight ? (bias ? fmaf(h, w[e], b[e]) : h * w[e]) : h;
     }
-    store_pack(out, at, dim, v[k]);
+    if (columns.any(k)) raw[k].put(v[k], out + columns.at[k]);
   }
 }
 
@@ -129,47 +165,61 @@ __global__ __launch_bounds__(1024) void k_norm_wide(T* __restrict__ y, float* __
 
 // dx row by row; the rows of a workgroup are its column sums' slice, kept in
 // registers (a lane holds the same columns of every row) and joined over the
-// workgroup's row groups at the end.  partial: [workgroup][2][dim], dw then db.
-template <typename T, typename W, int kLanes, int kPacks>
-__global__ __launch_bounds__(kLanes > kNormThreads ? kLanes : kNormThreads) void k_norm_gradient(
+// workgroup's row groups at the end.  The next row is on its way while a row's sums
+// cross the lanes.  partial: [workgroup][2][dim], dw then db.
+template <typename T, typename W, int kLanes, int kPacks, int kSize>
+__global__ __launch_bounds__(gradient_threads(kLanes)) void k_norm_gradient(
     T* __restrict__ dx, float* __restrict__ partial, const T* __restrict__ grad, const T* __restrict__ x,
     const float* __restrict__ means, const float* __restrict__ rstds, const W* __restrict__ weight, int64_t rows,
     int64_t dim, int64_t grad_stride, int64_t stride) {
-  constexpr int kSize = Pack<T>::kSize;
-  constexpr int kThreads = kLanes > kNormThreads ? kLanes : kNormThreads;
+  constexpr int kThreads = gradient_threads(kLanes);
   constexpr int kGroups = kThreads / kLanes;
   __shared__ float shared[kThreads / kWave];
   __shared__ float joined[kGroups > 1 ? kThreads * kSize : 1];
   const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const Columns<kLanes, kPacks, kSize> columns(lane, dim);
   float dw[kPacks][kSize] = {}, db[kPacks][kSize] = {}, w[kPacks][kSize];
 #pragma unroll
   for (int k = 0; k < kPacks; ++k)
-    if (weight) load_some<kSize>(weight, (int64_t)(k * kLanes + lane) * kSize, dim, w[k]);
+    if (weight) load_row_part<W, kSize>(weight + columns.at[k], w[k]);
   const float inverse = 1.0f / (float)dim;
+  const int64_t step = (int64_t)gridDim.x * kGroups;
+  Raw<T, kSize> next_x[kPacks], next_g[kPacks];
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  auto fetch = [&](int64_t row) {
+    if (row >= rows) return;
+#pragma unroll
+    for (int k = 0; k < kPacks; ++k) {
+      next_x[k].load(x + row * stride + columns.at[k]);
+      next_g[k].load(grad + row * grad_stride + columns.at[k]);
+    }
+    next_mean = means[row];
+    next_rstd = rstds[row];
+  };
+  int64_t row = (int64_t)blockIdx.x * kGroups + group;
+  fetch(row);
   // Where a row takes the whole workgroup, all its lanes run the same rows.
-  for (int64_t row = (int64_t)blockIdx.x * kGroups + group; row < rows; row += (int64_t)gridDim.x * kGroups) {
-    const T* in = x + row * stride;
-    const T* gin = grad + row * grad_stride;
+  for (; row < rows; row += step) {
     float h[kPacks][kSize], g[kPacks][kSize];
 #pragma unroll
     for (int k = 0; k < kPacks; ++k) {
-      const int64_t at = (int64_t)(k * kLanes + lane) * kSize;
-      load_pack(in, at, dim, h[k]);
-      load_pack(gin, at, dim, g[k]);
+      next_x[k].get(h[k]);
+      next_g[k].get(g[k]);
     }
-    const float mean = means[row], rstd = rstds[row];
+    const float mean = next_mean, rstd = next_rstd;
+    fetch(row + step);
     float s1 = 0.0f, s2 = 0.0f;
 #pragma unroll
     for (int k = 0; k < kPacks; ++k)
 #pragma unroll
       for (int e = 0; e < kSize; ++e) {
-        // Beyond the row g and h are 0 and add nothing.
-        h[k][e] = (int64_t)(k * kLanes + lane) * kSize + e < dim ? (h[k][e] - mean) * rstd : 0.0f;
+        h[k][e] = (h[k][e] - mean) * rstd;
         dw[k][e] = fmaf(g[k][e], h[k][e], dw[k][e]);
         db[k][e] += g[k][e];
         if (weight) g[k][e] *= w[k][e];
-        s1 += g[k][e];
-        s2 = fmaf(g[k][e], h[k][e], s2);
+        const float own = columns.own(k, e, g[k][e]);
+        s1 += own;
+        s2 = fmaf(own, columns.own(k, e, h[k][e]), s2);
       }
     s1 = row_sum<kLanes>(s1, shared) * inverse;
     s2 = row_sum<kLanes>(s2, shared) * inverse;
@@ -178,7 +228,7 @@ __global__ __launch_bounds__(kLanes > kNormThreads ? kLanes : kNormThreads) void
     for (int k = 0; k < kPacks; ++k) {
 #pragma unroll
       for (int e = 0; e < kSize; ++e) g[k][e] = rstd * (g[k][e] - fmaf(h[k][e], s2, s1));
-      store_pack(out, (int64_t)(k * kLanes + lane) * kSize, dim, g[k]);
+      if (columns.any(k)) Raw<T, kSize>().put(g[k], out + columns.at[k]);
     }
   }
   if (!partial) return;
@@ -198,10 +248,9 @@ __global__ __launch_bounds__(kLanes > kNormThreads ? kLanes : kNormThreads) void
 #pragma unroll
           for (int e = 0; e < kSize; ++e) mine[e] += joined[(other * kLanes + lane) * kSize + e];
       }
-      const int64_t at = (int64_t)(k * kLanes + lane) * kSize;
+      if (columns.any(k))
 #pragma unroll
-      for (int e = 0; e < kSize; ++e)
-        if (at + e < dim) slice[part * dim + at + e] = mine[e];
+        for (int e = 0; e < kSize; ++e) slice[part * dim + columns.at[k] + e] = mine[e];
     }
 }
 
@@ -273,6 +322,7 @@ __global__ __launch_bounds__(kReduceColumns* kReduceSlices) void k_norm_reduce(W
   const int64_t at = (int64_t)blockIdx.x * kReduceColumns + column;
   float sum = 0.0f;
   if (at < 2 * dim)
+#pragma unroll 8
     for (int s = part; s < slices; s += kReduceSlices) sum += partial[(int64_t)s * 2 * dim + at];
   sums[part][column] = sum;
   __syncthreads();
@@ -290,19 +340,20 @@ __global__ __launch_bounds__(kReduceColumns* kReduceSlices) void k_norm_reduce(W
 // each, then a workgroup's 256 and 1024 with kBlockElements.  Returns 0 where
 // the wide form takes the row.
 struct RowShape {
-  int lanes, packs;
+  int lanes, packs, size;  // size: values of a pack, 1 in rows narrower than one
 };
 
-RowShape row_shape(int64_t dim, int size, int block_elements) {
-  const int64_t packs = (dim + size - 1) / size;
+RowShape row_shape(int64_t dim, int pack, int block_elements) {
+  if (dim < pack) return {8, 1, 1};
+  const int64_t packs = (dim + pack - 1) / pack;
   int lanes = 8;
   while (lanes < 64 && lanes < packs) lanes *= 2;
-  if (lanes == 64 && packs > 64 * (kWaveElements / size)) lanes = 256;
-  if (lanes == 256 && packs > 256 * (kBlockElements / size)) lanes = 1024;
-  if (lanes == 1024 && packs > 1024 * (block_elements / size)) return {0, 0};
+  if (lanes == 64 && packs > 64 * (kWaveElements / pack)) lanes = 256;
+  if (lanes == 256 && packs > 256 * (kBlockElements / pack)) lanes = 1024;
+  if (lanes == 1024 && packs > 1024 * (block_elements / pack)) return {0, 0, pack};
   int each = 1;
   while ((int64_t)each * lanes < packs) each *= 2;
-  return {lanes, each};
+  return {lanes, each, pack};
 }
 
 // Calls fn(lanes, packs) with both as constants; the combinations row_shape gives.
@@ -319,7 +370,13 @@ bool with_packs(int packs, F&& fn) {
 
 template <int kSize, int kWideElements, typename F>
 bool with_shape(RowShape shape, F&& fn) {
-  auto lanes = [&](auto l) { return [&, l](auto p) { fn(l, p); }; };
+  using Size = std::integral_constant<int, kSize>;
+  using One = std::integral_constant<int, 1>;
+  auto lanes = [&](auto l) { return [&, l](auto p) { fn(l, p, Size()); }; };
+  if (shape.size == 1) {
+    fn(std::integral_constant<int, 8>(), One(), One());
+    return true;
+  }
   switch (shape.lanes) {
     case 8: return with_packs<1>(shape.packs, lanes(std::integral_constant<int, 8>()));
     case 16: return with_packs<1>(shape.packs, lanes(std::integral_constant<int, 16>()));
@@ -334,19 +391,19 @@ bool with_shape(RowShape shape, F&& fn) {
 template <typename T, typename W>
 int norm(T* y, float* mean, float* rstd, const T* x, const W* weight, const W* bias, int64_t rows, int64_t dim,
          int64_t stride, float eps, hipStream_t stream) {
-  constexpr int kSize = Pack<T>::kSize;
-  const RowShape shape = row_shape(dim, kSize, kBlockElements);
+  constexpr int kPack = Pack<T>::kSize;
+  const RowShape shape = row_shape(dim, kPack, kBlockElements);
   // A launch holds fewer than 2^32 lanes: very many narrow rows take several.
   constexpr int64_t kRowsAtOnce = int64_t(1) << 21;
   for (int64_t first = 0; first < rows; first += kRowsAtOnce) {
     const int64_t count = rows - first < kRowsAtOnce ? rows - first : kRowsAtOnce;
     const T* in = x + first * stride;
     T* out = y + first * dim;
-    const bool done = with_shape<kSize, kBlockElements>(shape, [&](auto l, auto p) {
-      constexpr int kLanes = decltype(l)::value, kPacks = decltype(p)::value;
+    const bool done = with_shape<kPack, kBlockElements>(shape, [&](auto l, auto p, auto z) {
+      constexpr int kLanes = decltype(l)::value, kPacks = decltype(p)::value, kSize = decltype(z)::value;
       constexpr int kThreads = kLanes > kNormThreads ? kLanes : kNormThreads;
       const uint32_t grid = (uint32_t)((count + kThreads / kLanes - 1) / (kThreads / kLanes));
-      hipLaunchKernelGGL((k_norm<T, W, kLanes, kPacks>), dim3(grid), dim3(kThreads), 0, stream, out, mean + first,
+      hipLaunchKernelGGL((k_norm<T, W, kLanes, kPacks, kSize>), dim3(grid), dim3(kThreads), 0, stream, out, mean + first,
                          rstd + first, in, weight, bias, count, dim, stride, eps);
     });
     if (!done)
@@ -359,15 +416,14 @@ int norm(T* y, float* mean, float* rstd, const T* x, const W* weight, const W* b
 
 // Gradient: 1024 lanes hold half as much of a row, for the column sums.
 constexpr int kGradientWideElements = 16;
-// Workgroups of 256: two to a CU keep the memory busy, and their slices of the
-// column sums stay small against the rows.
-constexpr int64_t kGradientGroups = 512;
+// One workgroup of 512 to a CU (two of 256), and more rows by turns: their slices
+// of the column sums stay small against the rows.
+constexpr int64_t kGradientGroups = 256;
 
 int64_t gradient_slices(int64_t rows, int64_t dim, int size) {
   const RowShape shape = row_shape(dim, size, kGradientWideElements);
-  const int64_t at_once = shape.lanes && shape.lanes < kNormThreads ? kNormThreads / shape.lanes : 1;
-  const int64_t most = shape.lanes == 1024 || !shape.lanes ? kGradientGroups / 2 : kGradientGroups;
-  const int64_t wanted = (rows + at_once - 1) / at_once;
+  const int64_t at_once = shape.lanes ? gradient_threads(shape.lanes) / shape.lanes : 1;
+  const int64_t wanted = (rows + at_once - 1) / at_once, most = shape.lanes == 256 ? 2 * kGradientGroups : kGradientGroups;
   return wanted < 1 ? 1 : wanted < most ? wanted : most;
 }
 
@@ -375,15 +431,15 @@ template <typename T, typename W>
 int norm_gradient(T* dx, W* dweight, W* dbias, const T* grad, const T* x, const float* mean, const float* rstd,
                   const W* weight, int64_t rows, int64_t dim, int64_t grad_stride, int64_t stride, float* partial,
                   hipStream_t stream) {
-  constexpr int kSize = Pack<T>::kSize;
-  const RowShape shape = row_shape(dim, kSize, kGradientWideElements);
-  const int64_t slices = gradient_slices(rows, dim, kSize);
+  constexpr int kPack = Pack<T>::kSize;
+  const RowShape shape = row_shape(dim, kPack, kGradientWideElements);
+  const int64_t slices = gradient_slices(rows, dim, kPack);
   if (!dweight) partial = nullptr;
   if (rows || partial) {
-    const bool done = with_shape<kSize, kGradientWideElements>(shape, [&](auto l, auto p) {
-      constexpr int kLanes = decltype(l)::value, kPacks = decltype(p)::value;
-      constexpr int kThreads = kLanes > kNormThreads ? kLanes : kNormThreads;
-      hipLaunchKernelGGL((k_norm_gradient<T, W, kLanes, kPacks>), dim3((uint32_t)slices), dim3(kThreads), 0, stream, dx,
+    const bool done = with_shape<kPack, kGradientWideElements>(shape, [&](auto l, auto p, auto z) {
+      constexpr int kLanes = decltype(l)::value, kPacks = decltype(p)::value, kSize = decltype(z)::value;
+      constexpr int kThreads = gradient_threads(kLanes);
+      hipLaunchKernelGGL((k_norm_gradient<T, W, kLanes, kPacks, kSize>), dim3((uint32_t)slices), dim3(kThreads), 0, stream, dx,
                          partial, grad, x, mean, rstd, weight, rows, dim, grad_stride, stride);
     });
     if (!done)
