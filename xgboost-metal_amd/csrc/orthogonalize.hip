@@ -3,13 +3,12 @@
 // ones transposed),
 //   X <- (a I + b A + c A^2) X,   A = X X^T,   `steps` times.
 // Every step is a polynomial Z in A applied from the left, so a segment of
-// steps runs among m x m matrices: A <- Z A Z and P <- Z P, all symmetric and
+// steps can run among m x m matrices: A <- Z A Z and P <- Z P, all symmetric and
 // commuting, and one product X <- P X ends it.  For n > m that leaves out most
 // products with n; symmetric results take half their tiles.  An error in A grows
-// by a^2 a step where X is small, so a segment has at most kSegment steps and
-// the next one takes A from X anew: with three, the result is as near the
-// exact one as binary32 products of the plain form come (low rank 512 x 2048:
-// 4e-5 of the norm against 2e-5; all five in one segment: 1e-4).
+// by a^2 a step where X is small, so a segment has at most two or three steps
+// and the next one takes A from X anew (low rank 512 x 2048: 4e-5 of the norm with
+// three, 2e-5 in plain binary32, 1e-4 with all five in one segment).
 //
 // The matrix instructions multiply binary16.  A small direction's part grows
 // a-fold a step, so operands of 11 bits would show in the result (4e-2 of the
@@ -331,6 +330,12 @@ __global__ __launch_bounds__(kWaves* kWave) void k_product_small(Product p) {
   if (!find_tile<kMode>((uint32_t)p.row_tiles, (uint32_t)p.column_tiles, &ti, &tj)) return;
   const half8* left = (const half8*)(job.left.data + batch * job.left.batch_stride + ti * job.left.blocks * 2 * kBlock) + lane;
   const half8* right = (const half8*)(job.right.data + batch * job.right.batch_stride + tj * job.right.blocks * 2 * kBlock) + lane;
+  // What the end adds is fetched with the first operands.
+  const Finish<kMode, T> finish(p, job, batch, total_factor(p, job, batch), ti, tj, ti != tj);
+  constexpr int kMine = kWaves > 1 ? 1 : 4;  // quarters of the tile that a wave finishes
+  Parts added[kMine];
+#pragma unroll
+  for (int q = 0; q < kMine; ++q) added[q] = finish.fetch(kWaves > 1 ? wave % 4 : q);
   struct Operands {
     half8 left[2], right[2];
   };
@@ -340,7 +345,13 @@ __global__ __launch_bounds__(kWaves* kWave) void k_product_small(Product p) {
     o.right[0] = right[k * 2 * kWave];
     if constexpr (kRightLow) o.right[1] = right[k * 2 * kWave + kWave];
   };
-  float16v sum = {};
+  // A sum for each kind of product: those of one sum wait for each other.
+  float16v sums[3] = {};
+  auto multiply = [&](const Operands& o) {
+    sums[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.left[0], o.right[0], sums[0], 0, 0, 0);
+    if constexpr (kLeftLow) sums[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.left[1], o.right[0], sums[1], 0, 0, 0);
+    if constexpr (kRightLow) sums[2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(o.left[0], o.right[1], sums[2], 0, 0, 0);
+  };
   const int64_t share = (p.depth + kWaves - 1) / kWaves, begin = wave * share;
   const int64_t steps = (begin + share < p.depth ? begin + share : p.depth) - begin;
   if (steps > 0) {
@@ -351,32 +362,29 @@ __global__ __launch_bounds__(kWaves* kWave) void k_product_small(Product p) {
     for (; k + kAhead <= steps; k += kAhead)
 #pragma unroll
       for (int q = 0; q < kAhead; ++q) {
-        multiply_block<kLeftLow, kRightLow>(ring[q].left, ring[q].right, sum);
+        multiply(ring[q]);
         const int64_t ahead = k + q + kAhead;
         fetch(ring[q], begin + (ahead < steps ? ahead : steps - 1));
       }
 #pragma unroll
     for (int q = 0; q < kAhead; ++q)
-      if (k + q < steps) multiply_block<kLeftLow, kRightLow>(ring[q].left, ring[q].right, sum);
+      if (k + q < steps) multiply(ring[q]);
   }
-  const Finish<kMode, T> finish(p, job, batch, total_factor(p, job, batch), ti, tj, ti != tj);
+  float16v sum = sums[0];
+  if constexpr (kLeftLow || kRightLow) sum += sums[1] + sums[2];
   if constexpr (kWaves > 1) {
     // The first four waves join and finish a quarter each.
 #pragma unroll
-    for (int g = 0; g < 4; ++g) joined[(wave * 4 + g) * kWave + lane] = four_of(sum, g);
+    for (int q = 0; q < 4; ++q) joined[(wave * 4 + q) * kWave + lane] = four_of(sum, q);
     __syncthreads();
     if (wave >= 4) return;
-    const Parts added = finish.fetch(wave);
     float4v v = joined[wave * kWave + lane];
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) v += joined[(w * 4 + wave) * kWave + lane];
-    finish(wave, v, added);
+    finish(wave, v, added[0]);
   } else {
-    Parts added[4];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) added[q] = finish.fetch(q);
-#pragma unroll
-    for (int q = 0; q < 4; ++q) finish(q, four_of(sum, q), added[q]);
+    for (int q = 0; q < 4; ++q) finish(q, four_of(sum, q), added[kWaves > 1 ? 0 : q]);
   }
 }
 
@@ -403,6 +411,17 @@ __global__ __launch_bounds__(4 * kWave, 1) void k_product(Product p) {
   const Job& job = p.job[blockIdx.y];
   uint32_t ti, tj;
   if (!find_tile<kMode>((uint32_t)(p.row_tiles / kSide), (uint32_t)(p.column_tiles / kSide), &ti, &tj)) return;
+  // What the end adds is fetched first.
+  constexpr int kSums = kHalf * kHalf;
+  const float factor = total_factor(p, job, batch);
+  auto finish_of = [&](int s) {
+    return Finish<kMode, T>(p, job, batch, factor, ti * kSide + wave / 2 * kHalf + s / kHalf, tj * kSide + wave % 2 * kHalf + s % kHalf, ti != tj);
+  };
+  Parts added[kSums][4];
+#pragma unroll
+  for (int s = 0; s < kSums; ++s)
+#pragma unroll
+    for (int q = 0; q < 4; ++q) added[s][q] = finish_of(s).fetch(q);
   // The blocks this wave loads of every stage.
   const _Float16* from[kLoads];
 #pragma unroll
@@ -445,7 +464,7 @@ __global__ __launch_bounds__(4 * kWave, 1) void k_product(Product p) {
     o.v[side][d][i][1 - high] = blocks[(d * (kLeft + kRight) + (side ? kLeft + wj : wi) + i + (high ? 0 : kSide)) * kWave];
   };
   // The instructions of a stage, those on one sum far apart.
-  constexpr int kSums = kHalf * kHalf, kProducts = 1 + kLeftLow + kRightLow, kCalls = kProducts * kDepth * kSums;
+  constexpr int kProducts = 1 + kLeftLow + kRightLow, kCalls = kProducts * kDepth * kSums;
   constexpr int kChains = kSums < 4 ? 2 : 1;  // sums of a block, where the blocks are few
   float16v sum[kSums][kChains] = {};
   auto multiply = [&](const Operands& o, int t) {
@@ -491,15 +510,6 @@ __global__ __launch_bounds__(4 * kWave, 1) void k_product(Product p) {
   }
   // Nothing may land in LDS after the workgroup has ended.
   __builtin_amdgcn_s_waitcnt(0x70);  // vmcnt(0) lgkmcnt(0)
-  const float factor = total_factor(p, job, batch);
-  auto finish_of = [&](int s) {
-    return Finish<kMode, T>(p, job, batch, factor, ti * kSide + wi + s / kHalf, tj * kSide + wj + s % kHalf, ti != tj);
-  };
-  Parts added[kSums][4];
-#pragma unroll
-  for (int s = 0; s < kSums; ++s)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) added[s][q] = finish_of(s).fetch(q);
 #pragma unroll
   for (int s = 0; s < kSums; ++s) {
     if constexpr (kChains > 1) sum[s][0] += sum[s][1];
@@ -833,7 +843,12 @@ int orthogonalize(T* out, const T* g, int64_t batch, int64_t rows, int64_t colum
     j.factor = scale;
     return j;
   };
-  const int segments = (steps + kMost - 1) / kMost;
+  // Segments of one step (the products as they stand in the formula) take three
+  // launches a step, longer ones 3.3 to 3.5, and multiplications with n in every
+  // step.  Measured, us: 1,500 x 2,048 489 and 501, 700 x 1,400 210 and 205;
+  // 128 x 1,000 89 and 94, 128 x 2,048 104 and 102.
+  const bool plain = 5 * pl.n <= 7 * pl.m || (pl.m <= 384 && pl.n <= 1024);
+  const int most = plain ? 1 : kMost, segments = (steps + most - 1) / most;
   for (int s = 0; s < segments; ++s) {
     const int length = steps / segments + (s < steps % segments ? 1 : 0);
     Product gram = square;
