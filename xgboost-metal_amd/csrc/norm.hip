@@ -166,16 +166,18 @@ __global__ __launch_bounds__(1024) void k_norm_wide(T* __restrict__ y, float* __
 // dx row by row; the rows of a workgroup are its column sums' slice, kept in
 // registers (a lane holds the same columns of every row) and joined over the
 // workgroup's row groups at the end.  The next row is on its way while a row's sums
-// cross the lanes.  partial: [workgroup][2][dim], dw then db.
+// cross the lanes.  partial: [workgroup][2][dim], dw then db; one workgroup alone
+// has the sums and stores them.
 template <typename T, typename W, int kLanes, int kPacks, int kSize>
 __global__ __launch_bounds__(gradient_threads(kLanes)) void k_norm_gradient(
-    T* __restrict__ dx, float* __restrict__ partial, const T* __restrict__ grad, const T* __restrict__ x,
-    const float* __restrict__ means, const float* __restrict__ rstds, const W* __restrict__ weight, int64_t rows,
-    int64_t dim, int64_t grad_stride, int64_t stride) {
+    T* __restrict__ dx, float* __restrict__ partial, W* __restrict__ dweight, W* __restrict__ dbias,
+    const T* __restrict__ grad, const T* __restrict__ x, const float* __restrict__ means,
+    const float* __restrict__ rstds, const W* __restrict__ weight, int64_t rows, int64_t dim, int64_t grad_stride,
+    int64_t stride) {
   constexpr int kThreads = gradient_threads(kLanes);
   constexpr int kGroups = kThreads / kLanes;
   __shared__ float shared[kThreads / kWave];
-  __shared__ float joined[kGroups > 1 ? kThreads * kSize : 1];
+  __shared__ float joined[kGroups > 1 ? kThreads / kWave * kLanes * kSize : 1];
   const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
   const Columns<kLanes, kPacks, kSize> columns(lane, dim);
   float dw[kPacks][kSize] = {}, db[kPacks][kSize] = {}, w[kPacks][kSize];
@@ -239,18 +241,30 @@ __global__ __launch_bounds__(gradient_threads(kLanes)) void k_norm_gradient(
     for (int k = 0; k < kPacks; ++k) {
       float* mine = part ? db[k] : dw[k];
       if constexpr (kGroups > 1) {
-        __syncthreads();
+        // The groups of a wave by exchanges, then the waves through LDS.
 #pragma unroll
-        for (int e = 0; e < kSize; ++e) joined[(group * kLanes + lane) * kSize + e] = mine[e];
+        for (int d = kLanes; d < kWave; d *= 2)
+#pragma unroll
+          for (int e = 0; e < kSize; ++e) mine[e] += __shfl_xor(mine[e], d, kWave);
+        __syncthreads();
+        if (threadIdx.x % kWave < kLanes)
+#pragma unroll
+          for (int e = 0; e < kSize; ++e) joined[(threadIdx.x / kWave * kLanes + lane) * kSize + e] = mine[e];
         __syncthreads();
         if (group) continue;
-        for (int other = 1; other < kGroups; ++other)
+#pragma unroll
+        for (int other = 1; other < kThreads / kWave; ++other)
 #pragma unroll
           for (int e = 0; e < kSize; ++e) mine[e] += joined[(other * kLanes + lane) * kSize + e];
       }
-      if (columns.any(k))
+      if (!columns.any(k)) continue;
+      if (gridDim.x > 1) {
 #pragma unroll
         for (int e = 0; e < kSize; ++e) slice[part * dim + columns.at[k] + e] = mine[e];
+      } else if (W* to = part ? dbias : dweight) {
+#pragma unroll
+        for (int e = 0; e < kSize; ++e) to[columns.at[k] + e] = (W)mine[e];
+      }
     }
 }
 
@@ -336,7 +350,7 @@ __global__ __launch_bounds__(kReduceColumns* kReduceSlices) void k_norm_reduce(W
   }
 }
 
-// Lanes and packs for a row: the least of 8 .. 64 lanes with kWaveElements
+// Lanes and packs for a row: the least of 1 .. 64 lanes with kWaveElements
 // each, then a workgroup's 256 and 1024 with kBlockElements.  Returns 0 where
 // the wide form takes the row.
 struct RowShape {
@@ -346,7 +360,7 @@ struct RowShape {
 RowShape row_shape(int64_t dim, int pack, int block_elements) {
   if (dim < pack) return {8, 1, 1};
   const int64_t packs = (dim + pack - 1) / pack;
-  int lanes = 8;
+  int lanes = 1;
   while (lanes < 64 && lanes < packs) lanes *= 2;
   if (lanes == 64 && packs > 64 * (kWaveElements / pack)) lanes = 256;
   if (lanes == 256 && packs > 256 * (kBlockElements / pack)) lanes = 1024;
@@ -378,6 +392,9 @@ bool with_shape(RowShape shape, F&& fn) {
     return true;
   }
   switch (shape.lanes) {
+    case 1: return with_packs<1>(shape.packs, lanes(std::integral_constant<int, 1>()));
+    case 2: return with_packs<1>(shape.packs, lanes(std::integral_constant<int, 2>()));
+    case 4: return with_packs<1>(shape.packs, lanes(std::integral_constant<int, 4>()));
     case 8: return with_packs<1>(shape.packs, lanes(std::integral_constant<int, 8>()));
     case 16: return with_packs<1>(shape.packs, lanes(std::integral_constant<int, 16>()));
     case 32: return with_packs<1>(shape.packs, lanes(std::integral_constant<int, 32>()));
@@ -424,7 +441,8 @@ int64_t gradient_slices(int64_t rows, int64_t dim, int size) {
   const RowShape shape = row_shape(dim, size, kGradientWideElements);
   const int64_t at_once = shape.lanes ? gradient_threads(shape.lanes) / shape.lanes : 1;
   const int64_t wanted = (rows + at_once - 1) / at_once, most = shape.lanes == 256 ? 2 * kGradientGroups : kGradientGroups;
-  return wanted < 1 ? 1 : wanted < most ? wanted : most;
+  // Two turns of one workgroup cost less than the launch that joins two.
+  return wanted <= 2 ? 1 : wanted < most ? wanted : most;
 }
 
 template <typename T, typename W>
@@ -439,13 +457,14 @@ int norm_gradient(T* dx, W* dweight, W* dbias, const T* grad, const T* x, const 
     const bool done = with_shape<kPack, kGradientWideElements>(shape, [&](auto l, auto p, auto z) {
       constexpr int kLanes = decltype(l)::value, kPacks = decltype(p)::value, kSize = decltype(z)::value;
       constexpr int kThreads = gradient_threads(kLanes);
-      hipLaunchKernelGGL((k_norm_gradient<T, W, kLanes, kPacks, kSize>), dim3((uint32_t)slices), dim3(kThreads), 0, stream, dx,
-                         partial, grad, x, mean, rstd, weight, rows, dim, grad_stride, stride);
+      hipLaunchKernelGGL((k_norm_gradient<T, W, kLanes, kPacks, kSize>), dim3((uint32_t)slices), dim3(kThreads), 0,
+                         stream, dx, partial, dweight, dbias, grad, x, mean, rstd, weight, rows, dim, grad_stride, stride);
     });
     if (!done)
       hipLaunchKernelGGL((k_norm_gradient_wide<T, W>), dim3((uint32_t)slices), dim3(1024), 0, stream, dx, partial, grad,
                          x, mean, rstd, weight, rows, dim, grad_stride, stride);
     MGB_LAUNCH_CHECK("layer norm gradient");
+    if (done && slices == 1) partial = nullptr;
   }
   if (partial) {
     hipLaunchKernelGGL((k_norm_reduce<W>), dim3((uint32_t)((2 * dim + kReduceColumns - 1) / kReduceColumns)),

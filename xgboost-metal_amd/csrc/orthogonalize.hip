@@ -30,9 +30,10 @@ constexpr int kNormGroups = 256;
 constexpr int64_t kMostSide = int64_t(1) << 20;
 constexpr float kMostCoefficient = 8.0f;
 
-// Steps of a segment at most.  Results of 24 bits show what a third step adds
-// (64 x 256: 4.4e-6 of the norm against 1.1e-6 with two), those of 11 and 8 do not.
-constexpr int kSegment32 = 2, kSegment16 = 3;
+// Steps of a segment at most: results of 24 bits show what a second step's error
+// adds (512 x 2048: 3.5e-6 of the norm, 1.5e-6 with one, plain binary32 2.8e-6),
+// those of 11 and 8 bits do not show a third's.
+constexpr int kSegment32 = 1, kSegment16 = 3;
 
 // Stored values are scaled so that the low part is a normal number: entries of X
 // and A are at most about 1, those of Z and P at most a^kSegment16 = 512.
@@ -736,8 +737,9 @@ int64_t padded(int64_t v) {
   return (v + to - 1) / to * to;
 }
 
-// The longer side up to which one workgroup takes a matrix of kOneSide rows.
-constexpr int64_t kOneLength = 1024;
+// The longer side up to which one workgroup takes a matrix of kOneSide rows.  Measured
+// with binary32, us: 64 x 256 51 and 77, 64 x 512 82 and 78.
+constexpr int64_t kOneLength = 448;
 
 // Where the matrices lie in the workspace.
 struct Plan {
@@ -844,9 +846,9 @@ int orthogonalize(T* out, const T* g, int64_t batch, int64_t rows, int64_t colum
     return j;
   };
   // Segments of one step (the products as they stand in the formula) take three
-  // launches a step, longer ones 3.3 to 3.5, and multiplications with n in every
-  // step.  Measured, us: 1,500 x 2,048 489 and 501, 700 x 1,400 210 and 205;
-  // 128 x 1,000 89 and 94, 128 x 2,048 104 and 102.
+  // launches a step, of three steps 3.3, and multiplications with n in every step.
+  // Measured with bfloat16, us: 1,500 x 2,048 461 and 464, 700 x 1,400 201 and 184;
+  // 128 x 1,000 88 and 90, 128 x 2,048 101 and 93.
   const bool plain = 5 * pl.n <= 7 * pl.m || (pl.m <= 384 && pl.n <= 1024);
   const int most = plain ? 1 : kMost, segments = (steps + most - 1) / most;
   for (int s = 0; s < segments; ++s) {
