@@ -116,7 +116,8 @@ def test_lookup_and_gradient(enc, rows, bag, table, dim, dtype):
     assert torch.equal(dw, enc.embedding_gradient(grad, tokens, table, scale=scale, pool=pool))
 
 
-@pytest.mark.parametrize("tokens,table", [(100000, 1), (70001, 3), (40000, 40000), (5000, 16777300)])
+@pytest.mark.parametrize("tokens,table", [(100000, 1), (70001, 3), (40000, 40000), (5000, 16777300),
+                                          (32768, 1), (30001, 3), (32768, 60000), (9, 300), (32769, 500)])
 def test_gradient_of_frequent_and_rare_tokens(enc, tokens, table):
     """One token for everything (its sum crosses every group), few, each once,
     and keys of four digits."""

@@ -291,93 +291,6 @@ __device__ __forceinline__ void clear(const Clear& c, uint32_t block, uint32_t b
   }
 }
 
-constexpr int kRangeThreads = 1024, kRangeWaves = kRangeThreads / kWave;
-constexpr uint32_t kRanges = 256;  // workgroups at most, and table rows of each at most
-
-// Few tokens: workgroup w sorts those of its `range` table rows.  Every workgroup
-// reads all tokens, a wave a sixteenth of them in their order, and so knows
-// without the others how many lie before its own: one launch.  Those beyond the
-// ranges clear.
-template <typename E, typename I>
-__global__ __launch_bounds__(kRangeThreads) void k_sort_ranges(E* __restrict__ out, const I* __restrict__ tokens, Sort s,
-                                                               uint32_t range, uint32_t ranges, uint32_t share,
-                                                               Clear zero) {
-  if (blockIdx.x >= ranges) {
-    clear<kRangeThreads>(zero, blockIdx.x - ranges, gridDim.x - ranges);
-    return;
-  }
-  extern __shared__ __align__(16) uint8_t lds[];
-  uint32_t(*counts)[kDigits] = (uint32_t(*)[kDigits])lds;  // [wave][table row]
-  uint32_t* totals = (uint32_t*)(counts + kRangeWaves);
-  uint32_t* shared = totals + kDigits;                     // a scan's words, then each wave's smaller tokens
-  uint32_t* smaller = shared + 2 * kRangeWaves;
-  E* mine = (E*)(smaller + kRangeWaves) + threadIdx.x / kWave * share;
-  const uint32_t lane = lane_id(), wave = threadIdx.x / kWave, n = (uint32_t)s.tokens;
-  const uint32_t low = blockIdx.x * range, none = ~0u;
-  const bool takes_none = s.vocabulary - low < range;
-  // (The last range may reach beyond the table: none of its tokens do.)
-  range = takes_none ? s.vocabulary - low : range;
-  for (uint32_t d = lane; d < kDigits; d += kWave) counts[wave][d] = 0;
-  const uint32_t begin = wave * share, end = begin + share < n ? begin + share : n;
-  uint32_t found = 0, before = 0;
-  for (uint32_t first = begin; first < end; first += kAhead * kWave) {
-    // What is compared is the token's low word: those outside the table become
-    // `none`, above every row, which only the last range (of the number
-    // `vocabulary`) takes in.
-    uint32_t key[kAhead];
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const uint32_t i = first + j * kWave + lane;
-      const I id = i < end ? tokens[i] : I(-1);
-      if constexpr (sizeof(I) == 8) key[j] = (uint64_t)id >> 31 ? none : (uint32_t)id;
-      else key[j] = (uint32_t)id;
-    }
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const uint32_t i = first + j * kWave + lane;
-      const bool in = key[j] - low < range || (takes_none && key[j] >= s.vocabulary && i < end);
-      const uint64_t all = __ballot(in);
-      before += (uint32_t)__popcll(__ballot(key[j] < low));
-      if (all == 0) continue;
-      if (in) {
-        const uint32_t row = key[j] < s.vocabulary ? key[j] : s.vocabulary;
-        mine[found + (uint32_t)__popcll(all & ((1ull << lane) - 1))] = (E)row << s.row_bits | i / s.bag;
-        atomicAdd(&counts[wave][row - low], 1u);
-      }
-      found += (uint32_t)__popcll(all);
-    }
-  }
-  if (lane == 0) smaller[wave] = before;
-  __syncthreads();
-  // A table row's tokens wave by wave, after the rows below it and the ranges below.
-  if (threadIdx.x < kDigits) {
-    uint32_t offset = 0;
-#pragma unroll
-    for (int w = 0; w < kRangeWaves; ++w) {
-      const uint32_t c = counts[w][threadIdx.x];
-      counts[w][threadIdx.x] = offset;
-      offset += c;
-    }
-    totals[threadIdx.x] = offset;
-  }
-  __syncthreads();
-  scan_digits(totals, shared);
-  uint32_t start = 0;
-#pragma unroll
-  for (int w = 0; w < kRangeWaves; ++w) start += smaller[w];
-  for (uint32_t first = 0; first < found; first += kWave) {
-    const bool valid = first + lane < found;
-    const E entry = valid ? mine[first + lane] : 0;
-    const uint32_t digit = valid ? (uint32_t)(entry >> s.row_bits) - low : 0;
-    const uint64_t same = equal_digits(digit, __ballot(valid));
-    const int leader = same ? __ffsll((unsigned long long)same) - 1 : (int)lane;
-    uint32_t at = 0;
-    if (valid && leader == (int)lane) at = atomicAdd(&counts[wave][digit], (uint32_t)__popcll(same));
-    at = __shfl(at, leader, kWave);
-    if (valid) out[start + totals[digit] + at + (uint32_t)__popcll(same & ((1ull << lane) - 1))] = entry;
-  }
-}
-
 constexpr int kSortThreads = 512, kSortWaves = kSortThreads / kWave;
 constexpr uint32_t kFewTiles = 64;  // at most, for the sort without scans between its passes
 
@@ -822,6 +735,164 @@ __global__ __launch_bounds__(kJoinThreads) void k_segment_join(T* __restrict__ o
   }
 }
 
+// ---- gradient: few tokens, in one launch ------------------------------------
+//
+// Workgroup w has `range` rows of the table.  It reads all tokens, a wave a
+// sixteenth of them in their order, keeps those of its rows, sorts them and sums
+// their segments; its rows that no token names become zero.
+
+constexpr int kRangeThreads = 1024, kRangeWaves = kRangeThreads / kWave;
+constexpr uint32_t kRanges = 256;  // workgroups at most, and table rows of each at most
+
+template <typename T, typename I, int kLanes, int kSize>
+__global__ __launch_bounds__(kRangeThreads) void k_range_gradient(T* __restrict__ out, uint32_t* __restrict__ sorted,
+                                                                  const T* __restrict__ grad,
+                                                                  const I* __restrict__ tokens, Sort s, int64_t dim,
+                                                                  int64_t stride, float scale, uint32_t range,
+                                                                  uint32_t share) {
+  constexpr uint32_t kGroups = kRangeThreads / kLanes;
+  extern __shared__ __align__(16) uint8_t lds[];
+  uint32_t(*counts)[kDigits] = (uint32_t(*)[kDigits])lds;  // [wave][table row]
+  uint32_t* totals = (uint32_t*)(counts + kRangeWaves);
+  uint32_t* shared = totals + kDigits;
+  uint32_t* smaller = shared + 2 * kRangeWaves;            // tokens of rows below, by wave
+  uint32_t* room = smaller + kRangeWaves;                  // the waves' tokens, then the groups' heads
+  const uint32_t lane = lane_id(), wave = threadIdx.x / kWave, n = (uint32_t)s.tokens;
+  const uint32_t low = blockIdx.x * range;
+  range = s.vocabulary - low < range ? s.vocabulary - low : range;
+  uint32_t* mine = room + wave * share;
+  for (uint32_t d = lane; d < kDigits; d += kWave) counts[wave][d] = 0;
+  const uint32_t begin = wave * share, end = begin + share < n ? begin + share : n;
+  uint32_t found = 0, before = 0;
+  for (uint32_t first = begin; first < end; first += kAhead * kWave) {
+    // A token's low word is compared; those outside the table lie above every row.
+    uint32_t key[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const uint32_t i = first + j * kWave + lane;
+      const I id = i < end ? tokens[i] : I(-1);
+      if constexpr (sizeof(I) == 8) key[j] = (uint64_t)id >> 31 ? ~0u : (uint32_t)id;
+      else key[j] = (uint32_t)id;
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const bool in = key[j] - low < range;
+      const uint64_t all = __ballot(in);
+      before += (uint32_t)__popcll(__ballot(key[j] < low));
+      if (all == 0) continue;
+      if (in) {
+        const uint32_t i = first + j * kWave + lane;
+        mine[found + (uint32_t)__popcll(all & ((1ull << lane) - 1))] = key[j] << s.row_bits | i / s.bag;
+        atomicAdd(&counts[wave][key[j] - low], 1u);
+      }
+      found += (uint32_t)__popcll(all);
+    }
+  }
+  if (lane == 0) smaller[wave] = before;
+  __syncthreads();
+  // A table row's tokens wave by wave, after the rows below it and the ranges below.
+  if (threadIdx.x < kDigits) {
+    uint32_t offset = 0;
+#pragma unroll
+    for (int w = 0; w < kRangeWaves; ++w) {
+      const uint32_t c = counts[w][threadIdx.x];
+      counts[w][threadIdx.x] = offset;
+      offset += c;
+    }
+    totals[threadIdx.x] = offset;
+  }
+  __syncthreads();
+  scan_digits(totals, shared);
+  uint32_t start = 0;
+#pragma unroll
+  for (int w = 0; w < kRangeWaves; ++w) start += smaller[w];
+  uint32_t* entries = sorted + start;
+  for (uint32_t first = 0; first < found; first += kWave) {
+    const bool valid = first + lane < found;
+    const uint32_t entry = valid ? mine[first + lane] : 0, digit = valid ? (entry >> s.row_bits) - low : 0;
+    const uint64_t same = equal_digits(digit, __ballot(valid));
+    const int leader = same ? __ffsll((unsigned long long)same) - 1 : (int)lane;
+    uint32_t at = 0;
+    if (valid && leader == (int)lane) at = atomicAdd(&counts[wave][digit], (uint32_t)__popcll(same));
+    at = __shfl(at, leader, kWave);
+    if (valid) entries[totals[digit] + at + (uint32_t)__popcll(same & ((1ull << lane) - 1))] = entry;
+  }
+  __syncthreads();
+  const uint32_t c = totals[kDigits - 1];  // all of them: no row is the last digit
+  // Sums.  A group of lanes takes `chunk` sorted tokens; what belongs to a segment of
+  // the chunk before goes to its head, and the group in whose chunk a segment begins
+  // adds the heads it runs through.
+  const uint32_t lane_in = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const uint32_t chunk = ((c + kGroups - 1) / kGroups + kAhead - 1) / kAhead * kAhead;
+  const uint32_t from = group * chunk < c ? group * chunk : c, to = c - from < chunk ? c : from + chunk;
+  const uint32_t mask = (1u << s.row_bits) - 1;
+  float* heads = (float*)room;
+  uint32_t* fronts = (uint32_t*)(heads + kRangeThreads * kSize);  // each group's first key, ~0 without tokens
+  if (lane_in == 0) fronts[group] = from < to ? entries[from] >> s.row_bits : ~0u;
+  const float one = runtime_one();
+  const int64_t width = (int64_t)kLanes * kSize;
+  for (int64_t column = 0; column < dim; column += width) {
+    const int64_t nominal = column + lane_in * kSize, at = nominal < dim - kSize ? nominal : dim - kSize;
+    const bool active = nominal < dim;
+    float sum[kSize] = {};
+    auto store = [&](uint32_t key) {
+      if (!active) return;
+#pragma unroll
+      for (int e = 0; e < kSize; ++e) sum[e] *= scale;
+      Raw<T, kSize>().put(sum, out + (int64_t)key * dim + at);
+    };
+    bool head = from > 0 && from < to && entries[from - 1] >> s.row_bits == entries[from] >> s.row_bits, tail = false;
+    uint32_t key = from < to ? entries[from] >> s.row_bits : 0;
+    // Entries are fetched an iteration ahead, with the one behind them.
+    uint32_t next[kAhead + 1];
+    auto fetch = [&](uint32_t i) {
+#pragma unroll
+      for (int j = 0; j <= kAhead; ++j) next[j] = entries[i + j < c ? i + j : c - 1];
+    };
+    if (from < to) fetch(from);
+    for (uint32_t i = from; i < to; i += kAhead) {
+      uint32_t entry[kAhead + 1];
+#pragma unroll
+      for (int j = 0; j <= kAhead; ++j) entry[j] = next[j];
+      if (i + kAhead < to) fetch(i + kAhead);
+      Raw<T, kSize> v[kAhead];
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) v[j].load(grad + (int64_t)(entry[j] & mask) * stride + at);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const uint32_t p = i + j + 1;
+        if (p > to) break;
+        add_one<T, kSize>(v[j], one, sum);
+        const uint32_t following = entry[j + 1] >> s.row_bits;
+        const bool ends = p >= c || following != key;
+        if (!ends && p < to) continue;
+        if (head) store_floats<kSize>(heads + (size_t)threadIdx.x * kSize, sum);
+        else if (ends) store(key);
+        else tail = true;
+        if (tail) break;
+        key = following;
+        head = false;
+#pragma unroll
+        for (int e = 0; e < kSize; ++e) sum[e] = 0.0f;
+      }
+    }
+    __syncthreads();
+    if (tail) {
+      for (uint32_t g = group + 1; g < kGroups && fronts[g] == key; ++g)
+        add_floats<kSize>(heads + (size_t)(g * kLanes + lane_in) * kSize, sum);
+      store(key);
+    }
+    // Rows without tokens.
+    for (uint32_t r = group; r < range; r += kGroups)
+      if (totals[r] == totals[r + 1]) {
+#pragma unroll
+        for (int e = 0; e < kSize; ++e) sum[e] = 0.0f;
+        store(low + r);
+      }
+    __syncthreads();
+  }
+}
+
 // The table from its windows' parts.
 template <typename T, int kLanes, int kSize>
 __global__ __launch_bounds__(kThreads) void k_segment_windows(T* __restrict__ out, uint32_t vocabulary,
@@ -919,8 +990,8 @@ int lookup(T* out, const T* weight, const I* tokens, int64_t rows, int64_t bag, 
 
 // A chiplet's cache, and the part of it that a window's rows of grad may take.
 constexpr int64_t kCache = int64_t(4) << 20, kWindowBytes = int64_t(9) << 18;
-// Most tokens for the sort by ranges (LDS holds them all, were they one row's).
-constexpr int64_t kRangeTokens = 32768, kRangeWideTokens = 16384;
+// Most tokens for the one launch by ranges (LDS holds them all, were they one range's).
+constexpr int64_t kRangeTokens = 32768;
 constexpr int64_t kLongTiles = int64_t(1) << 21;  // tokens from which a tile has 16 rounds, not 4
 
 // How the gradient of rows x bag tokens is computed and laid out in the workspace.
@@ -928,7 +999,7 @@ struct GradientPlan {
   Sort sort;
   Segments segments;
   RowLanes row;
-  bool wide, by_range, few;  // 64-bit entries; sort by ranges; few tiles
+  bool wide, by_range, few;  // 64-bit entries; one launch by ranges; few tiles
   int passes, rounds;
   size_t entries[2], counts, totals, heads, tails, parts, named, next_counts, clear_bytes, bytes;
 };
@@ -954,7 +1025,7 @@ GradientPlan gradient_plan(int64_t rows, int64_t bag, int64_t vocabulary, int64_
   const int key_bits = bits_of(vocabulary), row_bits = bits_of(window - 1);
   p.passes = (key_bits + kDigitBits - 1) / kDigitBits;
   p.wide = key_bits + row_bits > 32;
-  p.by_range = windows == 1 && n <= (p.wide ? kRangeWideTokens : kRangeTokens) && vocabulary < kRanges * kRanges;
+  p.by_range = windows == 1 && !p.wide && n <= kRangeTokens && vocabulary < kRanges * (kDigits - 1) && p.row.groups == 1;
   p.few = !p.by_range && windows == 1 && n <= (int64_t)kFewTiles * 4 * kSortThreads;
   p.rounds = p.few ? 1 : n < kLongTiles ? 4 : 16;
   while (p.few && n > (int64_t)kFewTiles * p.rounds * kSortThreads) p.rounds *= 2;
@@ -988,6 +1059,10 @@ GradientPlan gradient_plan(int64_t rows, int64_t bag, int64_t vocabulary, int64_
   if (!p.by_range) {
     p.counts = take((size_t)windows * kDigits * p.sort.tiles * sizeof(uint32_t));
     p.totals = take((size_t)windows * kDigits * sizeof(uint32_t));
+  }
+  if (p.by_range) {
+    p.bytes = at;
+    return p;
   }
   p.heads = take((size_t)windows * p.segments.chunks * dim * sizeof(float));
   p.tails = take((size_t)windows * p.segments.chunks * dim * sizeof(float));
@@ -1029,19 +1104,6 @@ uint32_t clear_blocks(const Clear& c, int threads) {
   return at_most((bytes + 128 * threads - 1) / (128 * threads), 1024);
 }
 
-template <typename E, typename I>
-int sort_ranges(const GradientPlan& p, E* out, const I* tokens, Clearing& clearing, hipStream_t stream) {
-  const uint32_t keys = p.sort.vocabulary + 1, range = (keys + kRanges - 1) / kRanges, ranges = (keys + range - 1) / range;
-  const uint32_t n = (uint32_t)p.sort.tokens, share = (n + kRangeThreads - 1) / kRangeThreads * kWave;
-  const uint32_t lds = (kRangeWaves * kDigits + kDigits + 3 * kRangeWaves) * 4 + kRangeWaves * share * (uint32_t)sizeof(E);
-  if (lds > 65536)
-    MGB_CHECK(hipFuncSetAttribute((const void*)k_sort_ranges<E, I>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-  const Clear zero = next_clear(clearing);
-  hipLaunchKernelGGL((k_sort_ranges<E, I>), dim3(ranges + clear_blocks(zero, kRangeThreads)), dim3(kRangeThreads), lds,
-                     stream, out, tokens, p.sort, range, ranges, share, zero);
-  return 0;
-}
-
 template <typename E, typename F, int kRounds, bool kFew>
 void sort_pass(const GradientPlan& p, uint8_t* ws, F from, E* out, int pass, Clearing& clearing, hipStream_t stream) {
   uint32_t *counts = (uint32_t*)(ws + p.counts), *totals = (uint32_t*)(ws + p.totals);
@@ -1062,12 +1124,11 @@ void sort_pass(const GradientPlan& p, uint8_t* ws, F from, E* out, int pass, Cle
                      kFew && pass + 1 < p.passes ? later + (size_t)pass * each : nullptr, p.sort, pass, zero);
 }
 
-// The sorted entries' place; null after an error.
+// The sorted entries' place.
 template <typename E, typename I>
 E* sort_tokens(const GradientPlan& p, uint8_t* ws, const I* tokens, Clearing clearing, hipStream_t stream) {
   E* entries[2] = {(E*)(ws + p.entries[0]), (E*)(ws + p.entries[1])};
-  clearing.launches = p.by_range ? 1 : p.few ? p.passes + 1 : 2 * p.passes;
-  if (p.by_range) return sort_ranges<E, I>(p, entries[0], tokens, clearing, stream) ? nullptr : entries[0];
+  clearing.launches = p.few ? p.passes + 1 : 2 * p.passes;
   int now = 0;
   for (int pass = 0; pass < p.passes; ++pass, now ^= 1) {
     auto run = [&](auto from) {
@@ -1088,6 +1149,31 @@ E* sort_tokens(const GradientPlan& p, uint8_t* ws, const I* tokens, Clearing cle
   return entries[now ^ 1];
 }
 
+template <typename T, typename I>
+int range_gradient(const GradientPlan& p, T* out, const T* grad, const I* tokens, uint8_t* ws, hipStream_t stream) {
+  const uint32_t rows = p.sort.vocabulary, range = (rows + kRanges - 1) / kRanges, ranges = (rows + range - 1) / range;
+  const uint32_t n = (uint32_t)p.sort.tokens, share = (n + kRangeThreads - 1) / kRangeThreads * kWave;
+  int status = 0;
+  with_lanes<T>(p.row, [&](auto l, auto size) {
+    constexpr int kLanes = decltype(l)::value, kSize = decltype(size)::value;
+    uint32_t room = kRangeWaves * share * 4;
+    const uint32_t sums = (kRangeThreads * kSize + kRangeThreads / kLanes) * 4;
+    if (room < sums) room = sums;
+    const uint32_t lds = (kRangeWaves * kDigits + kDigits + 3 * kRangeWaves) * 4 + room;
+    if (lds > 65536)
+      status = check(hipFuncSetAttribute((const void*)k_range_gradient<T, I, kLanes, kSize>,
+                                         hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds),
+                     "hipFuncSetAttribute(k_range_gradient)");
+    if (status == 0)
+      hipLaunchKernelGGL((k_range_gradient<T, I, kLanes, kSize>), dim3(ranges), dim3(kRangeThreads), lds, stream, out,
+                         (uint32_t*)(ws + p.entries[0]), grad, tokens, p.sort, p.segments.dim, p.segments.stride,
+                         p.segments.scale, range, share);
+  });
+  if (status) return -1;
+  MGB_LAUNCH_CHECK("embedding gradient: ranges");
+  return 0;
+}
+
 template <typename T, typename E, typename I>
 int lookup_gradient(GradientPlan& p, T* out, const T* grad, const I* tokens, uint8_t* ws, hipStream_t stream) {
   Clearing clearing = {};
@@ -1098,7 +1184,6 @@ int lookup_gradient(GradientPlan& p, T* out, const T* grad, const I* tokens, uin
     clearing.left = (uint64_t)p.sort.vocabulary * p.segments.dim * sizeof(T);
   }
   const E* sorted = sort_tokens<E, I>(p, ws, tokens, clearing, stream);
-  if (!sorted) return -1;
   MGB_LAUNCH_CHECK("embedding gradient: sort");
   with_lanes<T>(p.row, [&](auto l, auto size) {
     constexpr int kLanes = decltype(l)::value, kSize = decltype(size)::value;
@@ -1144,6 +1229,7 @@ int lookup_gradient(T* out, const T* grad, const I* tokens, int64_t rows, int64_
   p.segments.named = p.sort.windows > 1 ? ws + p.named : nullptr;
   p.segments.stride = stride;
   p.segments.scale = scale;
+  if (p.by_range) return range_gradient<T, I>(p, out, grad, tokens, ws, stream);
   return p.wide ? lookup_gradient<T, uint64_t, I>(p, out, grad, tokens, ws, stream)
                 : lookup_gradient<T, uint32_t, I>(p, out, grad, tokens, ws, stream);
 }
