@@ -576,3 +576,15 @@ def test_leaf_tokens_and_training(enc, xgb):
         adam.step()
         losses.append(loss.item())
     assert losses[-1] < 0.25 * losses[0]
+
+
+def test_example():
+    """The example trains an encoder on the leaves that predicts what the trees do, about as well."""
+    import importlib.util
+    from pathlib import Path
+    path = Path(__file__).resolve().parents[1] / "examples" / "leaf_encoder.py"
+    spec = importlib.util.spec_from_file_location("leaf_encoder", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    trees, leaves = example.main(rows=8000, rounds=20, dim=32, hidden=64, batch=1000, epochs=15)
+    assert leaves < 1.5 * trees
