@@ -149,6 +149,44 @@ def test_gradient_sorts(enc, rows, bag, table, dim, dtype):
     assert torch.equal(dw, enc.embedding_gradient(grad, tokens, table, scale=0.5, pool=True))
 
 
+# Many rows: a column's tokens from a narrow range of the table, from all of it,
+# or narrow ones followed by wide ones and narrow ones again; absent tokens among
+# them and a column of nothing else; infinities in the table.
+@pytest.mark.parametrize("wide", [(), (0,), (13,), (11, 12, 13, 14, 15, 16, 17, 18, 19, 20, 21, 22)], ids=["narrow", "first", "one", "late"])
+@pytest.mark.parametrize("rows,bag,leaves,dim,dtype,ids", [
+    (131072, 23, 256, 64, torch.bfloat16, torch.int32),
+    (140001, 23, 200, 32, torch.float32, torch.int64),
+    (131100, 25, 250, 96, torch.float16, torch.int32),
+    (131075, 24, 100, 128, torch.bfloat16, torch.int32),
+])
+def test_lookup_of_many_rows(enc, rows, bag, leaves, dim, dtype, ids, wide):
+    g = _gen(rows + bag + len(wide))
+    table = leaves * bag
+    tokens = torch.randint(0, leaves, (rows, bag), generator=g, device="cuda") + leaves * torch.arange(bag, device="cuda")
+    for c in wide:
+        tokens[:, c] = torch.randint(0, table, (rows,), generator=g, device="cuda")
+    gone = torch.rand(rows, bag, generator=g, device="cuda") < 0.01
+    tokens = torch.where(gone, torch.where(tokens % 2 == 0, -1, table), tokens)
+    tokens[:, 5] = -7
+    tokens[rows - 3] = table + 1
+    tokens = tokens.to(ids)
+    weight = _randn(g, table, dim, dtype=dtype)
+    weight[leaves * 2 + 1, 3] = float("inf")
+    got = enc.embedding_lookup(weight, tokens, scale=0.25, pool=True)
+    want, slack = torch.zeros(rows, dim, dtype=torch.float64, device="cuda"), torch.zeros(rows, dim, dtype=torch.float64, device="cuda")
+    padded = torch.cat([weight.double(), torch.zeros(1, dim, dtype=torch.float64, device="cuda")])
+    for column in tokens.long().unbind(1):
+        each = padded[torch.where((column < 0) | (column >= table), table, column)] * 0.25
+        want += each
+        slack += each.abs()
+    infinite = torch.isinf(want)
+    assert torch.equal(infinite, torch.isinf(got)) and bool(infinite.any())
+    # A sum of `bag` terms in binary32, then one rounding of the result.
+    bound = slack * (bag + 2) * 2.0 ** -24 + want.abs() * torch.finfo(dtype).eps / 2 + torch.finfo(dtype).tiny
+    assert bool(((got.double() - want).abs() <= bound)[~infinite].all())
+    assert bool((got[rows - 3] == 0).all())
+
+
 def test_lookup_leaves_unnamed_rows_alone(enc):
     """NaN and infinity in rows that no token names, row 0 among them, stay there."""
     weight = torch.ones(10, 40, device="cuda")

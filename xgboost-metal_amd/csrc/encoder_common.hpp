@@ -11,15 +11,6 @@
 
 namespace mgb {
 
-template <typename T>
-struct DTypeOf;
-template <>
-struct DTypeOf<float> { static constexpr int value = MGB_F32; };
-template <>
-struct DTypeOf<_Float16> { static constexpr int value = MGB_F16; };
-template <>
-struct DTypeOf<__bf16> { static constexpr int value = MGB_BF16; };
-
 // 16 bytes of elements.  Rows of any width and stride start anywhere, so packs
 // are moved by memcpy: global loads and stores of this chip take any byte
 // address, and an aligned pack costs no more for it.
@@ -115,8 +106,8 @@ struct Raw {
 
 // sum += v, and sum += a + b.  The chip adds binary16 to binary32 in one
 // instruction if it is a multiply-add (`one` is 1, from where the compiler does
-// not see it), and two bfloat16 by a dot product with (1, 1): 8 instructions
-// for a pack of two tokens' eight, where conversions and additions take 32.
+// not see it), and two bfloat16 by a dot product with (1, 1): 16 instructions
+// for two packs of eight, where conversions and additions take 32.
 template <typename T, int kSize>
 __device__ __forceinline__ void add_one(const Raw<T, kSize>& v, float one, float* sum) {
   T x[kSize];
