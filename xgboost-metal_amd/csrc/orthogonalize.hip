@@ -16,6 +16,10 @@
 // numbers, 22 bits, and a product takes three matrix instructions (high by
 // high, high by low, low by high; low by low is below binary32's rounding).
 // Sums are binary32.
+//
+// Measured (us, one MI355X): binary32 64 x 256 50 and 1,500 x 1,001 254, bfloat16
+// 2,048 x 4,096 940 (198 GFLOP, thrice in matrix instructions: 630 TFLOP/s of
+// those, where a library's large product reaches 1,130).
 #include <type_traits>
 #include <utility>
 
@@ -319,7 +323,8 @@ __device__ __forceinline__ float total_factor(const Product& p, const Job& job, 
 
 // Small products: a workgroup has a tile of 32 x 32, its kWaves waves a part of the
 // depth each, joined in LDS.  Operands go from memory to registers, a ring of
-// kAhead blocks, without a branch between a load and its use.
+// kAhead blocks, without a branch between a load and its use.  Bound by the launch
+// and one walk along the depth: 4 to 6 us for sides of 512.
 template <int kMode, typename T, int kWaves, bool kLeftLow, bool kRightLow>
 __global__ __launch_bounds__(kWaves* kWave) void k_product_small(Product p) {
   constexpr int kAhead = 4;
@@ -398,7 +403,11 @@ using SharedBytes = __attribute__((address_space(3))) void*;
 // them), so the waves share their operands in LDS.  Stages of kDepth blocks of 16
 // are loaded straight into a ring of kRing in LDS, a block as it lies in memory,
 // a lane's 16 bytes at 16 lane; a wave reads a stage into registers while it
-// multiplies the one before.
+// multiplies the one before.  2,048^3 of three instructions: symmetric 44 us (136
+// tiles, so 120 of 256 compute units stand idle; a half of its loop's time is the
+// matrix instructions', the rest waits for LDS's loads), 1,024 with tiles of 64 14;
+// 2,048 x 2,048 x 4,096 of three, whose tiles are two to a compute unit in turns,
+// 96 us, 1,070 TFLOP/s.  With four waves more that do nothing but load: 4 % slower.
 template <int kMode, typename T, int kHalf, bool kLeftLow, bool kRightLow>
 __global__ __launch_bounds__(4 * kWave, 1) void k_product(Product p) {
   constexpr int kRing = 4, kDepth = 4 / kHalf;
@@ -522,7 +531,8 @@ __global__ __launch_bounds__(4 * kWave, 1) void k_product(Product p) {
 
 // One workgroup for a whole matrix of at most 64 rows (after transposition): the
 // m x m matrices stay in LDS, X and its transpose in the workspace, where they
-// are in this compute unit's cache, and nothing waits for a launch.
+// are in this compute unit's cache, and nothing waits for a launch: 64 x 256 50 us,
+// by launches 77.
 constexpr int kOneSide = 64, kOneThreads = 512, kOneWaves = kOneThreads / kWave;
 constexpr int kSquare = kOneSide * kOneSide * 2;      // halves of a matrix in LDS
 constexpr int kJoined = kOneWaves / 2 * 3 * 4 * kWave;  // float4s of the partial sums of A
