@@ -1,0 +1,85 @@
+"""Orthogonalised updates at every form their products take, and the optimizer
+over them, against 64-bit forms.
+
+LARGE has what the products come in: tiles of 128, of 64 and of 32 with the depth
+in 1, 4 and 16 parts, single and by twos, symmetric or not, operands with and
+without low parts, segments of one step and of several, batches.
+"""
+import pytest
+import torch
+from test_gpu_encoder import COEFFICIENTS, U, _gen, _orthogonal64, _randn, enc  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+NAMES = ["f32", "f16", "bf16"]
+
+
+def _plain32(update, steps, coefficients=COEFFICIENTS, eps=1e-7):
+    a, b, c = coefficients
+    x = update.float()
+    x = x / (x.square().sum((-2, -1), keepdim=True).sqrt() + eps)
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.mT.contiguous() if tall else x
+    for _ in range(steps):
+        s = x @ x.mT.contiguous()
+        x = a * x + (b * s + c * (s @ s)) @ x
+    return x.mT.contiguous() if tall else x
+
+
+def _near_plain(got, update, steps, segmented):
+    """Against 64 bits, by the error that plain binary32 makes of the same input.
+    Operands of 22 bits where that has 24 are rounded four times as coarsely, and
+    the product of the two low parts, left out, is as much again: 8.  In a segment
+    of several steps A is carried on instead of taken from X, which adds
+    b a^2 / a^3 of a step's error to it, below 2: 16.  A result x of fewer bits:
+    |round(x) - want| <= |round(want) - want| + 2 |x - want|, as no number of the
+    type is nearer to x than round(x)."""
+    want = _orthogonal64(update, steps)
+    norm = want.norm()
+    error = ((_plain32(update, steps).double() - want).norm() / norm).item()
+    bound = (16 if segmented else 8) * error
+    if got.dtype != torch.float32:
+        bound = 2 * bound + ((want.to(got.dtype).double() - want).norm() / norm).item()
+    off = ((got.double() - want).norm() / norm).item()
+    assert off <= bound, f"{off:.2e} of the norm, bound {bound:.2e}, binary32 {error:.2e}"
+
+
+# shape, bits of the types it is for.  Tiles of 128: 2,048 x 4,096 (segments), 1,930 x
+# 2,100, the batches; of 64: 700 x 1,400 and 500 x 1,100 (segments), 1,500 x 1,100;
+# of 32: 400 x 2,500 and 128 x 2,048 (segments).
+LARGE = [((2048, 4096), (16,)), ((1930, 2100), (16, 32)), ((2100, 1930), (32,)), ((700, 1400), (16, 32)),
+         ((1500, 1100), (16, 32)), ((1100, 1500), (16, 32)), ((500, 1100), (16, 32)), ((400, 2500), (16, 32)),
+         ((2500, 450), (16,)), ((128, 2048), (16, 32)), ((2, 7, 512, 512), (16, 32)), ((14, 450, 900), (16, 32)),
+         ((3, 900, 450), (16,))]
+LARGE = [pytest.param(shape, dtype, id="x".join(map(str, shape)) + "-" + name) for shape, bits in LARGE
+         for dtype, name in zip(TYPES, NAMES) if (32 if dtype == torch.float32 else 16) in bits]
+
+
+@pytest.mark.parametrize("steps", [5, 1])
+@pytest.mark.parametrize("low_rank", [False, True], ids=["random", "low_rank"])
+@pytest.mark.parametrize("shape,dtype", LARGE)
+def test_products(enc, shape, dtype, low_rank, steps):  # noqa: F811
+    g = _gen(sum(shape) + steps)
+    if low_rank:  # a few directions, the others a thousand times smaller
+        update = _randn(g, *shape[:-1], 6) @ _randn(g, *shape[:-2], 6, shape[-1]) + 1e-3 * _randn(g, *shape)
+    else:
+        update = 0.01 * _randn(g, *shape)
+    update = update.to(dtype)
+    got = enc.orthogonalize(update, steps=steps)
+    assert got.shape == update.shape and got.dtype == dtype
+    for one, of in zip(got.reshape(-1, *shape[-2:]), update.reshape(-1, *shape[-2:])):
+        _near_plain(one, of, steps, dtype != torch.float32)
+    for _ in range(3):  # the same bits, launch after launch
+        assert torch.equal(got, enc.orthogonalize(update, steps=steps))
+
+
+@pytest.mark.parametrize("steps", [2, 3, 4, 6, 7])
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES)
+def test_segments(enc, dtype, steps):  # noqa: F811
+    """Segments of two and three steps and what follows them, few directions far above the others."""
+    g = _gen(steps)
+    update = (_randn(g, 450, 5) @ _randn(g, 5, 900) + 1e-3 * _randn(g, 450, 900)).to(dtype)
+    _near_plain(enc.orthogonalize(update, steps=steps), update, steps, dtype != torch.float32)
+    update = update.t()
+    _near_plain(enc.orthogonalize(update, steps=steps), update, steps, dtype != torch.float32)
