@@ -510,7 +510,9 @@ int mgb_layer_norm_gradient(void* dx, void* dweight, void* dbias, const void* gr
 /* `batch` matrices' updates by Newton-Schulz products: X = G / (|G|_F + eps),
  * then `steps` (1 to 100) times X <- (c0 I + c1 A + c2 A^2) X with A = X X^T
  * (matrices taller than wide transposed before and after).  Coefficients
- * within -8 and 8; sides up to 2^20.  out: matrices without gaps. */
+ * within -8 and 8, and such that the steps take no singular value of at most 1
+ * beyond about 4 before the last (A and Z as well stay within what the products
+ * hold; refused otherwise); eps >= 0; sides up to 2^20.  out: matrices without gaps. */
 size_t mgb_orthogonalize_workspace_bytes(int64_t batch, int64_t rows, int64_t columns);
 int mgb_orthogonalize(void* out, const void* update, int64_t batch, int64_t rows, int64_t columns, int64_t row_stride,
                       int64_t batch_stride, int steps, const float* coefficients, float eps, int dtype,

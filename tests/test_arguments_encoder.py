@@ -153,3 +153,25 @@ def test_package_refuses_mismatches(enc):
     for kind, text, call in bad:
         with pytest.raises(kind, match=text):
             call()
+
+
+def test_coefficients_that_leave_the_products_range_are_refused():
+    """Singular values begin within [0, 1]; where the steps can take one so far that
+    a product's operand passes what binary16 holds, the C entry refuses, before any
+    device work."""
+    lib = _lib()
+    one = P(256)  # never read: every call below is refused
+
+    def call(c, steps, dtype=0, eps=1e-7):
+        return lib.mgb_orthogonalize(one, one, I64(1), I64(1), I64(1), I64(1), I64(1), steps, (ctypes.c_float * 3)(*c),
+                                     F32(eps), dtype, one, ctypes.c_size_t(1 << 40), None)
+
+    for dtype in (0, 1, 2):
+        _refused(lib, call((5.0, 0.0, 0.0), 2, dtype), "coefficients")      # A = 25
+        _refused(lib, call((8.0, 0.0, 0.0), 2, dtype), "coefficients")      # A = 64
+        _refused(lib, call((2.0, 0.0, 0.0), 3, dtype), "coefficients")      # A = 16
+        _refused(lib, call((1.0, 4.0, -1.0), 2, dtype), "coefficients")     # the largest value at 1: 4
+        _refused(lib, call((8.0, -8.0, -8.0), 2, dtype), "coefficients")    # - 8 at 1
+        _refused(lib, call((3.4445, -4.775, 2.6), 6, dtype), "coefficients")  # grows with every step
+        _refused(lib, call((3.0, -4.0, 2.0), 5, dtype, -1e-3), "eps")
+        _refused(lib, call((3.0, -4.0, 2.0), 5, dtype, float("nan")), "eps")

@@ -83,3 +83,30 @@ def test_segments(enc, dtype, steps):  # noqa: F811
     _near_plain(enc.orthogonalize(update, steps=steps), update, steps, dtype != torch.float32)
     update = update.t()
     _near_plain(enc.orthogonalize(update, steps=steps), update, steps, dtype != torch.float32)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES)
+def test_orthogonalize_coefficients_at_the_limit(enc, dtype):  # noqa: F811
+    """What is accepted is right where singular values are as large as they can be, 1 at
+    first: a rank-one matrix' singular value runs through the polynomial.  Refused is
+    what would pass binary16's range."""
+    for shape in ((1, 1), (3, 200), (500, 800), (700, 1400)):
+        update = torch.zeros(shape, device="cuda", dtype=dtype)
+        update[0, 0] = 4.0
+        for coefficients, steps in (((3.9, 0.0, 0.0), 2), ((1.9, 0.0, 0.0), 3), ((8.0, 0.0, 0.0), 1), ((8.0, 8.0, 8.0), 1),
+                                    ((1.5, -0.5, 0.0), 20), (COEFFICIENTS, 100), ((3.4, -4.0, 1.5), 12)):
+            got = enc.orthogonalize(update, steps=steps, coefficients=coefficients)
+            s, slope = 1.0, 1.0
+            for _ in range(steps):
+                a, b, c = coefficients
+                slope = max(1.0, slope * abs(a + 3 * b * s ** 2 + 5 * c * s ** 4))
+                s = a * s + b * s ** 3 + c * s ** 5
+            # A value's rounding, 2^-22, a few times a step, through the steps behind it.
+            off = abs(got[0, 0].double().item() - s)
+            assert off <= abs(s) * (U[dtype] + 64 * steps * slope * 2.0 ** -22), (shape, coefficients, steps, off)
+            rest = got.double().clone()
+            rest[0, 0] = 0.0
+            assert not rest.any()
+        for coefficients, steps in (((5.0, 0.0, 0.0), 2), ((8.0, 8.0, 8.0), 2)):
+            with pytest.raises(ValueError, match="coefficients"):
+                enc.orthogonalize(update, steps=steps, coefficients=coefficients)

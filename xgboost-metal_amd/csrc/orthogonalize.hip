@@ -20,6 +20,7 @@
 // Measured (us, one MI355X): binary32 64 x 256 50 and 1,500 x 1,001 239, bfloat16
 // 2,048 x 4,096 882 to 940 (198 GFLOP, thrice in matrix instructions: 630 to 670
 // TFLOP/s of those, where a library's large product reaches 1,130).
+#include <cmath>
 #include <type_traits>
 #include <utility>
 
@@ -33,14 +34,17 @@ constexpr int kPad = 64;       // rows and columns of every matrix in the worksp
 constexpr int kNormGroups = 256;
 constexpr int64_t kMostSide = int64_t(1) << 20;
 constexpr float kMostCoefficient = 8.0f;
+constexpr double kMostHalf = 65504.0 * 0.99;  // binary16's largest value, and room for roundings
 
 // Steps of a segment at most: results of 24 bits show what a second step's error
 // adds (512 x 2048: 3.5e-6 of the norm, 1.5e-6 with one, plain binary32 2.8e-6),
 // those of 11 and 8 bits do not show a third's.
 constexpr int kSegment32 = 1, kSegment16 = 3;
 
-// Stored values are scaled so that the low part is a normal number: entries of X
-// and A are at most about 1, those of Z and P at most a^kSegment16 = 512.
+// What stored values are scaled by: X, A and U, whose entries may be up to 15.8 then
+// (about 1 with coefficients that converge), and Z and P, up to 1,013 (a^kSegment16
+// at most, which is 512).  in_range checks it.  A value of at least 2^-2 / scale keeps
+// 22 bits; a smaller one is off by 2^-25 / scale.
 constexpr float kScaleX = 4096.0f, kScaleZ = 64.0f;
 
 using half8 = __attribute__((ext_vector_type(8))) _Float16;
@@ -793,6 +797,42 @@ int64_t padded(int64_t v) {
   return (v + to - 1) / to * to;
 }
 
+// The largest |f(t)| of t in [0, end], where f' has the roots of u + v t + w t^2.
+template <typename F>
+double largest(F&& f, double end, double u, double v, double w) {
+  double most = std::fmax(std::fabs(f(0.0)), std::fabs(f(end)));
+  auto at = [&](double t) {
+    if (t > 0.0 && t < end) most = std::fmax(most, std::fabs(f(t)));
+  };
+  const double d = v * v - 4.0 * u * w;
+  if (d < 0.0) return most;
+  const double q = -0.5 * (v + std::copysign(std::sqrt(d), v));
+  if (w != 0.0) at(q / w);
+  if (q != 0.0) at(u / q);
+  return most;
+}
+
+// Whether all matrices stay within what their scales let binary16 hold.  Each is a
+// polynomial of X's singular values, which begin within [0, 1]; no entry is larger
+// than the largest singular value.  With `most` steps a segment.
+bool in_range(int steps, int most, double a, double b, double c) {
+  const double most_x = kMostHalf / kScaleX, most_z = kMostHalf / kScaleZ;
+  auto z = [&](double t) { return a + b * t + c * t * t; };  // t: eigenvalues of A
+  double end = 1.0, before[2] = {1.0, 1.0};                  // of A; of the steps before, Z's largest
+  for (int k = 0; k < steps; ++k) {
+    if (end > most_x) return false;  // A, and X with it
+    const double now = largest(z, end, b, 2.0 * c, 0.0);
+    if (now > most_z || (most > 1 && now * before[0] * before[1] > most_z)) return false;  // Z; P
+    if (k + 1 == steps) break;  // (the last step's result is the caller's)
+    if (most > 1 && largest([&](double t) { return t * z(t); }, end, a, 2.0 * b, 3.0 * c) > most_x) return false;  // U
+    const double s = largest([&](double t) { return std::sqrt(t) * z(t); }, end, a, 3.0 * b, 5.0 * c);
+    end = s * s;
+    before[1] = before[0];
+    before[0] = now;
+  }
+  return true;
+}
+
 // The longer side up to which one workgroup takes a matrix of kOneSide rows.  Measured
 // with binary32, us: 64 x 256 51 and 77, 64 x 512 82 and 78.
 constexpr int64_t kOneLength = 448;
@@ -985,12 +1025,17 @@ int mgb_orthogonalize(void* out, const void* update, int64_t batch, int64_t rows
   for (int k = 0; k < 3; ++k)
     MGB_REQUIRE(coefficients[k] >= -kMostCoefficient && coefficients[k] <= kMostCoefficient,
                 "orthogonalize: coefficients must lie within -8 and 8");
+  MGB_REQUIRE(eps >= 0.0f, "orthogonalize: eps must not be negative");
   if (batch == 0 || rows == 0 || columns == 0) return 0;
   MGB_REQUIRE(out && update && workspace, "orthogonalize: null pointer");
   MGB_REQUIRE(workspace_bytes >= mgb_orthogonalize_workspace_bytes(batch, rows, columns),
               "orthogonalize: workspace too small");
   auto run = [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
+    MGB_REQUIRE(in_range(steps, sizeof(T) == 4 ? kSegment32 : kSegment16, coefficients[0], coefficients[1],
+                         coefficients[2]),
+                "orthogonalize: with these coefficients and steps a singular value of at most 1 may grow beyond what "
+                "the products hold (about 4)");
     return orthogonalize<T>((T*)out, (const T*)update, batch, rows, columns, stride, batch_stride, steps,
                             coefficients[0], coefficients[1], coefficients[2], eps, (uint8_t*)workspace,
                             (hipStream_t)stream);

@@ -138,7 +138,8 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5,
     """The update with its singular values driven towards 1 (the Muon
     optimiser's): X = update / (norm + eps), then `steps` times
     X = (a I + b A + c A^2) X with A = X X^T, on the shorter side.  Leading axes
-    are a batch of matrices.  Works with 22 bits of each value whatever the
+    are a batch of matrices.  Coefficients that could take a singular value of at
+    most 1 beyond about 4 before the last step are refused.  Works with 22 bits of each value whatever the
     type; the result is rounded to it once."""
     return _encoder.orthogonalize(update, steps, coefficients, eps)
 
