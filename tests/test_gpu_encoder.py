@@ -626,3 +626,32 @@ def test_example():
     spec.loader.exec_module(example)
     trees, leaves = example.main(rows=8000, rounds=20, dim=32, hidden=64, batch=1000, epochs=15)
     assert leaves < 1.5 * trees
+
+
+def test_negated_views(enc):
+    """A view that torch negates on reading is read negated, as what it stands for."""
+    g = _gen(31)
+    x, dy, table, w, update = (_randn(g, *s) for s in ((6, 40), (6, 40), (9, 40), (40,), (20, 30)))
+    tokens = torch.randint(0, 9, (6, 5), generator=g, device="cuda")
+    y, mean, rstd = enc.layer_norm(x, w, w)
+    for call, values in ((lambda t: enc.embedding_lookup(t, tokens, pool=True), (table,)),
+                         (lambda t: enc.embedding_gradient(t, tokens, 9, pool=True), (dy,)),
+                         (lambda t: enc.embedding_lookup(table, t), (tokens,)),
+                         (lambda t: enc.orthogonalize(t), (update,)),
+                         (lambda t: enc.layer_norm(t, w, w), (x,)), (lambda t: enc.layer_norm(x, t, w), (w,)),
+                         (lambda t: enc.layer_norm(x, w, t), (w,)),
+                         (lambda t: enc.layer_norm_gradient(t, x, mean, rstd, w), (dy,)),
+                         (lambda t: enc.layer_norm_gradient(dy, t, mean, rstd, w), (x,)),
+                         (lambda t: enc.layer_norm_gradient(dy, x, t, rstd, w), (mean,)),
+                         (lambda t: enc.layer_norm_gradient(dy, x, mean, t, w), (rstd,)),
+                         (lambda t: enc.layer_norm_gradient(dy, x, mean, rstd, t), (w,))):
+        value, = values
+        got, want = call(torch._neg_view(-value)), call(value)
+        if isinstance(got, torch.Tensor):
+            got, want = (got,), (want,)
+        assert all(torch.equal(p, q) for p, q in zip(got, want))
+        got = call(torch._neg_view(value))
+        got = (got,) if isinstance(got, torch.Tensor) else got
+        want = call(-value)
+        want = (want,) if isinstance(want, torch.Tensor) else want
+        assert all(torch.equal(p, q) for p, q in zip(got, want))

@@ -41,10 +41,12 @@ std::string text(at::IntArrayRef shape) {
   return s + ")";
 }
 
-const Tensor& tensor(const char* name, PyObject* object) {
+// What a view that torch negates on reading stands for is a copy.
+Tensor tensor(const char* name, PyObject* object) {
   if (!THPVariable_Check(object))
     type_error(std::string(name) + " must be a torch.Tensor, got " + Py_TYPE(object)->tp_name);
-  return THPVariable_Unpack(object);
+  const Tensor& t = THPVariable_Unpack(object);
+  return t.is_neg() ? t.resolve_neg() : t;
 }
 
 // A tensor of one of the three types on a GPU.
@@ -124,7 +126,7 @@ struct Tokens {
 };
 
 Tokens tokens_of(PyObject* object, bool pool) {
-  const Tensor& t = tensor("tokens", object);
+  const Tensor t = tensor("tokens", object);
   if (t.scalar_type() != at::kInt && t.scalar_type() != at::kLong)
     type_error(std::string("tokens must be int32 or int64, are ") + toString(t.scalar_type()));
   if (pool && t.dim() == 0) value_error("pool needs tokens with an axis to sum over");
@@ -147,7 +149,7 @@ at::DimVector with_dim(at::IntArrayRef rows, int64_t dim) {
 PyObject* lookup(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   arguments("lookup", n, 4);
-  const Tensor& table = tensor("weight", args[0]);
+  const Tensor table = tensor("weight", args[0]);
   const int type = dtype("weight", table);
   if (table.dim() != 2) value_error("weight must be a table of rows, has shape " + text(table.sizes()));
   const Tokens tokens = tokens_of(args[1], truth(args[3]));
@@ -167,7 +169,7 @@ PyObject* lookup(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* lookup_gradient(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   arguments("lookup_gradient", n, 5);
-  const Tensor& given = tensor("grad", args[0]);
+  const Tensor given = tensor("grad", args[0]);
   const int type = dtype("grad", given);
   const Tokens tokens = tokens_of(args[1], truth(args[4]));
   same_device(given, "tokens", tokens.t);
@@ -196,7 +198,7 @@ void check_normalised(const Tensor& x) {
 // A parameter row of layer norm without gaps, or none.
 Tensor parameter(const char* name, PyObject* object, const Tensor& x) {
   if (object == Py_None) return {};
-  const Tensor& t = tensor(name, object);
+  const Tensor t = tensor(name, object);
   dtype(name, t);
   if (t.dim() != 1 || t.size(0) != x.size(-1))
     value_error(std::string(name) + " must have shape (" + std::to_string(x.size(-1)) + "), has " + text(t.sizes()));
@@ -218,7 +220,7 @@ void* pointer(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   arguments("norm", n, 4);
-  const Tensor& given = tensor("x", args[0]);
+  const Tensor given = tensor("x", args[0]);
   const int type = dtype("x", given);
   check_normalised(given);
   const Tensor weight = parameter("weight", args[1], given), bias = parameter("bias", args[2], given);
@@ -247,7 +249,7 @@ PyObject* norm(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* norm_gradient(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   arguments("norm_gradient", n, 5);
-  const Tensor &g = tensor("grad", args[0]), &given = tensor("x", args[1]);
+  const Tensor g = tensor("grad", args[0]), given = tensor("x", args[1]);
   const int type = dtype("x", given);
   if (dtype("grad", g) != type || g.sizes() != given.sizes())
     value_error(std::string("grad must be like x, ") + toString(given.scalar_type()) + " " + text(given.sizes()) +
@@ -258,7 +260,7 @@ PyObject* norm_gradient(PyObject*, PyObject* const* args, Py_ssize_t n) {
   const char* names[2] = {"mean", "rstd"};
   Tensor statistics[2];
   for (int k = 0; k < 2; ++k) {
-    const Tensor& t = tensor(names[k], args[2 + k]);
+    const Tensor t = tensor(names[k], args[2 + k]);
     if (t.scalar_type() != at::kFloat || t.sizes() != rows)
       value_error(std::string(names[k]) + " must be Float " + text(rows) + ", is " + toString(t.scalar_type()) + " " +
                   text(t.sizes()));
@@ -292,7 +294,7 @@ PyObject* norm_gradient(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* orthogonalize(PyObject*, PyObject* const* args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   arguments("orthogonalize", n, 4);
-  const Tensor& given = tensor("update", args[0]);
+  const Tensor given = tensor("update", args[0]);
   const int type = dtype("update", given);
   if (given.dim() < 2) value_error("update must be a matrix, has shape " + text(given.sizes()));
   float coefficients[3];
