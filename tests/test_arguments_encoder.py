@@ -175,3 +175,44 @@ def test_coefficients_that_leave_the_products_range_are_refused():
         _refused(lib, call((3.4445, -4.775, 2.6), 6, dtype), "coefficients")  # grows with every step
         _refused(lib, call((3.0, -4.0, 2.0), 5, dtype, -1e-3), "eps")
         _refused(lib, call((3.0, -4.0, 2.0), 5, dtype, float("nan")), "eps")
+
+
+# Without a GPU the first argument alone is looked at before the device is.
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def _calls(enc, device):
+    x, w, ids = torch.ones(4, 8, device=device), torch.ones(8, device=device), torch.zeros(4, dtype=torch.int64, device=device)
+    stat = torch.zeros(4, device=device)
+    first = (lambda t: enc.embedding_lookup(t, ids), lambda t: enc.embedding_gradient(t, ids, 5), lambda t: enc.layer_norm(t),
+             lambda t: enc.layer_norm_gradient(t, x, stat, stat), lambda t: enc.orthogonalize(t))
+    later = (lambda t: enc.layer_norm(x, t[0]), lambda t: enc.layer_norm(x, w, t[0]),
+             lambda t: enc.layer_norm_gradient(x, t, stat, stat), lambda t: enc.layer_norm_gradient(x, x, t[:, 0], stat),
+             lambda t: enc.layer_norm_gradient(x, x, stat, t[:, 0]), lambda t: enc.layer_norm_gradient(x, x, stat, stat, t[0]))
+    return x, first if device == "cpu" else first + later
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_forward_mode_derivatives_are_refused(enc, device):
+    """A dual tensor's tangent would be lost: no operator takes one."""
+    x, calls = _calls(enc, device)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        for call in calls:
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call(dual)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_tracing_is_refused(enc, device):
+    """A trace would hold the result as a constant."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, calls = _calls(enc, device)
+    for call in calls:
+        def result(t):
+            out = call(t)  # pylint: disable=cell-var-from-loop
+            return out if isinstance(out, torch.Tensor) else out[0]
+        for trace in (lambda: torch.jit.trace(result, x), lambda: make_fx(result)(x),
+                      lambda: make_fx(result, tracing_mode="fake")(x)):
+            with pytest.raises(NotImplementedError, match="trace"):
+                trace()

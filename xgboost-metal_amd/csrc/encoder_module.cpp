@@ -4,6 +4,8 @@
 // 12.3 us of host time that way), so those are here.
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -41,11 +43,30 @@ std::string text(at::IntArrayRef shape) {
   return s + ")";
 }
 
+[[noreturn]] void not_implemented(const std::string& message) {
+  PyErr_SetString(PyExc_NotImplementedError, message.c_str());
+  throw python_error();
+}
+
+// The calls are no operators of torch's, so what records operators does not see
+// them: a trace would hold their results as constants.
+bool recording() {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  using Key = c10::impl::TorchDispatchModeKey;
+  if (c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::Tracer)) return true;
+  return c10::impl::dispatch_mode_enabled() &&
+         (Modes::get_mode(Key::PROXY) || Modes::get_mode(Key::FAKE) || Modes::get_mode(Key::FUNCTIONAL));
+}
+
 // What a view that torch negates on reading stands for is a copy.
 Tensor tensor(const char* name, PyObject* object) {
   if (!THPVariable_Check(object))
     type_error(std::string(name) + " must be a torch.Tensor, got " + Py_TYPE(object)->tp_name);
+  if (recording()) not_implemented("the encoder's operators cannot be traced");
   const Tensor& t = THPVariable_Unpack(object);
+  // The tangent would be lost, and a tensor without one counts as constant.
+  if (t._fw_grad(0).defined())
+    not_implemented(std::string(name) + " has a forward-mode tangent, which the encoder's operators do not carry");
   return t.is_neg() ? t.resolve_neg() : t;
 }
 

@@ -17,7 +17,9 @@ Tensors are float32, float16 or bfloat16 on a GPU.  The operators run on the
 current stream of the tensors' device, wait for nothing, and keep nothing
 between calls; as with torch's own, a tensor that another stream still writes
 has to be waited for first.  Sums are in 32 bits and rounded once; no result
-depends on the order of atomics.  The module needs torch, which the rest of the
+depends on the order of atomics.  Derivatives are reverse-mode and of first order;
+forward-mode (dual) tensors and traces (torch.jit.trace, make_fx, torch.export)
+raise NotImplementedError.  The module needs torch, which the rest of the
 package does not: import torch before xgboost, so that both use one HIP runtime,
 then this module by name, `from xgboost import encoder`.
 """
