@@ -655,3 +655,33 @@ def test_negated_views(enc):
         want = call(-value)
         want = (want,) if isinstance(want, torch.Tensor) else want
         assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+def test_results_without_a_derivative_say_so(enc):
+    """What has no derivative gives values as ever, and an error where a gradient
+    would have to pass it, not a graph that ends there without a word."""
+    g = _gen(41)
+    x, dy, w = (_randn(g, *s) for s in ((6, 20), (6, 20), (20,)))
+    tokens = torch.randint(0, 5, (6,), generator=g, device="cuda")
+    _, mean, rstd = enc.layer_norm(x, w)
+    for call, given in ((lambda t: enc.orthogonalize(t), x), (lambda t: enc.embedding_gradient(t, tokens, 5), dy),
+                        (lambda t: enc.layer_norm_gradient(t, x, mean, rstd, w), dy),
+                        (lambda t: enc.layer_norm_gradient(dy, t, mean, rstd), x),
+                        (lambda t: enc.layer_norm_gradient(dy, x, mean, rstd, t), w)):
+        leaf = given.clone().requires_grad_()
+        want, got = call(given), call(leaf)
+        want, got = ((want,), (got,)) if isinstance(want, torch.Tensor) else (want, got)
+        for p, q in zip(want, got):
+            assert (p is None) == (q is None)
+            if p is not None:
+                assert torch.equal(p, q.detach()) and q.requires_grad and not p.requires_grad
+        with pytest.raises(NotImplementedError, match="derivative"):
+            got[0].sum().backward()
+        with torch.no_grad():
+            out = call(leaf)
+            assert not (out if isinstance(out, torch.Tensor) else out[0]).requires_grad
+    # Twice through the differentiable ones is an error as before.
+    x = x.requires_grad_()
+    once, = torch.autograd.grad(enc.layer_norm(x)[0].square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        once.sum().backward()

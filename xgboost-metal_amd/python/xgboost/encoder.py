@@ -55,14 +55,35 @@ except ImportError as missing:
                       "`python -c 'import __graft_entry__ as g; g.build()'`") from missing
 
 
+class _NoDerivative(torch.autograd.Function):
+    """An operator's results where an argument requires a gradient: one that would
+    have to pass them is an error, not a graph that ends there unseen."""
+
+    @staticmethod
+    def forward(ctx, name, operator, *arguments):  # pylint: disable=arguments-differ
+        ctx.name = name
+        return operator(*arguments)
+
+    @staticmethod
+    def backward(ctx, *_):  # pylint: disable=arguments-differ
+        raise NotImplementedError(f"{ctx.name} has no derivative")
+
+
+def _without_derivative(name: str, operator: Any, *arguments: Any) -> Any:
+    if torch.is_grad_enabled() and any(getattr(a, "requires_grad", False) for a in arguments):
+        return _NoDerivative.apply(name, operator, *arguments)
+    return operator(*arguments)
+
+
 # ---- embedding ---------------------------------------------------------------
 
 def embedding_gradient(grad: torch.Tensor, tokens: torch.Tensor, num_embeddings: int, *, scale: float = 1.0,
                        pool: bool = False) -> torch.Tensor:
     """The table's gradient, (num_embeddings, dim) in grad's type, from the
     gradient of `embedding_lookup`'s result: each table row's sum over the
-    tokens that name it.  Fewer than 2^31 tokens."""
-    return _encoder.lookup_gradient(grad, tokens, num_embeddings, scale, pool)
+    tokens that name it.  Fewer than 2^31 tokens.  Has no derivative itself: where
+    grad requires one, a backward pass through the result is an error."""
+    return _without_derivative("embedding_gradient", _encoder.lookup_gradient, grad, tokens, num_embeddings, scale, pool)
 
 
 class _EmbeddingLookup(torch.autograd.Function):
@@ -97,8 +118,8 @@ def layer_norm_gradient(grad: torch.Tensor, x: torch.Tensor, mean: torch.Tensor,
                         ) -> Tuple[torch.Tensor, Optional[torch.Tensor], Optional[torch.Tensor]]:
     """The gradients of `layer_norm`'s x, weight and bias from its result's
     gradient and the statistics it returned; without a weight the last two are
-    None."""
-    return _encoder.norm_gradient(grad, x, mean, rstd, weight)
+    None.  Has no derivative itself, like `embedding_gradient`."""
+    return _without_derivative("layer_norm_gradient", _encoder.norm_gradient, grad, x, mean, rstd, weight)
 
 
 class _LayerNorm(torch.autograd.Function):
@@ -142,8 +163,9 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5,
     X = (a I + b A + c A^2) X with A = X X^T, on the shorter side.  Leading axes
     are a batch of matrices.  Coefficients that could take a singular value of at
     most 1 beyond about 4 before the last step are refused.  Works with 22 bits of each value whatever the
-    type; the result is rounded to it once."""
-    return _encoder.orthogonalize(update, steps, coefficients, eps)
+    type; the result is rounded to it once.  Has no derivative: where the update
+    requires one, a backward pass through the result is an error."""
+    return _without_derivative("orthogonalize", _encoder.orthogonalize, update, steps, coefficients, eps)
 
 
 class Muon(torch.optim.Optimizer):
