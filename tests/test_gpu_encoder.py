@@ -685,3 +685,41 @@ def test_results_without_a_derivative_say_so(enc):
     once, = torch.autograd.grad(enc.layer_norm(x)[0].square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         once.sum().backward()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES)
+@pytest.mark.parametrize("dim", [2, 33, 512, 768, 777, 1000, 4100, 8192, 20000, 33000, 40001])
+def test_norm_far_from_zero(enc, dim, dtype):
+    """Rows of one value (y 0, the mean the value), and rows whose spread is small
+    against their mean.  No value takes part in more than 80 additions of a sum
+    (40 of a lane, 6 steps in a wave, 16 waves, and a few roundings), so a sum is
+    off by 80 2^-24 of its terms' sizes: the first mean by d of the row's, what is
+    left of it after centring by 80 2^-24 of the centred sizes, s at most, and y by
+    that and a few roundings of a centred value, times rstd; the variance by its
+    sum's and the square of that."""
+    g = _gen(dim)
+    rows = [torch.full((dim,), v, device="cuda") for v in (10000.1, 100000.3, 1234.567, -777.77, 3.0e-3)]
+    rows += [_randn(g, dim) * spread + at for spread, at in ((1.0, 1e4), (1e-2, 300.0), (1.0, -6e4), (1e-3, 0.1))]
+    x = torch.stack(rows).clamp(-65000, 65000).to(dtype)
+    y, mean, rstd = enc.layer_norm(x)
+    v = x.double()
+    wmean = v.mean(1)
+    centred = v - wmean[:, None]
+    wrstd = (centred.square().mean(1) + 1e-5) ** -0.5
+    d = 80 * E32 * v.abs().mean(1)
+    s = centred.abs().mean(1) + d
+    off = 80 * E32 * s + 4 * E32 * d
+    relative = 0.5 * (84 * E32 + off ** 2 * wrstd ** 2) + 4 * E32
+    h = centred * wrstd[:, None]
+    slack = wrstd[:, None] * (off[:, None] + 4 * E32 * centred.abs()) + h.abs() * relative[:, None]
+    _near(y, h, slack, "y")
+    _near(mean, wmean, off, "mean")
+    _near(rstd, wrstd, wrstd * relative, "rstd")
+    # The rows of one value have that mean, and so gradients without h.
+    assert torch.equal(mean[:5], x[:5, 0].float())
+    grad = _randn(g, len(x), dim, dtype=dtype)
+    dx, dw, db = enc.layer_norm_gradient(grad[:5], x[:5], mean[:5], rstd[:5], torch.ones(dim, device="cuda"))
+    assert not dw.any()
+    g64 = grad[:5].double()
+    want = wrstd[:5, None] * (g64 - g64.mean(1, keepdim=True))
+    _near(dx, want, wrstd[:5, None] * (relative[:5, None] + (dim + 8) * E32) * (g64.abs() + g64.abs().mean(1, keepdim=True)), "dx")

@@ -149,11 +149,23 @@ __device__ __forceinline__ float runtime_one() {
 }
 
 // Sum over aligned groups of kLanes (a power of two, at most a wave); every
-// lane of the group gets it.
+// lane of the group gets it.  Within 16 lanes the exchanges are lane moves, which
+// take no turn of LDS's: lanes 1 and 2 apart by quad permutations, and, as the
+// lanes of a quad then hold one value, and those of two quads, 4 and 8 apart by
+// mirrored halves of a row and mirrored rows.
+template <int kCtrl>
+__device__ __forceinline__ float lane_move(float v) {
+  return __uint_as_float(dpp_move<kCtrl, 0xf>(__float_as_uint(v)));
+}
+
 template <int kLanes>
 __device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-  for (int d = kLanes / 2; d > 0; d >>= 1) v += __shfl_xor(v, d, kWave);
+  if constexpr (kLanes >= 64) v += __shfl_xor(v, 32, kWave);
+  if constexpr (kLanes >= 32) v += __shfl_xor(v, 16, kWave);
+  if constexpr (kLanes >= 2) v += lane_move<0xb1>(v);
+  if constexpr (kLanes >= 4) v += lane_move<0x4e>(v);
+  if constexpr (kLanes >= 8) v += lane_move<0x141>(v);
+  if constexpr (kLanes >= 16) v += lane_move<0x140>(v);
   return v;
 }
 
@@ -169,6 +181,23 @@ __device__ __forceinline__ float block_sum(float v, float* shared) {
 #pragma unroll
   for (int w = 0; w < kThreads / kWave; ++w) total += shared[w];
   return total;
+}
+
+// Two sums at once; `shared` holds two floats per wave.
+template <int kThreads>
+__device__ __forceinline__ void block_sums(float& a, float& b, float* shared) {
+  constexpr int kWaves = kThreads / kWave;
+  a = group_sum<kWave>(a);
+  b = group_sum<kWave>(b);
+  __syncthreads();
+  if (lane_id() == 0) {
+    shared[threadIdx.x / kWave] = a;
+    shared[kWaves + threadIdx.x / kWave] = b;
+  }
+  __syncthreads();
+  // (A lane a wave's: 2 kWaves registers at once would cost a second workgroup.)
+  a = group_sum<kWaves>(shared[lane_id() % kWaves]);
+  b = group_sum<kWaves>(shared[kWaves + lane_id() % kWaves]);
 }
 
 // Host side: an argument's check that fails leaves its message.

@@ -8,8 +8,12 @@
 // Both passes are bound by memory: a row is read once into registers by the
 // lanes that hold it (a part of a wave, a wave or a workgroup, by its width),
 // the sums go over those lanes, and the row is written from the registers.
-// The variance is the sum of centred squares, not a difference of sums, so
-// rows far from zero lose nothing.  All sums are binary32.
+// All sums are binary32.  A mean rounded to it is off by up to an ulp or more, which
+// in a row far from zero is more than its spread, so the centred values are summed
+// once more: what is left of the mean is taken out of them, of the variance (a sum of
+// centred squares, not a difference of sums) and of the stored mean.  The gradient
+// centres by the stored mean, half an ulp of it off at most: h there is off by that
+// times rstd, 2^-13 where a row's spread is 2^12 ulps of its mean.
 //
 // Measured (us, one MI355X, whose copies reach 5.1 TB/s), with the bytes that
 // have to move: 65,536 x 1,024 bfloat16 forward 54 (5.0 TB/s), gradient 75 and the
@@ -42,6 +46,21 @@ __device__ __forceinline__ float row_sum(float v, float* shared) {
     return block_sum<kLanes>(v, shared);
   }
 }
+
+template <int kLanes>
+__device__ __forceinline__ void row_sums(float& a, float& b, float* shared) {
+  if constexpr (kLanes <= kWave) {
+    a = group_sum<kLanes>(a);
+    b = group_sum<kLanes>(b);
+  } else {
+    block_sums<kLanes>(a, b, shared);
+  }
+}
+
+// Given what is left of the mean and the mean square of values centred by all but
+// that: whether so much is left that the difference of squares would cancel, and the
+// values have to be centred anew.
+__device__ __forceinline__ bool far_off(float left, float square) { return 64.0f * left * left > square; }
 
 // A lane's columns of a row: kPacks times kSize, a pack or, in rows narrower than
 // a pack, one.  The last pack of a row that is no whole number of packs begins
@@ -79,7 +98,7 @@ __global__ __launch_bounds__(kLanes > kNormThreads ? kLanes : kNormThreads) void
     T* __restrict__ y, float* __restrict__ means, float* __restrict__ rstds, const T* __restrict__ x,
     const W* __restrict__ weight, const W* __restrict__ bias, int64_t rows, int64_t dim, int64_t stride, float eps) {
   constexpr int kThreads = kLanes > kNormThreads ? kLanes : kNormThreads;
-  __shared__ float shared[kThreads / kWave];
+  __shared__ float shared[2 * kThreads / kWave];
   const int lane = threadIdx.x % kLanes;
   const int64_t row = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
   // Lanes of a row beyond the last only occur where a row is at most a wave's:
@@ -98,16 +117,35 @@ __global__ __launch_bounds__(kLanes > kNormThreads ? kLanes : kNormThreads) void
 #pragma unroll
     for (int e = 0; e < kSize; ++e) sum += columns.own(k, e, v[k][e]);
   }
-  const float mean = row_sum<kLanes>(sum, shared) / (float)dim;
-  float squares = 0.0f;
+  float mean = row_sum<kLanes>(sum, shared) / (float)dim;
+  float left = 0.0f, variance = 0.0f;  // sums of the centred values and of their squares
 #pragma unroll
   for (int k = 0; k < kPacks; ++k)
 #pragma unroll
     for (int e = 0; e < kSize; ++e) {
       v[k][e] -= mean;
-      squares = fmaf(columns.own(k, e, v[k][e]), v[k][e], squares);
+      const float own = columns.own(k, e, v[k][e]);
+      left += own;
+      variance = fmaf(own, own, variance);
     }
-  const float rstd = 1.0f / sqrtf(row_sum<kLanes>(squares, shared) / (float)dim + eps);
+  row_sums<kLanes>(left, variance, shared);
+  left /= (float)dim;
+  variance /= (float)dim;
+  mean += left;
+  if (far_off(left, variance)) {  // the same for all lanes of a row
+    variance = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kPacks; ++k)
+#pragma unroll
+      for (int e = 0; e < kSize; ++e) {
+        const float own = columns.own(k, e, v[k][e] - left);
+        variance = fmaf(own, own, variance);
+      }
+    variance = row_sum<kLanes>(variance, shared) / (float)dim;
+  } else {
+    variance = fmaf(-left, left, variance);
+  }
+  const float rstd = 1.0f / sqrtf(variance + eps), shift = -left * rstd;
   if (lane == 0) {
     means[row] = mean;
     rstds[row] = rstd;
@@ -120,7 +158,7 @@ __global__ __launch_bounds__(kLanes > kNormThreads ? kLanes : kNormThreads) void
     if (bias) load_row_part<W, kSize>(bias + columns.at[k], b);
 #pragma unroll
     for (int e = 0; e < kSize; ++e) {
-      const float h = v[k][e] * rstd;
+      const float h = fmaf(v[k][e], rstd, shift);
       v[k][e] = weight ? (bias ? fmaf(h, w[e], b[e]) : h * w[e]) : h;
     }
     if (columns.any(k)) raw[k].put(v[k], out + columns.at[k]);
@@ -128,31 +166,49 @@ __global__ __launch_bounds__(kLanes > kNormThreads ? kLanes : kNormThreads) void
 }
 
 // Rows wider than the registers of 1024 lanes: three readings, the later two
-// from cache.
+// from cache (four where the first mean is far off).
 template <typename T, typename W>
 __global__ __launch_bounds__(1024) void k_norm_wide(T* __restrict__ y, float* __restrict__ means,
                                                     float* __restrict__ rstds, const T* __restrict__ x,
                                                     const W* __restrict__ weight, const W* __restrict__ bias,
                                                     int64_t dim, int64_t stride, float eps) {
   constexpr int kSize = Pack<T>::kSize;
-  __shared__ float shared[1024 / kWave];
+  __shared__ float shared[2 * 1024 / kWave];
   const int64_t row = blockIdx.x;
   const T* in = x + row * stride;
   float v[kSize], w[kSize], b[kSize];
-  float sum = 0.0f, squares = 0.0f;
+  float sum = 0.0f, left = 0.0f, variance = 0.0f;
   for (int64_t at = (int64_t)threadIdx.x * kSize; at < dim; at += 1024 * kSize) {
     load_pack(in, at, dim, v);
     for (int e = 0; e < kSize; ++e) sum += v[e];
   }
-  const float mean = block_sum<1024>(sum, shared) / (float)dim;
+  const float first = block_sum<1024>(sum, shared) / (float)dim;
   for (int64_t at = (int64_t)threadIdx.x * kSize; at < dim; at += 1024 * kSize) {
     load_pack(in, at, dim, v);
     for (int e = 0; e < kSize; ++e) {
-      const float c = at + e < dim ? v[e] - mean : 0.0f;
-      squares = fmaf(c, c, squares);
+      const float c = at + e < dim ? v[e] - first : 0.0f;
+      left += c;
+      variance = fmaf(c, c, variance);
     }
   }
-  const float rstd = 1.0f / sqrtf(block_sum<1024>(squares, shared) / (float)dim + eps);
+  block_sums<1024>(left, variance, shared);
+  left /= (float)dim;
+  variance /= (float)dim;
+  const float mean = first + left;
+  if (far_off(left, variance)) {  // the same for all lanes
+    variance = 0.0f;
+    for (int64_t at = (int64_t)threadIdx.x * kSize; at < dim; at += 1024 * kSize) {
+      load_pack(in, at, dim, v);
+      for (int e = 0; e < kSize; ++e) {
+        const float c = at + e < dim ? (v[e] - first) - left : 0.0f;
+        variance = fmaf(c, c, variance);
+      }
+    }
+    variance = block_sum<1024>(variance, shared) / (float)dim;
+  } else {
+    variance = fmaf(-left, left, variance);
+  }
+  const float rstd = 1.0f / sqrtf(variance + eps);
   if (threadIdx.x == 0) {
     means[row] = mean;
     rstds[row] = rstd;
@@ -162,7 +218,7 @@ __global__ __launch_bounds__(1024) void k_norm_wide(T* __restrict__ y, float* __
     if (weight) load_some<kSize>(weight, at, dim, w);
     if (bias) load_some<kSize>(bias, at, dim, b);
     for (int e = 0; e < kSize; ++e) {
-      const float h = (v[e] - mean) * rstd;
+      const float h = ((v[e] - first) - left) * rstd;
       v[e] = weight ? (bias ? fmaf(h, w[e], b[e]) : h * w[e]) : h;
     }
     store_pack(y + row * dim, at, dim, v);

@@ -146,7 +146,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
                eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(y, mean, rstd): x's last axis normalised to mean 0 and variance 1, times
     weight plus bias, and the statistics (float32) that `layer_norm_gradient`
-    reads.  weight and bias are float32 or x's type; a bias needs a weight.
+    reads.  y comes of the mean in more than 32 bits, the gradient of the one
+    returned.  weight and bias are float32 or x's type; a bias needs a weight.
     Differentiable in x, weight and bias through y."""
     if torch.is_grad_enabled() and (getattr(x, "requires_grad", False) or getattr(weight, "requires_grad", False) or
                                     getattr(bias, "requires_grad", False)):
