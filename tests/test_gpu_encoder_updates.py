@@ -5,6 +5,8 @@ LARGE has what the products come in: tiles of 128, of 64 and of 32 with the dept
 in 1, 4 and 16 parts, single and by twos, symmetric or not, operands with and
 without low parts, segments of one step and of several, batches.
 """
+import copy
+
 import pytest
 import torch
 from test_gpu_encoder import COEFFICIENTS, U, _gen, _orthogonal64, _randn, enc  # noqa: F401
@@ -110,3 +112,91 @@ def test_orthogonalize_coefficients_at_the_limit(enc, dtype):  # noqa: F811
         for coefficients, steps in (((5.0, 0.0, 0.0), 2), ((8.0, 8.0, 8.0), 2)):
             with pytest.raises(ValueError, match="coefficients"):
                 enc.orthogonalize(update, steps=steps, coefficients=coefficients)
+
+
+def _muon64(p, m, grad, lr, momentum, nesterov, decay, steps=5):
+    """The docstring's step in 64 bits: the weight and the momentum after it, and the update's norm."""
+    m = momentum * m + grad.double()
+    o = _orthogonal64(grad.double() + momentum * m if nesterov else m, steps)
+    size = lr * max(1.0, p.shape[0] / p.shape[1]) ** 0.5
+    return p - size * o - lr * decay * p, m, size * o.norm()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES)
+@pytest.mark.parametrize("nesterov,decay", [(True, 0.0), (False, 0.1), (True, 0.01)])
+@pytest.mark.parametrize("shape", [(40, 70), (90, 30), (70, 300)])
+def test_muon_steps(enc, shape, nesterov, decay, dtype):  # noqa: F811
+    """Eight steps by the formula.  An update is off by at most 2^-22 (a^5 + 5 a^4) of
+    its norm, a binary32 weight by 4 roundings a step.  16-bit weights are kept in
+    binary32 between the steps and show it rounded once, whatever the steps."""
+    g = _gen(sum(shape))
+    p = torch.nn.Parameter(_randn(g, *shape, dtype=dtype) * 0.2)
+    lr, momentum = 0.02, 0.9
+    opt = enc.Muon([p], lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=decay)
+    want, m = p.detach().double(), torch.zeros(shape, dtype=torch.float64, device="cuda")
+    a, slack = COEFFICIENTS[0], 0.0
+    for _ in range(8):
+        p.grad = _randn(g, *shape, dtype=dtype)
+        opt.step()
+        want, m, size = _muon64(want, m, p.grad, lr, momentum, nesterov, decay)
+        slack += (a ** 5 + 5 * a ** 4) * 2.0 ** -22 * size.item() + 4 * 2.0 ** -24 * want.abs().max().item()
+        bound = slack + U[dtype] * (want.abs() + slack)
+        assert p.dtype == dtype and ((p.detach().double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES)
+def test_muon_small_decay_and_momentum_last(enc, dtype):  # noqa: F811
+    """Without gradients only the decay is left, 1 - 2e-4 a step: 500 steps take a tenth,
+    although one is less than a 16-bit weight's rounding; each step rounds twice in binary32."""
+    p = torch.nn.Parameter(torch.ones(16, 24, device="cuda", dtype=dtype))
+    opt = enc.Muon([p], lr=0.02, weight_decay=0.01)
+    p.grad = torch.zeros_like(p)
+    for _ in range(500):
+        opt.step()
+    want = (1.0 - 0.02 * 0.01) ** 500
+    assert abs(p[3, 5].item() - want) <= (U[dtype] + 1000 * 2.0 ** -24) * want
+    # Momentum keeps what is below 2^-9 of it: 1 + 300 / 1024, not 1 (300 further roundings).
+    p = torch.nn.Parameter(torch.zeros(16, 24, device="cuda", dtype=dtype))
+    opt = enc.Muon([p], lr=0.0, momentum=1.0)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    p.grad = torch.full_like(p, 2.0 ** -10)
+    for _ in range(300):
+        opt.step()
+    m = opt.state[p]["momentum"]
+    assert m.dtype == torch.float32 and (m.double() - (1 + 300 / 1024)).abs().max() <= 300 * 2.0 ** -23
+
+
+def test_muon_weights_set_from_outside_and_resumed(enc):  # noqa: F811
+    """A 16-bit weight that was overwritten goes on from there, and a saved state goes on as if nothing was."""
+    g = _gen(7)
+    grads = [_randn(g, 20, 30, dtype=torch.bfloat16) for _ in range(6)]
+    start = _randn(g, 20, 30, dtype=torch.bfloat16)
+
+    def run(opt, p, some):
+        for grad in some:
+            p.grad = grad.clone()
+            opt.step()
+
+    def made(value):
+        p = torch.nn.Parameter(value.clone())
+        return p, enc.Muon([p], lr=1e-3, weight_decay=0.01)
+
+    p, opt = made(start)
+    run(opt, p, grads[:3])
+    saved, weight = copy.deepcopy(opt.state_dict()), p.detach().clone()
+    run(opt, p, grads[3:])
+    q, other = made(weight)
+    other.load_state_dict(saved)
+    run(other, q, grads[3:])
+    assert torch.equal(p, q)
+    for key in opt.state[p]:
+        assert torch.equal(opt.state[p][key], other.state[q][key])
+    other_values = opt.state[p]["weight"].to(p.dtype) != 2.0
+    with torch.no_grad():
+        p.fill_(2.0)
+    p.grad = torch.zeros_like(p)
+    opt.state[p]["momentum"].zero_()
+    opt.step()
+    assert (p == 2.0).all()  # 2 - 2e-5, rounded
+    assert (opt.state[p]["weight"][other_values] < 2.0).all() and other_values.sum() > 500

@@ -173,7 +173,12 @@ class Muon(torch.optim.Optimizer):
     """Matrices by orthogonalised momentum: m = momentum m + grad, and
     w -= lr (sqrt(max(1, rows / columns)) orthogonalize(grad + momentum m) + weight_decay w)
     (without `nesterov` orthogonalize(m)).  For weights of two axes; biases,
-    norms and embedding tables belong to another optimizer."""
+    norms and embedding tables belong to another optimizer.
+
+    The step is computed in float32.  Of a float16 or bfloat16 weight the state
+    keeps the float32 value too (`weight`, beside `momentum`), of which the
+    parameter is the rounding: steps and decays below half a unit of its type add
+    up.  A parameter set from outside goes on from what it was set to."""
 
     def __init__(self, params: Any, lr: float = 0.02, momentum: float = 0.95, nesterov: bool = True,
                  weight_decay: float = 0.0, steps: int = 5,
@@ -184,6 +189,14 @@ class Muon(torch.optim.Optimizer):
             for p in group["params"]:
                 if p.dim() != 2:
                     raise ValueError(f"Muon takes matrices, got a parameter of shape {tuple(p.shape)}")
+
+    def load_state_dict(self, state_dict: Any) -> None:
+        super().load_state_dict(state_dict)
+        # That rounds the state to the parameters' types.
+        saved = [k for group in state_dict["param_groups"] for k in group["params"]]
+        for k, p in zip(saved, (p for group in self.param_groups for p in group["params"])):
+            for name, value in state_dict["state"].get(k, {}).items():
+                self.state[p][name] = value.to(device=p.device, copy=True)
 
     @torch.no_grad()
     def step(self, closure: Any = None) -> Any:  # pylint: disable=arguments-differ
@@ -196,14 +209,23 @@ class Muon(torch.optim.Optimizer):
                 if p.grad is None:
                     continue
                 state = self.state[p]
+                short = p.dtype in (torch.float16, torch.bfloat16)
+                weight, grad = p, p.grad
                 if "momentum" not in state:
-                    state["momentum"] = torch.zeros_like(p)
-                m = state["momentum"].mul_(group["momentum"]).add_(p.grad)
-                update = torch.add(p.grad, m, alpha=group["momentum"]) if group["nesterov"] else m
+                    state["momentum"] = torch.zeros_like(p, dtype=torch.float32 if short else p.dtype)
+                if short:
+                    grad = grad.float()
+                    weight = state.get("weight")
+                    weight = p.float() if weight is None else torch.where(weight.to(p.dtype) == p, weight, p.float())
+                    state["weight"] = weight
+                m = state["momentum"].mul_(group["momentum"]).add_(grad)
+                update = torch.add(grad, m, alpha=group["momentum"]) if group["nesterov"] else m
                 update = orthogonalize(update, steps=group["steps"], coefficients=group["coefficients"])
                 if group["weight_decay"]:
-                    p.mul_(1.0 - group["lr"] * group["weight_decay"])
-                p.add_(update, alpha=-group["lr"] * max(1.0, p.shape[0] / p.shape[1]) ** 0.5)
+                    weight.mul_(1.0 - group["lr"] * group["weight_decay"])
+                weight.add_(update, alpha=-group["lr"] * max(1.0, p.shape[0] / p.shape[1]) ** 0.5)
+                if short:
+                    p.copy_(weight)
         return loss
 
 
