@@ -216,3 +216,13 @@ def test_tracing_is_refused(enc, device):
                       lambda: make_fx(result, tracing_mode="fake")(x)):
             with pytest.raises(NotImplementedError, match="trace"):
                 trace()
+
+
+def test_muon_refuses_later_groups(enc):
+    """A group that is added later is looked at as the first ones are, and left out if refused."""
+    opt = enc.Muon([torch.nn.Parameter(torch.zeros(4, 5))])
+    for shape in ((5,), (2, 3, 4), ()):
+        with pytest.raises(ValueError, match="matrices"):
+            opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(3, 3)), torch.nn.Parameter(torch.zeros(shape))]})
+    opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(2, 7))], "lr": 0.5})
+    assert [len(group["params"]) for group in opt.param_groups] == [1, 1] and opt.param_groups[1]["lr"] == 0.5

@@ -185,10 +185,13 @@ class Muon(torch.optim.Optimizer):
                  coefficients: Sequence[float] = (3.4445, -4.7750, 2.0315)) -> None:
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay,
                                       steps=steps, coefficients=tuple(coefficients)))
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.dim() != 2:
-                    raise ValueError(f"Muon takes matrices, got a parameter of shape {tuple(p.shape)}")
+
+    def add_param_group(self, param_group: Any) -> None:
+        super().add_param_group(param_group)
+        for p in self.param_groups[-1]["params"]:
+            if p.dim() != 2:
+                self.param_groups.pop()
+                raise ValueError(f"Muon takes matrices, got a parameter of shape {tuple(p.shape)}")
 
     def load_state_dict(self, state_dict: Any) -> None:
         super().load_state_dict(state_dict)
