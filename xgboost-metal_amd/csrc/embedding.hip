@@ -848,67 +848,64 @@ __global__ __launch_bounds__(kRangeThreads) void k_range_gradient(T* __restrict_
   uint32_t* fronts = (uint32_t*)(heads + kRangeThreads * kSize);  // each group's first key, ~0 without tokens
   if (lane_in == 0) fronts[group] = from < to ? entries[from] >> s.row_bits : ~0u;
   const float one = runtime_one();
-  const int64_t width = (int64_t)kLanes * kSize;
-  for (int64_t column = 0; column < dim; column += width) {
-    const int64_t nominal = column + lane_in * kSize, at = nominal < dim - kSize ? nominal : dim - kSize;
-    const bool active = nominal < dim;
-    float sum[kSize] = {};
-    auto store = [&](uint32_t key) {
-      if (!active) return;
+  // (The groups that take this path have all columns of a row at once.)
+  const int64_t nominal = lane_in * kSize, at = nominal < dim - kSize ? nominal : dim - kSize;
+  const bool active = nominal < dim;
+  float sum[kSize] = {};
+  auto store = [&](uint32_t key) {
+    if (!active) return;
 #pragma unroll
-      for (int e = 0; e < kSize; ++e) sum[e] *= scale;
-      Raw<T, kSize>().put(sum, out + (int64_t)key * dim + at);
-    };
-    bool head = from > 0 && from < to && entries[from - 1] >> s.row_bits == entries[from] >> s.row_bits, tail = false;
-    uint32_t key = from < to ? entries[from] >> s.row_bits : 0;
-    // Entries are fetched an iteration ahead, with the one behind them.
-    uint32_t next[kAhead + 1];
-    auto fetch = [&](uint32_t i) {
+    for (int e = 0; e < kSize; ++e) sum[e] *= scale;
+    Raw<T, kSize>().put(sum, out + (int64_t)key * dim + at);
+  };
+  bool head = from > 0 && from < to && entries[from - 1] >> s.row_bits == entries[from] >> s.row_bits, tail = false;
+  uint32_t key = from < to ? entries[from] >> s.row_bits : 0;
+  // Entries are fetched an iteration ahead, with the one behind them.
+  uint32_t next[kAhead + 1];
+  auto fetch = [&](uint32_t i) {
 #pragma unroll
-      for (int j = 0; j <= kAhead; ++j) next[j] = entries[i + j < c ? i + j : c - 1];
-    };
-    if (from < to) fetch(from);
-    for (uint32_t i = from; i < to; i += kAhead) {
-      uint32_t entry[kAhead + 1];
+    for (int j = 0; j <= kAhead; ++j) next[j] = entries[i + j < c ? i + j : c - 1];
+  };
+  if (from < to) fetch(from);
+  for (uint32_t i = from; i < to; i += kAhead) {
+    uint32_t entry[kAhead + 1];
 #pragma unroll
-      for (int j = 0; j <= kAhead; ++j) entry[j] = next[j];
-      if (i + kAhead < to) fetch(i + kAhead);
-      Raw<T, kSize> v[kAhead];
+    for (int j = 0; j <= kAhead; ++j) entry[j] = next[j];
+    if (i + kAhead < to) fetch(i + kAhead);
+    Raw<T, kSize> v[kAhead];
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) v[j].load(grad + (int64_t)(entry[j] & mask) * stride + at);
+    for (int j = 0; j < kAhead; ++j) v[j].load(grad + (int64_t)(entry[j] & mask) * stride + at);
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const uint32_t p = i + j + 1;
-        if (p > to) break;
-        add_one<T, kSize>(v[j], one, sum);
-        const uint32_t following = entry[j + 1] >> s.row_bits;
-        const bool ends = p >= c || following != key;
-        if (!ends && p < to) continue;
-        if (head) store_floats<kSize>(heads + (size_t)threadIdx.x * kSize, sum);
-        else if (ends) store(key);
-        else tail = true;
-        if (tail) break;
-        key = following;
-        head = false;
+    for (int j = 0; j < kAhead; ++j) {
+      const uint32_t p = i + j + 1;
+      if (p > to) break;
+      add_one<T, kSize>(v[j], one, sum);
+      const uint32_t following = entry[j + 1] >> s.row_bits;
+      const bool ends = p >= c || following != key;
+      if (!ends && p < to) continue;
+      if (head) store_floats<kSize>(heads + (size_t)threadIdx.x * kSize, sum);
+      else if (ends) store(key);
+      else tail = true;
+      if (tail) break;
+      key = following;
+      head = false;
 #pragma unroll
-        for (int e = 0; e < kSize; ++e) sum[e] = 0.0f;
-      }
+      for (int e = 0; e < kSize; ++e) sum[e] = 0.0f;
     }
-    __syncthreads();
-    if (tail) {
-      for (uint32_t g = group + 1; g < kGroups && fronts[g] == key; ++g)
-        add_floats<kSize>(heads + (size_t)(g * kLanes + lane_in) * kSize, sum);
-      store(key);
-    }
-    // Rows without tokens.
-    for (uint32_t r = group; r < range; r += kGroups)
-      if (totals[r] == totals[r + 1]) {
-#pragma unroll
-        for (int e = 0; e < kSize; ++e) sum[e] = 0.0f;
-        store(low + r);
-      }
-    __syncthreads();
   }
+  __syncthreads();
+  if (tail) {
+    for (uint32_t g = group + 1; g < kGroups && fronts[g] == key; ++g)
+      add_floats<kSize>(heads + (size_t)(g * kLanes + lane_in) * kSize, sum);
+    store(key);
+  }
+  // Rows without tokens.
+  for (uint32_t r = group; r < range; r += kGroups)
+    if (totals[r] == totals[r + 1]) {
+#pragma unroll
+      for (int e = 0; e < kSize; ++e) sum[e] = 0.0f;
+      store(low + r);
+    }
 }
 
 // The table from its windows' parts.
