@@ -54,7 +54,7 @@ __device__ __forceinline__ I share_of(const I* mine, int j) {
 // kLanes lanes share a row (further columns are other workgroups', blockIdx.y);
 // `split` groups share a row's tokens, kAhead in turn, and are joined through
 // LDS in their order.  O: byte offsets into the table, 32 bits where it is less
-// than 4 GB.  Many tokens are bound by what the chiplets' caches give the compute
+// than 4 GB (20,000 x 100 tokens of 64 columns 21.1 us, with 64 bits 25.9).  Many tokens are bound by what the chiplets' caches give the compute
 // units: 262,144 x 100 rows of 128 bytes take 153 us, 22 TB/s (90 % of the lines
 // hit there).  Instructions per token come next, so the lane that fetches a token
 // also checks it and finds its row.  Gathers from slices of the table in LDS, with
@@ -351,7 +351,8 @@ __global__ __launch_bounds__(kThreads) void k_sort_scan(uint32_t* __restrict__ c
 // A tile's entries are brought in order in LDS, so that those of one digit
 // leave it as one run.  With few tiles (kFew) a workgroup adds up the tiles'
 // counts itself, and counts the next pass's digits where its entries go: three
-// launches for two passes instead of six.
+// launches for two passes instead of six (whole gradients, us: 25,600 tokens 24.5 and
+// 32.0, 131,000 tokens 39.8 and 39.0).
 template <typename E, typename F, int kRounds, bool kFew>
 __global__ __launch_bounds__(kSortThreads) void k_sort_scatter(E* __restrict__ out, F from,
                                                                const uint32_t* __restrict__ counts,
@@ -525,7 +526,7 @@ struct Keys {
 };
 
 // O: byte offsets into a window's rows of grad, 32 bits where those are less
-// than 4 GB.
+// than 4 GB (30,000 x 300 tokens of 128 columns 265 us, with 64 bits 278).
 template <typename T, typename E, typename O, int kLanes, int kSize>
 __global__ __launch_bounds__(kThreads) void k_segment_sums(T* __restrict__ out, const T* __restrict__ grad,
                                                            const E* __restrict__ sorted, Sort s, Segments g) {
@@ -971,6 +972,9 @@ void with_lanes(const RowLanes& r, F&& fn) {
 }
 
 // Lanes that keep the chip's memory busy: four waves on each SIMD of 256 CUs.
+// Groups share a row's tokens below that (us, shared and a group a row): 16 x 100
+// tokens of 32 columns 3.4 and 9.2, 2,000 x 100 of 64 columns 6.9 and 10.2, 20,000 x 100
+// 21.7 and 21.1.
 constexpr int64_t kBusyLanes = int64_t(1) << 18;
 
 template <typename T, typename I>
@@ -1003,11 +1007,22 @@ int lookup(T* out, const T* weight, const I* tokens, int64_t rows, int64_t bag, 
   return 0;
 }
 
-// A chiplet's cache, and the part of it that a window's rows of grad may take.
+// A chiplet's cache, and the part of it that a window's rows of grad may take.  us
+// with one window, and with windows of 1, 2.25 and 4 MB: 65,536 x 100 tokens of 128
+// bytes 214, 180, 182, 191; 131,072 x 100 of 128 bytes 365, 269, 264, 279; 262,144 x 50
+// of 256 bytes 675, 619, 518, 452.
 constexpr int64_t kCache = int64_t(4) << 20, kWindowBytes = int64_t(9) << 18;
 // Most tokens for the one launch by ranges (LDS holds them all, were they one range's).
+// At 32,700 tokens 13.3 us, sorted in three launches 25.5 (32 columns); 17.0 and 29.1
+// (256 columns).
 constexpr int64_t kRangeTokens = 32768;
-constexpr int64_t kLongTiles = int64_t(1) << 21;  // tokens from which a tile has 16 rounds, not 4
+// Tokens from which a tile has 16 rounds, not 4 (us, 4 and 16): 1 million tokens of 64
+// columns 70 and 82, 3 million of 32 columns 117 and 118, 10 million of 16 columns 282
+// and 273.
+constexpr int64_t kLongTiles = int64_t(1) << 21;
+// Sorted tokens of a group at most (us, 64, 128, 512 and 2,048): 65,536 x 100 tokens of
+// 64 columns 191, 181, 182, 182; 262,144 x 50 of 128 columns 472, 454, 516, 517.
+constexpr int64_t kMostChunk = 512;
 
 // How the gradient of rows x bag tokens is computed and laid out in the workspace.
 struct GradientPlan {
@@ -1058,7 +1073,7 @@ GradientPlan gradient_plan(int64_t rows, int64_t bag, int64_t vocabulary, int64_
   // which leave fewer parts to join.
   int64_t chunk = n * p.row.lanes * p.row.groups / (2 * kBusyLanes);
   chunk = (chunk + kAhead - 1) / kAhead * kAhead;
-  chunk = chunk < kAhead ? kAhead : chunk > 512 ? 512 : chunk;
+  chunk = chunk < kAhead ? kAhead : chunk > kMostChunk ? kMostChunk : chunk;
   p.segments.chunk = (uint32_t)chunk;
   p.segments.chunks = (uint32_t)((window * bag + chunk - 1) / chunk);
   p.segments.dim = dim;

@@ -6,9 +6,10 @@
 // steps can run among m x m matrices: A <- Z A Z and P <- Z P, all symmetric and
 // commuting, and one product X <- P X ends it.  For n > m that leaves out most
 // products with n; symmetric results take half their tiles.  An error in A grows
-// by a^2 a step where X is small, so a segment has at most two or three steps
+// by a^2 a step where X is small, so a segment has at most three steps
 // and the next one takes A from X anew (low rank 512 x 2048: 4e-5 of the norm with
-// three, 2e-5 in plain binary32, 1e-4 with all five in one segment).
+// three, 2e-5 in plain binary32, 1e-4 with all five in one segment); with binary32
+// results a segment is one step.
 //
 // The matrix instructions multiply binary16.  A small direction's part grows
 // a-fold a step, so operands of 11 bits would show in the result (4e-2 of the
@@ -877,8 +878,13 @@ dim3 product_grid(const Product& p, int side, int jobs, int64_t batch) {
 }
 
 // Tiles of 128 where they are enough for half the compute units, of 64 where those
-// are enough for a quarter, else of 32 with the depth cut into as many parts as
-// help.
+// are enough for a quarter, else of 32 with the depth cut into parts.  us by this rule
+// and otherwise: 2,048 x 4,096 bfloat16 881, with tiles of 64 alone 955; 1,024 x 1,024
+// binary32 174, with 128 from 64 tiles on 222; 1,900 x 2,100 824, with 128 from 100 on
+// 798; 1,500 x 1,001 224, without tiles of 64 386; 512 x 512 97, with 64 from 32 tiles on
+// 124, from 100 on 87; 8 of 512 x 512 258 and 253 without tiles of 64.  Parts of the
+// depth: 512 x 512 97, in one up to a depth of 1,024 115, in 16 always 103, in 4 beyond
+// 256 98; 128 x 1,000 78, in 4 beyond 256 71.
 template <int kMode, typename T, bool kLeftLow, bool kRightLow>
 void product(const Product& p, int jobs, int64_t batch, hipStream_t stream) {
   auto tiles = [&](int side) {

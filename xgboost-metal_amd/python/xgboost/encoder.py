@@ -163,9 +163,10 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5,
     optimiser's): X = update / (norm + eps), then `steps` times
     X = (a I + b A + c A^2) X with A = X X^T, on the shorter side.  Leading axes
     are a batch of matrices.  Coefficients that could take a singular value of at
-    most 1 beyond about 4 before the last step are refused.  Works with 22 bits of each value whatever the
-    type; the result is rounded to it once.  Has no derivative: where the update
-    requires one, a backward pass through the result is an error."""
+    most 1 beyond about 4 before the last step are refused.  Whatever the type, a
+    value of X is kept to 22 bits, or to 2^-37 if it is below 2^-14 (X has norm 1
+    at first), and the result is rounded to its type once.  Has no derivative:
+    where the update requires one, a backward pass through the result is an error."""
     return _without_derivative("orthogonalize", _encoder.orthogonalize, update, steps, coefficients, eps)
 
 
