@@ -723,3 +723,16 @@ def test_norm_far_from_zero(enc, dim, dtype):
     g64 = grad[:5].double()
     want = wrstd[:5, None] * (g64 - g64.mean(1, keepdim=True))
     _near(dx, want, wrstd[:5, None] * (relative[:5, None] + (dim + 8) * E32) * (g64.abs() + g64.abs().mean(1, keepdim=True)), "dx")
+
+
+def test_leaf_tokens_of_rounds(enc, xgb):
+    """An end below 1 means all rounds and one beyond them the last, as in Booster.predict."""
+    rng = np.random.default_rng(5)
+    X = rng.normal(size=(300, 4)).astype(np.float32)
+    d = xgb.DMatrix(X, label=X[:, 0])
+    bst = xgb.train({"max_depth": 3}, d, 4)
+    whole = enc.LeafTokenizer(bst)(d)
+    for end in (0, -1, -3, 4, 9, 2):
+        tok = enc.LeafTokenizer(bst, (0, end))
+        leaves = bst.predict(d, pred_leaf=True, iteration_range=(0, end)).reshape(300, -1)
+        assert tok.trees == leaves.shape[1] and torch.equal(tok(d), whole[:, :tok.trees])

@@ -276,7 +276,7 @@ class LeafTokenizer:
         if begin != 0:
             raise ValueError("leaves are of the rounds [0, end)")
         trees = booster.trees_to_json()
-        trees = trees[:end] if end else trees
+        trees = trees[:end] if end > 0 else trees
         if not trees:
             raise ValueError("the model has no trees")
         nodes = max(len(t["left_children"]) for t in trees)
