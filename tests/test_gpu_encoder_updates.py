@@ -200,3 +200,52 @@ def test_muon_weights_set_from_outside_and_resumed(enc):  # noqa: F811
     opt.step()
     assert (p == 2.0).all()  # 2 - 2e-5, rounded
     assert (opt.state[p]["weight"][other_values] < 2.0).all() and other_values.sum() > 500
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=NAMES)
+def test_muon_captured(enc, dtype):  # noqa: F811
+    """A captured step, replayed with other gradients and eager work between, gives the eager steps' bits."""
+    g = _gen(9)
+    grads = [_randn(g, 30, 50, dtype=dtype) for _ in range(8)]
+    start = _randn(g, 30, 50, dtype=dtype)
+
+    def made():
+        p = torch.nn.Parameter(start.clone())
+        p.grad = grads[0].clone()
+        return p, enc.Muon([p], lr=1e-4, weight_decay=0.01)
+
+    p, eager = made()
+    q, captured = made()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        captured.step()
+    torch.cuda.current_stream().wait_stream(side)
+    eager.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured.step()
+    for grad in grads[1:]:
+        q.grad.copy_(grad)
+        graph.replay()
+        torch.cuda.synchronize()
+        p.grad.copy_(grad)
+        eager.step()
+        assert torch.equal(p, q)
+        for key, value in eager.state[p].items():
+            assert torch.equal(value, captured.state[q][key]), key
+
+
+def test_muon_state_of_other_types(enc):  # noqa: F811
+    """A state saved with a 16-bit momentum, or for weights of another type, is taken in the weight's state type."""
+    g = _gen(10)
+    for dtype, saved_type in ((torch.bfloat16, torch.bfloat16), (torch.float16, torch.float32), (torch.float32, torch.bfloat16)):
+        p = torch.nn.Parameter(_randn(g, 12, 18, dtype=dtype))
+        opt = enc.Muon([p])
+        m = _randn(g, 12, 18, dtype=saved_type)
+        opt.load_state_dict({"state": {0: {"momentum": m}}, "param_groups": opt.state_dict()["param_groups"]})
+        kept = opt.state[p]["momentum"]
+        assert kept.dtype == torch.float32 and torch.equal(kept, m.float())
+        p.grad = torch.zeros_like(p)
+        opt.step()
+        assert torch.equal(opt.state[p]["momentum"], m.float() * 0.95) and m.dtype == saved_type

@@ -200,7 +200,11 @@ class Muon(torch.optim.Optimizer):
         saved = [k for group in state_dict["param_groups"] for k in group["params"]]
         for k, p in zip(saved, (p for group in self.param_groups for p in group["params"])):
             for name, value in state_dict["state"].get(k, {}).items():
-                self.state[p][name] = value.to(device=p.device, copy=True)
+                self.state[p][name] = value.to(device=p.device, dtype=self._state_type(p), copy=True)
+
+    @staticmethod
+    def _state_type(p: torch.Tensor) -> torch.dtype:
+        return torch.float32 if p.dtype in (torch.float16, torch.bfloat16) else p.dtype
 
     @torch.no_grad()
     def step(self, closure: Any = None) -> Any:  # pylint: disable=arguments-differ
@@ -213,15 +217,16 @@ class Muon(torch.optim.Optimizer):
                 if p.grad is None:
                     continue
                 state = self.state[p]
-                short = p.dtype in (torch.float16, torch.bfloat16)
+                short = p.dtype != self._state_type(p)
                 weight, grad = p, p.grad
                 if "momentum" not in state:
-                    state["momentum"] = torch.zeros_like(p, dtype=torch.float32 if short else p.dtype)
+                    state["momentum"] = torch.zeros_like(p, dtype=self._state_type(p))
                 if short:
                     grad = grad.float()
-                    weight = state.get("weight")
-                    weight = p.float() if weight is None else torch.where(weight.to(p.dtype) == p, weight, p.float())
-                    state["weight"] = weight
+                    if "weight" not in state:
+                        state["weight"] = p.float()
+                    weight = state["weight"]  # written in place: a captured step's replays go on from it
+                    torch.where(weight.to(p.dtype) == p, weight, p.float(), out=weight)
                 m = state["momentum"].mul_(group["momentum"]).add_(grad)
                 update = torch.add(grad, m, alpha=group["momentum"]) if group["nesterov"] else m
                 update = orthogonalize(update, steps=group["steps"], coefficients=group["coefficients"])
