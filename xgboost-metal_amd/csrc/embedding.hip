@@ -13,8 +13,8 @@
 //
 // Measured (us, one MI355X, whose copies reach 5.1 TB/s): lookup 262,144 x 100
 // bfloat16 tokens of a table of 25,600 x 64 153, 8,191 rows of 1,024 6.2 (at the
-// copies' rate); gradient of 65,536 x 100 tokens 190 (sorts 88, sums 79, join 15,
-// windows 7), of 16,411 tokens and rows of 1,024 53, of 256 x 100 tokens 13.
+// copies' rate); gradient of 65,536 x 100 tokens 181 (sorts 88, sums 79, join 15,
+// windows 7), of 16,411 tokens and rows of 1,024 52, of 256 x 100 tokens 13.
 #include <type_traits>
 
 #include "encoder_common.hpp"

@@ -16,9 +16,9 @@
 // times rstd, 2^-13 where a row's spread is 2^12 ulps of its mean.
 //
 // Measured (us, one MI355X, whose copies reach 5.1 TB/s), with the bytes that
-// have to move: 65,536 x 1,024 bfloat16 forward 54 (5.0 TB/s), gradient 75 and the
-// joining of its column sums 5 (5.0 TB/s); 5,003 x 1,000 binary32 gradient 13 and
-// 3 (3.8 TB/s: the second launch, and eight waves a CU with 2.4 rows each); 16 x 32
+// have to move: 65,536 x 1,024 bfloat16 forward 54 (5.0 TB/s), gradient 74 and the
+// joining of its column sums 5 (5.1 TB/s); 5,003 x 1,000 binary32 gradient 13 and
+// 4 (3.6 TB/s: the second launch, and eight waves a CU with 2.4 rows each); 16 x 32
 // 1.9, a launch.
 #include <type_traits>
 

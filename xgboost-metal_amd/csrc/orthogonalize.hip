@@ -18,9 +18,10 @@
 // high, high by low, low by high; low by low is below binary32's rounding).
 // Sums are binary32.
 //
-// Measured (us, one MI355X): binary32 64 x 256 50 and 1,500 x 1,001 239, bfloat16
-// 2,048 x 4,096 882 to 940 (198 GFLOP, thrice in matrix instructions: 630 to 670
-// TFLOP/s of those, where a library's large product reaches 1,130).
+// Measured (us, one MI355X, a call among others and from a graph): binary32 64 x 256 51
+// and 1,500 x 1,001 252 and 224, bfloat16 2,048 x 4,096 943 and 881 (198 GFLOP, thrice in
+// matrix instructions: 630 to 670 TFLOP/s of those, where a library's large product
+// reaches 1,130).
 #include <cmath>
 #include <type_traits>
 #include <utility>
