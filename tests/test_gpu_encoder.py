@@ -736,3 +736,21 @@ def test_leaf_tokens_of_rounds(enc, xgb):
         tok = enc.LeafTokenizer(bst, (0, end))
         leaves = bst.predict(d, pred_leaf=True, iteration_range=(0, end)).reshape(300, -1)
         assert tok.trees == leaves.shape[1] and torch.equal(tok(d), whole[:, :tok.trees])
+
+
+def test_pooled_beyond_32_bit_offsets(enc):
+    """Rows of the table, and of the gradient, more than 4 GB apart."""
+    rows, stride = 1100, 2_000_000
+    big = torch.zeros(rows, stride, device="cuda", dtype=torch.float16)  # 4.4 GB
+    g = _gen(11)
+    big[:, 5:45] = _randn(g, rows, 40, dtype=torch.float16)
+    weight = big[:, 5:45]
+    tokens = torch.randint(-1, rows + 1, (300, 17), generator=g, device="cuda")
+    tokens[0, 0] = rows - 1
+    want, size = _lookup64(weight, tokens, 0.5, True)
+    _near(enc.embedding_lookup(weight, tokens, scale=0.5, pool=True), want, size * 19 * E32)
+    # 200 tokens a row: more than one launch takes; and fewer, which one does.
+    for bag in (200, 10):
+        tokens = _tokens(g, (rows, bag), 700, torch.int32, 0.1)
+        want, size, count = _gradient64(weight, tokens, 700, 2.0, True)
+        _near(enc.embedding_gradient(weight, tokens, 700, scale=2.0, pool=True), want, size * (count + 1) * E32)
