@@ -754,3 +754,16 @@ def test_pooled_beyond_32_bit_offsets(enc):
         tokens = _tokens(g, (rows, bag), 700, torch.int32, 0.1)
         want, size, count = _gradient64(weight, tokens, 700, 2.0, True)
         _near(enc.embedding_gradient(weight, tokens, 700, scale=2.0, pool=True), want, size * (count + 1) * E32)
+
+
+@pytest.mark.parametrize("dim", [3, 100, 5000, 40001])
+def test_norm_statistics_of_infinite_rows(enc, dim):
+    """The mean of a row with infinities is what their sum is; rstd is not a number, nor is y."""
+    x = _randn(_gen(6), 5, dim)
+    inf = float("inf")
+    x[0, 1], x[1, 0], x[2, dim - 1] = inf, -inf, float("nan")
+    x[3, 0], x[3, 2] = inf, -inf
+    y, mean, rstd = enc.layer_norm(x)
+    assert mean[0].item() == inf and mean[1].item() == -inf and torch.isnan(mean[2:4]).all()
+    assert torch.isnan(rstd[:4]).all() and torch.isnan(y[:4]).all()
+    assert torch.isfinite(mean[4]) and torch.isfinite(y[4]).all()

@@ -67,6 +67,9 @@ __device__ __forceinline__ void row_sums(float& a, float& b, float* shared) {
 // values have to be centred anew.
 __device__ __forceinline__ bool far_off(float left, float square) { return 64.0f * left * left > square; }
 
+// (A row with an infinity keeps its infinite mean.)
+__device__ __forceinline__ float finite_or_zero(float v) { return fabsf(v) < INFINITY ? v : 0.0f; }
+
 // A lane's columns of a row: kPacks times kSize, a pack or, in rows narrower than
 // a pack, one.  The last pack of a row that is no whole number of packs begins
 // early, so that it ends with the row, and lanes beyond the row take that too:
@@ -134,7 +137,7 @@ __global__ __launch_bounds__(kLanes > kNormThreads ? kLanes : kNormThreads) void
       variance = fmaf(own, own, variance);
     }
   row_sums<kLanes>(left, variance, shared);
-  left /= (float)dim;
+  left = finite_or_zero(left / (float)dim);
   variance /= (float)dim;
   mean += left;
   if (far_off(left, variance)) {  // the same for all lanes of a row
@@ -197,7 +200,7 @@ __global__ __launch_bounds__(1024) void k_norm_wide(T* __restrict__ y, float* __
     }
   }
   block_sums<1024>(left, variance, shared);
-  left /= (float)dim;
+  left = finite_or_zero(left / (float)dim);
   variance /= (float)dim;
   const float mean = first + left;
   if (far_off(left, variance)) {  // the same for all lanes
