@@ -518,6 +518,88 @@ int mgb_orthogonalize(void* out, const void* update, int64_t batch, int64_t rows
                       int64_t batch_stride, int steps, const float* coefficients, float eps, int dtype,
                       void* workspace, size_t workspace_bytes, void* stream);
 
+/* The gated feed-forward block: y = (act(x gate^T) * (x up^T)) down^T for `rows`
+ * rows of `dim` values, gate and up (hidden, dim), down (dim, hidden), all of
+ * dtype; y without gaps.  kept, NULL or (rows, 2, hidden) binary32, gets the
+ * rows' x gate^T, then x up^T, for the gradient.  The hidden values are rounded
+ * to dtype (as operands of the second product); sums are binary32.  Sides up to
+ * 2^20. */
+enum { MGB_SILU = 0, MGB_GELU = 1 };
+typedef struct {
+  void* y;
+  float* kept;
+  const void *x, *gate, *up, *down;
+  int64_t rows, dim, hidden, x_stride, gate_stride, up_stride, down_stride;
+  int activation, dtype;
+} MgbFeedForward;
+size_t mgb_feed_forward_workspace_bytes(const MgbFeedForward* p);
+int mgb_feed_forward(const MgbFeedForward* p, void* workspace, size_t workspace_bytes, void* stream);
+/* Its gradients from y's (`grad`) and what was kept: dx, dgate, dup and ddown,
+ * each without gaps, or NULL where it is not wanted. */
+typedef struct {
+  void *dx, *dgate, *dup, *ddown;
+  const void *grad, *x;
+  const float* kept;
+  const void *gate, *up, *down;
+  int64_t rows, dim, hidden, grad_stride, x_stride, gate_stride, up_stride, down_stride;
+  int activation, dtype;
+} MgbFeedForwardGradient;
+size_t mgb_feed_forward_gradient_workspace_bytes(const MgbFeedForwardGradient* p);
+int mgb_feed_forward_gradient(const MgbFeedForwardGradient* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rows in 8 bits: `blocks` blocks of 128 e4m3 values (a row's rest filled with
+ * zeros), `stride` bytes (a multiple of 16) from row to row, and for each block a
+ * byte of exponent + 127 of the power of two that its values are times, whole
+ * words a row, `scale_stride` bytes from row to row.  Values begin at 16 bytes,
+ * scales at 4. */
+typedef struct {
+  void *values, *scales;
+  int64_t rows, blocks, stride, scale_stride;
+} MgbBlocks;
+/* x (out->rows rows of dim values) so: the smallest power of two that takes a
+ * block's largest finite magnitude to at most 448, values rounded to nearest even;
+ * infinities and NaN become NaN. */
+int mgb_quantize_blocks(const MgbBlocks* out, const void* x, int64_t dim, int64_t x_stride, int dtype, void* stream);
+/* out (x.rows, weight.rows), without gaps, = x weight^T of what the blocks stand
+ * for.  Sums of 16-bit results in the 8-bit instructions' precision (about 1.5e-5 of
+ * the norm), of binary32 ones in binary32. */
+typedef struct {
+  void* out;
+  MgbBlocks x, weight;
+  int dtype;
+} MgbBlockMatmul;
+size_t mgb_block_matmul_workspace_bytes(const MgbBlockMatmul* p);
+int mgb_block_matmul(const MgbBlockMatmul* p, void* workspace, size_t workspace_bytes, void* stream);
+/* mgb_feed_forward with its matrices as blocks; x and the hidden values are
+ * rounded to blocks too.  gate and up must lie alike. */
+typedef struct {
+  void* y;
+  const void* x;
+  MgbBlocks gate, up, down;
+  int64_t rows, dim, hidden, x_stride;
+  int activation, dtype;
+} MgbBlockFeedForward;
+size_t mgb_block_feed_forward_workspace_bytes(const MgbBlockFeedForward* p);
+int mgb_block_feed_forward(const MgbBlockFeedForward* p, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Distillation from a teacher's largest logits: with q = softmax(logits / T) and p the
+ * softmax of values / T over a row's `top` (at most 1,024) entries whose index lies
+ * in [0, classes), loss = T^2 sum p (log p - log q at the index), 0 for a row
+ * without entries; lse = log sum exp(logits / T).  The gradient takes the loss's
+ * (`grad`, a value a row) and lse: dlogits (rows without gaps) = grad T (q - p). */
+typedef struct {
+  float *loss, *lse;
+  void* dlogits;
+  const float* grad;
+  const void *logits, *values, *indices;
+  int64_t rows, classes, top, stride, value_stride, index_stride, grad_stride;
+  float temperature;
+  int dtype, value_dtype, index_bytes;
+} MgbDistillation;
+size_t mgb_distillation_loss_workspace_bytes(const MgbDistillation* p);
+int mgb_distillation_loss(const MgbDistillation* p, void* workspace, size_t workspace_bytes, void* stream);
+int mgb_distillation_gradient(const MgbDistillation* p, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,340 @@
+// Products in 8 bits with a scale for each block of 128 values, and the encoder's
+// block served that way.
+//
+// A row's values are kept as e4m3 (4 bits of exponent, 3 of mantissa, up to 448), each
+// 128 of them times the smallest power of two that takes the largest to at most 448.
+// A power of two scales without rounding, is a byte, and is what the matrix
+// instruction applies by itself: a step of a product is one block, and its sums need
+// no other arithmetic.  Padding to whole blocks is zeros.
+//
+// The 8-bit instructions add a few products at a time with about 16 bits (1.5e-5 of
+// the norm for normal values, whatever the depth), which 16-bit results do not show.
+// Binary32 results, and the hidden values of a block in binary32 and binary16 (which
+// are rounded to e4m3 next: what crosses a border there shows), come of the bfloat16
+// instructions, which take e4m3 values with their scales exactly.
+#include "feed_forward.hpp"
+
+namespace mgb {
+namespace block {
+namespace {
+
+constexpr int kBlock = 128, kQuantThreads = 256, kQuantLanes = kBlock / 8;
+
+__device__ __forceinline__ float group_max16(float v) {
+  v = fmaxf(v, lane_move<0xb1>(v));
+  v = fmaxf(v, lane_move<0x4e>(v));
+  v = fmaxf(v, lane_move<0x141>(v));
+  return fmaxf(v, lane_move<0x140>(v));
+}
+
+// The exponent + 127 of the smallest power of two that takes `largest` to at most
+// 448 = 1.75 2^8; 127 where there is none.
+__device__ __forceinline__ uint32_t scale_of(float largest) {
+  const uint32_t bits = __float_as_uint(largest);
+  const int exponent = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return largest == 0.0f ? 127u : exponent > 0 ? (uint32_t)exponent : 0u;
+}
+
+// Eight values as e4m3, rounded to nearest even; infinities and NaN become its NaN.
+__device__ __forceinline__ uint2 round_eight(const float* v, float factor) {
+  int word[2] = {};
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    word[w] = __builtin_amdgcn_cvt_pk_fp8_f32(v[w * 4] * factor, v[w * 4 + 1] * factor, word[w], false);
+    word[w] = __builtin_amdgcn_cvt_pk_fp8_f32(v[w * 4 + 2] * factor, v[w * 4 + 3] * factor, word[w], true);
+  }
+  return {(uint32_t)word[0], (uint32_t)word[1]};
+}
+
+// 16 lanes a block of 128, 8 values a lane.
+template <typename T>
+__global__ __launch_bounds__(kQuantThreads) void k_quantize(uint8_t* __restrict__ values, uint8_t* __restrict__ scales,
+                                                            const T* __restrict__ x, int64_t rows, int64_t dim,
+                                                            int64_t stride, int64_t blocks, int64_t value_stride,
+                                                            int64_t scale_stride) {
+  const int64_t all = rows * blocks, step = (int64_t)gridDim.x * (kQuantThreads / kQuantLanes);
+  const int64_t step_rows = step / blocks, step_blocks = step % blocks;
+  const int lane = threadIdx.x % kQuantLanes;
+  int64_t at = (int64_t)blockIdx.x * (kQuantThreads / kQuantLanes) + threadIdx.x / kQuantLanes;
+  int64_t row = at / blocks, block = at % blocks;
+  for (; at < all; at += step) {
+    float v[8];
+    load_some<8>(x + row * stride, block * kBlock + lane * 8, dim, v);
+    float largest = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.0f);
+    const uint32_t scale = scale_of(group_max16(largest));
+    const uint2 word = round_eight(v, __uint_as_float((254u - scale) << 23));
+    __builtin_memcpy(__builtin_assume_aligned(values + row * value_stride + block * kBlock + lane * 8, 8), &word, 8);
+    if (lane == 0) scales[row * scale_stride + block] = (uint8_t)scale;
+    row += step_rows;
+    block += step_blocks;
+    if (block >= blocks) {
+      block -= blocks;
+      ++row;
+    }
+  }
+}
+
+template <typename T>
+void quantize(uint8_t* values, uint8_t* scales, const T* x, int64_t rows, int64_t dim, int64_t stride, int64_t value_stride,
+              int64_t scale_stride, hipStream_t stream) {
+  const int64_t blocks = (dim + kBlock - 1) / kBlock, each = kQuantThreads / kQuantLanes;
+  const int64_t groups = std::min<int64_t>((rows * blocks + each - 1) / each, 4096);
+  k_quantize<T><<<(uint32_t)groups, kQuantThreads, 0, stream>>>(values, scales, x, rows, dim, stride, blocks, value_stride,
+                                                                 scale_stride);
+}
+
+// What blocks stand for, as bfloat16, which has their bits and exponents.
+__global__ __launch_bounds__(kQuantThreads) void k_widen(__bf16* __restrict__ to, MgbBlocks m) {
+  const int64_t all = m.rows * m.blocks, step = (int64_t)gridDim.x * (kQuantThreads / kQuantLanes);
+  const int lane = threadIdx.x % kQuantLanes;
+  for (int64_t at = (int64_t)blockIdx.x * (kQuantThreads / kQuantLanes) + threadIdx.x / kQuantLanes; at < all; at += step) {
+    const int64_t row = at / m.blocks, block = at % m.blocks;
+    uint32_t word[2];
+    __builtin_memcpy(word, (const uint8_t*)m.values + row * m.stride + block * kBlock + lane * 8, 8);
+    const int exponent = (int)((const uint8_t*)m.scales)[row * m.scale_stride + block] - 127;
+    __bf16 v[8];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const auto low = __builtin_amdgcn_cvt_pk_f32_fp8((int)word[w], false);
+      const auto high = __builtin_amdgcn_cvt_pk_f32_fp8((int)word[w], true);
+      v[w * 4] = (__bf16)ldexpf(low[0], exponent);
+      v[w * 4 + 1] = (__bf16)ldexpf(low[1], exponent);
+      v[w * 4 + 2] = (__bf16)ldexpf(high[0], exponent);
+      v[w * 4 + 3] = (__bf16)ldexpf(high[1], exponent);
+    }
+    __builtin_memcpy(to + (row * m.blocks + block) * kBlock + lane * 8, v, sizeof(v));
+  }
+}
+
+Laid widen(Space& space, const MgbBlocks& m, hipStream_t stream, bool run) {
+  const int64_t width = m.blocks * kBlock * 2;
+  char* to = space.take(m.rows * width);
+  if (run) {
+    const int64_t each = kQuantThreads / kQuantLanes;
+    k_widen<<<(uint32_t)std::min<int64_t>((m.rows * m.blocks + each - 1) / each, 4096), kQuantThreads, 0, stream>>>(
+        (__bf16*)to, m);
+  }
+  return {to, width, 0};
+}
+
+product::Operand operand8(const MgbBlocks& m) {
+  return {{(const char*)m.values, nullptr}, {m.stride, m.stride}, 0, m.rows, m.blocks * kBlock};
+}
+
+// out = x weight^T.  The depth's steps are blocks, of which a workgroup holds the
+// scales of kScaleSteps.
+template <typename T>
+int multiply(T* out, const MgbBlocks& x, const MgbBlocks& weight, Space& space, hipStream_t stream, bool run) {
+  Params p = {};
+  p.jobs = 1;
+  p.sources = 1;
+  p.pairs = 1;
+  p.depth = x.blocks * kBlock;
+  p.job[0].out = out;
+  p.job[0].out_stride = weight.rows;
+  p.job[0].rows = x.rows;
+  p.job[0].columns = weight.rows;
+  const Size size = choose(p, false);
+  if constexpr (sizeof(T) == 4) {
+    const Laid left = widen(space, x, stream, run), right = widen(space, weight, stream, run);
+    p.job[0].left = operand(left, x.rows, p.depth);
+    p.job[0].right = operand(right, weight.rows, p.depth);
+    split_depth(p, size, space);
+    if (run) store_product<__bf16, T, false, false>(p, size, stream);
+  } else {
+    p.job[0].left = operand8(x);
+    p.job[0].right = operand8(weight);
+    p.left_scales = (const uint8_t*)x.scales;
+    p.right_scales[0] = (const uint8_t*)weight.scales;
+    p.left_scale_stride = x.scale_stride;
+    p.right_scale_stride = weight.scale_stride;
+    split_depth(p, size, space, kBlock, product::kScaleSteps);
+    if (run) store_product<product::E4m3, T, false, false>(p, size, stream);
+  }
+  return 0;
+}
+
+struct GatedFloat {
+  static constexpr bool kDual = true;
+  const Params& p;
+  __device__ __forceinline__ GatedFloat(const Params& params, const product::Job&, uint32_t) : p(params) {}
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, const float* gate, const float* up) const {
+    float h[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = activate<true>(gate[e], p.activation) * up[e];
+    product::store_eight((float*)p.hidden + m * p.hidden_stride, n, p.true_columns, h);
+  }
+};
+
+template <typename T>
+int serve(const MgbBlockFeedForward& a, Space& space, hipStream_t stream, bool run) {
+  const int64_t dim = a.gate.blocks * kBlock, hidden = a.down.blocks * kBlock;
+  const int64_t x_scales = (a.gate.blocks + 3) / 4 * 4, hidden_scales = (a.down.blocks + 3) / 4 * 4;
+  MgbBlocks x = {space.take(a.rows * dim), space.take(a.rows * x_scales), a.rows, a.gate.blocks, dim, x_scales};
+  if (run) quantize<T>((uint8_t*)x.values, (uint8_t*)x.scales, (const T*)a.x, a.rows, a.dim, a.x_stride, dim, x_scales, stream);
+  Params p = {};
+  p.jobs = 1;
+  p.sources = 1;
+  p.pairs = 1;
+  p.depth = dim;
+  p.true_columns = a.hidden;
+  p.hidden_stride = a.hidden;
+  p.hidden = space.take(a.rows * a.hidden * sizeof(float));
+  p.activation = a.activation;
+  p.job[0].rows = a.rows;
+  p.job[0].columns = a.hidden;
+  const Size size = choose(p, true);
+  if constexpr (std::is_same_v<T, __bf16>) {
+    p.job[0].left = operand8(x);
+    p.job[0].right = {{(const char*)a.gate.values, (const char*)a.up.values}, {a.gate.stride, a.up.stride}, 0, a.hidden, dim};
+    p.left_scales = (const uint8_t*)x.scales;
+    p.right_scales[0] = (const uint8_t*)a.gate.scales;
+    p.right_scales[1] = (const uint8_t*)a.up.scales;
+    p.left_scale_stride = x.scale_stride;
+    p.right_scale_stride = a.gate.scale_stride;
+    whole_depth(p, kBlock);
+    if (run) launch_product<product::E4m3, false, false, GatedFloat>(p, size, stream);
+  } else {
+    const Laid left = widen(space, x, stream, run);
+    const Laid gate = widen(space, a.gate, stream, run), up = widen(space, a.up, stream, run);
+    p.job[0].left = operand(left, a.rows, dim);
+    p.job[0].right = operands(gate, up, a.hidden, dim);
+    whole_depth(p);
+    if (run) launch_product<__bf16, false, false, GatedFloat>(p, size, stream);
+  }
+  MgbBlocks h = {space.take(a.rows * hidden), space.take(a.rows * hidden_scales), a.rows, a.down.blocks, hidden, hidden_scales};
+  if (run)
+    quantize<float>((uint8_t*)h.values, (uint8_t*)h.scales, (const float*)p.hidden, a.rows, a.hidden, a.hidden, hidden,
+                    hidden_scales, stream);
+  return multiply<T>((T*)a.y, h, a.down, space, stream, run);
+}
+
+template <class Call>
+int with_type(int dtype, const Call& call) {
+  switch (dtype) {
+    case MGB_F32: return call((float*)nullptr);
+    case MGB_F16: return call((_Float16*)nullptr);
+    case MGB_BF16: return call((__bf16*)nullptr);
+  }
+  set_error("blocks: types must be float32, float16 or bfloat16");
+  return -1;
+}
+
+int check_blocks(const MgbBlocks& m) {
+  MGB_REQUIRE(m.rows >= 0 && m.rows < kMostRows, "blocks: rows must be below 2^31");
+  MGB_REQUIRE(m.blocks >= 1 && m.blocks <= kMostSide / kBlock, "blocks: a row must have 1 to 8,192 blocks");
+  MGB_REQUIRE(m.stride >= m.blocks * kBlock && m.stride <= kMostSide && m.stride % 16 == 0,
+              "blocks: rows of values must be 16-byte multiples apart, at most 2^20");
+  MGB_REQUIRE(m.scale_stride >= (m.blocks + 3) / 4 * 4 && m.scale_stride % 4 == 0,
+              "blocks: rows of scales must be whole words");
+  MGB_REQUIRE((uintptr_t)m.values % 16 == 0 && (uintptr_t)m.scales % 4 == 0, "blocks: values must begin at 16 bytes, scales at 4");
+  return 0;
+}
+
+int check_matmul(const MgbBlockMatmul* a) {
+  MGB_REQUIRE(a, "block matmul: null pointer");
+  if (check_blocks(a->x) || check_blocks(a->weight)) return -1;
+  MGB_REQUIRE(a->x.blocks == a->weight.blocks, "block matmul: both must have the same blocks a row");
+  MGB_REQUIRE(a->weight.rows <= kMostSide, "block matmul: a weight must have at most 2^20 rows");
+  MGB_REQUIRE(a->dtype >= MGB_F32 && a->dtype <= MGB_BF16, "block matmul: types must be float32, float16 or bfloat16");
+  return 0;
+}
+
+int check_serve(const MgbBlockFeedForward* a) {
+  MGB_REQUIRE(a, "block feed forward: null pointer");
+  if (check_blocks(a->gate) || check_blocks(a->up) || check_blocks(a->down)) return -1;
+  MGB_REQUIRE(a->rows >= 0 && a->rows < kMostRows, "block feed forward: rows must be below 2^31");
+  MGB_REQUIRE(a->dim >= 1 && a->hidden >= 1 && a->dim <= kMostSide && a->hidden <= kMostSide,
+              "block feed forward: a matrix' sides must be 1 to 2^20");
+  MGB_REQUIRE(a->gate.rows == a->hidden && a->up.rows == a->hidden && a->down.rows == a->dim &&
+                  a->gate.blocks == (a->dim + kBlock - 1) / kBlock && a->up.blocks == a->gate.blocks &&
+                  a->down.blocks == (a->hidden + kBlock - 1) / kBlock,
+              "block feed forward: the matrices' sizes do not fit");
+  MGB_REQUIRE(a->gate.stride == a->up.stride && a->gate.scale_stride == a->up.scale_stride,
+              "block feed forward: gate and up must lie alike");
+  MGB_REQUIRE(a->gate.blocks <= product::kScaleSteps || a->dtype != MGB_BF16,
+              "block feed forward: rows of bfloat16 must be at most 8,192 wide");
+  MGB_REQUIRE(a->activation == MGB_SILU || a->activation == MGB_GELU, "block feed forward: activation must be silu or gelu");
+  MGB_REQUIRE(a->dtype >= MGB_F32 && a->dtype <= MGB_BF16, "block feed forward: types must be float32, float16 or bfloat16");
+  MGB_REQUIRE(a->x_stride < (int64_t(1) << 40) && a->x_stride > -(int64_t(1) << 40), "block feed forward: row stride out of range");
+  return 0;
+}
+
+}  // namespace
+}  // namespace block
+}  // namespace mgb
+
+using namespace mgb;
+
+extern "C" {
+
+int mgb_quantize_blocks(const MgbBlocks* out, const void* x, int64_t dim, int64_t x_stride, int dtype, void* stream) {
+  MGB_REQUIRE(out, "quantize blocks: null pointer");
+  if (block::check_blocks(*out)) return -1;
+  MGB_REQUIRE(dim >= 1 && out->blocks == (dim + block::kBlock - 1) / block::kBlock,
+              "quantize blocks: a row's blocks must hold its values");
+  MGB_REQUIRE(x_stride < (int64_t(1) << 40) && x_stride > -(int64_t(1) << 40), "quantize blocks: row stride out of range");
+  MGB_REQUIRE(dtype >= MGB_F32 && dtype <= MGB_BF16, "quantize blocks: types must be float32, float16 or bfloat16");
+  if (out->rows == 0) return 0;
+  MGB_REQUIRE(out->values && out->scales && x, "quantize blocks: null pointer");
+  return block::with_type(dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    block::quantize<T>((uint8_t*)out->values, (uint8_t*)out->scales, (const T*)x, out->rows, dim, x_stride, out->stride,
+                       out->scale_stride, (hipStream_t)stream);
+    MGB_LAUNCH_CHECK("quantize blocks");
+    return 0;
+  });
+}
+
+size_t mgb_block_matmul_workspace_bytes(const MgbBlockMatmul* a) {
+  if (block::check_matmul(a) || a->x.rows == 0 || a->weight.rows == 0) return 0;
+  block::Space space = {};
+  block::with_type(a->dtype, [&](auto* t) { return block::multiply(t, a->x, a->weight, space, nullptr, false); });
+  return space.used;
+}
+
+int mgb_block_matmul(const MgbBlockMatmul* a, void* workspace, size_t workspace_bytes, void* stream) {
+  if (block::check_matmul(a)) return -1;
+  if (a->x.rows == 0 || a->weight.rows == 0) return 0;
+  const size_t need = mgb_block_matmul_workspace_bytes(a);
+  MGB_REQUIRE(a->out && a->x.values && a->x.scales && a->weight.values && a->weight.scales && (workspace || need == 0),
+              "block matmul: null pointer");
+  MGB_REQUIRE(workspace_bytes >= need, "block matmul: workspace too small");
+  MGB_REQUIRE((uintptr_t)workspace % 256 == 0, "block matmul: the workspace must begin at 256 bytes");
+  block::Space space = {(char*)workspace, 0};
+  return block::with_type(a->dtype, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    if (block::multiply((T*)a->out, a->x, a->weight, space, (hipStream_t)stream, true)) return -1;
+    MGB_LAUNCH_CHECK("block matmul");
+    return 0;
+  });
+}
+
+size_t mgb_block_feed_forward_workspace_bytes(const MgbBlockFeedForward* a) {
+  if (block::check_serve(a) || a->rows == 0) return 0;
+  block::Space space = {};
+  block::with_type(a->dtype, [&](auto* t) {
+    return block::serve<std::remove_pointer_t<decltype(t)>>(*a, space, nullptr, false);
+  });
+  return space.used;
+}
+
+int mgb_block_feed_forward(const MgbBlockFeedForward* a, void* workspace, size_t workspace_bytes, void* stream) {
+  if (block::check_serve(a)) return -1;
+  if (a->rows == 0) return 0;
+  MGB_REQUIRE(a->y && a->x && a->gate.values && a->gate.scales && a->up.values && a->up.scales && a->down.values &&
+                  a->down.scales && workspace,
+              "block feed forward: null pointer");
+  MGB_REQUIRE(workspace_bytes >= mgb_block_feed_forward_workspace_bytes(a), "block feed forward: workspace too small");
+  MGB_REQUIRE((uintptr_t)workspace % 256 == 0, "block feed forward: the workspace must begin at 256 bytes");
+  block::Space space = {(char*)workspace, 0};
+  return block::with_type(a->dtype, [&](auto* t) {
+    if (block::serve<std::remove_pointer_t<decltype(t)>>(*a, space, (hipStream_t)stream, true)) return -1;
+    MGB_LAUNCH_CHECK("block feed forward");
+    return 0;
+  });
+}
+
+}  // extern "C"

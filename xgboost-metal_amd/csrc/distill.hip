@@ -1,0 +1,353 @@
+// Distillation: a row's loss is how far its logits z are from a teacher's largest
+// ones, given as values t_j at columns i_j:
+//   q = softmax(z / T),  p = softmax over the given j of t / T,
+//   loss = T^2 sum_j p_j (log p_j - log q_{i_j}),  dz = grad T (q - p at the i_j).
+// An entry whose column lies outside the row is absent; a row without entries has
+// loss and gradient 0.  Entries of the same column add up.
+//
+// Bound by memory: the loss reads z once, with the running largest value and sum of a
+// softmax in each lane; the gradient reads it once and writes dz.  Sums are binary32.
+#include <algorithm>
+
+#include "encoder_common.hpp"
+
+namespace mgb {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr float kLog2e = 1.44269504f, kLowest = -3.40282347e38f;
+constexpr int64_t kMostClasses = int64_t(1) << 31;
+
+struct Teacher {
+  const void* values;
+  const void* indices;
+  int64_t count, value_stride, index_stride;
+  int value_type, index_bytes;
+
+  __device__ __forceinline__ float value(int64_t row, int64_t j) const {
+    const int64_t at = row * value_stride + j;
+    switch (value_type) {
+      case MGB_F32: return ((const float*)values)[at];
+      case MGB_F16: return (float)((const _Float16*)values)[at];
+      default: return (float)((const __bf16*)values)[at];
+    }
+  }
+  __device__ __forceinline__ int64_t column(int64_t row, int64_t j) const {
+    const int64_t at = row * index_stride + j;
+    return index_bytes == 4 ? ((const int32_t*)indices)[at] : ((const int64_t*)indices)[at];
+  }
+};
+
+// The running largest value and the sum of exp((v - largest) / T).
+struct Running {
+  float largest, sum;
+  __device__ __forceinline__ void join(float other_largest, float other_sum, float c) {
+    const float most = fmaxf(largest, other_largest);
+    sum = sum * __builtin_amdgcn_exp2f((largest - most) * c) + other_sum * __builtin_amdgcn_exp2f((other_largest - most) * c);
+    largest = most;
+  }
+};
+
+template <int kLanes>
+__device__ __forceinline__ Running join_lanes(Running r, float c, Running* shared) {
+#pragma unroll
+  for (int d = (kLanes < kWave ? kLanes : kWave) / 2; d > 0; d /= 2) r.join(__shfl_xor(r.largest, d, kWave), __shfl_xor(r.sum, d, kWave), c);
+  if constexpr (kLanes > kWave) {
+    __syncthreads();
+    if (threadIdx.x % kWave == 0) shared[threadIdx.x / kWave] = r;
+    __syncthreads();
+    r = shared[0];
+#pragma unroll
+    for (int w = 1; w < kLanes / kWave; ++w) r.join(shared[w].largest, shared[w].sum, c);
+  }
+  return r;
+}
+
+template <int kLanes>
+__device__ __forceinline__ float sum_lanes(float v, float* shared) {
+  if constexpr (kLanes <= kWave) return group_sum<kLanes>(v);
+  else return block_sum<kLanes>(v, shared);
+}
+
+// The teacher's largest value and sum, over the lanes of a row.
+template <int kLanes>
+__device__ __forceinline__ Running teach(const Teacher& teacher, int64_t row, int64_t classes, int lane, float c, Running* shared) {
+  Running r = {kLowest, 0.0f};
+  for (int64_t j = lane; j < teacher.count; j += kLanes) {
+    const int64_t column = teacher.column(row, j);
+    if (column < 0 || column >= classes) continue;
+    const float v = teacher.value(row, j);
+    if (v == -INFINITY) continue;  // a probability of 0, as none
+    r.join(v, 1.0f, c);
+  }
+  return join_lanes<kLanes>(r, c, shared);
+}
+
+template <typename T, int kLanes>
+__device__ __forceinline__ Running sweep(const T* z, int64_t begin, int64_t end, int lane, float c) {
+  constexpr int kSize = Pack<T>::kSize, kAhead = 4;
+  Running r = {kLowest, 0.0f};
+  auto take = [&](const float* v) {
+    float most = r.largest;
+#pragma unroll
+    for (int e = 0; e < kSize; ++e) most = fmaxf(most, v[e]);
+    float sum = r.sum * __builtin_amdgcn_exp2f((r.largest - most) * c);
+#pragma unroll
+    for (int e = 0; e < kSize; ++e) sum += __builtin_amdgcn_exp2f((v[e] - most) * c);
+    r = {most, sum};
+  };
+  int64_t at = begin + (int64_t)lane * kSize;
+  for (; at + (int64_t)(kAhead - 1) * kLanes * kSize + kSize <= end; at += (int64_t)kAhead * kLanes * kSize) {
+    Raw<T, kSize> raw[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) raw[k].load(z + at + (int64_t)k * kLanes * kSize);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      float v[kSize];
+      raw[k].get(v);
+      take(v);
+    }
+  }
+  for (; at < end; at += (int64_t)kLanes * kSize) {
+    float v[kSize];
+    load_pack(z, at, end, v);
+#pragma unroll
+    for (int e = 0; e < kSize; ++e)
+      if (at + e >= end) v[e] = -INFINITY;
+    take(v);
+  }
+  return r;
+}
+
+// log sum exp(z / T), and the row's loss.
+template <typename T, int kLanes>
+__device__ __forceinline__ void finish_row(float* loss, float* lses, const T* z, const Teacher& teacher, Running r, int64_t row,
+                                           int64_t classes, int lane, float temperature, float c, Running* shared) {
+  const float inverse = 1.0f / temperature;
+  const float lse = fmaf(r.largest, inverse, logf(r.sum));
+  const Running t = teach<kLanes>(teacher, row, classes, lane, c, shared);
+  const float log_total = logf(t.sum);
+  float sum = 0.0f;
+  for (int64_t j = lane; j < teacher.count; j += kLanes) {
+    const int64_t column = teacher.column(row, j);
+    if (column < 0 || column >= classes) continue;
+    const float v = teacher.value(row, j);
+    if (v == -INFINITY) continue;
+    const float log_p = (v - t.largest) * inverse - log_total, p = expf(log_p);
+    if (p != 0.0f) sum = fmaf(p, log_p - ((float)z[column] * inverse - lse), sum);
+  }
+  sum = sum_lanes<kLanes>(sum, (float*)shared);
+  if (lane == 0) {
+    loss[row] = t.sum > 0.0f || t.sum != t.sum ? sum * temperature * temperature : 0.0f;
+    lses[row] = lse;
+  }
+}
+
+// A row by kLanes lanes; with `partial` a part of it, columns blockIdx.y each.
+template <typename T, int kLanes>
+__global__ __launch_bounds__(kThreads) void k_loss(float* __restrict__ loss, float* __restrict__ lses, Running* __restrict__ partial,
+                                                   const T* __restrict__ logits, Teacher teacher, int64_t rows, int64_t classes,
+                                                   int64_t stride, int64_t part, float temperature) {
+  __shared__ Running shared[kThreads / kWave];
+  const int lane = threadIdx.x % kLanes;
+  const int64_t row = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
+  if (row >= rows) return;  // (no barrier follows where a workgroup has several rows)
+  const float c = kLog2e / temperature;
+  const T* z = logits + row * stride;
+  const int64_t begin = (int64_t)blockIdx.y * part, end = begin + part < classes ? begin + part : classes;
+  const Running r = join_lanes<kLanes>(sweep<T, kLanes>(z, begin, end, lane, c), c, shared);
+  if (partial) {
+    if (lane == 0) partial[row * gridDim.y + blockIdx.y] = r;
+    return;
+  }
+  finish_row<T, kLanes>(loss, lses, z, teacher, r, row, classes, lane, temperature, c, shared);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kWave) void k_loss_join(float* __restrict__ loss, float* __restrict__ lses,
+                                                     const Running* __restrict__ partial, int parts, const T* __restrict__ logits,
+                                                     Teacher teacher, int64_t classes, int64_t stride, float temperature) {
+  const int lane = threadIdx.x;
+  const int64_t row = blockIdx.x;
+  const float c = kLog2e / temperature;
+  Running r = {kLowest, 0.0f};
+  for (int k = lane; k < parts; k += kWave) r.join(partial[row * parts + k].largest, partial[row * parts + k].sum, c);
+  r = join_lanes<kWave>(r, c, nullptr);
+  finish_row<T, kWave>(loss, lses, logits + row * stride, teacher, r, row, classes, lane, temperature, c, nullptr);
+}
+
+// dz of a part of a row: q everywhere, then the teacher's columns once more, by the
+// lane of a column's first entry.  The entries' columns and probabilities lie in LDS.
+struct Entry {
+  int32_t column;  // -1: absent
+  float p;
+};
+
+template <typename T, int kLanes>
+__global__ __launch_bounds__(kThreads) void k_loss_gradient(T* __restrict__ dz, const float* __restrict__ grad,
+                                                            const T* __restrict__ logits, const float* __restrict__ lses,
+                                                            Teacher teacher, int64_t rows, int64_t classes, int64_t grad_stride,
+                                                            int64_t stride, int64_t part, float temperature) {
+  extern __shared__ Entry all_entries[];
+  __shared__ Running shared[kThreads / kWave];
+  constexpr int kSize = Pack<T>::kSize;
+  const int lane = threadIdx.x % kLanes, count = (int)teacher.count;
+  const int64_t row = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
+  const bool there = row < rows;
+  if (kLanes > kWave && !there) return;
+  Entry* const entries = all_entries + threadIdx.x / kLanes * count;
+  const float inverse = 1.0f / temperature;
+  const int64_t begin = (int64_t)blockIdx.y * part, end = begin + part < classes ? begin + part : classes;
+  float factor = 0.0f, lse = 0.0f;
+  bool empty = true;
+  const T* z = logits;
+  T* out = dz;
+  auto slope = [&](float v) { return __builtin_amdgcn_exp2f(fmaf(v, inverse, -lse) * kLog2e); };
+  if (there) {
+    z = logits + row * stride;
+    out = dz + row * classes;
+    const Running t = teach<kLanes>(teacher, row, classes, lane, kLog2e / temperature, shared);
+    const float log_total = logf(t.sum);
+    for (int j = lane; j < count; j += kLanes) {
+      const int64_t column = teacher.column(row, j);
+      const float v = teacher.value(row, j);
+      const bool present = column >= 0 && column < classes && v != -INFINITY;
+      entries[j] = {present ? (int32_t)column : -1, present ? expf((v - t.largest) * inverse - log_total) : 0.0f};
+    }
+    empty = t.sum == 0.0f;
+    factor = grad[row * grad_stride] * temperature;
+    lse = lses[row];
+    for (int64_t at = begin + (int64_t)lane * kSize; at < end; at += (int64_t)kLanes * kSize) {
+      float v[kSize];
+      load_pack(z, at, end, v);
+#pragma unroll
+      for (int e = 0; e < kSize; ++e) v[e] = empty ? 0.0f : factor * slope(v[e]);
+      store_pack(out, at, end, v);
+    }
+  }
+  __syncthreads();
+  if (empty) return;
+  for (int j = lane; j < count; j += kLanes) {
+    const int32_t column = entries[j].column;
+    if (column < begin || column >= end) continue;
+    bool first = true;
+    float p = 0.0f;
+    for (int k = 0; k < count; ++k) {
+      const bool same = entries[k].column == column;
+      first = first && !(same && k < j);
+      p += same ? entries[k].p : 0.0f;
+    }
+    if (first) out[column] = (T)(factor * (slope((float)z[column]) - p));
+  }
+}
+
+struct Plan {
+  int lanes;       // of a row
+  int64_t parts, part;
+};
+
+// Rows of up to 2,048 columns by a wave, wider ones by a workgroup; where there are
+// few of those, in parts of at least 8,192 columns.
+Plan plan(int64_t rows, int64_t classes) {
+  Plan p = {classes <= 2048 ? kWave : kThreads, 1, classes};
+  if (p.lanes == kThreads && rows < 1024) {
+    p.parts = std::max<int64_t>(1, std::min((classes + 8191) / 8192, 1024 / std::max<int64_t>(rows, 1)));
+    p.part = ((classes + p.parts - 1) / p.parts + 7) / 8 * 8;
+    p.parts = (classes + p.part - 1) / p.part;
+  }
+  return p;
+}
+
+int check_arguments(const MgbDistillation* a) {
+  MGB_REQUIRE(a, "distillation: null pointer");
+  MGB_REQUIRE(a->rows >= 0 && a->rows < (int64_t(1) << 31), "distillation: rows must be below 2^31");
+  MGB_REQUIRE(a->classes >= 1 && a->classes < kMostClasses, "distillation: a row must have 1 to 2^31 - 1 logits");
+  MGB_REQUIRE(a->top >= 0 && a->top <= 1024, "distillation: a teacher's row must have at most 1,024 entries");
+  MGB_REQUIRE(a->temperature > 0.0f && a->temperature < INFINITY, "distillation: the temperature must be positive");
+  MGB_REQUIRE(a->index_bytes == 4 || a->index_bytes == 8, "distillation: indices must be int32 or int64");
+  for (const int type : {a->dtype, a->value_dtype})
+    MGB_REQUIRE(type >= MGB_F32 && type <= MGB_BF16, "distillation: types must be float32, float16 or bfloat16");
+  for (const int64_t stride : {a->stride, a->value_stride, a->index_stride, a->grad_stride})
+    MGB_REQUIRE(stride < (int64_t(1) << 40) && stride > -(int64_t(1) << 40), "distillation: row stride out of range");
+  return 0;
+}
+
+Teacher teacher_of(const MgbDistillation& a) {
+  return {a.values, a.indices, a.top, a.value_stride, a.index_stride, a.value_dtype, a.index_bytes};
+}
+
+template <typename T>
+int loss(const MgbDistillation& a, void* workspace, hipStream_t stream) {
+  const Plan p = plan(a.rows, a.classes);
+  Running* partial = p.parts > 1 ? (Running*)workspace : nullptr;
+  const Teacher teacher = teacher_of(a);
+  const T* logits = (const T*)a.logits;
+  const dim3 grid((uint32_t)((a.rows * p.lanes + kThreads - 1) / kThreads), (uint32_t)p.parts);
+  if (p.lanes == kWave)
+    k_loss<T, kWave><<<grid, kThreads, 0, stream>>>(a.loss, a.lse, partial, logits, teacher, a.rows, a.classes, a.stride, p.part,
+                                                    a.temperature);
+  else
+    k_loss<T, kThreads><<<grid, kThreads, 0, stream>>>(a.loss, a.lse, partial, logits, teacher, a.rows, a.classes, a.stride, p.part,
+                                                       a.temperature);
+  if (partial)
+    k_loss_join<T><<<(uint32_t)a.rows, kWave, 0, stream>>>(a.loss, a.lse, partial, (int)p.parts, logits, teacher, a.classes,
+                                                           a.stride, a.temperature);
+  MGB_LAUNCH_CHECK("distillation loss");
+  return 0;
+}
+
+template <typename T>
+int gradient(const MgbDistillation& a, hipStream_t stream) {
+  const Plan p = plan(a.rows, a.classes);
+  const dim3 grid((uint32_t)((a.rows * p.lanes + kThreads - 1) / kThreads), (uint32_t)p.parts);
+  const uint32_t lds = (uint32_t)(kThreads / p.lanes * a.top * sizeof(Entry));
+  if (p.lanes == kWave)
+    k_loss_gradient<T, kWave><<<grid, kThreads, lds, stream>>>((T*)a.dlogits, a.grad, (const T*)a.logits, a.lse, teacher_of(a), a.rows,
+                                                             a.classes, a.grad_stride, a.stride, p.part, a.temperature);
+  else
+    k_loss_gradient<T, kThreads><<<grid, kThreads, lds, stream>>>((T*)a.dlogits, a.grad, (const T*)a.logits, a.lse, teacher_of(a),
+                                                                a.rows, a.classes, a.grad_stride, a.stride, p.part, a.temperature);
+  MGB_LAUNCH_CHECK("distillation gradient");
+  return 0;
+}
+
+}  // namespace
+}  // namespace mgb
+
+using namespace mgb;
+
+extern "C" {
+
+size_t mgb_distillation_loss_workspace_bytes(const MgbDistillation* a) {
+  if (check_arguments(a) || a->rows == 0) return 0;
+  const Plan p = plan(a->rows, a->classes);
+  return p.parts > 1 ? (size_t)a->rows * p.parts * sizeof(Running) : 0;
+}
+
+int mgb_distillation_loss(const MgbDistillation* a, void* workspace, size_t workspace_bytes, void* stream) {
+  if (check_arguments(a)) return -1;
+  if (a->rows == 0) return 0;
+  const size_t need = mgb_distillation_loss_workspace_bytes(a);
+  MGB_REQUIRE(a->loss && a->lse && a->logits && (a->top == 0 || (a->values && a->indices)) && (workspace || need == 0),
+              "distillation loss: null pointer");
+  MGB_REQUIRE(workspace_bytes >= need, "distillation loss: workspace too small");
+  switch (a->dtype) {
+    case MGB_F32: return loss<float>(*a, workspace, (hipStream_t)stream);
+    case MGB_F16: return loss<_Float16>(*a, workspace, (hipStream_t)stream);
+    default: return loss<__bf16>(*a, workspace, (hipStream_t)stream);
+  }
+}
+
+int mgb_distillation_gradient(const MgbDistillation* a, void* stream) {
+  if (check_arguments(a)) return -1;
+  if (a->rows == 0) return 0;
+  MGB_REQUIRE(a->dlogits && a->grad && a->lse && a->logits && (a->top == 0 || (a->values && a->indices)),
+              "distillation gradient: null pointer");
+  switch (a->dtype) {
+    case MGB_F32: return gradient<float>(*a, (hipStream_t)stream);
+    case MGB_F16: return gradient<_Float16>(*a, (hipStream_t)stream);
+    default: return gradient<__bf16>(*a, (hipStream_t)stream);
+  }
+}
+
+}  // extern "C"

@@ -7,11 +7,15 @@
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
+#include <cstring>
 #include <string>
+#include <utility>
+#include <vector>
 
 #include "mgb_kernels.h"
 
@@ -344,9 +348,360 @@ PyObject* orthogonalize(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+int activation_of(PyObject* object) {
+  const char* name = PyUnicode_Check(object) ? PyUnicode_AsUTF8(object) : nullptr;
+  if (PyErr_Occurred()) throw python_error();
+  if (name && !strcmp(name, "silu")) return MGB_SILU;
+  if (name && !strcmp(name, "gelu")) return MGB_GELU;
+  value_error("activation must be \"silu\" or \"gelu\"");
+}
+
+// The block's matrices, in x's type and on its device.
+struct Matrices {
+  Rows gate, up, down;
+  int64_t dim, hidden;
+};
+
+Matrices matrices_of(const Tensor& x, PyObject* const* args) {
+  if (x.dim() == 0 || x.size(-1) == 0) value_error("x must have a last axis, has shape " + text(x.sizes()));
+  const char* names[3] = {"gate", "up", "down"};
+  Tensor t[3];
+  for (int k = 0; k < 3; ++k) {
+    t[k] = tensor(names[k], args[k]);
+    dtype(names[k], t[k]);
+    if (t[k].scalar_type() != x.scalar_type())
+      type_error(std::string(names[k]) + " must be " + toString(x.scalar_type()) + " as x, is " +
+                 toString(t[k].scalar_type()));
+    same_device(x, names[k], t[k]);
+  }
+  const int64_t dim = x.size(-1), hidden = t[0].dim() == 2 ? t[0].size(0) : 0;
+  if (t[0].dim() != 2 || t[0].size(1) != dim || hidden == 0)
+    value_error("gate must have shape (hidden, " + std::to_string(dim) + "), has " + text(t[0].sizes()));
+  if (t[1].sizes() != t[0].sizes()) value_error("up must have shape " + text(t[0].sizes()) + ", has " + text(t[1].sizes()));
+  if (t[2].dim() != 2 || t[2].size(0) != dim || t[2].size(1) != hidden)
+    value_error("down must have shape (" + std::to_string(dim) + ", " + std::to_string(hidden) + "), has " +
+                text(t[2].sizes()));
+  return {rows_of(t[0]), rows_of(t[1]), rows_of(t[2]), dim, hidden};
+}
+
+at::IntArrayRef rows_shape(const Tensor& x) { return x.sizes().slice(0, x.dim() - 1); }
+
+// (x, gate, up, down, activation, keep)
+PyObject* feed_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments("feed_forward", n, 6);
+  const Tensor given = tensor("x", args[0]);
+  const int type = dtype("x", given);
+  const Matrices m = matrices_of(given, args + 1);
+  const int activation = activation_of(args[4]);
+  const bool keep = truth(args[5]);
+  const Rows x = rows_of(given);
+  const c10::DeviceGuard guard(given.device());
+  Tensor y = empty(given.sizes(), given.scalar_type(), given), kept;
+  if (keep) {
+    at::DimVector shape = with_dim(rows_shape(given), 2);
+    shape.push_back(m.hidden);
+    kept = empty(shape, at::kFloat, given);
+  }
+  const MgbFeedForward p = {y.data_ptr(), (float*)pointer(kept), x.t.data_ptr(), m.gate.t.data_ptr(), m.up.t.data_ptr(),
+                            m.down.t.data_ptr(), count(rows_shape(given)), m.dim, m.hidden, x.stride, m.gate.stride,
+                            m.up.stride, m.down.stride, activation, type};
+  const size_t need = mgb_feed_forward_workspace_bytes(&p);
+  const Tensor space = workspace(need, given);
+  check(mgb_feed_forward(&p, space.data_ptr(), need, stream_of(given)));
+  if (!keep) return THPVariable_Wrap(std::move(y));
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(y)), THPVariable_Wrap(std::move(kept)));
+  END_HANDLE_TH_ERRORS
+}
+
+// (grad, x, kept, gate, up, down, activation, which of the four are wanted)
+PyObject* feed_forward_gradient(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments("feed_forward_gradient", n, 8);
+  const Tensor g = tensor("grad", args[0]), given = tensor("x", args[1]);
+  const int type = dtype("x", given);
+  if (dtype("grad", g) != type || g.sizes() != given.sizes())
+    value_error(std::string("grad must be like x, ") + toString(given.scalar_type()) + " " + text(given.sizes()) +
+                ", is " + toString(g.scalar_type()) + " " + text(g.sizes()));
+  same_device(given, "grad", g);
+  const Matrices m = matrices_of(given, args + 3);
+  at::DimVector kept_shape = with_dim(rows_shape(given), 2);
+  kept_shape.push_back(m.hidden);
+  Tensor kept = tensor("kept", args[2]);
+  if (kept.scalar_type() != at::kFloat || kept.sizes() != at::IntArrayRef(kept_shape))
+    value_error("kept must be Float " + text(kept_shape) + ", is " + toString(kept.scalar_type()) + " " +
+                text(kept.sizes()));
+  same_device(given, "kept", kept);
+  if (!kept.is_contiguous()) kept = kept.contiguous();
+  const int activation = activation_of(args[6]);
+  const int64_t wanted = integer(args[7]);
+  const Rows x = rows_of(given), grad = rows_of(g);
+  const c10::DeviceGuard guard(given.device());
+  Tensor out[4];
+  if (wanted & 1) out[0] = empty(given.sizes(), given.scalar_type(), given);
+  if (wanted & 2) out[1] = empty({m.hidden, m.dim}, given.scalar_type(), given);
+  if (wanted & 4) out[2] = empty({m.hidden, m.dim}, given.scalar_type(), given);
+  if (wanted & 8) out[3] = empty({m.dim, m.hidden}, given.scalar_type(), given);
+  const MgbFeedForwardGradient p = {pointer(out[0]), pointer(out[1]), pointer(out[2]), pointer(out[3]),
+                                    grad.t.data_ptr(), x.t.data_ptr(), (const float*)kept.data_ptr(),
+                                    m.gate.t.data_ptr(), m.up.t.data_ptr(), m.down.t.data_ptr(),
+                                    count(rows_shape(given)), m.dim, m.hidden, grad.stride, x.stride, m.gate.stride,
+                                    m.up.stride, m.down.stride, activation, type};
+  const size_t need = mgb_feed_forward_gradient_workspace_bytes(&p);
+  const Tensor space = workspace(need, given);
+  check(mgb_feed_forward_gradient(&p, space.data_ptr(), need, stream_of(given)));
+  PyObject* result = PyTuple_New(4);
+  if (!result) throw python_error();
+  for (int k = 0; k < 4; ++k) {
+    PyObject* item = Py_None;
+    if (out[k].defined()) item = THPVariable_Wrap(std::move(out[k]));
+    else Py_INCREF(item);
+    PyTuple_SET_ITEM(result, k, item);
+  }
+  return result;
+  END_HANDLE_TH_ERRORS
+}
+
+constexpr int64_t kBlock = 128;
+
+// (values, scales) as quantize_blocks gives them: whole blocks in 8 bits, their
+// scales in rows of whole words.  Others are laid out anew.
+struct Blocks {
+  Tensor values, scales;
+  MgbBlocks blocks;
+};
+
+Blocks blocks_of(const char* name, PyObject* values_object, PyObject* scales_object) {
+  Tensor values = tensor(name, values_object), scales = tensor(name, scales_object);
+  if (values.scalar_type() != at::kFloat8_e4m3fn)
+    type_error(std::string(name) + "'s values must be float8_e4m3fn, are " + toString(values.scalar_type()));
+  if (scales.scalar_type() != at::kFloat8_e8m0fnu)
+    type_error(std::string(name) + "'s scales must be float8_e8m0fnu, are " + toString(scales.scalar_type()));
+  if (!values.is_cuda()) value_error(std::string(name) + " must be on a GPU, is on " + values.device().str());
+  same_device(values, "its scales", scales);
+  if (values.dim() == 0 || values.size(-1) == 0 || values.size(-1) % kBlock)
+    value_error(std::string(name) + "'s values must be rows of whole blocks of 128, have shape " + text(values.sizes()));
+  const int64_t blocks = values.size(-1) / kBlock;
+  at::DimVector want(values.sizes().begin(), values.sizes().end());
+  want.back() = blocks;
+  if (scales.sizes() != at::IntArrayRef(want))
+    value_error(std::string(name) + "'s scales must have shape " + text(want) + ", have " + text(scales.sizes()));
+  Rows v = rows_of(values);
+  if (v.stride % 16 || v.stride < values.size(-1) || v.stride > (int64_t(1) << 20) || (uintptr_t)v.t.data_ptr() % 16)
+    v = {values.clone(at::MemoryFormat::Contiguous), values.size(-1)};
+  const int64_t rows = count(values.sizes().slice(0, values.dim() - 1)), words = (blocks + 3) / 4 * 4;
+  // Rows of scales: the view that quantize_blocks gives has whole words behind it.
+  bool well = scales.stride(-1) == 1 && (uintptr_t)scales.data_ptr() % 4 == 0;
+  int64_t step = words;
+  for (int64_t axis = scales.dim() - 2; axis >= 0 && well; --axis) {
+    well = scales.size(axis) <= 1 || scales.stride(axis) == step;
+    step *= scales.size(axis);
+  }
+  well = well && (scales.storage_offset() + rows * words) * (int64_t)scales.element_size() <= (int64_t)scales.storage().nbytes();
+  if (!well) {
+    at::DimVector wide(want);
+    wide.back() = words;
+    const c10::DeviceGuard guard(values.device());
+    Tensor copy = empty(wide, at::kFloat8_e8m0fnu, scales);
+    copy.narrow(-1, 0, blocks).copy_(scales);
+    scales = copy;
+  }
+  return {v.t, scales, {v.t.data_ptr(), scales.data_ptr(), rows, blocks, v.stride, words}};
+}
+
+// (x) -> values (..., whole blocks), scales (..., blocks)
+PyObject* quantize_blocks(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments("quantize_blocks", n, 1);
+  const Tensor given = tensor("x", args[0]);
+  const int type = dtype("x", given);
+  if (given.dim() == 0 || given.size(-1) == 0) value_error("x must have a last axis, has shape " + text(given.sizes()));
+  const Rows x = rows_of(given);
+  const int64_t dim = given.size(-1), blocks = (dim + kBlock - 1) / kBlock, words = (blocks + 3) / 4 * 4;
+  const c10::DeviceGuard guard(given.device());
+  Tensor values = empty(with_dim(rows_shape(given), blocks * kBlock), at::kFloat8_e4m3fn, given);
+  Tensor scales = empty(with_dim(rows_shape(given), words), at::kFloat8_e8m0fnu, given);
+  const MgbBlocks out = {values.data_ptr(), scales.data_ptr(), count(rows_shape(given)), blocks, blocks * kBlock, words};
+  check(mgb_quantize_blocks(&out, x.t.data_ptr(), dim, x.stride, type, stream_of(given)));
+  if (words != blocks) scales = scales.narrow(-1, 0, blocks);
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(values)), THPVariable_Wrap(std::move(scales)));
+  END_HANDLE_TH_ERRORS
+}
+
+at::ScalarType result_type(PyObject* object, int* code) {
+  if (!THPDtype_Check(object)) type_error(std::string("dtype must be a torch.dtype, got ") + Py_TYPE(object)->tp_name);
+  const at::ScalarType type = reinterpret_cast<THPDtype*>(object)->scalar_type;
+  switch (type) {
+    case at::kFloat: *code = MGB_F32; break;
+    case at::kHalf: *code = MGB_F16; break;
+    case at::kBFloat16: *code = MGB_BF16; break;
+    default: type_error(std::string("dtype must be float32, float16 or bfloat16, is ") + toString(type));
+  }
+  return type;
+}
+
+// (x values, x scales, weight values, weight scales, dtype)
+PyObject* block_matmul(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments("block_matmul", n, 5);
+  int type = 0;
+  const at::ScalarType result = result_type(args[4], &type);
+  const Blocks x = blocks_of("x", args[0], args[1]), weight = blocks_of("weight", args[2], args[3]);
+  same_device(x.values, "weight", weight.values);
+  if (weight.values.dim() != 2) value_error("weight must be a matrix, has shape " + text(weight.values.sizes()));
+  if (x.blocks.blocks != weight.blocks.blocks)
+    value_error("x and weight must have rows of as many blocks, have " + std::to_string(x.blocks.blocks) + " and " +
+                std::to_string(weight.blocks.blocks));
+  const c10::DeviceGuard guard(x.values.device());
+  Tensor out = empty(with_dim(rows_shape(x.values), weight.blocks.rows), result, x.values);
+  const MgbBlockMatmul p = {out.data_ptr(), x.blocks, weight.blocks, type};
+  const size_t need = mgb_block_matmul_workspace_bytes(&p);
+  const Tensor space = workspace(need, x.values);
+  check(mgb_block_matmul(&p, space.data_ptr(), need, stream_of(x.values)));
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
+// (x, gate values, scales, up values, scales, down values, scales, activation)
+PyObject* block_feed_forward(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments("block_feed_forward", n, 8);
+  const Tensor given = tensor("x", args[0]);
+  const int type = dtype("x", given);
+  if (given.dim() == 0 || given.size(-1) == 0) value_error("x must have a last axis, has shape " + text(given.sizes()));
+  const char* names[3] = {"gate", "up", "down"};
+  std::vector<Blocks> m;
+  for (int k = 0; k < 3; ++k) {
+    m.push_back(blocks_of(names[k], args[1 + 2 * k], args[2 + 2 * k]));
+    same_device(given, names[k], m[k].values);
+    if (m[k].values.dim() != 2)
+      value_error(std::string(names[k]) + " must be a matrix, has shape " + text(m[k].values.sizes()));
+  }
+  const int64_t dim = given.size(-1), hidden = m[0].blocks.rows;
+  const int64_t blocks = (dim + kBlock - 1) / kBlock, hidden_blocks = (hidden + kBlock - 1) / kBlock;
+  if (hidden == 0 || m[0].blocks.blocks != blocks)
+    value_error("gate must have rows of " + std::to_string(blocks) + " blocks, has shape " + text(m[0].values.sizes()));
+  if (m[1].values.sizes() != m[0].values.sizes())
+    value_error("up must have shape " + text(m[0].values.sizes()) + ", has " + text(m[1].values.sizes()));
+  if (m[2].blocks.rows != dim || m[2].blocks.blocks != hidden_blocks)
+    value_error("down must have " + std::to_string(dim) + " rows of " + std::to_string(hidden_blocks) +
+                " blocks, has shape " + text(m[2].values.sizes()));
+  if (m[0].blocks.stride != m[1].blocks.stride)
+    for (int k = 0; k < 2; ++k)
+      if (m[k].blocks.stride != m[k].values.size(-1)) {
+        m[k].values = m[k].values.clone(at::MemoryFormat::Contiguous);
+        m[k].blocks.values = m[k].values.data_ptr();
+        m[k].blocks.stride = m[k].values.size(-1);
+      }
+  const int activation = activation_of(args[7]);
+  const Rows x = rows_of(given);
+  const c10::DeviceGuard guard(given.device());
+  Tensor y = empty(given.sizes(), given.scalar_type(), given);
+  const MgbBlockFeedForward p = {y.data_ptr(), x.t.data_ptr(), m[0].blocks, m[1].blocks, m[2].blocks,
+                                 count(rows_shape(given)), dim, hidden, x.stride, activation, type};
+  const size_t need = mgb_block_feed_forward_workspace_bytes(&p);
+  const Tensor space = workspace(need, given);
+  check(mgb_block_feed_forward(&p, space.data_ptr(), need, stream_of(given)));
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// Rows of logits and a teacher's entries for each.
+struct Distillation {
+  Rows logits, values, indices;
+  at::IntArrayRef rows;
+  MgbDistillation p;
+};
+
+Distillation distillation_of(const Tensor& logits, PyObject* values_object, PyObject* indices_object, PyObject* temperature) {
+  Distillation d = {};
+  const int type = dtype("logits", logits);
+  if (logits.dim() == 0 || logits.size(-1) == 0)
+    value_error("logits must have a last axis, have shape " + text(logits.sizes()));
+  const Tensor values = tensor("values", values_object), indices = tensor("indices", indices_object);
+  const int value_type = dtype("values", values);
+  if (indices.scalar_type() != at::kInt && indices.scalar_type() != at::kLong)
+    type_error(std::string("indices must be int32 or int64, are ") + toString(indices.scalar_type()));
+  same_device(logits, "values", values);
+  same_device(logits, "indices", indices);
+  d.rows = rows_shape(logits);
+  if (values.dim() != logits.dim() || rows_shape(values) != d.rows)
+    value_error("values must have shape " + text(d.rows) + " and a last axis for these logits, have " + text(values.sizes()));
+  if (indices.sizes() != values.sizes())
+    value_error("indices must have shape " + text(values.sizes()) + " as values, have " + text(indices.sizes()));
+  if (values.size(-1) > 1024)
+    value_error("a teacher's row must have at most 1,024 entries, has " + std::to_string(values.size(-1)));
+  const double t = real(temperature);
+  if (!((float)t > 0.0f && (float)t <= 3.4e38f)) value_error("temperature must be positive, is " + std::to_string(t));
+  d.logits = rows_of(logits);
+  d.values = rows_of(values);
+  d.indices = rows_of(indices);
+  d.p.logits = d.logits.t.data_ptr();
+  d.p.values = d.values.t.data_ptr();
+  d.p.indices = d.indices.t.data_ptr();
+  d.p.rows = count(d.rows);
+  d.p.classes = logits.size(-1);
+  d.p.top = values.size(-1);
+  d.p.stride = d.logits.stride;
+  d.p.value_stride = d.values.stride;
+  d.p.index_stride = d.indices.stride;
+  d.p.temperature = (float)t;
+  d.p.dtype = type;
+  d.p.value_dtype = value_type;
+  d.p.index_bytes = indices.scalar_type() == at::kInt ? 4 : 8;
+  return d;
+}
+
+// (logits, values, indices, temperature) -> loss, lse
+PyObject* distillation_loss(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments("distillation_loss", n, 4);
+  const Tensor given = tensor("logits", args[0]);
+  Distillation d = distillation_of(given, args[1], args[2], args[3]);
+  const c10::DeviceGuard guard(given.device());
+  Tensor loss = empty(d.rows, at::kFloat, given), lse = empty(d.rows, at::kFloat, given);
+  d.p.loss = (float*)loss.data_ptr();
+  d.p.lse = (float*)lse.data_ptr();
+  const size_t need = mgb_distillation_loss_workspace_bytes(&d.p);
+  const Tensor space = workspace(need, given);
+  check(mgb_distillation_loss(&d.p, space.data_ptr(), need, stream_of(given)));
+  return Py_BuildValue("(NN)", THPVariable_Wrap(std::move(loss)), THPVariable_Wrap(std::move(lse)));
+  END_HANDLE_TH_ERRORS
+}
+
+// (grad, logits, lse, values, indices, temperature)
+PyObject* distillation_gradient(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments("distillation_gradient", n, 6);
+  Tensor grad = tensor("grad", args[0]);
+  const Tensor given = tensor("logits", args[1]);
+  Tensor lse = tensor("lse", args[2]);
+  Distillation d = distillation_of(given, args[3], args[4], args[5]);
+  for (const auto& [name, t] : {std::pair<const char*, Tensor*>{"grad", &grad}, {"lse", &lse}}) {
+    if (t->scalar_type() != at::kFloat || t->sizes() != d.rows)
+      value_error(std::string(name) + " must be Float " + text(d.rows) + ", is " + toString(t->scalar_type()) + " " +
+                  text(t->sizes()));
+    same_device(given, name, *t);
+  }
+  if (!lse.is_contiguous()) lse = lse.contiguous();
+  // The gradient of a sum is one value for all rows.
+  d.p.grad_stride = grad.dim() == 1 ? grad.stride(0) : 1;
+  if (grad.dim() != 1 && !grad.is_contiguous()) grad = grad.contiguous();
+  const c10::DeviceGuard guard(given.device());
+  Tensor out = empty(given.sizes(), given.scalar_type(), given);
+  d.p.dlogits = out.data_ptr();
+  d.p.grad = (const float*)grad.data_ptr();
+  d.p.lse = (float*)lse.data_ptr();
+  check(mgb_distillation_gradient(&d.p, stream_of(given)));
+  return THPVariable_Wrap(std::move(out));
+  END_HANDLE_TH_ERRORS
+}
+
 #define ENTRY(fn) {#fn, (PyCFunction)(void (*)(void))fn, METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {ENTRY(lookup), ENTRY(lookup_gradient), ENTRY(norm), ENTRY(norm_gradient),
-                           ENTRY(orthogonalize), {nullptr, nullptr, 0, nullptr}};
+                           ENTRY(orthogonalize), ENTRY(feed_forward), ENTRY(feed_forward_gradient),
+                           ENTRY(quantize_blocks), ENTRY(block_matmul), ENTRY(block_feed_forward), ENTRY(distillation_loss),
+                           ENTRY(distillation_gradient), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_encoder", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1,0 +1,340 @@
+// What the block's forward and backward passes share (feed_forward.hip,
+// feed_forward_gradient.hip): the operands' layout, the plan of a product, the
+// activations.
+#pragma once
+#include <algorithm>
+#include <vector>
+
+#include "product.hpp"
+
+namespace mgb {
+namespace block {
+
+using product::Params;
+using product::float4v;
+
+constexpr int64_t kMostSide = int64_t(1) << 20, kMostRows = int64_t(1) << 31;
+
+// The matrix instructions' type for values of T, and the parts that hold one.
+// Binary32 values are three bfloat16, 24 bits (or 2^-134, where bfloat16's steps end),
+// whose products take six instructions; the type has binary32's range, so nothing is
+// scaled.
+template <typename T>
+struct Kind {
+  using E = T;
+  static constexpr int kParts = 1, kPairs = 1;
+};
+template <>
+struct Kind<float> {
+  using E = __bf16;
+  static constexpr int kParts = 3, kPairs = 6;
+};
+
+// v as the sum of three bfloat16.  What is not finite stays as it is in the first;
+// a value that would round to an infinity is cut instead.
+__device__ __forceinline__ void split_parts(float v, __bf16* part) {
+  __bf16 first = (__bf16)v;
+  if (!(fabsf((float)first) < INFINITY)) {
+    const uint32_t cut = __float_as_uint(v) & 0xffff0000u;
+    if (fabsf(v) < INFINITY) first = (__bf16)__uint_as_float(cut);
+  }
+  float rest = v - (float)first;
+  if (!(fabsf(rest) < INFINITY)) rest = 0.0f;
+  part[0] = first;
+  part[1] = (__bf16)rest;
+  part[2] = (__bf16)(rest - (float)part[1]);
+}
+
+// Workspace in pieces; without a base it counts.
+struct Space {
+  char* base;
+  size_t used;
+  char* take(size_t bytes) {
+    char* at = base ? base + used : nullptr;
+    used += (bytes + 255) / 256 * 256;
+    return at;
+  }
+};
+
+// ---- layout ------------------------------------------------------------------
+// The products load 16 bytes a lane, whole ones of a row.  16-bit matrices whose
+// rows begin at 16 bytes and hold whole ones are read where they lie; others are
+// copied with their rows padded with zeros, and binary32 ones split into parts.
+struct LayJob {
+  const void* from;
+  char* to;
+  int64_t rows, columns, stride, chunks, part;  // stride in elements, chunks of 8, part in bytes
+};
+constexpr int kMostLay = 5;
+struct LayJobs {
+  LayJob job[kMostLay];
+  int count;
+};
+
+constexpr int kLayThreads = 256;
+
+template <typename T>
+__global__ __launch_bounds__(kLayThreads) void k_lay_out(LayJobs jobs) {
+  using E = typename Kind<T>::E;
+  constexpr int kParts = Kind<T>::kParts;
+  const LayJob job = jobs.job[blockIdx.y];
+  const int64_t all = job.rows * job.chunks, step = (int64_t)gridDim.x * kLayThreads;
+  const int64_t step_rows = step / job.chunks, step_chunks = step % job.chunks;
+  int64_t at = (int64_t)blockIdx.x * kLayThreads + threadIdx.x, row = at / job.chunks, chunk = at % job.chunks;
+  for (; at < all; at += step) {
+    float v[8];
+    load_some<8>((const T*)job.from + row * job.stride, chunk * 8, job.columns, v);
+    E part[kParts][8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (kParts == 3) {
+        __bf16 three[3];
+        split_parts(v[e], three);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) part[q][e] = three[q];
+      } else {
+        part[0][e] = (E)v[e];
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kParts; ++q)
+      __builtin_memcpy(__builtin_assume_aligned(job.to + q * job.part + (row * job.chunks + chunk) * 16, 16), part[q], 16);
+    row += step_rows;
+    chunk += step_chunks;
+    if (chunk >= job.chunks) {
+      chunk -= job.chunks;
+      ++row;
+    }
+  }
+}
+
+// A matrix as a product takes it.
+struct Laid {
+  const char* data;
+  int64_t stride, part;  // bytes
+};
+
+inline int64_t padded(int64_t n) { return (n + 7) / 8 * 8; }
+
+template <typename T>
+bool lies_well(const void* data, int64_t rows, int64_t columns, int64_t stride) {
+  return sizeof(T) == 2 && columns % 8 == 0 && (uintptr_t)data % 16 == 0 &&
+         (rows <= 1 || (stride % 8 == 0 && stride >= columns && stride <= kMostSide));
+}
+
+template <typename T>
+Laid lay(Space& space, LayJobs& jobs, const void* data, int64_t rows, int64_t columns, int64_t stride, bool copy) {
+  if (!copy) return {(const char*)data, (rows > 1 ? stride : columns) * 2, 0};
+  const int64_t width = padded(columns) * 2, part = width * rows;
+  char* to = space.take(part * Kind<T>::kParts);
+  jobs.job[jobs.count++] = {data, to, rows, columns, stride, width / 16, part};
+  return {to, width, part};
+}
+
+template <typename T>
+Laid lay(Space& space, LayJobs& jobs, const void* data, int64_t rows, int64_t columns, int64_t stride) {
+  return lay<T>(space, jobs, data, rows, columns, stride, !lies_well<T>(data, rows, columns, stride));
+}
+
+template <typename T>
+void lay_out(const LayJobs& jobs, hipStream_t stream) {
+  int64_t most = 0;
+  for (int k = 0; k < jobs.count; ++k) most = std::max(most, jobs.job[k].rows * jobs.job[k].chunks);
+  if (most == 0) return;
+  const int64_t groups = std::min<int64_t>((most + kLayThreads - 1) / kLayThreads, 2048);
+  k_lay_out<T><<<dim3((uint32_t)groups, jobs.count), kLayThreads, 0, stream>>>(jobs);
+}
+
+// ---- a product's plan ----------------------------------------------------------
+enum Size { kLarge, kMedium, kSmall };
+inline int side(Size size) { return size == kLarge ? 256 : size == kMedium ? 128 : 64; }
+
+inline uint32_t lay_tiles(Params& p, Size size, bool dual) {
+  const int64_t m = side(size), n = dual ? m / 2 : m;
+  p.tiles = 0;
+  for (int j = 0; j < p.jobs; ++j) {
+    auto& job = p.job[j];
+    job.first_tile = p.tiles;
+    job.row_tiles = (uint32_t)((job.rows + m - 1) / m);
+    job.column_tiles = (uint32_t)((job.columns + n - 1) / n);
+    p.tiles += job.row_tiles * job.column_tiles;
+  }
+  return p.tiles;
+}
+
+inline int64_t steps_of(const Params& p, int values) {
+  return std::max<int64_t>(1, (p.depth + values - 1) / values) * p.pairs * p.sources;
+}
+
+// The size of the tiles: the largest that still gives most compute units one.
+inline Size choose(Params& p, bool dual) {
+  if (lay_tiles(p, kLarge, dual) >= 160) return kLarge;
+  if (lay_tiles(p, kMedium, dual) >= 160) return kMedium;
+  lay_tiles(p, kSmall, dual);
+  return kSmall;
+}
+
+// Shares of the depth, where there are few tiles: partial sums in binary32, added
+// in their order by k_join.
+inline void split_depth(Params& p, Size size, Space& space, int values = 64, int64_t most_steps = INT32_MAX) {
+  const int64_t steps = steps_of(p, values), groups = size == kLarge ? 256 : size == kMedium ? 512 : 1024;
+  int64_t splits = std::max<int64_t>(1, std::min(groups / p.tiles, steps / 8));
+  splits = std::max(splits, (steps + most_steps - 1) / most_steps);
+  p.steps_per_split = (uint32_t)((steps + splits - 1) / splits);
+  p.splits = (uint32_t)((steps + p.steps_per_split - 1) / p.steps_per_split);
+  p.partial_size = 0;
+  for (int j = 0; j < p.jobs; ++j) {
+    p.job[j].partial = p.partial_size;
+    p.partial_size += (p.job[j].rows * p.job[j].columns + 3) / 4 * 4;
+  }
+  p.partials = p.splits > 1 ? (float*)space.take(p.splits * p.partial_size * sizeof(float)) : nullptr;
+}
+
+inline void whole_depth(Params& p, int values = 64) {
+  p.splits = 1;
+  p.steps_per_split = (uint32_t)steps_of(p, values);
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_join(Params p) {
+  const product::Job& job = p.job[blockIdx.y];
+  const int64_t all = job.rows * job.columns, step = (int64_t)gridDim.x * 256 * 4;
+  T* out = (T*)job.out;
+  for (int64_t at = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; at < all; at += step) {
+    const float* from = p.partials + job.partial + at;
+    float4v sum = *(const float4v*)from;
+    for (uint32_t s = 1; s < p.splits; ++s) sum += *(const float4v*)(from + s * p.partial_size);
+    if (at + 4 <= all) {
+      T r[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) r[e] = (T)sum[e];
+      __builtin_memcpy(out + at, r, sizeof(r));
+    } else {
+      for (int e = 0; at + e < all; ++e) out[at + e] = (T)sum[e];
+    }
+  }
+}
+
+template <typename E, bool kLeftTurned, bool kRightTurned, class Finish>
+void launch_product(const Params& p, Size size, hipStream_t stream) {
+  const uint32_t groups = (p.tiles * p.splits + 7) / 8 * 8;
+  switch (size) {
+    case kLarge:
+      product::k_product<E, kLeftTurned, kRightTurned, product::Large, Finish>
+          <<<groups, product::Large::kThreads, 0, stream>>>(p);
+      break;
+    case kMedium:
+      product::k_product<E, kLeftTurned, kRightTurned, product::Medium, Finish>
+          <<<groups, product::Medium::kThreads, 0, stream>>>(p);
+      break;
+    case kSmall:
+      product::k_product<E, kLeftTurned, kRightTurned, product::Small, Finish>
+          <<<groups, product::Small::kThreads, 0, stream>>>(p);
+  }
+}
+
+// Products whose results are stored as they are, without gaps.
+template <typename E, typename T, bool kLeftTurned, bool kRightTurned>
+void store_product(const Params& p, Size size, hipStream_t stream) {
+  if (p.splits == 1) {
+    launch_product<E, kLeftTurned, kRightTurned, product::Store<T>>(p, size, stream);
+    return;
+  }
+  launch_product<E, kLeftTurned, kRightTurned, product::Partial>(p, size, stream);
+  int64_t most = 0;
+  for (int j = 0; j < p.jobs; ++j) most = std::max(most, p.job[j].rows * p.job[j].columns);
+  k_join<T><<<dim3((uint32_t)std::min<int64_t>((most + 1023) / 1024, 2048), p.jobs), 256, 0, stream>>>(p);
+}
+
+// ---- activations -----------------------------------------------------------------
+__device__ __forceinline__ float exp2_fast(float v) { return __builtin_amdgcn_exp2f(v); }
+__device__ __forceinline__ float inverse(float v) { return __builtin_amdgcn_rcpf(v); }
+
+// Both of 1 ulp, as is the exponent's rounding times |g|: silu is off by about
+// (|g| + 3) 2^-24 of itself.
+__device__ __forceinline__ float logistic(float g) { return inverse(1.0f + exp2_fast(g * -1.44269504f)); }
+
+// The normal distribution's function Phi(g), and exp(-g^2 / 2).  For z = |g| / sqrt(2)
+// and t = 1 / (1 + c z), Phi(-|g|) = exp(-z^2) t P(t) / 2, with P fitted to
+// t^-1 exp(z^2) erfc(z) by least squares, weighted until the relative error is even:
+// 7e-6 with six coefficients (16-bit results), 1.1e-8 with nine (binary32 results,
+// where the roundings are 4e-7 for g above -12).
+template <bool kExact>
+__device__ __forceinline__ float normal(float g, float* density) {
+  constexpr float kC = kExact ? 0.375f : 0.425f;
+  const float e = exp2_fast(g * g * -0.72134752f);
+  *density = e;
+  const float t = inverse(fmaf(fabsf(g), kC * 0.70710678f, 1.0f));
+  float poly;
+  if constexpr (kExact) {
+    poly = fmaf(t, 0.0616967715f, -0.288076133f);
+    poly = fmaf(t, poly, 0.43389535f);
+    poly = fmaf(t, poly, -0.231078207f);
+    poly = fmaf(t, poly, 0.274845332f);
+    poly = fmaf(t, poly, 0.121038452f);
+    poly = fmaf(t, poly, 0.205430552f);
+    poly = fmaf(t, poly, 0.210633487f);
+    poly = fmaf(t, poly, 0.211614415f);
+  } else {
+    poly = fmaf(t, -0.154950291f, 0.431325078f);
+    poly = fmaf(t, poly, -0.0336631872f);
+    poly = fmaf(t, poly, 0.288952172f);
+    poly = fmaf(t, poly, 0.227761433f);
+    poly = fmaf(t, poly, 0.2405819f);
+  }
+  const float tail = 0.5f * t * poly * e;
+  return g < 0.0f ? tail : 1.0f - tail;
+}
+
+template <bool kExact>
+__device__ __forceinline__ float activate(float g, int activation) {
+  if (activation == MGB_SILU) return g * logistic(g);
+  float density;
+  return g * normal<kExact>(g, &density);
+}
+
+// act(g), and its derivative.
+template <bool kExact>
+__device__ __forceinline__ float activate(float g, int activation, float* slope) {
+  if (activation == MGB_SILU) {
+    const float s = logistic(g);
+    *slope = s * fmaf(g, 1.0f - s, 1.0f);
+    return g * s;
+  }
+  float density;
+  const float phi = normal<kExact>(g, &density);
+  *slope = fmaf(g * density, 0.39894228f, phi);
+  return g * phi;
+}
+
+// Eight values of a row of the block's inner matrices, in parts.
+template <typename T>
+__device__ __forceinline__ void store_inner(char* matrix, int64_t part, int64_t at, const float* v) {
+  using E = typename Kind<T>::E;
+  constexpr int kParts = Kind<T>::kParts;
+  E eight[kParts][8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if constexpr (kParts == 3) {
+      __bf16 three[3];
+      split_parts(v[e], three);
+#pragma unroll
+      for (int q = 0; q < 3; ++q) eight[q][e] = three[q];
+    } else {
+      eight[0][e] = (E)v[e];
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < kParts; ++q)
+    __builtin_memcpy(__builtin_assume_aligned(matrix + (q * part + at) * 2, 16), eight[q], 16);
+}
+
+inline product::Operand operand(const Laid& m, int64_t extent, int64_t depth) {
+  return {{m.data, nullptr}, {m.stride, m.stride}, m.part, extent, depth};
+}
+inline product::Operand operands(const Laid& m, const Laid& second, int64_t extent, int64_t depth) {
+  return {{m.data, second.data}, {m.stride, second.stride}, m.part, extent, depth};
+}
+
+}  // namespace block
+}  // namespace mgb

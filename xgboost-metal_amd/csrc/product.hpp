@@ -1,0 +1,597 @@
+// Matrix products by tiles, result = sum over k of left(m, k) right(n, k), for the
+// encoder's block (feed_forward.hip) and its 8-bit products (blocks.hip).
+//
+// A workgroup has a tile of kTileM x kTileN.  A step of the depth is 128 bytes of
+// every row (64 16-bit values, 128 8-bit ones); its operands lie in LDS in four
+// regions, the upper and lower half of the tile's rows (A0, A1) and of its columns
+// (B0, B1), two steps of each.  A wave has a part of all four quarters and works a
+// step off in four phases, each one quarter:
+//   phase      reads into registers   multiplies   fills (from memory)
+//     0        A0 of this step        A0 B0        B0 of the step after the next
+//     1        B1                     A0 B1        A0
+//     2        A1                     A1 B1        B1
+//     3        B0 of the next step    A1 B0        A1
+// so a region is filled again in the phase after the one that read it, and has six
+// phases to arrive.  With eight waves, two a SIMD, the second four are half a phase
+// behind: while one wave of a SIMD multiplies, the other reads, and a barrier
+// between the halves keeps them so.
+//
+// An operand's rows either hold the depth without gaps ("straight"), or the depth
+// goes from row to row ("turned": the transpose of a matrix as it lies); turned ones
+// are transposed by the LDS reads that do so (ds_read_b64_tr_b16).  Chunks of 16
+// bytes are permuted within the LDS rows so that lanes that read together hit
+// different banks; as loads to LDS go to consecutive places, the lanes fetch their
+// chunks permuted.  Whatever lies outside an operand is read as zero by the bounds
+// of its buffer descriptor: rows beyond the last, and the depth's end inside a step.
+//
+// Measured (one MI355X): DESIGN has the cases; 8,192 x 4,096 x 4,096 bfloat16.
+#pragma once
+#include <type_traits>
+
+#include "encoder_common.hpp"
+
+namespace mgb {
+namespace product {
+
+using int4v = __attribute__((ext_vector_type(4))) int;
+using int8v = __attribute__((ext_vector_type(8))) int;
+using short4v = __attribute__((ext_vector_type(4))) short;
+using float4v = __attribute__((ext_vector_type(4))) float;
+using bf16x8 = __attribute__((ext_vector_type(8))) __bf16;
+using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
+using SharedBytes = __attribute__((address_space(3))) void*;
+
+struct E4m3 {};  // 8-bit values with a scale (a power of two, its exponent + 127) for each 128
+
+constexpr int kStepBytes = 128;
+constexpr int kScaleSteps = 64;  // of 8-bit operands, a workgroup's most
+
+// Binary32 values as three bfloat16 (24 bits) make six products; the three that
+// are left out are below 2^-24 of the largest.
+__host__ __device__ constexpr int left_part(int pair) { return (0x201100 >> (4 * pair)) & 15; }
+__host__ __device__ constexpr int right_part(int pair) { return (0x021010 >> (4 * pair)) & 15; }
+
+// One operand: up to two matrices whose products are added (`data[1]` may be null).
+struct Operand {
+  const char* data[2];
+  int64_t stride[2];   // bytes from row to row as they lie
+  int64_t part;        // bytes between the parts of binary32 values
+  int64_t extent;      // rows (straight), columns (turned) that there are
+  int64_t depth;       // values along the depth that there are; straight: whole chunks of 16 bytes
+};
+
+constexpr int kMostJobs = 3;
+struct Job {
+  Operand left, right;
+  void* out;
+  int64_t out_stride;  // elements
+  int64_t rows, columns;
+  int64_t partial;     // where its partial sums begin, elements
+  uint32_t row_tiles, column_tiles, first_tile;
+};
+
+struct Params {
+  Job job[kMostJobs];
+  int jobs;
+  int sources, pairs;
+  int64_t depth;             // the larger of the operands'
+  uint32_t tiles, splits, steps_per_split;
+  float* partials;           // [split][partial_size]
+  int64_t partial_size;
+  // 8-bit operands: a byte of exponent for each row and step, rows of whole words
+  const uint8_t* left_scales;
+  const uint8_t* right_scales[2];  // the second for the dual form
+  int64_t left_scale_stride, right_scale_stride;
+  // the block's epilogues
+  float* kept;               // [row][2][hidden], binary32, or null
+  char* hidden;              // act(gate) up, in parts
+  char* dgate;               // [2][row][stride], in parts: dgate, then dup
+  int64_t hidden_stride, hidden_part, gradient_part, gradient_second;  // elements
+  int64_t true_columns;      // columns of `kept`
+  int activation;
+};
+
+__device__ __forceinline__ void wait_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// vmcnt(n) lgkmcnt(0)
+template <int kLoads>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(kLoads < 64, "vmcnt");
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(0x70 | (kLoads & 15) | (kLoads >> 4) << 14);
+  asm volatile("" ::: "memory");
+}
+
+template <typename E>
+constexpr int element_bytes() { return std::is_same_v<E, E4m3> ? 1 : 2; }
+
+// A 16 x 16 tile's operand of one step: 32 bytes a lane.
+struct Fragment {
+  int8v v;
+  __device__ __forceinline__ int4v half(int h) const {
+    return h ? __builtin_shufflevector(v, v, 4, 5, 6, 7) : __builtin_shufflevector(v, v, 0, 1, 2, 3);
+  }
+};
+
+__device__ __forceinline__ void hold(Fragment& f) { asm volatile("" : "+v"(f.v)); }
+
+// sum[4 (lane / 16) + e of right][lane % 16 of left]
+template <typename E>
+__device__ __forceinline__ float4v multiply(const Fragment& left, const Fragment& right, float4v sum) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    if constexpr (std::is_same_v<E, __bf16>) {
+      sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, right.half(h)),
+                                                    __builtin_bit_cast(bf16x8, left.half(h)), sum, 0, 0, 0);
+    } else {
+      sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, right.half(h)),
+                                                   __builtin_bit_cast(f16x8, left.half(h)), sum, 0, 0, 0);
+    }
+  }
+  return sum;
+}
+
+// The scales' lowest bytes count.
+__device__ __forceinline__ float4v multiply8(const Fragment& left, const Fragment& right, int left_scale, int right_scale,
+                                             float4v sum) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(right.v, left.v, sum, 0, 0, 0, right_scale, 0, left_scale);
+}
+
+// A tile's shape: waves kWavesM x kWavesN; of each region's rows a wave has kRowsM or kRowsN.
+template <int kM, int kN, int kWM, int kWN>
+struct Tile {
+  static constexpr int kTileM = kM, kTileN = kN, kWavesM = kWM, kWavesN = kWN;
+  static constexpr int kWaves = kWM * kWN, kThreads = kWaves * kWave;
+  static constexpr int kHalfM = kM / 2, kHalfN = kN / 2;
+  static constexpr int kRowsM = kHalfM / kWM, kRowsN = kHalfN / kWN;
+  static constexpr int kTilesM = kRowsM / 16, kTilesN = kRowsN / 16;
+  static constexpr int kRegionM = kHalfM * kStepBytes, kRegionN = kHalfN * kStepBytes;
+  static constexpr int kLoadsM = kRegionM / (kThreads * 16), kLoadsN = kRegionN / (kThreads * 16);
+  static constexpr int kBytes = 4 * kRegionM + 4 * kRegionN;
+  static constexpr bool kAlternate = kWaves == 8;
+  static_assert(kLoadsM * kThreads * 16 == kRegionM && kLoadsN * kThreads * 16 == kRegionN, "whole loads");
+};
+using Large = Tile<256, 256, 2, 4>;
+using Medium = Tile<128, 128, 2, 2>;
+using Small = Tile<64, 64, 2, 2>;
+
+// The tile of a workgroup: an eighth of the workgroups (a chiplet's, which takes
+// every eighth) has a stretch of an order that goes by bands of kBand tile rows,
+// column by column, so that what a chiplet works on at one time shares operands.
+constexpr uint32_t kBand = 4;
+__device__ __forceinline__ bool find_tile(const Params& p, uint32_t* job, uint32_t* ti, uint32_t* tj, uint32_t* split) {
+  const uint32_t total = p.tiles * p.splits, each = (total + 7) / 8;
+  const uint32_t at = blockIdx.x % 8 * each + blockIdx.x / 8;
+  if (blockIdx.x / 8 >= each || at >= total) return false;
+  *split = at / p.tiles;
+  uint32_t tile = at % p.tiles, j = 0;
+  while (j + 1 < (uint32_t)p.jobs && tile >= p.job[j + 1].first_tile) ++j;
+  tile -= p.job[j].first_tile;
+  const uint32_t rows = p.job[j].row_tiles, columns = p.job[j].column_tiles;
+  const uint32_t band = tile / (kBand * columns), in = tile % (kBand * columns);
+  const uint32_t height = rows - band * kBand < kBand ? rows - band * kBand : kBand;
+  *job = j;
+  *ti = band * kBand + in % height;
+  *tj = in / height;
+  return true;
+}
+
+// What is read of an operand: a cursor that goes over its steps, the products of
+// the parts, and the matrices.  All of it is the same for a workgroup's lanes.
+template <bool kTurned, int kHalf, int kLoads, int kWaves>
+struct Reader {
+  const char* from[2];       // the regions' first rows, now
+  int64_t left[2];           // bytes from there to the end of what the region has
+  int64_t stride, depth;
+  uint32_t offset[kLoads];   // this lane's, from `from`
+  uint32_t chunk;            // straight: where in the step the lane's 16 bytes are
+
+  __device__ __forceinline__ void lanes(int64_t row_stride) {
+    const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q) {
+      if constexpr (!kTurned) {
+        const int row = (q * kWaves + wave) * 8 + lane / 8;
+        chunk = ((lane % 8) ^ (row & 7)) * 16;
+        offset[q] = (uint32_t)(row * row_stride) + chunk;
+      } else {
+        // A row of kHalf values is kHalf / 8 chunks.
+        constexpr int kChunks = kHalf / 8;
+        const int slot = (q * kWaves + wave) * kWave + lane, row = slot / kChunks, at = slot % kChunks;
+        offset[q] = (uint32_t)(row * row_stride) + ((at ^ (2 * (row & 7) % kChunks)) * 16);
+      }
+    }
+  }
+};
+
+// The exponents of the 8-bit operands' rows, of up to 64 steps: words of a step's
+// left rows, then of its right rows.
+template <typename S>
+struct Scales {
+  static constexpr int kWordsM = 2 * S::kTilesM / 4 > 0 ? 2 * S::kTilesM / 4 : 1;  // of a lane's rows
+  static constexpr int kWordsN = 2 * S::kTilesN / 4 > 0 ? 2 * S::kTilesN / 4 : 1;
+  static constexpr int kM = S::kWavesM * 16 * kWordsM, kN = S::kWavesN * 16 * kWordsN;
+  static constexpr int kBytes = (kM + kN) * 4;  // a step's
+
+  template <int kHalf, int kWaves, int kRows, int kTiles, int kWords>
+  static __device__ __forceinline__ int place(int row) {  // byte
+    const int half = row / kHalf, in = row % kHalf, wave = in / kRows, tile = in % kRows / 16;
+    const int byte = half * kTiles + tile;
+    return ((wave * 16 + in % 16) * kWords + byte / 4) * 4 + byte % 4;
+  }
+  static __device__ __forceinline__ void fill(char* panel, const Params& p, int64_t row0, int64_t rows, int64_t column0,
+                                              int64_t columns, bool dual, uint32_t begin, uint32_t end) {
+    const int quads = (int)(end - begin + 3) / 4;
+    for (int at = threadIdx.x; at < (S::kTileM + S::kTileN) * quads; at += S::kThreads) {
+      const int row = at / quads, quad = at % quads;
+      const uint8_t* from = nullptr;
+      int to;
+      if (row < S::kTileM) {
+        if (row0 + row < rows) from = p.left_scales + (row0 + row) * p.left_scale_stride;
+        to = place<S::kHalfM, S::kWavesM, S::kRowsM, S::kTilesM, kWordsM>(row);
+      } else {
+        const int r = row - S::kTileM;
+        const int64_t column = column0 + (dual ? r % S::kHalfN : r);
+        if (column < columns) from = p.right_scales[dual ? r / S::kHalfN : 0] + column * p.right_scale_stride;
+        to = kM * 4 + place<S::kHalfN, S::kWavesN, S::kRowsN, S::kTilesN, kWordsN>(r);
+      }
+      // (Rows are whole words: a word that begins in a row ends in it.)
+      const uint32_t word = from ? *(const uint32_t*)(from + begin + quad * 4) : 0x7f7f7f7fu;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (quad * 4 + e < (int)(end - begin)) panel[(quad * 4 + e) * kBytes + to] = (char)(word >> (8 * e));
+    }
+  }
+};
+
+template <typename E, bool kLeftTurned, bool kRightTurned, typename S, class Finish>
+__global__ __launch_bounds__(S::kThreads, 2) void k_product(Params p) {
+  constexpr bool k8 = std::is_same_v<E, E4m3>;
+  constexpr int kBytes = element_bytes<E>();
+  constexpr int kStep = kStepBytes / kBytes;  // elements
+  static_assert(!k8 || (!kLeftTurned && !kRightTurned), "8-bit operands lie straight");
+  __shared__ __attribute__((aligned(1024))) char lds[S::kBytes + (k8 ? Scales<S>::kBytes * kScaleSteps : 0)];
+
+  uint32_t which, ti, tj, split;
+  if (!find_tile(p, &which, &ti, &tj, &split)) return;
+  const Job& job = p.job[which];
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int wm = wave / S::kWavesN, wn = wave % S::kWavesN;
+
+  // ---- memory to LDS
+  Reader<kLeftTurned, S::kHalfM, S::kLoadsM, S::kWaves> left;
+  Reader<kRightTurned, S::kHalfN, S::kLoadsN, S::kWaves> right;
+  const int64_t row0 = (int64_t)ti * S::kTileM;
+  // The dual form has the columns of one matrix in B0 and the same ones of the other in B1.
+  const int64_t column0 = (int64_t)tj * (Finish::kDual ? S::kHalfN : S::kTileN);
+  left.depth = job.left.depth;
+  right.depth = job.right.depth;
+  const uint32_t each = p.depth > 0 ? (uint32_t)((p.depth + kStep - 1) / kStep) : 1;
+  const uint32_t all = each * p.pairs * p.sources;
+  const uint32_t begin = split * p.steps_per_split;
+  const uint32_t end = begin + p.steps_per_split < all ? begin + p.steps_per_split : all;
+
+  // The cursor: step k of the depth, of a product of parts, of a matrix.
+  uint32_t ahead = begin;  // the next step to fetch
+  uint32_t k = begin % each, pair = begin / each % p.pairs, source = begin / each / p.pairs;
+  auto place = [&] {
+    const int s = Finish::kDual ? 0 : source;
+    auto base = [&](const Operand& o, int matrix, int part) { return o.data[matrix] + part * o.part; };
+    left.stride = job.left.stride[s];
+    right.stride = job.right.stride[s];
+    const int lp = p.pairs > 1 ? left_part(pair) : 0, rp = p.pairs > 1 ? right_part(pair) : 0;
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const int64_t row = row0 + r * S::kHalfM;
+      if constexpr (!kLeftTurned) {
+        left.from[r] = base(job.left, s, lp) + row * left.stride + (int64_t)k * kStepBytes;
+        const int64_t rows = job.left.extent - row < S::kHalfM ? job.left.extent - row : S::kHalfM;
+        left.left[r] = rows > 0 ? (rows - 1) * left.stride + (left.depth * kBytes - (int64_t)k * kStepBytes) : 0;
+      } else {
+        left.from[r] = base(job.left, s, lp) + (int64_t)k * kStep * left.stride + row * kBytes;
+        left.left[r] = row < job.left.extent ? (job.left.extent - row) * kBytes : 0;
+      }
+      const int64_t column = column0 + (Finish::kDual ? 0 : r * S::kHalfN);
+      const int matrix = Finish::kDual ? r : s;
+      const int64_t stride = job.right.stride[matrix];
+      if constexpr (!kRightTurned) {
+        right.from[r] = base(job.right, matrix, rp) + column * stride + (int64_t)k * kStepBytes;
+        const int64_t rows = job.right.extent - column < S::kHalfN ? job.right.extent - column : S::kHalfN;
+        right.left[r] = rows > 0 ? (rows - 1) * stride + (right.depth * kBytes - (int64_t)k * kStepBytes) : 0;
+      } else {
+        right.from[r] = base(job.right, matrix, rp) + (int64_t)k * kStep * stride + column * kBytes;
+        right.left[r] = column < job.right.extent ? (job.right.extent - column) * kBytes : 0;
+      }
+    }
+  };
+  if (begin < end) place();
+  // (Both matrices of an operand lie at the same distance: the entries see to that.)
+  left.lanes(job.left.stride[0]);
+  right.lanes(job.right.stride[0]);
+  auto advance = [&] {
+    ++ahead;
+    if (++k < each) {
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        left.from[r] += kLeftTurned ? kStep * left.stride : kStepBytes;
+        right.from[r] += kRightTurned ? kStep * right.stride : kStepBytes;
+        if (!kLeftTurned && left.left[r] > 0) left.left[r] -= kStepBytes;
+        if (!kRightTurned && right.left[r] > 0) right.left[r] -= kStepBytes;
+      }
+    } else {
+      k = 0;
+      if (++pair == (uint32_t)p.pairs) {
+        pair = 0;
+        ++source;
+      }
+      if (ahead < end) place();
+    }
+  };
+  // Loads of steps beyond the last have an empty buffer: they read nothing and fill
+  // with zeros, and the count of loads in flight stays what the waits take it for.
+  auto fetch = [&](auto& reader, int r, char* to, auto turned, auto loads) {
+    int64_t bytes = reader.left[r];
+    if constexpr (decltype(turned)::value) {
+      const int64_t depth = reader.depth - (int64_t)k * kStep < kStep ? reader.depth - (int64_t)k * kStep : kStep;
+      bytes = bytes > 0 && depth > 0 ? bytes + (depth - 1) * reader.stride : 0;
+    }
+    if (ahead >= end) bytes = 0;
+    const __amdgpu_buffer_rsrc_t buffer =
+        __builtin_amdgcn_make_buffer_rsrc((void*)reader.from[r], 0, (int)bytes, 0x00020000);
+#pragma unroll
+    for (int q = 0; q < decltype(loads)::value; ++q) {
+      uint32_t offset = reader.offset[q];
+      if constexpr (!decltype(turned)::value)
+        offset = (int64_t)k * kStepBytes + reader.chunk < reader.depth * kBytes ? offset : 0x80000000u;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(buffer, (SharedBytes)(to + (q * S::kWaves + wave) * (kWave * 16)), 16,
+                                               (int)offset, 0, 0, 0);
+    }
+  };
+  using LeftTurned = std::bool_constant<kLeftTurned>;
+  using RightTurned = std::bool_constant<kRightTurned>;
+  using LoadsM = std::integral_constant<int, S::kLoadsM>;
+  using LoadsN = std::integral_constant<int, S::kLoadsN>;
+  char* const lds_right = lds + 4 * S::kRegionM;
+  auto left_region = [&](int r, int stage) { return lds + (r * 2 + stage) * S::kRegionM; };
+  auto right_region = [&](int r, int stage) { return lds_right + (r * 2 + stage) * S::kRegionN; };
+  auto fetch_left = [&](int r, int stage) { fetch(left, r, left_region(r, stage), LeftTurned{}, LoadsM{}); };
+  auto fetch_right = [&](int r, int stage) { fetch(right, r, right_region(r, stage), RightTurned{}, LoadsN{}); };
+
+  // ---- LDS to registers
+  // Straight: lane l has row l % 16, chunks l / 16 and l / 16 + 4 of it.  Turned: its 8
+  // values of a half are 8 l / 16 .. + 7 of the depth, by two reads of 4 x 16 that
+  // transpose: lane l gives the place of row l % 16 / 4, columns l % 4 * 4 .. + 3.
+  auto straight_place = [&](int row, int half) {
+    return (row + lane % 16) * kStepBytes + (((lane / 16) ^ (lane & 7)) ^ (half * 4)) * 16;
+  };
+  auto read = [&](Fragment* f, const char* region, int first_row, auto tiles, auto turned, auto half_rows) {
+#pragma unroll
+    for (int t = 0; t < decltype(tiles)::value; ++t) {
+      int4v part[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if constexpr (!decltype(turned)::value) {
+          part[h] = *(const int4v*)(region + straight_place(first_row, h) + t * 16 * kStepBytes);
+        } else {
+          constexpr int kPitch = decltype(half_rows)::value * 2, kGranules = decltype(half_rows)::value / 16;
+          short4v four[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int row = h * 32 + lane / 16 * 8 + j * 4 + lane % 16 / 4;
+            const int granule = (first_row / 16 + t) ^ ((row & 7) % kGranules);
+            four[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                (__attribute__((address_space(3))) short4v*)(region + row * kPitch + granule * 32 + lane % 4 * 8));
+          }
+          __builtin_memcpy(&part[h], four, sizeof(four));
+        }
+      }
+      f[t].v = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  };
+  using TilesM = std::integral_constant<int, S::kTilesM>;
+  using TilesN = std::integral_constant<int, S::kTilesN>;
+  using HalfM = std::integral_constant<int, S::kHalfM>;
+  using HalfN = std::integral_constant<int, S::kHalfN>;
+  Fragment a[S::kTilesM], b[2][S::kTilesN];
+  auto read_left = [&](int r, int stage) { read(a, left_region(r, stage), wm * S::kRowsM, TilesM{}, LeftTurned{}, HalfM{}); };
+  auto read_right = [&](Fragment* f, int r, int stage) {
+    read(f, right_region(r, stage), wn * S::kRowsN, TilesN{}, RightTurned{}, HalfN{});
+  };
+
+  // A row's exponents of a step: bytes kTilesM x + i of words that lanes l % 16 of the
+  // rows' waves read, for all of its steps.
+  using Panel = Scales<S>;
+  uint32_t left_scales[Panel::kWordsM] = {}, right_scales[Panel::kWordsN] = {};
+  auto read_scales = [&](uint32_t step) {
+    const uint32_t* words = (const uint32_t*)(lds + S::kBytes) + step * (Panel::kBytes / 4);
+    __builtin_memcpy(left_scales, words + (wm * 16 + lane % 16) * Panel::kWordsM, sizeof(left_scales));
+    __builtin_memcpy(right_scales, words + Panel::kM + (wn * 16 + lane % 16) * Panel::kWordsN, sizeof(right_scales));
+  };
+
+  float4v sum[2][2][S::kTilesM][S::kTilesN] = {};
+  // Matrix instructions have no order of their own among barriers and loads: empty
+  // statements that name their operands before and their results after hold them
+  // between a phase's two barriers.
+  auto multiply_quarter = [&](int x, int y, Fragment* f) {
+#pragma unroll
+    for (int i = 0; i < S::kTilesM; ++i) hold(a[i]);
+#pragma unroll
+    for (int j = 0; j < S::kTilesN; ++j) hold(f[j]);
+#pragma unroll
+    for (int i = 0; i < S::kTilesM; ++i)
+#pragma unroll
+      for (int j = 0; j < S::kTilesN; ++j) {
+        if constexpr (k8) {
+          const int l = x * S::kTilesM + i, r = y * S::kTilesN + j;
+          sum[x][y][i][j] = multiply8(a[i], f[j], (int)(left_scales[l / 4] >> (l % 4 * 8)),
+                                      (int)(right_scales[r / 4] >> (r % 4 * 8)), sum[x][y][i][j]);
+        } else {
+          sum[x][y][i][j] = multiply<E>(a[i], f[j], sum[x][y][i][j]);
+        }
+      }
+#pragma unroll
+    for (int i = 0; i < S::kTilesM; ++i)
+#pragma unroll
+      for (int j = 0; j < S::kTilesN; ++j) asm volatile("" : "+v"(sum[x][y][i][j]));
+  };
+
+  // ---- the steps
+  constexpr int kFlight = 3 * (S::kLoadsM + S::kLoadsN);  // loads issued after the region that is waited for
+  // The four quarters of a step, with B0 of this step in b[kStage] already.
+  auto phase_end = [&] {
+    __builtin_amdgcn_sched_barrier(0);
+    wait_loads<kFlight>();
+    wait_barrier();
+    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (S::kAlternate) __builtin_amdgcn_s_setprio(1);
+  };
+  auto quarter_end = [&] {
+    if constexpr (S::kAlternate) {
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_setprio(0);
+      wait_barrier();
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto step = [&](auto stage_constant, uint32_t t) {
+    constexpr int kStage = decltype(stage_constant)::value;
+    if constexpr (k8) read_scales(t);
+    read_left(0, kStage);
+    fetch_right(0, kStage);
+    phase_end();
+    multiply_quarter(0, 0, b[kStage]);
+    quarter_end();
+    read_right(b[1 - kStage], 1, kStage);
+    fetch_left(0, kStage);
+    phase_end();
+    multiply_quarter(0, 1, b[1 - kStage]);
+    quarter_end();
+    read_left(1, kStage);
+    fetch_right(1, kStage);
+    phase_end();
+    multiply_quarter(1, 1, b[1 - kStage]);
+    quarter_end();
+    read_right(b[1 - kStage], 0, 1 - kStage);
+    fetch_left(1, kStage);
+    advance();
+    phase_end();
+    multiply_quarter(1, 0, b[kStage]);
+    quarter_end();
+  };
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    fetch_right(0, s);
+    fetch_left(0, s);
+    fetch_right(1, s);
+    fetch_left(1, s);
+    advance();
+  }
+  if constexpr (k8) {
+    Panel::fill(lds + S::kBytes, p, row0, job.left.extent, column0, job.right.extent, Finish::kDual, begin, end);
+    wait_loads<0>();
+  } else {
+    wait_loads<kFlight>();
+  }
+  wait_barrier();
+  read_right(b[0], 0, 0);
+  wait_loads<kFlight>();
+  wait_barrier();
+  if constexpr (S::kAlternate)
+    if (wave >= S::kWaves / 2) wait_barrier();
+  const uint32_t steps = end > begin ? end - begin : 0;
+  for (uint32_t t = 0; t + 2 <= steps; t += 2) {
+    step(std::integral_constant<int, 0>{}, t);
+    step(std::integral_constant<int, 1>{}, t + 1);
+  }
+  if (steps % 2) step(std::integral_constant<int, 0>{}, steps - 1);
+  if constexpr (S::kAlternate)
+    if (wave < S::kWaves / 2) wait_barrier();
+  // Nothing may land in LDS after the workgroup has ended.
+  wait_loads<0>();
+
+  // ---- what becomes of the sums: through LDS, half of the rows at a time, so that a
+  // lane then has 8 columns of a row.  (16 bytes go to place c ^ row % 16 of a row.)
+  constexpr int kQuads = S::kTileN / 4;
+  float4v* const rows = (float4v*)lds;
+  const Finish finish(p, job, split);
+#pragma unroll
+  for (int x = 0; x < 2; ++x) {
+    wait_barrier();
+#pragma unroll
+    for (int i = 0; i < S::kTilesM; ++i)
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int j = 0; j < S::kTilesN; ++j) {
+          const int row = wm * S::kRowsM + i * 16 + lane % 16;
+          const int quad = (y * S::kHalfN + wn * S::kRowsN + j * 16) / 4 + lane / 16;
+          rows[row * kQuads + (quad ^ lane % 16)] = sum[x][y][i][j];
+        }
+    wait_loads<0>();
+    wait_barrier();
+    constexpr int kEights = (Finish::kDual ? S::kHalfN : S::kTileN) / 8;
+#pragma unroll 1
+    for (int at = threadIdx.x; at < S::kHalfM * kEights; at += S::kThreads) {
+      const int row = at / kEights, eight = at % kEights;
+      const int64_t m = row0 + x * S::kHalfM + row;
+      if (m >= job.rows) break;
+      float v[Finish::kDual ? 2 : 1][8];
+#pragma unroll
+      for (int y = 0; y < (Finish::kDual ? 2 : 1); ++y)
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const float4v four = rows[row * kQuads + ((y * (S::kHalfN / 4) + eight * 2 + q) ^ (row % 16))];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[y][q * 4 + e] = four[e];
+        }
+      if constexpr (Finish::kDual) finish(m, column0 + eight * 8, v[0], v[1]);
+      else finish(m, column0 + eight * 8, v[0]);
+    }
+  }
+}
+
+// Eight values of a row, to the type rounded once; those beyond `columns` are not stored.
+template <typename T>
+__device__ __forceinline__ void store_eight(T* row, int64_t n, int64_t columns, const float* v) {
+  T r[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) r[e] = (T)v[e];
+  if (n + 8 <= columns) {
+    __builtin_memcpy(row + n, r, sizeof(r));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (n + e < columns) row[n + e] = r[e];
+  }
+}
+
+template <typename T>
+struct Store {
+  static constexpr bool kDual = false;
+  T* out;
+  int64_t stride, columns;
+  __device__ __forceinline__ Store(const Params&, const Job& job, uint32_t)
+      : out((T*)job.out), stride(job.out_stride), columns(job.columns) {}
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, const float* v) const {
+    store_eight(out + m * stride, n, columns, v);
+  }
+};
+
+// A share of the depth, added up by k_join.
+struct Partial {
+  static constexpr bool kDual = false;
+  float* out;
+  int64_t columns;
+  __device__ __forceinline__ Partial(const Params& p, const Job& job, uint32_t split)
+      : out(p.partials + split * p.partial_size + job.partial), columns(job.columns) {}
+  __device__ __forceinline__ void operator()(int64_t m, int64_t n, const float* v) const {
+    store_eight(out + m * columns, n, columns, v);
+  }
+};
+
+}  // namespace product
+}  // namespace mgb

@@ -25,15 +25,17 @@ then this module by name, `from xgboost import encoder`.
 """
 from __future__ import annotations
 
-from typing import Any, Optional, Sequence, Tuple
+from typing import Any, NamedTuple, Optional, Sequence, Tuple
 
 import numpy as np
 import torch
 
 from .core import Booster, DMatrix
 
-__all__ = ["Embedding", "LayerNorm", "LeafTokenizer", "Muon", "embedding_gradient", "embedding_lookup", "layer_norm",
-           "layer_norm_gradient", "orthogonalize"]
+__all__ = ["BlockScaled", "Embedding", "FeedForward", "LayerNorm", "LeafTokenizer", "Muon", "QuantizedFeedForward",
+           "block_feed_forward", "block_matmul", "distillation_gradient", "distillation_loss", "embedding_gradient", "embedding_lookup",
+           "feed_forward", "feed_forward_gradient", "layer_norm", "layer_norm_gradient", "orthogonalize",
+           "quantize_blocks"]
 
 
 def _one_runtime() -> None:
@@ -170,6 +172,152 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5,
     return _without_derivative("orthogonalize", _encoder.orthogonalize, update, steps, coefficients, eps)
 
 
+# ---- gated feed-forward block ---------------------------------------------------
+
+def feed_forward_gradient(grad: torch.Tensor, x: torch.Tensor, kept: torch.Tensor, gate: torch.Tensor, up: torch.Tensor,
+                          down: torch.Tensor, *, activation: str = "silu"
+                          ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """The gradients of `feed_forward`'s x, gate, up and down from its result's
+    gradient and what it kept.  Has no derivative itself, like
+    `embedding_gradient`."""
+    return _without_derivative("feed_forward_gradient", _encoder.feed_forward_gradient, grad, x, kept, gate, up, down,
+                               activation, 15)
+
+
+class _FeedForward(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gate, up, down, activation):  # pylint: disable=arguments-differ
+        y, kept = _encoder.feed_forward(x, gate, up, down, activation, True)
+        ctx.save_for_backward(x, kept, gate, up, down)
+        ctx.activation = activation
+        ctx.mark_non_differentiable(kept)
+        ctx.set_materialize_grads(False)
+        return y, kept
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, _):  # pylint: disable=arguments-differ
+        if grad is None:
+            return None, None, None, None, None
+        x, kept, gate, up, down = ctx.saved_tensors
+        wanted = sum(1 << k for k in range(4) if ctx.needs_input_grad[k])
+        return (*_encoder.feed_forward_gradient(grad, x, kept, gate, up, down, ctx.activation, wanted), None)
+
+
+def feed_forward(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor, *, activation: str = "silu",
+                 keep: bool = False) -> Any:
+    """(act(x gate^T) * (x up^T)) down^T over x's last axis: gate and up are
+    (hidden, dim), down (dim, hidden), all of x's type; `activation` is "silu" or
+    "gelu" (by the normal distribution's function).  With `keep` the result is
+    (y, kept), kept being x gate^T and x up^T, float32 (..., 2, hidden), which
+    `feed_forward_gradient` reads.  The hidden values are rounded to x's type.
+    Float32 values are multiplied as three bfloat16 each; an infinity among them
+    gives NaN.  Differentiable in x and the matrices through y."""
+    if torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in (x, gate, up, down)):
+        y, kept = _FeedForward.apply(x, gate, up, down, activation)
+        return (y, kept) if keep else y
+    return _encoder.feed_forward(x, gate, up, down, activation, keep)
+
+
+# ---- products in 8 bits -----------------------------------------------------------
+
+class BlockScaled(NamedTuple):
+    """Rows in 8 bits: `values`, float8_e4m3fn, rows of whole blocks of 128 (the rest
+    of the last one zeros), and `scales`, float8_e8m0fnu, the power of two that each
+    block is times.  `dim` is the rows' length before."""
+    values: torch.Tensor
+    scales: torch.Tensor
+    dim: int
+
+    def dequantize(self) -> torch.Tensor:
+        """The values that the blocks stand for, float32."""
+        blocks = self.values.float().unflatten(-1, (-1, 128)) * self.scales.float()[..., None]
+        return blocks.flatten(-2)[..., :self.dim]
+
+
+def _blocks(name: str, m: BlockScaled) -> BlockScaled:
+    if not isinstance(m, BlockScaled):
+        raise TypeError(f"{name} must be a BlockScaled (see quantize_blocks), got {type(m).__name__}")
+    return m
+
+
+def quantize_blocks(x: torch.Tensor) -> BlockScaled:
+    """x's last axis in 8 bits with a scale for each 128 values: the smallest power of
+    two that takes the largest finite magnitude to at most 448, the values rounded to
+    nearest even.  An infinity or NaN becomes NaN.  Has no derivative, like the
+    products of what it gives: where x requires one, a backward pass is an error."""
+    return BlockScaled(*_without_derivative("quantize_blocks", _encoder.quantize_blocks, x), x.shape[-1])
+
+
+def block_matmul(x: BlockScaled, weight: BlockScaled, *, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """x weight^T in `dtype`, of what the blocks stand for: x (..., dim) and weight
+    (rows, dim).  16-bit results come of the 8-bit matrix instructions (off by about
+    1.5e-5 of the norm before they are rounded), float32 ones of bfloat16's, which
+    take the values exactly."""
+    x, weight = _blocks("x", x), _blocks("weight", weight)
+    if x.dim != weight.dim:
+        raise ValueError(f"x and weight must have rows of one length, have {x.dim} and {weight.dim}")
+    return _without_derivative("block_matmul", _encoder.block_matmul, x.values, x.scales, weight.values, weight.scales,
+                               dtype)
+
+
+def block_feed_forward(x: torch.Tensor, gate: BlockScaled, up: BlockScaled, down: BlockScaled, *,
+                       activation: str = "silu") -> torch.Tensor:
+    """`feed_forward` as it is served: the matrices as `quantize_blocks` keeps them, x
+    and the hidden values rounded so in the call.  The products of bfloat16 rows are
+    `block_matmul`'s 16-bit ones; those of float16 and float32 rows, up to the hidden
+    values' rounding, are exact.  Has no derivative: where x requires one, a backward
+    pass through the result is an error."""
+    gate, up, down = _blocks("gate", gate), _blocks("up", up), _blocks("down", down)
+    return _without_derivative("block_feed_forward", _encoder.block_feed_forward, x, gate.values, gate.scales, up.values,
+                               up.scales, down.values, down.scales, activation)
+
+
+# ---- distillation -----------------------------------------------------------------
+
+def distillation_gradient(grad: torch.Tensor, logits: torch.Tensor, lse: torch.Tensor, values: torch.Tensor,
+                          indices: torch.Tensor, *, temperature: float = 1.0) -> torch.Tensor:
+    """The logits' gradient from that of `distillation_loss`'s loss (float32, a value a
+    row) and the lse it returned.  Has no derivative itself, like
+    `embedding_gradient`."""
+    return _without_derivative("distillation_gradient", _encoder.distillation_gradient, grad, logits, lse, values, indices,
+                               temperature)
+
+
+class _Distillation(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, values, indices, temperature):  # pylint: disable=arguments-differ
+        loss, lse = _encoder.distillation_loss(logits, values, indices, temperature)
+        ctx.save_for_backward(logits, lse, values, indices)
+        ctx.temperature = temperature
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        return loss, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, _):  # pylint: disable=arguments-differ
+        if grad is None:
+            return None, None, None, None
+        logits, lse, values, indices = ctx.saved_tensors
+        return _encoder.distillation_gradient(grad, logits, lse, values, indices, ctx.temperature), None, None, None
+
+
+def distillation_loss(logits: torch.Tensor, values: torch.Tensor, indices: torch.Tensor, *, temperature: float = 1.0
+                      ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(loss, lse) of each row of logits (..., classes): how far softmax(logits / T) is
+    from a teacher, whose largest logits are `values` (..., top) at the columns
+    `indices` (int32 or int64): T^2 times the Kullback-Leibler divergence from the
+    softmax of values / T over the entries, and log sum exp(logits / T), which
+    `distillation_gradient` reads, both float32.  An entry whose index lies outside the
+    row, -1 for padding, or whose value is -inf is absent; a row without entries has
+    loss 0.  At most 1,024 entries.  Differentiable in logits through the loss; the
+    teacher is constant."""
+    if torch.is_grad_enabled() and getattr(logits, "requires_grad", False):
+        return _Distillation.apply(logits, values, indices, temperature)
+    return _encoder.distillation_loss(logits, values, indices, temperature)
+
+
 class Muon(torch.optim.Optimizer):
     """Matrices by orthogonalised momentum: m = momentum m + grad, and
     w -= lr (sqrt(max(1, rows / columns)) orthogonalize(grad + momentum m) + weight_decay w)
@@ -266,6 +414,44 @@ class LayerNorm(torch.nn.Module):
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return layer_norm(x, self.weight, self.bias, eps=self.eps)[0]
+
+
+class FeedForward(torch.nn.Module):
+    """`feed_forward` with matrices of its own, drawn from normal distributions of
+    variance 1 / dim (gate, up) and 1 / hidden (down)."""
+
+    def __init__(self, dim: int, hidden: int, *, activation: str = "silu", device: Any = "cuda",
+                 dtype: torch.dtype = torch.float32) -> None:
+        super().__init__()
+        self.activation = activation
+
+        def matrix(rows: int, columns: int) -> torch.nn.Parameter:
+            return torch.nn.Parameter(torch.randn(rows, columns, device=device, dtype=dtype) * columns ** -0.5)
+        self.gate, self.up, self.down = matrix(hidden, dim), matrix(hidden, dim), matrix(dim, hidden)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return feed_forward(x, self.gate, self.up, self.down, activation=self.activation)
+
+    def quantized(self) -> "QuantizedFeedForward":
+        """The block with its matrices in 8 bits, as they are now, to serve it with."""
+        return QuantizedFeedForward(self)
+
+
+class QuantizedFeedForward(torch.nn.Module):
+    """`block_feed_forward` with a `FeedForward`'s matrices, laid out once."""
+
+    def __init__(self, block: FeedForward) -> None:
+        super().__init__()
+        self.activation, self.dim, self.hidden = block.activation, block.gate.shape[1], block.gate.shape[0]
+        for name in ("gate", "up", "down"):
+            kept = quantize_blocks(getattr(block, name).detach())
+            self.register_buffer(name + "_values", kept.values)
+            self.register_buffer(name + "_scales", kept.scales)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        matrices = (BlockScaled(getattr(self, name + "_values"), getattr(self, name + "_scales"), dim)
+                    for name, dim in (("gate", self.dim), ("up", self.dim), ("down", self.hidden)))
+        return block_feed_forward(x, *matrices, activation=self.activation)
 
 
 class LeafTokenizer:
