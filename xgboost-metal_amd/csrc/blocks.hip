@@ -12,7 +12,7 @@
 // Binary32 results, and the hidden values of a block in binary32 and binary16 (which
 // are rounded to e4m3 next: what crosses a border there shows), come of the bfloat16
 // instructions, which take e4m3 values with their scales exactly.
-#include "feed_forward.hpp"
+#include "few_rows.hpp"
 
 namespace mgb {
 namespace block {
@@ -25,25 +25,6 @@ __device__ __forceinline__ float group_max16(float v) {
   v = fmaxf(v, lane_move<0x4e>(v));
   v = fmaxf(v, lane_move<0x141>(v));
   return fmaxf(v, lane_move<0x140>(v));
-}
-
-// The exponent + 127 of the smallest power of two that takes `largest` to at most
-// 448 = 1.75 2^8; 127 where there is none.
-__device__ __forceinline__ uint32_t scale_of(float largest) {
-  const uint32_t bits = __float_as_uint(largest);
-  const int exponent = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return largest == 0.0f ? 127u : exponent > 0 ? (uint32_t)exponent : 0u;
-}
-
-// Eight values as e4m3, rounded to nearest even; infinities and NaN become its NaN.
-__device__ __forceinline__ uint2 round_eight(const float* v, float factor) {
-  int word[2] = {};
-#pragma unroll
-  for (int w = 0; w < 2; ++w) {
-    word[w] = __builtin_amdgcn_cvt_pk_fp8_f32(v[w * 4] * factor, v[w * 4 + 1] * factor, word[w], false);
-    word[w] = __builtin_amdgcn_cvt_pk_fp8_f32(v[w * 4 + 2] * factor, v[w * 4 + 3] * factor, word[w], true);
-  }
-  return {(uint32_t)word[0], (uint32_t)word[1]};
 }
 
 // 16 lanes a block of 128, 8 values a lane.
@@ -91,20 +72,10 @@ __global__ __launch_bounds__(kQuantThreads) void k_widen(__bf16* __restrict__ to
   const int lane = threadIdx.x % kQuantLanes;
   for (int64_t at = (int64_t)blockIdx.x * (kQuantThreads / kQuantLanes) + threadIdx.x / kQuantLanes; at < all; at += step) {
     const int64_t row = at / m.blocks, block = at % m.blocks;
-    uint32_t word[2];
-    __builtin_memcpy(word, (const uint8_t*)m.values + row * m.stride + block * kBlock + lane * 8, 8);
-    const int exponent = (int)((const uint8_t*)m.scales)[row * m.scale_stride + block] - 127;
-    __bf16 v[8];
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const auto low = __builtin_amdgcn_cvt_pk_f32_fp8((int)word[w], false);
-      const auto high = __builtin_amdgcn_cvt_pk_f32_fp8((int)word[w], true);
-      v[w * 4] = (__bf16)ldexpf(low[0], exponent);
-      v[w * 4 + 1] = (__bf16)ldexpf(low[1], exponent);
-      v[w * 4 + 2] = (__bf16)ldexpf(high[0], exponent);
-      v[w * 4 + 3] = (__bf16)ldexpf(high[1], exponent);
-    }
-    __builtin_memcpy(to + (row * m.blocks + block) * kBlock + lane * 8, v, sizeof(v));
+    uint2 bytes;
+    __builtin_memcpy(&bytes, (const uint8_t*)m.values + row * m.stride + block * kBlock + lane * 8, 8);
+    const product::bf16x8 v = widen_eight(bytes, ((const uint8_t*)m.scales)[row * m.scale_stride + block]);
+    __builtin_memcpy(to + (row * m.blocks + block) * kBlock + lane * 8, &v, sizeof(v));
   }
 }
 
@@ -127,6 +98,23 @@ product::Operand operand8(const MgbBlocks& m) {
 // scales of kScaleSteps.
 template <typename T>
 int multiply(T* out, const MgbBlocks& x, const MgbBlocks& weight, Space& space, hipStream_t stream, bool run) {
+  if (x.rows <= kMostFewRows) {
+    Few f = {};
+    f.x = x.values;
+    f.w[0] = weight.values;
+    f.x_scales = (const uint8_t*)x.scales;
+    f.w_scales[0] = (const uint8_t*)weight.scales;
+    f.x_stride = x.stride;
+    f.w_stride[0] = weight.stride;
+    f.x_scale_stride = x.scale_stride;
+    f.w_scale_stride = weight.scale_stride;
+    f.rows = x.rows;
+    f.columns = weight.rows;
+    f.depth = x.blocks * kBlock;
+    f.out = out;
+    if (run) few_rows<InBlocks, InBlocks, T, false>(f, stream);
+    return 0;
+  }
   Params p = {};
   p.jobs = 1;
   p.sources = 1;
@@ -160,16 +148,48 @@ struct GatedFloat {
   static constexpr bool kDual = true;
   const Params& p;
   __device__ __forceinline__ GatedFloat(const Params& params, const product::Job&, uint32_t) : p(params) {}
+  template <int kCount>
   __device__ __forceinline__ void operator()(int64_t m, int64_t n, const float* gate, const float* up) const {
-    float h[8];
+    float h[kCount];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) h[e] = activate<true>(gate[e], p.activation) * up[e];
-    product::store_eight((float*)p.hidden + m * p.hidden_stride, n, p.true_columns, h);
+    for (int e = 0; e < kCount; ++e) h[e] = activate<true>(gate[e], p.activation) * up[e];
+    product::store_some<kCount>((float*)p.hidden + m * p.hidden_stride, n, p.true_columns, h);
   }
 };
 
 template <typename T>
 int serve(const MgbBlockFeedForward& a, Space& space, hipStream_t stream, bool run) {
+  if (a.rows <= kMostFewRows) {
+    Few f = {};
+    f.x = a.x;
+    f.w[0] = a.gate.values;
+    f.w[1] = a.up.values;
+    f.w_scales[0] = (const uint8_t*)a.gate.scales;
+    f.w_scales[1] = (const uint8_t*)a.up.scales;
+    f.x_stride = a.x_stride;
+    f.w_stride[0] = a.gate.stride;
+    f.w_stride[1] = a.up.stride;
+    f.w_scale_stride = a.gate.scale_stride;
+    f.rows = a.rows;
+    f.columns = a.hidden;
+    f.depth = a.dim;
+    f.out = space.take(a.rows * a.hidden * sizeof(float));
+    f.activation = a.activation;
+    if (run) few_rows<Rounded<T>, InBlocks, float, true>(f, stream);
+    Few g = {};
+    g.x = f.out;
+    g.w[0] = a.down.values;
+    g.w_scales[0] = (const uint8_t*)a.down.scales;
+    g.x_stride = a.hidden;
+    g.w_stride[0] = a.down.stride;
+    g.w_scale_stride = a.down.scale_stride;
+    g.rows = a.rows;
+    g.columns = a.dim;
+    g.depth = a.hidden;
+    g.out = a.y;
+    if (run) few_rows<Rounded<float>, InBlocks, T, false>(g, stream);
+    return 0;
+  }
   const int64_t dim = a.gate.blocks * kBlock, hidden = a.down.blocks * kBlock;
   const int64_t x_scales = (a.gate.blocks + 3) / 4 * 4, hidden_scales = (a.down.blocks + 3) / 4 * 4;
   MgbBlocks x = {space.take(a.rows * dim), space.take(a.rows * x_scales), a.rows, a.gate.blocks, dim, x_scales};

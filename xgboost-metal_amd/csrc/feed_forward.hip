@@ -4,7 +4,7 @@
 // workgroup, so that gate and up never leave its registers (but for a gradient,
 // which reads them in binary32: rounded to 16 bits they would show in it), the
 // second is y's.  hidden is rounded to x's type once; sums are binary32.
-#include "feed_forward.hpp"
+#include "few_rows.hpp"
 
 namespace mgb {
 namespace block {
@@ -15,17 +15,18 @@ struct Gated {
   static constexpr bool kDual = true;
   const Params& p;
   __device__ __forceinline__ Gated(const Params& params, const product::Job&, uint32_t) : p(params) {}
+  template <int kCount>
   __device__ __forceinline__ void operator()(int64_t m, int64_t n, const float* gate, const float* up) const {
-    if (n >= p.hidden_stride) return;
-    float h[8];
+    if (n >= p.hidden_columns) return;
+    float h[kCount];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) h[e] = activate<sizeof(T) == 4>(gate[e], p.activation) * up[e];
+    for (int e = 0; e < kCount; ++e) h[e] = activate<sizeof(T) == 4>(gate[e], p.activation) * up[e];
     // (Columns that pad hidden's rows are products with zeros.)
-    store_inner<T>(p.hidden, p.hidden_part, m * p.hidden_stride + n, h);
+    store_inner<T, kCount>(p.hidden, p.hidden_part, m * p.hidden_stride + n, h);
     if (p.kept) {
       float* to = p.kept + m * 2 * p.true_columns;
-      product::store_eight(to, n, p.true_columns, gate);
-      product::store_eight(to + p.true_columns, n, p.true_columns, up);
+      product::store_some<kCount>(to, n, p.true_columns, gate);
+      product::store_some<kCount>(to + p.true_columns, n, p.true_columns, up);
     }
   }
 };
@@ -33,6 +34,36 @@ struct Gated {
 template <typename T>
 int forward(const MgbFeedForward& a, Space& space, hipStream_t stream, bool run) {
   using E = typename Kind<T>::E;
+  if (a.rows <= kMostFewRows) {
+    Few f = {};
+    f.x = a.x;
+    f.w[0] = a.gate;
+    f.w[1] = a.up;
+    f.x_stride = a.x_stride;
+    f.w_stride[0] = a.gate_stride;
+    f.w_stride[1] = a.up_stride;
+    f.rows = a.rows;
+    f.columns = a.hidden;
+    f.depth = a.dim;
+    f.out = space.take(a.rows * a.hidden * sizeof(T));
+    f.kept = a.kept;
+    f.activation = a.activation;
+    Few g = {};
+    g.x = f.out;
+    g.w[0] = a.down;
+    g.x_stride = a.hidden;
+    g.w_stride[0] = a.down_stride;
+    g.rows = a.rows;
+    g.columns = a.dim;
+    g.depth = a.hidden;
+    g.out = a.y;
+    if (run) {
+      few_rows<Plain<T>, Plain<T>, T, true>(f, stream);
+      few_rows<Plain<T>, Plain<T>, T, false>(g, stream);
+      MGB_LAUNCH_CHECK("feed forward");
+    }
+    return 0;
+  }
   LayJobs jobs = {};
   const bool copy = !lies_well<T>(a.gate, a.hidden, a.dim, a.gate_stride) ||
                     !lies_well<T>(a.up, a.hidden, a.dim, a.up_stride) ||
@@ -48,8 +79,9 @@ int forward(const MgbFeedForward& a, Space& space, hipStream_t stream, bool run)
   inner.sources = 1;
   inner.pairs = Kind<T>::kPairs;
   inner.depth = dim;
-  inner.hidden_stride = hidden;
-  inner.hidden_part = a.rows * hidden;
+  inner.hidden_columns = hidden;
+  inner.hidden_stride = inner_stride(hidden);
+  inner.hidden_part = a.rows * inner.hidden_stride;
   inner.hidden = space.take(inner.hidden_part * Kind<T>::kParts * 2);
   inner.kept = a.kept;
   inner.true_columns = a.hidden;
@@ -66,7 +98,7 @@ int forward(const MgbFeedForward& a, Space& space, hipStream_t stream, bool run)
   outer.sources = 1;
   outer.pairs = Kind<T>::kPairs;
   outer.depth = hidden;
-  outer.job[0].left = operand({inner.hidden, hidden * 2, inner.hidden_part * 2}, a.rows, hidden);
+  outer.job[0].left = operand({inner.hidden, inner.hidden_stride * 2, inner.hidden_part * 2}, a.rows, hidden);
   outer.job[0].right = operand(down, a.dim, hidden);
   outer.job[0].out = a.y;
   outer.job[0].out_stride = a.dim;

@@ -56,6 +56,11 @@ struct Space {
   }
 };
 
+// Rows of the inner matrices: those of whole 2 KB would all begin in the same few
+// of the cache's channels (products of 8,192 x 8,192 x 8,192: 862 us, and 770 with rows
+// of 1 KB more), so they are 256 bytes longer.
+inline int64_t inner_stride(int64_t columns) { return columns % 1024 ? columns : columns + 128; }
+
 // ---- layout ------------------------------------------------------------------
 // The products load 16 bytes a lane, whole ones of a row.  16-bit matrices whose
 // rows begin at 16 bytes and hold whole ones are read where they lie; others are
@@ -63,7 +68,7 @@ struct Space {
 struct LayJob {
   const void* from;
   char* to;
-  int64_t rows, columns, stride, chunks, part;  // stride in elements, chunks of 8, part in bytes
+  int64_t rows, columns, stride, chunks, part;  // stride in elements, chunks of 8 a row of `to`, part in bytes
 };
 constexpr int kMostLay = 5;
 struct LayJobs {
@@ -108,6 +113,53 @@ __global__ __launch_bounds__(kLayThreads) void k_lay_out(LayJobs jobs) {
   }
 }
 
+// The same, transposed: rows of `to` are columns of `from`.
+constexpr int kTurnSide = 64;
+template <typename T>
+__global__ __launch_bounds__(kLayThreads) void k_turn(LayJobs jobs) {
+  using E = typename Kind<T>::E;
+  constexpr int kParts = Kind<T>::kParts;
+  __shared__ float tile[kTurnSide][kTurnSide + 1];
+  const LayJob job = jobs.job[blockIdx.y];
+  const int64_t across = (job.columns + kTurnSide - 1) / kTurnSide, down = (job.rows + kTurnSide - 1) / kTurnSide;
+  for (int64_t at = blockIdx.x; at < across * down; at += gridDim.x) {
+    const int64_t row0 = at / across * kTurnSide, column0 = at % across * kTurnSide;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kTurnSide * kTurnSide / 8 / kLayThreads; ++k) {
+      const int eight = k * kLayThreads + threadIdx.x, row = eight / (kTurnSide / 8), column = eight % (kTurnSide / 8) * 8;
+      float v[8] = {};
+      if (row0 + row < job.rows) load_some<8>((const T*)job.from + (row0 + row) * job.stride, column0 + column, job.columns, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) tile[row][column + e] = v[e];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < kTurnSide * kTurnSide / 8 / kLayThreads; ++k) {
+      // (lanes that follow each other take rows of `to`: columns of the tile lie in different banks)
+      const int eight = k * kLayThreads + threadIdx.x, row = eight % kTurnSide, chunk = eight / kTurnSide;
+      if (column0 + row >= job.columns || row0 / 8 + chunk >= job.chunks) continue;
+      E part[kParts][8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float v = tile[chunk * 8 + e][row];
+        if constexpr (kParts == 3) {
+          __bf16 three[3];
+          split_parts(v, three);
+#pragma unroll
+          for (int q = 0; q < 3; ++q) part[q][e] = three[q];
+        } else {
+          part[0][e] = (E)v;
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < kParts; ++q)
+        __builtin_memcpy(__builtin_assume_aligned(job.to + q * job.part + ((column0 + row) * job.chunks + row0 / 8 + chunk) * 16, 16),
+                         part[q], 16);
+    }
+  }
+}
+
 // A matrix as a product takes it.
 struct Laid {
   const char* data;
@@ -134,6 +186,23 @@ Laid lay(Space& space, LayJobs& jobs, const void* data, int64_t rows, int64_t co
 template <typename T>
 Laid lay(Space& space, LayJobs& jobs, const void* data, int64_t rows, int64_t columns, int64_t stride) {
   return lay<T>(space, jobs, data, rows, columns, stride, !lies_well<T>(data, rows, columns, stride));
+}
+
+// The transpose (columns, rows) of a matrix.
+template <typename T>
+Laid lay_turned(Space& space, LayJobs& jobs, const void* data, int64_t rows, int64_t columns, int64_t stride) {
+  const int64_t width = inner_stride(padded(rows)) * 2, part = width * columns;
+  char* to = space.take(part * Kind<T>::kParts);
+  jobs.job[jobs.count++] = {data, to, rows, columns, stride, width / 16, part};
+  return {to, width, part};
+}
+
+template <typename T>
+void turn(const LayJobs& jobs, hipStream_t stream) {
+  int64_t most = 0;
+  for (int k = 0; k < jobs.count; ++k)
+    most = std::max(most, ((jobs.job[k].rows + kTurnSide - 1) / kTurnSide) * ((jobs.job[k].columns + kTurnSide - 1) / kTurnSide));
+  if (most > 0) k_turn<T><<<dim3((uint32_t)std::min<int64_t>(most, 4096), jobs.count), kLayThreads, 0, stream>>>(jobs);
 }
 
 template <typename T>
@@ -307,26 +376,26 @@ __device__ __forceinline__ float activate(float g, int activation, float* slope)
   return g * phi;
 }
 
-// Eight values of a row of the block's inner matrices, in parts.
-template <typename T>
+// Values of a row of the block's inner matrices, in parts.
+template <typename T, int kCount>
 __device__ __forceinline__ void store_inner(char* matrix, int64_t part, int64_t at, const float* v) {
   using E = typename Kind<T>::E;
   constexpr int kParts = Kind<T>::kParts;
-  E eight[kParts][8];
+  E some[kParts][kCount];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
+  for (int e = 0; e < kCount; ++e) {
     if constexpr (kParts == 3) {
       __bf16 three[3];
       split_parts(v[e], three);
 #pragma unroll
-      for (int q = 0; q < 3; ++q) eight[q][e] = three[q];
+      for (int q = 0; q < 3; ++q) some[q][e] = three[q];
     } else {
-      eight[0][e] = (E)v[e];
+      some[0][e] = (E)v[e];
     }
   }
 #pragma unroll
   for (int q = 0; q < kParts; ++q)
-    __builtin_memcpy(__builtin_assume_aligned(matrix + (q * part + at) * 2, 16), eight[q], 16);
+    __builtin_memcpy(__builtin_assume_aligned(matrix + (q * part + at) * 2, kCount * 2), some[q], kCount * 2);
 }
 
 inline product::Operand operand(const Laid& m, int64_t extent, int64_t depth) {

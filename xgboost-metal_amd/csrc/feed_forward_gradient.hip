@@ -11,19 +11,22 @@ namespace mgb {
 namespace block {
 namespace {
 
+constexpr int64_t kTurnRows = 4096;
+
 template <typename T>
 struct Slope {
   static constexpr bool kDual = false;
   const Params& p;
   __device__ __forceinline__ Slope(const Params& params, const product::Job&, uint32_t) : p(params) {}
+  template <int kCount>
   __device__ __forceinline__ void operator()(int64_t m, int64_t n, const float* dh) const {
-    if (n >= p.hidden_stride) return;
+    if (n >= p.hidden_columns) return;
     const float* from = p.kept + m * 2 * p.true_columns;
-    float gate[8], up[8], dgate[8], dup[8], hidden[8];
-    load_some<8>(from, n, p.true_columns, gate);
-    load_some<8>(from + p.true_columns, n, p.true_columns, up);
+    float gate[kCount], up[kCount], dgate[kCount], dup[kCount], hidden[kCount];
+    load_some<kCount>(from, n, p.true_columns, gate);
+    load_some<kCount>(from + p.true_columns, n, p.true_columns, up);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int e = 0; e < kCount; ++e) {
       float slope;
       const float act = activate<sizeof(T) == 4>(gate[e], p.activation, &slope);
       const bool there = n + e < p.true_columns;  // columns that pad a row are zero whatever dy holds
@@ -32,9 +35,9 @@ struct Slope {
       dup[e] = there ? dh[e] * act : 0.0f;
     }
     const int64_t at = m * p.hidden_stride + n;
-    store_inner<T>(p.dgate, p.gradient_part, at, dgate);
-    store_inner<T>(p.dgate, p.gradient_part, p.gradient_second + at, dup);
-    if (p.hidden) store_inner<T>(p.hidden, p.hidden_part, at, hidden);
+    store_inner<T, kCount>(p.dgate, p.gradient_part, at, dgate);
+    store_inner<T, kCount>(p.dgate, p.gradient_part, p.gradient_second + at, dup);
+    if (p.hidden) store_inner<T, kCount>(p.hidden, p.hidden_part, at, hidden);
   }
 };
 
@@ -62,16 +65,24 @@ int gradient(const MgbFeedForwardGradient& a, Space& space, hipStream_t stream, 
     MGB_LAUNCH_CHECK("feed forward gradient");
     return 0;
   }
-  LayJobs jobs = {};
+  LayJobs jobs = {}, turned = {};
+  // Matrices whose products go along their columns are transposed first where that
+  // costs little: binary32 ones, which are laid out anyhow, and others of many rows
+  // of x (16,384 x 1,024 x 4,096: two products of 322 and 280 us become TBD).
+  const bool turn_weights = sizeof(T) == 4 || a.rows >= kTurnRows;
   const int64_t dim = padded(a.dim), hidden = padded(a.hidden);
   const bool copy = !lies_well<T>(a.gate, a.hidden, a.dim, a.gate_stride) ||
                     !lies_well<T>(a.up, a.hidden, a.dim, a.up_stride) ||
                     (a.hidden > 1 && a.gate_stride != a.up_stride);
   const Laid grad = lay<T>(space, jobs, a.grad, a.rows, a.dim, a.grad_stride);
-  const Laid down = lay<T>(space, jobs, a.down, a.dim, a.hidden, a.down_stride);
+  const Laid down = turn_weights ? lay_turned<T>(space, turned, a.down, a.dim, a.hidden, a.down_stride)
+                                 : lay<T>(space, jobs, a.down, a.dim, a.hidden, a.down_stride);
   Laid x = {}, gate = {}, up = {};
   if (a.dgate || a.dup) x = lay<T>(space, jobs, a.x, a.rows, a.dim, a.x_stride);
-  if (a.dx) {
+  if (a.dx && turn_weights) {
+    gate = lay_turned<T>(space, turned, a.gate, a.hidden, a.dim, a.gate_stride);
+    up = lay_turned<T>(space, turned, a.up, a.hidden, a.dim, a.up_stride);
+  } else if (a.dx) {
     gate = lay<T>(space, jobs, a.gate, a.hidden, a.dim, a.gate_stride, copy);
     up = lay<T>(space, jobs, a.up, a.hidden, a.dim, a.up_stride, copy);
   }
@@ -81,23 +92,24 @@ int gradient(const MgbFeedForwardGradient& a, Space& space, hipStream_t stream, 
   inner.sources = 1;
   inner.pairs = Kind<T>::kPairs;
   inner.depth = dim;
-  inner.hidden_stride = hidden;
-  inner.hidden_part = a.rows * hidden;
-  inner.gradient_second = a.rows * hidden;
-  inner.gradient_part = 2 * a.rows * hidden;
+  inner.hidden_columns = hidden;
+  inner.hidden_stride = inner_stride(hidden);
+  inner.hidden_part = a.rows * inner.hidden_stride;
+  inner.gradient_second = inner.hidden_part;
+  inner.gradient_part = 2 * inner.hidden_part;
   inner.dgate = space.take(inner.gradient_part * kParts * 2);
-  const Laid dgate = {inner.dgate, hidden * 2, inner.gradient_part * 2};
-  const Laid dup = {inner.dgate + inner.gradient_second * 2, hidden * 2, inner.gradient_part * 2};
+  const Laid dgate = {inner.dgate, inner.hidden_stride * 2, inner.gradient_part * 2};
+  const Laid dup = {inner.dgate + inner.gradient_second * 2, inner.hidden_stride * 2, inner.gradient_part * 2};
   Laid middle = {};
   if (a.ddown) {
     inner.hidden = space.take(inner.hidden_part * kParts * 2);
-    middle = {inner.hidden, hidden * 2, inner.hidden_part * 2};
+    middle = {inner.hidden, inner.hidden_stride * 2, inner.hidden_part * 2};
   }
   inner.kept = const_cast<float*>(a.kept);
   inner.true_columns = a.hidden;
   inner.activation = a.activation;
   inner.job[0].left = operand(grad, a.rows, dim);
-  inner.job[0].right = operand(down, hidden, a.dim);
+  inner.job[0].right = turn_weights ? operand(down, a.hidden, dim) : operand(down, hidden, a.dim);
   inner.job[0].rows = a.rows;
   inner.job[0].columns = hidden;
   const Size inner_size = choose(inner, false);
@@ -111,7 +123,7 @@ int gradient(const MgbFeedForwardGradient& a, Space& space, hipStream_t stream, 
     input.pairs = Kind<T>::kPairs;
     input.depth = hidden;
     input.job[0].left = operands(dgate, dup, a.rows, hidden);
-    input.job[0].right = operands(gate, up, dim, a.hidden);
+    input.job[0].right = turn_weights ? operands(gate, up, a.dim, hidden) : operands(gate, up, dim, a.hidden);
     input.job[0].out = a.dx;
     input.job[0].out_stride = a.dim;
     input.job[0].rows = a.rows;
@@ -144,8 +156,14 @@ int gradient(const MgbFeedForwardGradient& a, Space& space, hipStream_t stream, 
   }
   if (!run) return 0;
   lay_out<T>(jobs, stream);
-  launch_product<E, false, true, Slope<T>>(inner, inner_size, stream);
-  if (a.dx) store_product<E, T, false, true>(input, input_size, stream);
+  turn<T>(turned, stream);
+  if (turn_weights) {
+    launch_product<E, false, false, Slope<T>>(inner, inner_size, stream);
+    if (a.dx) store_product<E, T, false, false>(input, input_size, stream);
+  } else if constexpr (sizeof(T) == 2) {
+    launch_product<E, false, true, Slope<T>>(inner, inner_size, stream);
+    if (a.dx) store_product<E, T, false, true>(input, input_size, stream);
+  }
   if (matrices) store_product<E, T, true, true>(weights, weights_size, stream);
   MGB_LAUNCH_CHECK("feed forward gradient");
   return 0;

@@ -1,0 +1,334 @@
+// Products with few rows (a request's, a single token's), out = x w^T: bound by the
+// reading of w, once, and by the launch.
+//
+// A workgroup has 16 rows of w (result columns), its waves a share of the depth
+// each, in units of one or four instructions (32 or 128 values), whose loads are all
+// in flight; the waves' sums meet in LDS.  Operands go from memory to registers in the matrix instruction's
+// layout, whatever their alignment, and become bfloat16 or binary16 there: binary32
+// values three bfloat16 each (six instructions a product), blocks of 8 bits the values
+// they stand for, exactly, and x, where the other operand is blocks, is rounded to
+// blocks on the way (a block is a unit, and lies in the registers of four lanes).
+#pragma once
+#include "feed_forward.hpp"
+
+namespace mgb {
+namespace block {
+
+constexpr int kMostFewRows = 32;
+
+struct Few {
+  const void* x;
+  const void* w[2];              // the second for the dual form
+  const uint8_t *x_scales, *w_scales[2];
+  int64_t x_stride, w_stride[2];  // elements
+  int64_t x_scale_stride, w_scale_stride;
+  int64_t rows, columns, depth;
+  void* out;                     // (rows, columns) without gaps
+  float* kept;                   // (rows, 2, columns) or null
+  int activation;
+};
+
+// How an operand lies: values of T; e4m3 blocks; x of T that is rounded to blocks.
+template <typename T>
+struct Plain {
+  using Type = T;
+  static constexpr int kParts = Kind<T>::kParts;
+};
+struct InBlocks {
+  using Type = uint8_t;
+  static constexpr int kParts = 1;
+};
+template <typename T>
+struct Rounded {
+  using Type = T;
+  static constexpr int kParts = 1;
+};
+
+// The exponent + 127 of the smallest power of two that takes `largest` to at most
+// 448 = 1.75 2^8; 127 where there is none.
+__device__ __forceinline__ uint32_t scale_of(float largest) {
+  const uint32_t bits = __float_as_uint(largest);
+  const int exponent = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return largest == 0.0f ? 127u : exponent > 0 ? (uint32_t)exponent : 0u;
+}
+
+__device__ __forceinline__ float scale_value(uint32_t scale) {  // 2^(scale - 127)
+  return __uint_as_float(scale ? scale << 23 : 0x400000u);
+}
+
+// Eight values as e4m3, rounded to nearest even; infinities and NaN become its NaN.
+__device__ __forceinline__ uint2 round_eight(const float* v, float factor) {
+  int word[2] = {};
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    word[w] = __builtin_amdgcn_cvt_pk_fp8_f32(v[w * 4] * factor, v[w * 4 + 1] * factor, word[w], false);
+    word[w] = __builtin_amdgcn_cvt_pk_fp8_f32(v[w * 4 + 2] * factor, v[w * 4 + 3] * factor, word[w], true);
+  }
+  return {(uint32_t)word[0], (uint32_t)word[1]};
+}
+
+// What eight e4m3 values times 2^(scale - 127) are, as bfloat16 (whose steps end at 2^-133).
+__device__ __forceinline__ product::bf16x8 widen_eight(uint2 bytes, uint32_t scale) {
+  const float factor = scale_value(scale);
+  product::bf16x8 v;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) {
+    const int word = (int)(w ? bytes.y : bytes.x);
+    const auto low = __builtin_amdgcn_cvt_pk_f32_fp8(word, false), high = __builtin_amdgcn_cvt_pk_f32_fp8(word, true);
+    v[w * 4] = (__bf16)(low[0] * factor);
+    v[w * 4 + 1] = (__bf16)(low[1] * factor);
+    v[w * 4 + 2] = (__bf16)(high[0] * factor);
+    v[w * 4 + 3] = (__bf16)(high[1] * factor);
+  }
+  return v;
+}
+
+// A unit of 16 rows: lane l has 8 values of row l % 16 for each of kSteps instructions.
+template <class Kind_, int kSteps>
+struct Unit {
+  using T = typename Kind_::Type;
+  static constexpr bool kBlocks = std::is_same_v<Kind_, InBlocks>;
+  // 16 bytes a lane and load: 8 16-bit values, half of 8 binary32 ones, 16 of 8 bits.
+  static constexpr int kLoads = kBlocks ? 2 : kSteps * (int)sizeof(T) / 2;
+  static_assert(kSteps == 4 || !kBlocks, "a block is a unit");
+  uint4 raw[kLoads];
+  uint32_t scale;
+
+  // Lane l / 16's 8 values of instruction s begin here; the same for both operands.
+  static __device__ __forceinline__ int place(int s, int quarter, bool blocks) {
+    return blocks ? s / 2 * 64 + quarter * 16 + s % 2 * 8 : s * 32 + quarter * 8;
+  }
+  // Rows beyond the last are read as zeros, as is the depth's end.
+  __device__ __forceinline__ void load(const T* row, const uint8_t* scales, int64_t unit, int64_t depth, bool there,
+                                       int quarter, bool with_blocks) {
+    const int64_t begin = unit * (32 * kSteps);
+    if constexpr (kBlocks) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        raw[k] = there ? *(const uint4*)(row + begin + k * 64 + quarter * 16) : uint4{};
+      scale = there ? scales[unit] : 127u;
+    } else {
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const int64_t at = begin + place(s, quarter, with_blocks);
+        uint4 piece[sizeof(T) / 2] = {};
+        if (there && at + 8 <= depth) {
+          __builtin_memcpy(piece, row + at, sizeof(piece));
+        } else if (there && at < depth) {
+          T v[8] = {};
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (at + e < depth) v[e] = row[at + e];
+          __builtin_memcpy(piece, v, sizeof(piece));
+        }
+#pragma unroll
+        for (int k = 0; k < (int)sizeof(T) / 2; ++k) raw[s * (sizeof(T) / 2) + k] = piece[k];
+      }
+    }
+  }
+  __device__ __forceinline__ void values(int s, float* v) const {
+    T t[8];
+    __builtin_memcpy(t, &raw[s * (sizeof(T) / 2)], sizeof(t));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = (float)t[e];
+  }
+};
+
+// x rounded to blocks: a unit's scale, of the four lanes that hold a row's.
+template <class Kind_, int kSteps>
+__device__ __forceinline__ void find_scale(Unit<Kind_, kSteps>& u) {
+  if constexpr (std::is_same_v<Kind_, Rounded<typename Kind_::Type>>) {
+    float largest = 0.0f;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      float v[8];
+      u.values(s, v);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.0f);
+    }
+    largest = fmaxf(largest, __shfl_xor(largest, 16, kWave));
+    largest = fmaxf(largest, __shfl_xor(largest, 32, kWave));
+    u.scale = scale_of(largest);
+  }
+}
+
+// Instruction s's operand of a unit, in parts, from what was loaded.
+template <class Kind_, int kSteps>
+__device__ __forceinline__ void operand_of(const Unit<Kind_, kSteps>& u, int s, product::int4v* out) {
+  if constexpr (std::is_same_v<Kind_, InBlocks>) {
+    const uint2 bytes = s % 2 ? uint2{u.raw[s / 2].z, u.raw[s / 2].w} : uint2{u.raw[s / 2].x, u.raw[s / 2].y};
+    out[0] = __builtin_bit_cast(product::int4v, widen_eight(bytes, u.scale));
+  } else if constexpr (std::is_same_v<Kind_, Rounded<typename Kind_::Type>>) {
+    float v[8];
+    u.values(s, v);
+    const uint2 bytes = round_eight(v, __uint_as_float((254u - u.scale) << 23));
+    out[0] = __builtin_bit_cast(product::int4v, widen_eight(bytes, u.scale));
+  } else if constexpr (Kind_::kParts == 3) {
+    float v[8];
+    u.values(s, v);
+    product::bf16x8 part[3];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      __bf16 three[3];
+      split_parts(v[e], three);
+#pragma unroll
+      for (int q = 0; q < 3; ++q) part[q][e] = three[q];
+    }
+#pragma unroll
+    for (int q = 0; q < 3; ++q) out[q] = __builtin_bit_cast(product::int4v, part[q]);
+  } else {
+    out[0] = __builtin_bit_cast(product::int4v, u.raw[s]);
+  }
+}
+
+template <bool kHalf>
+__device__ __forceinline__ float4v multiply_one(product::int4v w, product::int4v x, float4v sum) {
+  if constexpr (kHalf)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(product::f16x8, w), __builtin_bit_cast(product::f16x8, x),
+                                                  sum, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(product::bf16x8, w),
+                                                   __builtin_bit_cast(product::bf16x8, x), sum, 0, 0, 0);
+}
+
+// kTiles of 16 rows of x; kDual: out = act(x w0^T) (x w1^T).
+template <class X, class W, typename Out, int kTiles, bool kDual, int kWaves, int kSteps>
+__global__ __launch_bounds__(kWaves* kWave) void k_few(Few p) {
+  constexpr int kMatrices = kDual ? 2 : 1;
+  constexpr bool kBlocks = std::is_same_v<W, InBlocks>;
+  static_assert(X::kParts == W::kParts, "both in as many parts");
+  __shared__ float4v shared[kWaves][kMatrices][kTiles][kWave];
+  using XT = typename X::Type;
+  using WT = typename W::Type;
+  const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int quarter = lane / 16;
+  const int64_t column0 = (int64_t)blockIdx.x * 16, column = column0 + lane % 16;
+  const bool column_there = column < p.columns;
+  const WT* w[kMatrices];
+  const uint8_t* w_scales[kMatrices];
+#pragma unroll
+  for (int m = 0; m < kMatrices; ++m) {
+    w[m] = (const WT*)p.w[m] + (column_there ? column * p.w_stride[m] : 0);
+    w_scales[m] = kBlocks ? p.w_scales[m] + (column_there ? column * p.w_scale_stride : 0) : nullptr;
+  }
+  const XT* x[kTiles];
+  const uint8_t* x_scales[kTiles];
+  bool row_there[kTiles];
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t) {
+    const int64_t row = t * 16 + lane % 16;
+    row_there[t] = row < p.rows;
+    x[t] = (const XT*)p.x + (row_there[t] ? row * p.x_stride : 0);
+    x_scales[t] = std::is_same_v<X, InBlocks> ? p.x_scales + (row_there[t] ? row * p.x_scale_stride : 0) : nullptr;
+  }
+  float4v sum[kMatrices][kTiles] = {};
+  const int64_t units = (p.depth + 32 * kSteps - 1) / (32 * kSteps);
+  int64_t unit = units * wave / kWaves;
+  const int64_t end = units * (wave + 1) / kWaves;
+  Unit<W, kSteps> next_w[kMatrices];
+  Unit<X, kSteps> next_x[kTiles];
+  auto fetch = [&] {
+#pragma unroll
+    for (int m = 0; m < kMatrices; ++m) next_w[m].load(w[m], w_scales[m], unit, p.depth, column_there, quarter, kBlocks);
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) next_x[t].load(x[t], x_scales[t], unit, p.depth, row_there[t], quarter, kBlocks);
+  };
+  // The next unit's loads are on their way while one is multiplied, where the
+  // registers hold both.
+  constexpr int kRaw = 4 * (kMatrices * Unit<W, kSteps>::kLoads + kTiles * Unit<X, kSteps>::kLoads);
+  constexpr bool kAhead = 2 * kRaw <= (kWaves > 8 ? 64 : 192);
+  if (kAhead && unit < end) fetch();
+  while (unit < end) {
+    if constexpr (!kAhead) fetch();
+    Unit<W, kSteps> this_w[kMatrices];
+    Unit<X, kSteps> this_x[kTiles];
+#pragma unroll
+    for (int m = 0; m < kMatrices; ++m) this_w[m] = next_w[m];
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) this_x[t] = next_x[t];
+    ++unit;
+    if (kAhead && unit < end) fetch();
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) find_scale(this_x[t]);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      product::int4v of_w[kMatrices][W::kParts];
+#pragma unroll
+      for (int m = 0; m < kMatrices; ++m) operand_of(this_w[m], s, of_w[m]);
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t) {
+        product::int4v of_x[X::kParts];
+        operand_of(this_x[t], s, of_x);
+#pragma unroll
+        for (int pair = 0; pair < (X::kParts == 3 ? Kind<float>::kPairs : 1); ++pair) {
+          const int xp = X::kParts == 3 ? product::left_part(pair) : 0, wp = X::kParts == 3 ? product::right_part(pair) : 0;
+#pragma unroll
+          for (int m = 0; m < kMatrices; ++m)
+            sum[m][t] = multiply_one<std::is_same_v<X, Plain<_Float16>>>(of_w[m][wp], of_x[xp], sum[m][t]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 0; m < kMatrices; ++m)
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) shared[wave][m][t][lane] = sum[m][t];
+  __syncthreads();
+  // A lane joins four columns of a row.
+  for (int at = threadIdx.x; at < kTiles * kWave; at += kWaves * kWave) {
+    const int t = at / kWave, l = at % kWave;
+    float4v total[kMatrices];
+#pragma unroll
+    for (int m = 0; m < kMatrices; ++m) {
+      total[m] = shared[0][m][t][l];
+#pragma unroll
+      for (int k = 1; k < kWaves; ++k) total[m] += shared[k][m][t][l];
+    }
+    const int64_t row = t * 16 + l % 16, first = column0 + l / 16 * 4;
+    if (row >= p.rows) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (first + e >= p.columns) continue;
+      float v = total[0][e];
+      if constexpr (kDual) {
+        if (p.kept) {
+          p.kept[row * 2 * p.columns + first + e] = total[0][e];
+          p.kept[(row * 2 + 1) * p.columns + first + e] = total[kMatrices - 1][e];
+        }
+        v = activate<sizeof(Out) == 4>(v, p.activation) * total[kMatrices - 1][e];
+      }
+      ((Out*)p.out)[row * p.columns + first + e] = (Out)v;
+    }
+  }
+}
+
+template <class X, class W, typename Out, bool kDual>
+void few_rows(const Few& p, hipStream_t stream) {
+  const uint32_t groups = (uint32_t)((p.columns + 15) / 16);
+  // Waves for every unit, up to as many as the registers of their loads allow; units of
+  // one instruction where there are fewer of four than waves.
+  constexpr int kMost = kDual ? 8 : 16;
+  constexpr bool kBlocks = std::is_same_v<W, InBlocks>;
+  auto launch = [&](auto tiles, auto waves, auto steps) {
+    constexpr int kWaves = decltype(waves)::value;
+    k_few<X, W, Out, decltype(tiles)::value, kDual, kWaves, decltype(steps)::value><<<groups, kWaves * kWave, 0, stream>>>(p);
+  };
+  auto with_tiles = [&](auto tiles) {
+    using Four = std::integral_constant<int, 4>;
+    using Most = std::integral_constant<int, kMost>;
+    if constexpr (kBlocks) {
+      if (p.depth > 512) launch(tiles, Most{}, Four{});
+      else launch(tiles, Four{}, Four{});
+    } else {
+      using One = std::integral_constant<int, 1>;
+      if (p.depth <= 128) launch(tiles, Four{}, One{});
+      else if (sizeof(typename X::Type) == 4 || p.depth < 128 * kMost) launch(tiles, Most{}, One{});
+      else launch(tiles, Most{}, Four{});
+    }
+  };
+  if (p.rows <= 16) with_tiles(std::integral_constant<int, 1>{});
+  else with_tiles(std::integral_constant<int, 2>{});
+}
+
+}  // namespace block
+}  // namespace mgb

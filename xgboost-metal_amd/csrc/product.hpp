@@ -6,13 +6,15 @@
 // regions, the upper and lower half of the tile's rows (A0, A1) and of its columns
 // (B0, B1), two steps of each.  A wave has a part of all four quarters and works a
 // step off in four phases, each one quarter:
-//   phase      reads into registers   multiplies   fills (from memory)
-//     0        A0 of this step        A0 B0        B0 of the step after the next
-//     1        B1                     A0 B1        A0
-//     2        A1                     A1 B1        B1
-//     3        B0 of the next step    A1 B0        A1
-// so a region is filled again in the phase after the one that read it, and has six
-// phases to arrive.  With eight waves, two a SIMD, the second four are half a phase
+//   phase  multiplies   reads into registers      fills (from memory, two steps on)
+//     0      A0 B0       B1                        A0
+//     1      A0 B1       A1                        B0
+//     2      A1 B1       A0 of the next step       B1
+//     3      A1 B0       B0 of the next step       A1
+// What a phase reads is multiplied in the next; a region is filled again two phases
+// after the one that read it, and has five phases to arrive.  (Turned operands, below,
+// are read in the phase that multiplies them, each a phase later, and filled again in
+// the phase after.)  With eight waves, two a SIMD, the second four are half a phase
 // behind: while one wave of a SIMD multiplies, the other reads, and a barrier
 // between the halves keeps them so.
 //
@@ -87,6 +89,7 @@ struct Params {
   char* hidden;              // act(gate) up, in parts
   char* dgate;               // [2][row][stride], in parts: dgate, then dup
   int64_t hidden_stride, hidden_part, gradient_part, gradient_second;  // elements
+  int64_t hidden_columns;    // whole chunks of 8, the rest zeros
   int64_t true_columns;      // columns of `kept`
   int activation;
 };
@@ -117,22 +120,15 @@ struct Fragment {
   }
 };
 
-__device__ __forceinline__ void hold(Fragment& f) { asm volatile("" : "+v"(f.v)); }
-
-// sum[4 (lane / 16) + e of right][lane % 16 of left]
+// sum[4 (lane / 16) + e of right][lane % 16 of left], of half a step
 template <typename E>
-__device__ __forceinline__ float4v multiply(const Fragment& left, const Fragment& right, float4v sum) {
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    if constexpr (std::is_same_v<E, __bf16>) {
-      sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, right.half(h)),
-                                                    __builtin_bit_cast(bf16x8, left.half(h)), sum, 0, 0, 0);
-    } else {
-      sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, right.half(h)),
-                                                   __builtin_bit_cast(f16x8, left.half(h)), sum, 0, 0, 0);
-    }
-  }
-  return sum;
+__device__ __forceinline__ float4v multiply(int4v left, int4v right, float4v sum) {
+  if constexpr (std::is_same_v<E, __bf16>)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, right), __builtin_bit_cast(bf16x8, left), sum,
+                                                   0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, right), __builtin_bit_cast(f16x8, left), sum, 0,
+                                                  0, 0);
 }
 
 // The scales' lowest bytes count.
@@ -180,9 +176,30 @@ __device__ __forceinline__ bool find_tile(const Params& p, uint32_t* job, uint32
   return true;
 }
 
+// Straight columns in pairs of 16 x 16 tiles: column 8 a + 4 j + b of 32 is row 4 a + b of
+// tile j, so that a lane's sums of a pair are 8 columns that follow each other.
+template <bool kTurned, typename S>
+constexpr bool paired() { return !kTurned && S::kTilesN % 2 == 0; }
+// The chunks of a row are permuted by this, which differs among the 8 rows that lanes
+// read together: 8 that follow each other, or 8 a + b for a pair's.
+template <bool kPairs>
+__device__ __forceinline__ int straight_key(int row) {
+  return kPairs ? (row & 3) | (row >> 3 & 1) << 2 : row & 7;
+}
+
+// How the 32-byte granules of a turned row in LDS are permuted: the 32 lanes that
+// are served together read four rows from 4 k on and the four 8 rows further, 32 bytes
+// of each, which are to lie in different banks (of 256 bytes) whatever the rows' length.
+template <int kGranules>
+__device__ __forceinline__ int turned_key(int row) {
+  if constexpr (kGranules == 8) return (row & 3) | (row >> 3 & 1) << 2;
+  if constexpr (kGranules == 4) return (row >> 1 & 1) | (row >> 3 & 1) << 1;
+  return row >> 3 & 1;
+}
+
 // What is read of an operand: a cursor that goes over its steps, the products of
 // the parts, and the matrices.  All of it is the same for a workgroup's lanes.
-template <bool kTurned, int kHalf, int kLoads, int kWaves>
+template <bool kTurned, bool kPairs, int kHalf, int kLoads, int kWaves>
 struct Reader {
   const char* from[2];       // the regions' first rows, now
   int64_t left[2];           // bytes from there to the end of what the region has
@@ -196,13 +213,13 @@ struct Reader {
     for (int q = 0; q < kLoads; ++q) {
       if constexpr (!kTurned) {
         const int row = (q * kWaves + wave) * 8 + lane / 8;
-        chunk = ((lane % 8) ^ (row & 7)) * 16;
+        chunk = ((lane % 8) ^ straight_key<kPairs>(row)) * 16;  // (the same for all q)
         offset[q] = (uint32_t)(row * row_stride) + chunk;
       } else {
         // A row of kHalf values is kHalf / 8 chunks.
         constexpr int kChunks = kHalf / 8;
         const int slot = (q * kWaves + wave) * kWave + lane, row = slot / kChunks, at = slot % kChunks;
-        offset[q] = (uint32_t)(row * row_stride) + ((at ^ (2 * (row & 7) % kChunks)) * 16);
+        offset[q] = (uint32_t)(row * row_stride) + ((at ^ (2 * turned_key<kChunks / 2>(row))) * 16);
       }
     }
   }
@@ -217,11 +234,13 @@ struct Scales {
   static constexpr int kM = S::kWavesM * 16 * kWordsM, kN = S::kWavesN * 16 * kWordsN;
   static constexpr int kBytes = (kM + kN) * 4;  // a step's
 
-  template <int kHalf, int kWaves, int kRows, int kTiles, int kWords>
+  template <int kHalf, int kRows, int kTiles, int kWords, bool kPairs>
   static __device__ __forceinline__ int place(int row) {  // byte
-    const int half = row / kHalf, in = row % kHalf, wave = in / kRows, tile = in % kRows / 16;
+    const int half = row / kHalf, wave = row % kHalf / kRows, in = row % kRows;
+    const int tile = kPairs ? in / 32 * 2 + in / 4 % 2 : in / 16;
+    const int lane = kPairs ? in % 32 / 8 * 4 + in % 4 : in % 16;
     const int byte = half * kTiles + tile;
-    return ((wave * 16 + in % 16) * kWords + byte / 4) * 4 + byte % 4;
+    return ((wave * 16 + lane) * kWords + byte / 4) * 4 + byte % 4;
   }
   static __device__ __forceinline__ void fill(char* panel, const Params& p, int64_t row0, int64_t rows, int64_t column0,
                                               int64_t columns, bool dual, uint32_t begin, uint32_t end) {
@@ -232,12 +251,12 @@ struct Scales {
       int to;
       if (row < S::kTileM) {
         if (row0 + row < rows) from = p.left_scales + (row0 + row) * p.left_scale_stride;
-        to = place<S::kHalfM, S::kWavesM, S::kRowsM, S::kTilesM, kWordsM>(row);
+        to = place<S::kHalfM, S::kRowsM, S::kTilesM, kWordsM, false>(row);
       } else {
         const int r = row - S::kTileM;
         const int64_t column = column0 + (dual ? r % S::kHalfN : r);
         if (column < columns) from = p.right_scales[dual ? r / S::kHalfN : 0] + column * p.right_scale_stride;
-        to = kM * 4 + place<S::kHalfN, S::kWavesN, S::kRowsN, S::kTilesN, kWordsN>(r);
+        to = kM * 4 + place<S::kHalfN, S::kRowsN, S::kTilesN, kWordsN, paired<false, S>()>(r);
       }
       // (Rows are whole words: a word that begins in a row ends in it.)
       const uint32_t word = from ? *(const uint32_t*)(from + begin + quad * 4) : 0x7f7f7f7fu;
@@ -254,6 +273,10 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_product(Params p) {
   constexpr int kBytes = element_bytes<E>();
   constexpr int kStep = kStepBytes / kBytes;  // elements
   static_assert(!k8 || (!kLeftTurned && !kRightTurned), "8-bit operands lie straight");
+  // Straight operands are read a phase before they are multiplied (A0 and A1 in
+  // registers of their own); the turned ones' addresses leave no registers for that.
+  constexpr bool kAhead = !kLeftTurned && !kRightTurned;
+  constexpr bool kPairs = paired<kRightTurned, S>();
   __shared__ __attribute__((aligned(1024))) char lds[S::kBytes + (k8 ? Scales<S>::kBytes * kScaleSteps : 0)];
 
   uint32_t which, ti, tj, split;
@@ -263,8 +286,8 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_product(Params p) {
   const int wm = wave / S::kWavesN, wn = wave % S::kWavesN;
 
   // ---- memory to LDS
-  Reader<kLeftTurned, S::kHalfM, S::kLoadsM, S::kWaves> left;
-  Reader<kRightTurned, S::kHalfN, S::kLoadsN, S::kWaves> right;
+  Reader<kLeftTurned, false, S::kHalfM, S::kLoadsM, S::kWaves> left;
+  Reader<kRightTurned, kPairs, S::kHalfN, S::kLoadsN, S::kWaves> right;
   const int64_t row0 = (int64_t)ti * S::kTileM;
   // The dual form has the columns of one matrix in B0 and the same ones of the other in B1.
   const int64_t column0 = (int64_t)tj * (Finish::kDual ? S::kHalfN : S::kTileN);
@@ -362,130 +385,169 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_product(Params p) {
   auto fetch_right = [&](int r, int stage) { fetch(right, r, right_region(r, stage), RightTurned{}, LoadsN{}); };
 
   // ---- LDS to registers
-  // Straight: lane l has row l % 16, chunks l / 16 and l / 16 + 4 of it.  Turned: its 8
-  // values of a half are 8 l / 16 .. + 7 of the depth, by two reads of 4 x 16 that
-  // transpose: lane l gives the place of row l % 16 / 4, columns l % 4 * 4 .. + 3.
-  auto straight_place = [&](int row, int half) {
-    return (row + lane % 16) * kStepBytes + (((lane / 16) ^ (lane & 7)) ^ (half * 4)) * 16;
-  };
-  auto read = [&](Fragment* f, const char* region, int first_row, auto tiles, auto turned, auto half_rows) {
+  // Straight: lane l has row l % 16 (of a pair 8 (l % 16 / 4) + l % 4), chunks l / 16 and
+  // l / 16 + 4 of it.  Turned: its 8 values of a half are 8 l / 16 .. + 7 of the depth, by
+  // two reads of 4 x 16 that transpose: lane l gives the place of row l % 16 / 4, columns
+  // l % 4 * 4 .. + 3.
+  auto read = [&](const char* region, int first_row, int t, auto turned, auto pairs, auto half_rows) {
+    int4v part[2];
 #pragma unroll
-    for (int t = 0; t < decltype(tiles)::value; ++t) {
-      int4v part[2];
+    for (int h = 0; h < 2; ++h) {
+      if constexpr (!decltype(turned)::value) {
+        constexpr bool kIn = decltype(pairs)::value;
+        const int row = kIn ? lane % 16 / 4 * 8 + lane % 4 : lane % 16;
+        const int chunk = (lane / 16 ^ (lane & 7)) ^ (h * 4);
+        part[h] = *(const int4v*)(region + (first_row + row) * kStepBytes + chunk * 16 +
+                                  (kIn ? t / 2 * 32 + t % 2 * 4 : t * 16) * kStepBytes);
+      } else {
+        constexpr int kPitch = decltype(half_rows)::value * 2, kGranules = decltype(half_rows)::value / 16;
+        short4v four[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        if constexpr (!decltype(turned)::value) {
-          part[h] = *(const int4v*)(region + straight_place(first_row, h) + t * 16 * kStepBytes);
-        } else {
-          constexpr int kPitch = decltype(half_rows)::value * 2, kGranules = decltype(half_rows)::value / 16;
-          short4v four[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int row = h * 32 + lane / 16 * 8 + j * 4 + lane % 16 / 4;
-            const int granule = (first_row / 16 + t) ^ ((row & 7) % kGranules);
-            four[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) short4v*)(region + row * kPitch + granule * 32 + lane % 4 * 8));
-          }
-          __builtin_memcpy(&part[h], four, sizeof(four));
+        for (int j = 0; j < 2; ++j) {
+          const int row = h * 32 + lane / 16 * 8 + j * 4 + lane % 16 / 4;
+          const int granule = (first_row / 16 + t) ^ turned_key<kGranules>(row);
+          four[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) short4v*)(region + row * kPitch + granule * 32 + lane % 4 * 8));
         }
+        __builtin_memcpy(&part[h], four, sizeof(four));
       }
-      f[t].v = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
     }
+    Fragment f;
+    f.v = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
+    return f;
   };
-  using TilesM = std::integral_constant<int, S::kTilesM>;
-  using TilesN = std::integral_constant<int, S::kTilesN>;
   using HalfM = std::integral_constant<int, S::kHalfM>;
   using HalfN = std::integral_constant<int, S::kHalfN>;
-  Fragment a[S::kTilesM], b[2][S::kTilesN];
-  auto read_left = [&](int r, int stage) { read(a, left_region(r, stage), wm * S::kRowsM, TilesM{}, LeftTurned{}, HalfM{}); };
-  auto read_right = [&](Fragment* f, int r, int stage) {
-    read(f, right_region(r, stage), wn * S::kRowsN, TilesN{}, RightTurned{}, HalfN{});
+  Fragment a[kAhead ? 2 : 1][S::kTilesM], b[2][S::kTilesN];
+  auto read_left = [&](int r, int stage, int t) { return read(left_region(r, stage), wm * S::kRowsM, t, LeftTurned{}, std::false_type{}, HalfM{}); };
+  auto read_right = [&](int r, int stage, int t) {
+    return read(right_region(r, stage), wn * S::kRowsN, t, RightTurned{}, std::bool_constant<kPairs>{}, HalfN{});
   };
 
   // A row's exponents of a step: bytes kTilesM x + i of words that lanes l % 16 of the
   // rows' waves read, for all of its steps.
   using Panel = Scales<S>;
-  uint32_t left_scales[Panel::kWordsM] = {}, right_scales[Panel::kWordsN] = {};
+  struct Words {
+    uint32_t left[Panel::kWordsM], right[Panel::kWordsN];
+  };
+  Words scales = {}, next_scales = {};
   auto read_scales = [&](uint32_t step) {
-    const uint32_t* words = (const uint32_t*)(lds + S::kBytes) + step * (Panel::kBytes / 4);
-    __builtin_memcpy(left_scales, words + (wm * 16 + lane % 16) * Panel::kWordsM, sizeof(left_scales));
-    __builtin_memcpy(right_scales, words + Panel::kM + (wn * 16 + lane % 16) * Panel::kWordsN, sizeof(right_scales));
+    Words w = {};
+    if constexpr (k8) {
+      const uint32_t* words = (const uint32_t*)(lds + S::kBytes) + step * (Panel::kBytes / 4);
+      __builtin_memcpy(w.left, words + (wm * 16 + lane % 16) * Panel::kWordsM, sizeof(w.left));
+      __builtin_memcpy(w.right, words + Panel::kM + (wn * 16 + lane % 16) * Panel::kWordsN, sizeof(w.right));
+    }
+    return w;
   };
 
   float4v sum[2][2][S::kTilesM][S::kTilesN] = {};
+  // Tiles i and j of a quarter; without a 8-bit step, half of it.
+  auto multiply_tile = [&](int x, int y, int i, int j, int h, const Fragment& right) {
+    if constexpr (k8) {
+      const int l = x * S::kTilesM + i, r = y * S::kTilesN + j;
+      if (h == 0)
+        sum[x][y][i][j] = multiply8(a[kAhead ? x : 0][i], right, (int)(scales.left[l / 4] >> (l % 4 * 8)),
+                                    (int)(scales.right[r / 4] >> (r % 4 * 8)), sum[x][y][i][j]);
+    } else {
+      sum[x][y][i][j] = multiply<E>(a[kAhead ? x : 0][i].half(h), right.half(h), sum[x][y][i][j]);
+    }
+  };
+
+  // ---- the steps
+  constexpr int kFlight = (kAhead ? 5 : 6) * S::kLoadsM;  // loads issued after the region that is waited for
+  static_assert(S::kLoadsM == S::kLoadsN, "regions of one size");
+  auto order = [] { __builtin_amdgcn_sched_barrier(0); };
   // Matrix instructions have no order of their own among barriers and loads: empty
-  // statements that name their operands before and their results after hold them
-  // between a phase's two barriers.
-  auto multiply_quarter = [&](int x, int y, Fragment* f) {
-#pragma unroll
-    for (int i = 0; i < S::kTilesM; ++i) hold(a[i]);
-#pragma unroll
-    for (int j = 0; j < S::kTilesN; ++j) hold(f[j]);
-#pragma unroll
-    for (int i = 0; i < S::kTilesM; ++i)
-#pragma unroll
-      for (int j = 0; j < S::kTilesN; ++j) {
-        if constexpr (k8) {
-          const int l = x * S::kTilesM + i, r = y * S::kTilesN + j;
-          sum[x][y][i][j] = multiply8(a[i], f[j], (int)(left_scales[l / 4] >> (l % 4 * 8)),
-                                      (int)(right_scales[r / 4] >> (r % 4 * 8)), sum[x][y][i][j]);
-        } else {
-          sum[x][y][i][j] = multiply<E>(a[i], f[j], sum[x][y][i][j]);
-        }
-      }
+  // statements that name the sums hold them within a phase.
+  auto hold = [&](int x, int y) {
 #pragma unroll
     for (int i = 0; i < S::kTilesM; ++i)
 #pragma unroll
       for (int j = 0; j < S::kTilesN; ++j) asm volatile("" : "+v"(sum[x][y][i][j]));
   };
-
-  // ---- the steps
-  constexpr int kFlight = 3 * (S::kLoadsM + S::kLoadsN);  // loads issued after the region that is waited for
-  // The four quarters of a step, with B0 of this step in b[kStage] already.
-  auto phase_end = [&] {
-    __builtin_amdgcn_sched_barrier(0);
-    wait_loads<kFlight>();
-    wait_barrier();
-    __builtin_amdgcn_sched_barrier(0);
-    if constexpr (S::kAlternate) __builtin_amdgcn_s_setprio(1);
+  // The regions that the next phase reads are there, and what this one read is out of LDS.
+  auto arrived = [] {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xf70 | (kFlight & 15) | (kFlight >> 4) << 14);  // vmcnt(kFlight)
+    asm volatile("" ::: "memory");
   };
-  auto quarter_end = [&] {
-    if constexpr (S::kAlternate) {
-      __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_s_setprio(0);
+  auto taken = [] {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
+    asm volatile("" ::: "memory");
+  };
+  // The end of a phase, after its reads and loads are issued.
+  auto multiply_quarter = [&](int x, int y, const Fragment* right) {
+    order();
+    if constexpr (!kAhead) taken();
+    if constexpr (!kAhead || S::kAlternate) {
+      arrived();
       wait_barrier();
     }
-    __builtin_amdgcn_sched_barrier(0);
+    if constexpr (S::kAlternate) __builtin_amdgcn_s_setprio(1);
+    order();
+    hold(x, y);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {  // (those of one sum far apart: one waits for the other)
+#pragma unroll
+      for (int i = 0; i < S::kTilesM; ++i)
+#pragma unroll
+        for (int j = 0; j < S::kTilesN; ++j) multiply_tile(x, y, i, j, h, right[j]);
+      order();
+    }
+    hold(x, y);
+    order();
+    if constexpr (S::kAlternate) __builtin_amdgcn_s_setprio(0);
+    if constexpr (kAhead) taken();
+    if constexpr (kAhead && !S::kAlternate) arrived();
+    if constexpr (kAhead || S::kAlternate) wait_barrier();
+    order();
+  };
+  auto take_left = [&](int r, int stage) {
+#pragma unroll
+    for (int i = 0; i < S::kTilesM; ++i) a[kAhead ? r : 0][i] = read_left(r, stage, i);
+  };
+  auto take_right = [&](Fragment* to, int r, int stage) {
+#pragma unroll
+    for (int j = 0; j < S::kTilesN; ++j) to[j] = read_right(r, stage, j);
   };
   auto step = [&](auto stage_constant, uint32_t t) {
     constexpr int kStage = decltype(stage_constant)::value;
-    if constexpr (k8) read_scales(t);
-    read_left(0, kStage);
-    fetch_right(0, kStage);
-    phase_end();
-    multiply_quarter(0, 0, b[kStage]);
-    quarter_end();
-    read_right(b[1 - kStage], 1, kStage);
-    fetch_left(0, kStage);
-    phase_end();
-    multiply_quarter(0, 1, b[1 - kStage]);
-    quarter_end();
-    read_left(1, kStage);
-    fetch_right(1, kStage);
-    phase_end();
-    multiply_quarter(1, 1, b[1 - kStage]);
-    quarter_end();
-    read_right(b[1 - kStage], 0, 1 - kStage);
+    Fragment *const now = b[kStage], *const other = b[1 - kStage];
+    if constexpr (kAhead) {
+      take_right(other, 1, kStage);
+      fetch_left(0, kStage);
+      multiply_quarter(0, 0, now);
+      take_left(1, kStage);
+      fetch_right(0, kStage);
+      multiply_quarter(0, 1, other);
+      take_left(0, 1 - kStage);
+      fetch_right(1, kStage);
+      multiply_quarter(1, 1, other);
+    } else {
+      take_left(0, kStage);
+      fetch_right(0, kStage);
+      multiply_quarter(0, 0, now);
+      take_right(other, 1, kStage);
+      fetch_left(0, kStage);
+      multiply_quarter(0, 1, other);
+      take_left(1, kStage);
+      fetch_right(1, kStage);
+      multiply_quarter(1, 1, other);
+    }
+    take_right(other, 0, 1 - kStage);
+    next_scales = read_scales(t + 1);
     fetch_left(1, kStage);
     advance();
-    phase_end();
-    multiply_quarter(1, 0, b[kStage]);
-    quarter_end();
+    multiply_quarter(1, 0, now);
+    scales = next_scales;
   };
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
+    if constexpr (kAhead) fetch_left(0, s);
     fetch_right(0, s);
-    fetch_left(0, s);
+    if constexpr (!kAhead) fetch_left(0, s);
     fetch_right(1, s);
     fetch_left(1, s);
     advance();
@@ -497,7 +559,9 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_product(Params p) {
     wait_loads<kFlight>();
   }
   wait_barrier();
-  read_right(b[0], 0, 0);
+  scales = read_scales(0);
+  take_right(b[0], 0, 0);
+  if constexpr (kAhead) take_left(0, 0);
   wait_loads<kFlight>();
   wait_barrier();
   if constexpr (S::kAlternate)
@@ -513,58 +577,44 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_product(Params p) {
   // Nothing may land in LDS after the workgroup has ended.
   wait_loads<0>();
 
-  // ---- what becomes of the sums: through LDS, half of the rows at a time, so that a
-  // lane then has 8 columns of a row.  (16 bytes go to place c ^ row % 16 of a row.)
-  constexpr int kQuads = S::kTileN / 4;
-  float4v* const rows = (float4v*)lds;
+  // ---- what becomes of the sums: a lane has 4 or, of pairs, 8 columns of a row
   const Finish finish(p, job, split);
+  constexpr int kCount = kPairs ? 8 : 4;
 #pragma unroll
-  for (int x = 0; x < 2; ++x) {
-    wait_barrier();
+  for (int x = 0; x < 2; ++x)
 #pragma unroll
-    for (int i = 0; i < S::kTilesM; ++i)
+    for (int i = 0; i < S::kTilesM; ++i) {
+      const int64_t m = row0 + x * S::kHalfM + wm * S::kRowsM + i * 16 + lane % 16;
+      if (m >= job.rows) continue;
 #pragma unroll
-      for (int y = 0; y < 2; ++y)
+      for (int j = 0; j < S::kTilesN; j += kCount / 4) {
+        const int64_t n = column0 + wn * S::kRowsN + j * 16 + lane / 16 * kCount;
+        float v[2][kCount];
 #pragma unroll
-        for (int j = 0; j < S::kTilesN; ++j) {
-          const int row = wm * S::kRowsM + i * 16 + lane % 16;
-          const int quad = (y * S::kHalfN + wn * S::kRowsN + j * 16) / 4 + lane / 16;
-          rows[row * kQuads + (quad ^ lane % 16)] = sum[x][y][i][j];
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int e = 0; e < kCount; ++e) v[y][e] = sum[x][y][i][j + e / 4][e % 4];
+        if constexpr (Finish::kDual) {
+          finish.template operator()<kCount>(m, n, v[0], v[1]);
+        } else {
+#pragma unroll
+          for (int y = 0; y < 2; ++y) finish.template operator()<kCount>(m, n + y * S::kHalfN, v[y]);
         }
-    wait_loads<0>();
-    wait_barrier();
-    constexpr int kEights = (Finish::kDual ? S::kHalfN : S::kTileN) / 8;
-#pragma unroll 1
-    for (int at = threadIdx.x; at < S::kHalfM * kEights; at += S::kThreads) {
-      const int row = at / kEights, eight = at % kEights;
-      const int64_t m = row0 + x * S::kHalfM + row;
-      if (m >= job.rows) break;
-      float v[Finish::kDual ? 2 : 1][8];
-#pragma unroll
-      for (int y = 0; y < (Finish::kDual ? 2 : 1); ++y)
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const float4v four = rows[row * kQuads + ((y * (S::kHalfN / 4) + eight * 2 + q) ^ (row % 16))];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[y][q * 4 + e] = four[e];
-        }
-      if constexpr (Finish::kDual) finish(m, column0 + eight * 8, v[0], v[1]);
-      else finish(m, column0 + eight * 8, v[0]);
+      }
     }
-  }
 }
 
-// Eight values of a row, to the type rounded once; those beyond `columns` are not stored.
-template <typename T>
-__device__ __forceinline__ void store_eight(T* row, int64_t n, int64_t columns, const float* v) {
-  T r[8];
+// Values of a row, to the type rounded once; those beyond `columns` are not stored.
+template <int kCount, typename T>
+__device__ __forceinline__ void store_some(T* row, int64_t n, int64_t columns, const float* v) {
+  T r[kCount];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) r[e] = (T)v[e];
-  if (n + 8 <= columns) {
+  for (int e = 0; e < kCount; ++e) r[e] = (T)v[e];
+  if (n + kCount <= columns) {
     __builtin_memcpy(row + n, r, sizeof(r));
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (int e = 0; e < kCount; ++e)
       if (n + e < columns) row[n + e] = r[e];
   }
 }
@@ -576,8 +626,9 @@ struct Store {
   int64_t stride, columns;
   __device__ __forceinline__ Store(const Params&, const Job& job, uint32_t)
       : out((T*)job.out), stride(job.out_stride), columns(job.columns) {}
+  template <int kCount>
   __device__ __forceinline__ void operator()(int64_t m, int64_t n, const float* v) const {
-    store_eight(out + m * stride, n, columns, v);
+    store_some<kCount>(out + m * stride, n, columns, v);
   }
 };
 
@@ -588,8 +639,9 @@ struct Partial {
   int64_t columns;
   __device__ __forceinline__ Partial(const Params& p, const Job& job, uint32_t split)
       : out(p.partials + split * p.partial_size + job.partial), columns(job.columns) {}
+  template <int kCount>
   __device__ __forceinline__ void operator()(int64_t m, int64_t n, const float* v) const {
-    store_eight(out + m * columns, n, columns, v);
+    store_some<kCount>(out + m * columns, n, columns, v);
   }
 };
 
