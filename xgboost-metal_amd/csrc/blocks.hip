@@ -124,12 +124,11 @@ int multiply(T* out, const MgbBlocks& x, const MgbBlocks& weight, Space& space, 
   p.job[0].out_stride = weight.rows;
   p.job[0].rows = x.rows;
   p.job[0].columns = weight.rows;
-  const Size size = choose(p, false);
   if constexpr (sizeof(T) == 4) {
     const Laid left = widen(space, x, stream, run), right = widen(space, weight, stream, run);
     p.job[0].left = operand(left, x.rows, p.depth);
     p.job[0].right = operand(right, weight.rows, p.depth);
-    split_depth(p, size, space);
+    const Size size = choose_shares(p, space, false);
     if (run) store_product<__bf16, T, false, false>(p, size, stream);
   } else {
     p.job[0].left = operand8(x);
@@ -138,7 +137,7 @@ int multiply(T* out, const MgbBlocks& x, const MgbBlocks& weight, Space& space, 
     p.right_scales[0] = (const uint8_t*)weight.scales;
     p.left_scale_stride = x.scale_stride;
     p.right_scale_stride = weight.scale_stride;
-    split_depth(p, size, space, kBlock, product::kScaleSteps);
+    const Size size = choose_shares(p, space, false, kBlock, product::kScaleSteps);
     if (run) store_product<product::E4m3, T, false, false>(p, size, stream);
   }
   return 0;
@@ -205,7 +204,7 @@ int serve(const MgbBlockFeedForward& a, Space& space, hipStream_t stream, bool r
   p.activation = a.activation;
   p.job[0].rows = a.rows;
   p.job[0].columns = a.hidden;
-  const Size size = choose(p, true);
+  const Size size = choose(p, true, std::is_same_v<T, __bf16> ? kBlock : 64);
   if constexpr (std::is_same_v<T, __bf16>) {
     p.job[0].left = operand8(x);
     p.job[0].right = {{(const char*)a.gate.values, (const char*)a.up.values}, {a.gate.stride, a.up.stride}, 0, a.hidden, dim};
@@ -214,14 +213,12 @@ int serve(const MgbBlockFeedForward& a, Space& space, hipStream_t stream, bool r
     p.right_scales[1] = (const uint8_t*)a.up.scales;
     p.left_scale_stride = x.scale_stride;
     p.right_scale_stride = a.gate.scale_stride;
-    whole_depth(p, kBlock);
     if (run) launch_product<product::E4m3, false, false, GatedFloat>(p, size, stream);
   } else {
     const Laid left = widen(space, x, stream, run);
     const Laid gate = widen(space, a.gate, stream, run), up = widen(space, a.up, stream, run);
     p.job[0].left = operand(left, a.rows, dim);
     p.job[0].right = operands(gate, up, a.hidden, dim);
-    whole_depth(p);
     if (run) launch_product<__bf16, false, false, GatedFloat>(p, size, stream);
   }
   MgbBlocks h = {space.take(a.rows * hidden), space.take(a.rows * hidden_scales), a.rows, a.down.blocks, hidden, hidden_scales};

@@ -91,7 +91,6 @@ int forward(const MgbFeedForward& a, Space& space, hipStream_t stream, bool run)
   inner.job[0].rows = a.rows;
   inner.job[0].columns = hidden;
   const Size inner_size = choose(inner, true);
-  whole_depth(inner);
 
   Params outer = {};
   outer.jobs = 1;
@@ -104,8 +103,7 @@ int forward(const MgbFeedForward& a, Space& space, hipStream_t stream, bool run)
   outer.job[0].out_stride = a.dim;
   outer.job[0].rows = a.rows;
   outer.job[0].columns = a.dim;
-  const Size outer_size = choose(outer, false);
-  split_depth(outer, outer_size, space);
+  const Size outer_size = choose_shares(outer, space, false);
   if (!run) return 0;
   lay_out<T>(jobs, stream);
   launch_product<E, false, false, Gated<T>>(inner, inner_size, stream);

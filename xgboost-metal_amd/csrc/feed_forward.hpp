@@ -235,33 +235,92 @@ inline int64_t steps_of(const Params& p, int values) {
   return std::max<int64_t>(1, (p.depth + values - 1) / values) * p.pairs * p.sources;
 }
 
-// The size of the tiles: the largest that still gives most compute units one.
-inline Size choose(Params& p, bool dual) {
-  if (lay_tiles(p, kLarge, dual) >= 160) return kLarge;
-  if (lay_tiles(p, kMedium, dual) >= 160) return kMedium;
-  lay_tiles(p, kSmall, dual);
-  return kSmall;
+// Estimated times, in us, of a workgroup's step and of what comes before and after its
+// steps, with 1, 2, .. workgroups a compute unit (measured with 64 to 1,024 tiles and
+// depths of 512 to 4,096; turned operands' steps take a third longer).  Products of few
+// tiles are short of workgroups, those of many small ones of LDS' rate: the estimate
+// finds sizes and shares between.
+struct Rate {
+  int most;       // workgroups a compute unit
+  float step[4], fixed[4];
+};
+constexpr Rate kRates[3] = {{1, {1.42f}, {10.0f}},
+                            {2, {0.575f, 0.87f}, {6.4f, 8.8f}},
+                            {4, {0.346f, 0.446f, 0.6f, 0.748f}, {4.9f, 5.3f, 6.5f, 7.6f}}};
+constexpr int64_t kUnits = 256;  // compute units
+
+inline float estimate(Size size, int64_t workgroups, int64_t steps, bool turned) {
+  const Rate& r = kRates[size];
+  const int64_t each = (workgroups + kUnits - 1) / kUnits;
+  float time = 0.0f;
+  for (int64_t left = each; left > 0;) {  // rounds of r.most, the last of what is left
+    const int64_t rounds = left >= r.most ? left / r.most : 1, now = left >= r.most ? r.most : left;
+    time += rounds * (r.fixed[now - 1] + steps * r.step[now - 1] * (turned ? 1.3f : 1.0f));
+    left -= rounds * now;
+  }
+  return time;
 }
 
-// Shares of the depth, where there are few tiles: partial sums in binary32, added
-// in their order by k_join.
-inline void split_depth(Params& p, Size size, Space& space, int values = 64, int64_t most_steps = INT32_MAX) {
-  const int64_t steps = steps_of(p, values), groups = size == kLarge ? 256 : size == kMedium ? 512 : 1024;
-  int64_t splits = std::max<int64_t>(1, std::min(groups / p.tiles, steps / 8));
-  splits = std::max(splits, (steps + most_steps - 1) / most_steps);
-  p.steps_per_split = (uint32_t)((steps + splits - 1) / splits);
-  p.splits = (uint32_t)((steps + p.steps_per_split - 1) / p.steps_per_split);
+// The size of the tiles where the depth stays whole.
+inline Size choose(Params& p, bool dual, int values = 64) {
+  Size best = kSmall;
+  float least = INFINITY;
+  for (const Size size : {kLarge, kMedium, kSmall}) {
+    const float time = estimate(size, lay_tiles(p, size, dual), steps_of(p, values), false);
+    if (time < least) {
+      least = time;
+      best = size;
+    }
+  }
+  lay_tiles(p, best, dual);
+  p.splits = 1;
+  p.first_steps = p.other_steps = (uint32_t)steps_of(p, values);
+  return best;
+}
+
+// The same where the depth may be shared: each tile's shares are workgroups of their own,
+// whose partial sums, in binary32, k_join adds in their order.  Shares of one length,
+// or, of large tiles that leave compute units idle, a first one as long as the whole
+// work is to take and shorter ones for the idle units.
+inline Size choose_shares(Params& p, Space& space, bool turned, int values = 64, int64_t most_steps = INT32_MAX) {
+  const int64_t steps = steps_of(p, values);
+  Size best = kSmall;
+  int64_t best_first = 0, best_other = 0;
+  float least = INFINITY;
+  auto consider = [&](Size size, int64_t first, int64_t other, float time) {
+    if (time >= least || first > most_steps || other > most_steps) return;
+    least = time;
+    best = size;
+    best_first = first;
+    best_other = other;
+  };
+  for (const Size size : {kLarge, kMedium, kSmall}) {
+    const int64_t tiles = lay_tiles(p, size, false);
+    const float area = (float)side(size) * side(size) * tiles * 8.0f / 5e6f;  // written and read again, 5 TB/s
+    for (int64_t shares = 1; shares <= 64; shares += shares < 8 ? 1 : shares < 16 ? 2 : 8) {
+      const int64_t each = (steps + shares - 1) / shares;
+      if (shares > 1 && each < 4 && each * (shares - 1) >= steps) break;
+      consider(size, each, each, estimate(size, tiles * shares, each, turned) + (shares > 1 ? 3.0f + area * shares : 0.0f));
+    }
+    if (size != kLarge || tiles <= kUnits / 2 || tiles >= kUnits) continue;
+    const int64_t first = (steps * tiles + kUnits - 1) / kUnits, rest = steps - first;
+    for (int64_t shares = 1; shares <= 6 && rest >= shares; ++shares) {
+      const int64_t other = (rest + shares - 1) / shares, rounds = (tiles * shares + kUnits - tiles - 1) / (kUnits - tiles);
+      const float idle = rounds * estimate(size, 1, other, turned), own = estimate(size, 1, first, turned);
+      consider(size, first, other, std::max(idle, own) + 3.0f + area * (1 + shares));
+    }
+  }
+  lay_tiles(p, best, false);
+  p.first_steps = (uint32_t)std::min(best_first, steps);
+  p.other_steps = (uint32_t)best_other;
+  p.splits = steps > best_first ? 1 + (uint32_t)((steps - best_first + best_other - 1) / best_other) : 1;
   p.partial_size = 0;
   for (int j = 0; j < p.jobs; ++j) {
     p.job[j].partial = p.partial_size;
     p.partial_size += (p.job[j].rows * p.job[j].columns + 3) / 4 * 4;
   }
   p.partials = p.splits > 1 ? (float*)space.take(p.splits * p.partial_size * sizeof(float)) : nullptr;
-}
-
-inline void whole_depth(Params& p, int values = 64) {
-  p.splits = 1;
-  p.steps_per_split = (uint32_t)steps_of(p, values);
+  return best;
 }
 
 template <typename T>
@@ -286,7 +345,7 @@ __global__ __launch_bounds__(256) void k_join(Params p) {
 
 template <typename E, bool kLeftTurned, bool kRightTurned, class Finish>
 void launch_product(const Params& p, Size size, hipStream_t stream) {
-  const uint32_t groups = (p.tiles * p.splits + 7) / 8 * 8;
+  const uint32_t groups = (p.tiles + 7) / 8 * 8 * p.splits;
   switch (size) {
     case kLarge:
       product::k_product<E, kLeftTurned, kRightTurned, product::Large, Finish>

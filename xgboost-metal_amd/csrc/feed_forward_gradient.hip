@@ -113,7 +113,6 @@ int gradient(const MgbFeedForwardGradient& a, Space& space, hipStream_t stream, 
   inner.job[0].rows = a.rows;
   inner.job[0].columns = hidden;
   const Size inner_size = choose(inner, false);
-  whole_depth(inner);
 
   Params input = {};
   Size input_size = kSmall;
@@ -128,8 +127,7 @@ int gradient(const MgbFeedForwardGradient& a, Space& space, hipStream_t stream, 
     input.job[0].out_stride = a.dim;
     input.job[0].rows = a.rows;
     input.job[0].columns = a.dim;
-    input_size = choose(input, false);
-    split_depth(input, input_size, space);
+    input_size = choose_shares(input, space, !turn_weights);
   }
 
   Params weights = {};
@@ -151,8 +149,7 @@ int gradient(const MgbFeedForwardGradient& a, Space& space, hipStream_t stream, 
     add(a.dgate, dgate, a.hidden, x, a.dim);
     add(a.dup, dup, a.hidden, x, a.dim);
     add(a.ddown, grad, a.dim, middle, a.hidden);
-    weights_size = choose(weights, false);
-    split_depth(weights, weights_size, space);
+    weights_size = choose_shares(weights, space, true);
   }
   if (!run) return 0;
   lay_out<T>(jobs, stream);

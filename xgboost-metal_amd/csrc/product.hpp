@@ -77,7 +77,7 @@ struct Params {
   int jobs;
   int sources, pairs;
   int64_t depth;             // the larger of the operands'
-  uint32_t tiles, splits, steps_per_split;
+  uint32_t tiles, splits, first_steps, other_steps;  // the depth's shares: the first, and the others
   float* partials;           // [split][partial_size]
   int64_t partial_size;
   // 8-bit operands: a byte of exponent for each row and step, rows of whole words
@@ -158,13 +158,13 @@ using Small = Tile<64, 64, 2, 2>;
 // The tile of a workgroup: an eighth of the workgroups (a chiplet's, which takes
 // every eighth) has a stretch of an order that goes by bands of kBand tile rows,
 // column by column, so that what a chiplet works on at one time shares operands.
+// The shares of the depth follow each other, the longest first.
 constexpr uint32_t kBand = 4;
 __device__ __forceinline__ bool find_tile(const Params& p, uint32_t* job, uint32_t* ti, uint32_t* tj, uint32_t* split) {
-  const uint32_t total = p.tiles * p.splits, each = (total + 7) / 8;
-  const uint32_t at = blockIdx.x % 8 * each + blockIdx.x / 8;
-  if (blockIdx.x / 8 >= each || at >= total) return false;
-  *split = at / p.tiles;
-  uint32_t tile = at % p.tiles, j = 0;
+  const uint32_t each = (p.tiles + 7) / 8, local = blockIdx.x / 8;
+  uint32_t tile = blockIdx.x % 8 * each + local % each, j = 0;
+  *split = local / each;
+  if (tile >= p.tiles || *split >= p.splits) return false;
   while (j + 1 < (uint32_t)p.jobs && tile >= p.job[j + 1].first_tile) ++j;
   tile -= p.job[j].first_tile;
   const uint32_t rows = p.job[j].row_tiles, columns = p.job[j].column_tiles;
@@ -195,6 +195,47 @@ __device__ __forceinline__ int turned_key(int row) {
   if constexpr (kGranules == 8) return (row & 3) | (row >> 3 & 1) << 2;
   if constexpr (kGranules == 4) return (row >> 1 & 1) | (row >> 3 & 1) << 1;
   return row >> 3 & 1;
+}
+
+// 16 columns and the step's depth of turned rows in LDS, transposed, for tiles at `at`
+// (bytes of LDS): four reads of 8 values of the depth each, 4 x 16 values at a time.  The
+// compiler would wait for all loads to LDS before its own form of these reads; here
+// the wait for the reads alone stands in the same statement.
+template <int kPitch, int kOffset, int kTiles>
+__device__ __forceinline__ void read_turned(const uint32_t* at, Fragment* f) {
+  using int2v = __attribute__((ext_vector_type(2))) int;
+  // Offsets of the depth's 4 rows from 0, 4, 32 and 36 on.
+  constexpr int k0 = kOffset, k1 = kOffset + 4 * kPitch, k2 = kOffset + 32 * kPitch, k3 = kOffset + 36 * kPitch;
+  static_assert(k3 < 65536, "the instruction's offsets");
+  int2v v[kTiles][4];
+#define MGB_READS(t)                                      \
+  "ds_read_b64_tr_b16 %[a" #t "], %[at" #t "] offset:%[k0]\n" \
+  "ds_read_b64_tr_b16 %[b" #t "], %[at" #t "] offset:%[k1]\n" \
+  "ds_read_b64_tr_b16 %[c" #t "], %[at" #t "] offset:%[k2]\n" \
+  "ds_read_b64_tr_b16 %[d" #t "], %[at" #t "] offset:%[k3]\n"
+#define MGB_OUT(t) [a##t] "=&v"(v[t][0]), [b##t] "=&v"(v[t][1]), [c##t] "=&v"(v[t][2]), [d##t] "=&v"(v[t][3])
+#define MGB_OFFSETS [k0] "n"(k0), [k1] "n"(k1), [k2] "n"(k2), [k3] "n"(k3)
+  if constexpr (kTiles == 4) {
+    asm volatile(MGB_READS(0) MGB_READS(1) MGB_READS(2) MGB_READS(3) "s_waitcnt lgkmcnt(0)"
+                 : MGB_OUT(0), MGB_OUT(1), MGB_OUT(2), MGB_OUT(3)
+                 : [at0] "v"(at[0]), [at1] "v"(at[1]), [at2] "v"(at[2]), [at3] "v"(at[3]), MGB_OFFSETS
+                 : "memory");
+  } else if constexpr (kTiles == 2) {
+    asm volatile(MGB_READS(0) MGB_READS(1) "s_waitcnt lgkmcnt(0)"
+                 : MGB_OUT(0), MGB_OUT(1)
+                 : [at0] "v"(at[0]), [at1] "v"(at[1]), MGB_OFFSETS
+                 : "memory");
+  } else {
+    static_assert(kTiles == 1, "tiles of a wave");
+    asm volatile(MGB_READS(0) "s_waitcnt lgkmcnt(0)" : MGB_OUT(0) : [at0] "v"(at[0]), MGB_OFFSETS : "memory");
+  }
+#undef MGB_READS
+#undef MGB_OUT
+#undef MGB_OFFSETS
+#pragma unroll
+  for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) f[t].v[k] = v[t][k / 2][k % 2];
 }
 
 // What is read of an operand: a cursor that goes over its steps, the products of
@@ -295,8 +336,8 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_product(Params p) {
   right.depth = job.right.depth;
   const uint32_t each = p.depth > 0 ? (uint32_t)((p.depth + kStep - 1) / kStep) : 1;
   const uint32_t all = each * p.pairs * p.sources;
-  const uint32_t begin = split * p.steps_per_split;
-  const uint32_t end = begin + p.steps_per_split < all ? begin + p.steps_per_split : all;
+  const uint32_t begin = split ? p.first_steps + (split - 1) * p.other_steps : 0, share = split ? p.other_steps : p.first_steps;
+  const uint32_t end = begin + share < all ? begin + share : all;
 
   // The cursor: step k of the depth, of a product of parts, of a matrix.
   uint32_t ahead = begin;  // the next step to fetch
@@ -389,39 +430,51 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_product(Params p) {
   // l / 16 + 4 of it.  Turned: its 8 values of a half are 8 l / 16 .. + 7 of the depth, by
   // two reads of 4 x 16 that transpose: lane l gives the place of row l % 16 / 4, columns
   // l % 4 * 4 .. + 3.
-  auto read = [&](const char* region, int first_row, int t, auto turned, auto pairs, auto half_rows) {
+  auto straight = [&](const char* region, int first_row, int t, auto pairs) {
     int4v part[2];
+    constexpr bool kIn = decltype(pairs)::value;
+    const int row = kIn ? lane % 16 / 4 * 8 + lane % 4 : lane % 16;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      if constexpr (!decltype(turned)::value) {
-        constexpr bool kIn = decltype(pairs)::value;
-        const int row = kIn ? lane % 16 / 4 * 8 + lane % 4 : lane % 16;
-        const int chunk = (lane / 16 ^ (lane & 7)) ^ (h * 4);
-        part[h] = *(const int4v*)(region + (first_row + row) * kStepBytes + chunk * 16 +
-                                  (kIn ? t / 2 * 32 + t % 2 * 4 : t * 16) * kStepBytes);
-      } else {
-        constexpr int kPitch = decltype(half_rows)::value * 2, kGranules = decltype(half_rows)::value / 16;
-        short4v four[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          const int row = h * 32 + lane / 16 * 8 + j * 4 + lane % 16 / 4;
-          const int granule = (first_row / 16 + t) ^ turned_key<kGranules>(row);
-          four[j] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) short4v*)(region + row * kPitch + granule * 32 + lane % 4 * 8));
-        }
-        __builtin_memcpy(&part[h], four, sizeof(four));
-      }
+      const int chunk = (lane / 16 ^ (lane & 7)) ^ (h * 4);
+      part[h] = *(const int4v*)(region + (first_row + row) * kStepBytes + chunk * 16 +
+                                (kIn ? t / 2 * 32 + t % 2 * 4 : t * 16) * kStepBytes);
     }
     Fragment f;
     f.v = __builtin_shufflevector(part[0], part[1], 0, 1, 2, 3, 4, 5, 6, 7);
     return f;
   };
-  using HalfM = std::integral_constant<int, S::kHalfM>;
-  using HalfN = std::integral_constant<int, S::kHalfN>;
+  auto turned_places = [&](uint32_t* at, const char* first_region, int first_row, int tiles, auto half_rows) {
+    constexpr int kPitch = decltype(half_rows)::value * 2, kGranules = decltype(half_rows)::value / 16;
+    const int row = lane / 16 * 8 + lane % 16 / 4;
+    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)first_region;
+#pragma unroll
+    for (int t = 0; t < tiles; ++t)
+      at[t] = base + row * kPitch + ((first_row / 16 + t) ^ turned_key<kGranules>(row)) * 32 + lane % 4 * 8;
+  };
+  uint32_t left_at[S::kTilesM], right_at[S::kTilesN];
+  if constexpr (kLeftTurned) turned_places(left_at, lds, wm * S::kRowsM, S::kTilesM, std::integral_constant<int, S::kHalfM>{});
+  if constexpr (kRightTurned) turned_places(right_at, lds_right, wn * S::kRowsN, S::kTilesN, std::integral_constant<int, S::kHalfN>{});
   Fragment a[kAhead ? 2 : 1][S::kTilesM], b[2][S::kTilesN];
-  auto read_left = [&](int r, int stage, int t) { return read(left_region(r, stage), wm * S::kRowsM, t, LeftTurned{}, std::false_type{}, HalfM{}); };
-  auto read_right = [&](int r, int stage, int t) {
-    return read(right_region(r, stage), wn * S::kRowsN, t, RightTurned{}, std::bool_constant<kPairs>{}, HalfN{});
+  auto take_left = [&](auto r, auto stage) {
+    constexpr int kR = decltype(r)::value, kStage = decltype(stage)::value;
+    if constexpr (kLeftTurned) {
+      read_turned<S::kHalfM * 2, (kR * 2 + kStage) * S::kRegionM, S::kTilesM>(left_at, a[0]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::kTilesM; ++i)
+        a[kAhead ? kR : 0][i] = straight(left_region(kR, kStage), wm * S::kRowsM, i, std::false_type{});
+    }
+  };
+  auto take_right = [&](Fragment* to, auto r, auto stage) {
+    constexpr int kR = decltype(r)::value, kStage = decltype(stage)::value;
+    if constexpr (kRightTurned) {
+      read_turned<S::kHalfN * 2, (kR * 2 + kStage) * S::kRegionN, S::kTilesN>(right_at, to);
+    } else {
+#pragma unroll
+      for (int j = 0; j < S::kTilesN; ++j)
+        to[j] = straight(right_region(kR, kStage), wn * S::kRowsN, j, std::bool_constant<kPairs>{});
+    }
   };
 
   // A row's exponents of a step: bytes kTilesM x + i of words that lanes l % 16 of the
@@ -504,44 +557,44 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_product(Params p) {
     if constexpr (kAhead || S::kAlternate) wait_barrier();
     order();
   };
-  auto take_left = [&](int r, int stage) {
-#pragma unroll
-    for (int i = 0; i < S::kTilesM; ++i) a[kAhead ? r : 0][i] = read_left(r, stage, i);
-  };
-  auto take_right = [&](Fragment* to, int r, int stage) {
-#pragma unroll
-    for (int j = 0; j < S::kTilesN; ++j) to[j] = read_right(r, stage, j);
-  };
+  using Zero = std::integral_constant<int, 0>;
+  using One = std::integral_constant<int, 1>;
   auto step = [&](auto stage_constant, uint32_t t) {
     constexpr int kStage = decltype(stage_constant)::value;
+    using Now = std::integral_constant<int, kStage>;
+    using Next = std::integral_constant<int, 1 - kStage>;
     Fragment *const now = b[kStage], *const other = b[1 - kStage];
     if constexpr (kAhead) {
-      take_right(other, 1, kStage);
+      take_right(other, One{}, Now{});
       fetch_left(0, kStage);
       multiply_quarter(0, 0, now);
-      take_left(1, kStage);
+      take_left(One{}, Now{});
       fetch_right(0, kStage);
       multiply_quarter(0, 1, other);
-      take_left(0, 1 - kStage);
+      take_left(Zero{}, Next{});
       fetch_right(1, kStage);
       multiply_quarter(1, 1, other);
+      take_right(other, Zero{}, Next{});
+      next_scales = read_scales(t + 1);
+      fetch_left(1, kStage);
+      advance();
+      multiply_quarter(1, 0, now);
+      scales = next_scales;
     } else {
-      take_left(0, kStage);
       fetch_right(0, kStage);
+      take_left(Zero{}, Now{});
       multiply_quarter(0, 0, now);
-      take_right(other, 1, kStage);
       fetch_left(0, kStage);
+      take_right(other, One{}, Now{});
       multiply_quarter(0, 1, other);
-      take_left(1, kStage);
       fetch_right(1, kStage);
+      take_left(One{}, Now{});
       multiply_quarter(1, 1, other);
+      fetch_left(1, kStage);
+      advance();
+      take_right(other, Zero{}, Next{});
+      multiply_quarter(1, 0, now);
     }
-    take_right(other, 0, 1 - kStage);
-    next_scales = read_scales(t + 1);
-    fetch_left(1, kStage);
-    advance();
-    multiply_quarter(1, 0, now);
-    scales = next_scales;
   };
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
@@ -560,8 +613,8 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_product(Params p) {
   }
   wait_barrier();
   scales = read_scales(0);
-  take_right(b[0], 0, 0);
-  if constexpr (kAhead) take_left(0, 0);
+  take_right(b[0], Zero{}, Zero{});
+  if constexpr (kAhead) take_left(Zero{}, Zero{});
   wait_loads<kFlight>();
   wait_barrier();
   if constexpr (S::kAlternate)
