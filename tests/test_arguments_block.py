@@ -92,6 +92,9 @@ def test_workspaces_are_checked(lib):
     assert need > 0
     _refused(lib, lib.mgb_block_feed_forward(ctypes.byref(s), P(HERE), ctypes.c_size_t(need - 1), None), "too small")
     b = Matmul(HERE, m, m, 0)
+    assert lib.mgb_block_matmul_workspace_bytes(ctypes.byref(b)) == 0  # (few rows are read as they are)
+    many = Blocks(HERE, HERE, 64, 1, 128, 4)
+    b = Matmul(HERE, many, m, 0)
     need = lib.mgb_block_matmul_workspace_bytes(ctypes.byref(b))
     assert need > 0
     _refused(lib, lib.mgb_block_matmul(ctypes.byref(b), P(HERE), ctypes.c_size_t(need - 1), None), "too small")

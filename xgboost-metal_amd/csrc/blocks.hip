@@ -66,8 +66,16 @@ void quantize(uint8_t* values, uint8_t* scales, const T* x, int64_t rows, int64_
                                                                  scale_stride);
 }
 
-// What blocks stand for, as bfloat16, which has their bits and exponents.
-__global__ __launch_bounds__(kQuantThreads) void k_widen(__bf16* __restrict__ to, MgbBlocks m) {
+// What blocks stand for, as bfloat16, which has their bits and exponents; matrices
+// blockIdx.y.
+struct Widen {
+  __bf16* to[3];
+  MgbBlocks m[3];
+  int count;
+};
+
+__global__ __launch_bounds__(kQuantThreads) void k_widen(Widen w) {
+  const MgbBlocks& m = w.m[blockIdx.y];
   const int64_t all = m.rows * m.blocks, step = (int64_t)gridDim.x * (kQuantThreads / kQuantLanes);
   const int lane = threadIdx.x % kQuantLanes;
   for (int64_t at = (int64_t)blockIdx.x * (kQuantThreads / kQuantLanes) + threadIdx.x / kQuantLanes; at < all; at += step) {
@@ -75,19 +83,23 @@ __global__ __launch_bounds__(kQuantThreads) void k_widen(__bf16* __restrict__ to
     uint2 bytes;
     __builtin_memcpy(&bytes, (const uint8_t*)m.values + row * m.stride + block * kBlock + lane * 8, 8);
     const product::bf16x8 v = widen_eight(bytes, ((const uint8_t*)m.scales)[row * m.scale_stride + block]);
-    __builtin_memcpy(to + (row * m.blocks + block) * kBlock + lane * 8, &v, sizeof(v));
+    __builtin_memcpy(w.to[blockIdx.y] + (row * m.blocks + block) * kBlock + lane * 8, &v, sizeof(v));
   }
 }
 
-Laid widen(Space& space, const MgbBlocks& m, hipStream_t stream, bool run) {
+Laid widened(Space& space, Widen& w, const MgbBlocks& m) {
   const int64_t width = m.blocks * kBlock * 2;
   char* to = space.take(m.rows * width);
-  if (run) {
-    const int64_t each = kQuantThreads / kQuantLanes;
-    k_widen<<<(uint32_t)std::min<int64_t>((m.rows * m.blocks + each - 1) / each, 4096), kQuantThreads, 0, stream>>>(
-        (__bf16*)to, m);
-  }
+  w.to[w.count] = (__bf16*)to;
+  w.m[w.count++] = m;
   return {to, width, 0};
+}
+
+void widen(const Widen& w, hipStream_t stream) {
+  const int64_t each = kQuantThreads / kQuantLanes;
+  int64_t most = 0;
+  for (int k = 0; k < w.count; ++k) most = std::max(most, w.m[k].rows * w.m[k].blocks);
+  k_widen<<<dim3((uint32_t)std::min<int64_t>((most + each - 1) / each, 4096), w.count), kQuantThreads, 0, stream>>>(w);
 }
 
 product::Operand operand8(const MgbBlocks& m) {
@@ -125,7 +137,9 @@ int multiply(T* out, const MgbBlocks& x, const MgbBlocks& weight, Space& space, 
   p.job[0].rows = x.rows;
   p.job[0].columns = weight.rows;
   if constexpr (sizeof(T) == 4) {
-    const Laid left = widen(space, x, stream, run), right = widen(space, weight, stream, run);
+    Widen w = {};
+    const Laid left = widened(space, w, x), right = widened(space, w, weight);
+    if (run) widen(w, stream);
     p.job[0].left = operand(left, x.rows, p.depth);
     p.job[0].right = operand(right, weight.rows, p.depth);
     const Size size = choose_shares(p, space, false);
@@ -143,18 +157,48 @@ int multiply(T* out, const MgbBlocks& x, const MgbBlocks& weight, Space& space, 
   return 0;
 }
 
-struct GatedFloat {
+struct GatedFloat : product::Plainly {
   static constexpr bool kDual = true;
   const Params& p;
-  __device__ __forceinline__ GatedFloat(const Params& params, const product::Job&, uint32_t) : p(params) {}
-  template <int kCount>
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, const float* gate, const float* up) const {
+  int64_t rows;
+  __device__ __forceinline__ GatedFloat(const Params& params, const product::Job& job, uint32_t) : p(params), rows(job.rows) {}
+  template <int kCount, bool kWhole, typename L>
+  __device__ __forceinline__ void store(int64_t m, int64_t n, const float* gate, const float* up, const L&) const {
+    if (!kWhole && m >= rows) return;
     float h[kCount];
 #pragma unroll
     for (int e = 0; e < kCount; ++e) h[e] = activate<true>(gate[e], p.activation) * up[e];
-    product::store_some<kCount>((float*)p.hidden + m * p.hidden_stride, n, p.true_columns, h);
+    product::store_some<kCount, kWhole>((float*)p.hidden + m * p.hidden_stride, n, p.true_columns, h);
   }
 };
+
+// The same rounded to blocks in the workgroup that has them: large tiles, whose 128
+// columns of both products are a block.
+struct GatedBlocks : product::Plainly {
+  static constexpr bool kDual = true, kBlocks = true;
+  const Params& p;
+  __device__ __forceinline__ GatedBlocks(const Params& params, const product::Job&, uint32_t) : p(params) {}
+  __device__ __forceinline__ float value(float gate, float up) const { return activate<true>(gate, p.activation) * up; }
+  __device__ __forceinline__ void store(int64_t m, int64_t n, uint32_t block, const float* v, float top, bool first) const {
+    const uint32_t scale = scale_of(top);
+    const uint2 bytes = round_eight(v, __uint_as_float((254u - scale) << 23));
+    __builtin_memcpy(__builtin_assume_aligned(p.hidden + m * p.hidden_stride + n, 8), &bytes, 8);
+    if (first) p.dgate[m * p.gradient_part + block] = (char)scale;
+  }
+};
+
+template <class E, class Finish>
+void launch_small(const Params& p, Size size, hipStream_t stream) {
+  const uint32_t groups = (p.tiles + 7) / 8 * 8 * p.splits;
+  if (size == kMedium) product::k_product<E, false, false, product::Medium, Finish><<<groups, product::Medium::kThreads, 0, stream>>>(p);
+  else product::k_product<E, false, false, product::Small, Finish><<<groups, product::Small::kThreads, 0, stream>>>(p);
+}
+
+template <class E>
+void launch_blocks(const Params& p, hipStream_t stream) {
+  product::k_product<E, false, false, product::Large, GatedBlocks>
+      <<<(p.tiles + 7) / 8 * 8 * p.splits, product::Large::kThreads, 0, stream>>>(p);
+}
 
 template <typename T>
 int serve(const MgbBlockFeedForward& a, Space& space, hipStream_t stream, bool run) {
@@ -199,12 +243,21 @@ int serve(const MgbBlockFeedForward& a, Space& space, hipStream_t stream, bool r
   p.pairs = 1;
   p.depth = dim;
   p.true_columns = a.hidden;
-  p.hidden_stride = a.hidden;
-  p.hidden = space.take(a.rows * a.hidden * sizeof(float));
+  MgbBlocks h = {space.take(a.rows * hidden), space.take(a.rows * hidden_scales), a.rows, a.down.blocks, hidden, hidden_scales};
   p.activation = a.activation;
   p.job[0].rows = a.rows;
   p.job[0].columns = a.hidden;
   const Size size = choose(p, true, std::is_same_v<T, __bf16> ? kBlock : 64);
+  const bool rounds = size == kLarge;
+  if (rounds) {
+    p.hidden = (char*)h.values;
+    p.hidden_stride = hidden;
+    p.dgate = (char*)h.scales;
+    p.gradient_part = hidden_scales;
+  } else {
+    p.hidden_stride = a.hidden;
+    p.hidden = space.take(a.rows * a.hidden * sizeof(float));
+  }
   if constexpr (std::is_same_v<T, __bf16>) {
     p.job[0].left = operand8(x);
     p.job[0].right = {{(const char*)a.gate.values, (const char*)a.up.values}, {a.gate.stride, a.up.stride}, 0, a.hidden, dim};
@@ -213,16 +266,18 @@ int serve(const MgbBlockFeedForward& a, Space& space, hipStream_t stream, bool r
     p.right_scales[1] = (const uint8_t*)a.up.scales;
     p.left_scale_stride = x.scale_stride;
     p.right_scale_stride = a.gate.scale_stride;
-    if (run) launch_product<product::E4m3, false, false, GatedFloat>(p, size, stream);
+    if (run && rounds) launch_blocks<product::E4m3>(p, stream);
+    else if (run) launch_small<product::E4m3, GatedFloat>(p, size, stream);
   } else {
-    const Laid left = widen(space, x, stream, run);
-    const Laid gate = widen(space, a.gate, stream, run), up = widen(space, a.up, stream, run);
+    Widen w = {};
+    const Laid left = widened(space, w, x), gate = widened(space, w, a.gate), up = widened(space, w, a.up);
+    if (run) widen(w, stream);
     p.job[0].left = operand(left, a.rows, dim);
     p.job[0].right = operands(gate, up, a.hidden, dim);
-    if (run) launch_product<__bf16, false, false, GatedFloat>(p, size, stream);
+    if (run && rounds) launch_blocks<__bf16>(p, stream);
+    else if (run) launch_small<__bf16, GatedFloat>(p, size, stream);
   }
-  MgbBlocks h = {space.take(a.rows * hidden), space.take(a.rows * hidden_scales), a.rows, a.down.blocks, hidden, hidden_scales};
-  if (run)
+  if (run && !rounds)
     quantize<float>((uint8_t*)h.values, (uint8_t*)h.scales, (const float*)p.hidden, a.rows, a.hidden, a.hidden, hidden,
                     hidden_scales, stream);
   return multiply<T>((T*)a.y, h, a.down, space, stream, run);

@@ -6,8 +6,12 @@
 // loss and gradient 0.  Entries of the same column add up.
 //
 // Bound by memory: the loss reads z once, with the running largest value and sum of a
-// softmax in each lane; the gradient reads it once and writes dz.  Sums are binary32.
+// softmax in each lane, 32 bfloat16 values between two changes of it; the gradient
+// reads it once and writes dz.  8,192 rows of 32,768 bfloat16: loss 84 us, 6.4 TB/s of
+// the logits (a plain read reaches 6.2, one past the caches 7.1); gradient 193 us, 5.6
+// TB/s (a large copy 5.0).  Sums are binary32.
 #include <algorithm>
+#include <type_traits>
 
 #include "encoder_common.hpp"
 
@@ -16,6 +20,10 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr float kLog2e = 1.44269504f, kLowest = -3.40282347e38f;
+// Logits of this many bytes go past the caches, of whose last level this is the size.
+// 8,192 rows of 32,768 in bfloat16 (537 MB): loss 84 us, gradient 193, through the
+// caches 95 and 208; a quarter of them 24 and 51, through the caches 26 and 48.
+constexpr int64_t kStreamBytes = 256 << 20;
 constexpr int64_t kMostClasses = int64_t(1) << 31;
 
 struct Teacher {
@@ -48,19 +56,29 @@ struct Running {
   }
 };
 
+// Two of them joined over the lanes of a row; `shared` holds two a wave.
 template <int kLanes>
-__device__ __forceinline__ Running join_lanes(Running r, float c, Running* shared) {
+__device__ __forceinline__ void join_lanes(Running& a, Running& b, float c, Running* shared) {
 #pragma unroll
-  for (int d = (kLanes < kWave ? kLanes : kWave) / 2; d > 0; d /= 2) r.join(__shfl_xor(r.largest, d, kWave), __shfl_xor(r.sum, d, kWave), c);
+  for (int d = (kLanes < kWave ? kLanes : kWave) / 2; d > 0; d /= 2) {
+    a.join(__shfl_xor(a.largest, d, kWave), __shfl_xor(a.sum, d, kWave), c);
+    b.join(__shfl_xor(b.largest, d, kWave), __shfl_xor(b.sum, d, kWave), c);
+  }
   if constexpr (kLanes > kWave) {
     __syncthreads();
-    if (threadIdx.x % kWave == 0) shared[threadIdx.x / kWave] = r;
+    if (threadIdx.x % kWave == 0) {
+      shared[threadIdx.x / kWave * 2] = a;
+      shared[threadIdx.x / kWave * 2 + 1] = b;
+    }
     __syncthreads();
-    r = shared[0];
+    a = shared[0];
+    b = shared[1];
 #pragma unroll
-    for (int w = 1; w < kLanes / kWave; ++w) r.join(shared[w].largest, shared[w].sum, c);
+    for (int w = 1; w < kLanes / kWave; ++w) {
+      a.join(shared[2 * w].largest, shared[2 * w].sum, c);
+      b.join(shared[2 * w + 1].largest, shared[2 * w + 1].sum, c);
+    }
   }
-  return r;
 }
 
 template <int kLanes>
@@ -69,44 +87,84 @@ __device__ __forceinline__ float sum_lanes(float v, float* shared) {
   else return block_sum<kLanes>(v, shared);
 }
 
-// The teacher's largest value and sum, over the lanes of a row.
-template <int kLanes>
-__device__ __forceinline__ Running teach(const Teacher& teacher, int64_t row, int64_t classes, int lane, float c, Running* shared) {
-  Running r = {kLowest, 0.0f};
-  for (int64_t j = lane; j < teacher.count; j += kLanes) {
-    const int64_t column = teacher.column(row, j);
-    if (column < 0 || column >= classes) continue;
-    const float v = teacher.value(row, j);
-    if (v == -INFINITY) continue;  // a probability of 0, as none
-    r.join(v, 1.0f, c);
-  }
-  return join_lanes<kLanes>(r, c, shared);
+// An entry of the teacher's; absent ones have value -inf.
+struct Entry {
+  int32_t column;
+  float value;
+};
+
+__device__ __forceinline__ Entry entry_of(const Teacher& teacher, int64_t row, int64_t classes, int64_t j) {
+  const int64_t column = teacher.column(row, j);
+  const bool there = column >= 0 && column < classes;
+  return {there ? (int32_t)column : -1, there ? teacher.value(row, j) : -INFINITY};
 }
 
-template <typename T, int kLanes>
+// A lane's first entry, without a branch on what is fetched.
+__device__ __forceinline__ Entry first_entry(const Teacher& teacher, int64_t row, int64_t classes, int lane) {
+  if (lane >= teacher.count) return {-1, -INFINITY};
+  const int64_t column = teacher.column(row, lane);
+  const float value = teacher.value(row, lane);
+  const bool there = column >= 0 && column < classes;
+  return {there ? (int32_t)column : -1, there ? value : -INFINITY};
+}
+
+// A lane's entries (`first` is its first): the largest value and the sum.
+template <int kLanes>
+__device__ __forceinline__ Running teach(const Teacher& teacher, const Entry& first, int64_t row, int64_t classes, int lane,
+                                         float c) {
+  Running r = {kLowest, 0.0f};
+  for (int64_t j = lane; j < teacher.count; j += kLanes) {
+    const float v = j == lane ? first.value : entry_of(teacher, row, classes, j).value;
+    if (v != -INFINITY) r.join(v, 1.0f, c);
+  }
+  return r;
+}
+
+// 16 bytes of a row, or from it past the caches.
+template <bool kStream, typename T>
+__device__ __forceinline__ void load_raw(Raw<T, Pack<T>::kSize>& raw, const T* from) {
+  using Loose = __attribute__((ext_vector_type(4), aligned(2))) uint32_t;
+  if constexpr (kStream) raw.bits = __builtin_nontemporal_load((const Loose*)from);
+  else raw.load(from);
+}
+
+template <bool kStream, typename T>
+__device__ __forceinline__ void store_raw(const float* v, T* to) {
+  using Loose = __attribute__((ext_vector_type(4), aligned(2))) uint32_t;
+  T r[Pack<T>::kSize];
+#pragma unroll
+  for (int e = 0; e < Pack<T>::kSize; ++e) r[e] = (T)v[e];
+  Loose bits;
+  __builtin_memcpy(&bits, r, sizeof(bits));
+  if constexpr (kStream) __builtin_nontemporal_store(bits, (Loose*)to);
+  else __builtin_memcpy(to, r, sizeof(r));
+}
+
+// The running value and sum of a lane's part of a row, kAhead packs at a time: values
+// v count as 2^(c v - base), c = log2(e) / T.
+template <bool kStream, typename T, int kLanes>
 __device__ __forceinline__ Running sweep(const T* z, int64_t begin, int64_t end, int lane, float c) {
   constexpr int kSize = Pack<T>::kSize, kAhead = 4;
   Running r = {kLowest, 0.0f};
-  auto take = [&](const float* v) {
+  auto take = [&](const float* v, auto count) {
+    constexpr int kCount = decltype(count)::value;
     float most = r.largest;
 #pragma unroll
-    for (int e = 0; e < kSize; ++e) most = fmaxf(most, v[e]);
-    float sum = r.sum * __builtin_amdgcn_exp2f((r.largest - most) * c);
+    for (int e = 0; e < kCount; ++e) most = fmaxf(most, v[e]);
+    float sum[2] = {r.sum * __builtin_amdgcn_exp2f((r.largest - most) * c), 0.0f};
 #pragma unroll
-    for (int e = 0; e < kSize; ++e) sum += __builtin_amdgcn_exp2f((v[e] - most) * c);
-    r = {most, sum};
+    for (int e = 0; e < kCount; ++e) sum[e % 2] += __builtin_amdgcn_exp2f((v[e] - most) * c);
+    r = {most, sum[0] + sum[1]};
   };
   int64_t at = begin + (int64_t)lane * kSize;
   for (; at + (int64_t)(kAhead - 1) * kLanes * kSize + kSize <= end; at += (int64_t)kAhead * kLanes * kSize) {
     Raw<T, kSize> raw[kAhead];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) raw[k].load(z + at + (int64_t)k * kLanes * kSize);
+    for (int k = 0; k < kAhead; ++k) load_raw<kStream>(raw[k], z + at + (int64_t)k * kLanes * kSize);
+    float v[kAhead * kSize];
 #pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      float v[kSize];
-      raw[k].get(v);
-      take(v);
-    }
+    for (int k = 0; k < kAhead; ++k) raw[k].get(v + k * kSize);
+    take(v, std::integral_constant<int, kAhead * kSize>{});
   }
   for (; at < end; at += (int64_t)kLanes * kSize) {
     float v[kSize];
@@ -114,27 +172,28 @@ __device__ __forceinline__ Running sweep(const T* z, int64_t begin, int64_t end,
 #pragma unroll
     for (int e = 0; e < kSize; ++e)
       if (at + e >= end) v[e] = -INFINITY;
-    take(v);
+    take(v, std::integral_constant<int, kSize>{});
   }
   return r;
 }
 
 // log sum exp(z / T), and the row's loss.
 template <typename T, int kLanes>
-__device__ __forceinline__ void finish_row(float* loss, float* lses, const T* z, const Teacher& teacher, Running r, int64_t row,
-                                           int64_t classes, int lane, float temperature, float c, Running* shared) {
+__device__ __forceinline__ void finish_row(float* loss, float* lses, const T* z, const Teacher& teacher,
+                                           const Entry& first, Running r, int64_t row, int64_t classes, int lane,
+                                           float temperature, float c, Running* shared) {
   const float inverse = 1.0f / temperature;
-  const float lse = fmaf(r.largest, inverse, logf(r.sum));
-  const Running t = teach<kLanes>(teacher, row, classes, lane, c, shared);
-  const float log_total = logf(t.sum);
+  const float logit = first.value != -INFINITY ? (float)z[first.column] : 0.0f;
+  Running t = teach<kLanes>(teacher, first, row, classes, lane, c);
+  join_lanes<kLanes>(r, t, c, shared);
+  const float lse = fmaf(r.largest, inverse, logf(r.sum)), log_total = logf(t.sum);
   float sum = 0.0f;
   for (int64_t j = lane; j < teacher.count; j += kLanes) {
-    const int64_t column = teacher.column(row, j);
-    if (column < 0 || column >= classes) continue;
-    const float v = teacher.value(row, j);
-    if (v == -INFINITY) continue;
-    const float log_p = (v - t.largest) * inverse - log_total, p = expf(log_p);
-    if (p != 0.0f) sum = fmaf(p, log_p - ((float)z[column] * inverse - lse), sum);
+    const Entry e = j == lane ? first : entry_of(teacher, row, classes, j);
+    if (e.value == -INFINITY) continue;
+    const float log_p = (e.value - t.largest) * inverse - log_total, p = expf(log_p);
+    const float there = j == lane ? logit : (float)z[e.column];
+    if (p != 0.0f) sum = fmaf(p, log_p - (there * inverse - lse), sum);
   }
   sum = sum_lanes<kLanes>(sum, (float*)shared);
   if (lane == 0) {
@@ -144,23 +203,26 @@ __device__ __forceinline__ void finish_row(float* loss, float* lses, const T* z,
 }
 
 // A row by kLanes lanes; with `partial` a part of it, columns blockIdx.y each.
-template <typename T, int kLanes>
+template <bool kStream, typename T, int kLanes>
 __global__ __launch_bounds__(kThreads) void k_loss(float* __restrict__ loss, float* __restrict__ lses, Running* __restrict__ partial,
                                                    const T* __restrict__ logits, Teacher teacher, int64_t rows, int64_t classes,
                                                    int64_t stride, int64_t part, float temperature) {
-  __shared__ Running shared[kThreads / kWave];
+  __shared__ Running shared[2 * kThreads / kWave];
   const int lane = threadIdx.x % kLanes;
   const int64_t row = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
   if (row >= rows) return;  // (no barrier follows where a workgroup has several rows)
   const float c = kLog2e / temperature;
   const T* z = logits + row * stride;
   const int64_t begin = (int64_t)blockIdx.y * part, end = begin + part < classes ? begin + part : classes;
-  const Running r = join_lanes<kLanes>(sweep<T, kLanes>(z, begin, end, lane, c), c, shared);
   if (partial) {
+    Running r = sweep<kStream, T, kLanes>(z, begin, end, lane, c), none = {kLowest, 0.0f};
+    join_lanes<kLanes>(r, none, c, shared);
     if (lane == 0) partial[row * gridDim.y + blockIdx.y] = r;
     return;
   }
-  finish_row<T, kLanes>(loss, lses, z, teacher, r, row, classes, lane, temperature, c, shared);
+  const Entry first = first_entry(teacher, row, classes, lane);  // (on its way during the sweep)
+  const Running r = sweep<kStream, T, kLanes>(z, begin, end, lane, c);
+  finish_row<T, kLanes>(loss, lses, z, teacher, first, r, row, classes, lane, temperature, c, shared);
 }
 
 template <typename T>
@@ -170,26 +232,22 @@ __global__ __launch_bounds__(kWave) void k_loss_join(float* __restrict__ loss, f
   const int lane = threadIdx.x;
   const int64_t row = blockIdx.x;
   const float c = kLog2e / temperature;
+  const T* z = logits + row * stride;
+  const Entry first = first_entry(teacher, row, classes, lane);
   Running r = {kLowest, 0.0f};
   for (int k = lane; k < parts; k += kWave) r.join(partial[row * parts + k].largest, partial[row * parts + k].sum, c);
-  r = join_lanes<kWave>(r, c, nullptr);
-  finish_row<T, kWave>(loss, lses, logits + row * stride, teacher, r, row, classes, lane, temperature, c, nullptr);
+  finish_row<T, kWave>(loss, lses, z, teacher, first, r, row, classes, lane, temperature, c, nullptr);
 }
 
 // dz of a part of a row: q everywhere, then the teacher's columns once more, by the
 // lane of a column's first entry.  The entries' columns and probabilities lie in LDS.
-struct Entry {
-  int32_t column;  // -1: absent
-  float p;
-};
-
-template <typename T, int kLanes>
+template <bool kStream, typename T, int kLanes>
 __global__ __launch_bounds__(kThreads) void k_loss_gradient(T* __restrict__ dz, const float* __restrict__ grad,
                                                             const T* __restrict__ logits, const float* __restrict__ lses,
                                                             Teacher teacher, int64_t rows, int64_t classes, int64_t grad_stride,
                                                             int64_t stride, int64_t part, float temperature) {
   extern __shared__ Entry all_entries[];
-  __shared__ Running shared[kThreads / kWave];
+  __shared__ Running shared[2 * kThreads / kWave];
   constexpr int kSize = Pack<T>::kSize;
   const int lane = threadIdx.x % kLanes, count = (int)teacher.count;
   const int64_t row = (int64_t)blockIdx.x * (kThreads / kLanes) + threadIdx.x / kLanes;
@@ -206,18 +264,34 @@ __global__ __launch_bounds__(kThreads) void k_loss_gradient(T* __restrict__ dz, 
   if (there) {
     z = logits + row * stride;
     out = dz + row * classes;
-    const Running t = teach<kLanes>(teacher, row, classes, lane, kLog2e / temperature, shared);
+    Running t = teach<kLanes>(teacher, first_entry(teacher, row, classes, lane), row, classes, lane, kLog2e / temperature);
+    Running none = {kLowest, 0.0f};
+    join_lanes<kLanes>(t, none, kLog2e / temperature, shared);
     const float log_total = logf(t.sum);
     for (int j = lane; j < count; j += kLanes) {
-      const int64_t column = teacher.column(row, j);
-      const float v = teacher.value(row, j);
-      const bool present = column >= 0 && column < classes && v != -INFINITY;
-      entries[j] = {present ? (int32_t)column : -1, present ? expf((v - t.largest) * inverse - log_total) : 0.0f};
+      Entry e = entry_of(teacher, row, classes, j);
+      const bool there = e.value != -INFINITY;
+      entries[j] = {there ? e.column : -1, there ? expf((e.value - t.largest) * inverse - log_total) : 0.0f};
     }
     empty = t.sum == 0.0f;
     factor = grad[row * grad_stride] * temperature;
     lse = lses[row];
-    for (int64_t at = begin + (int64_t)lane * kSize; at < end; at += (int64_t)kLanes * kSize) {
+    constexpr int kAhead = 4;
+    int64_t at = begin + (int64_t)lane * kSize;
+    for (; at + (int64_t)(kAhead - 1) * kLanes * kSize + kSize <= end; at += (int64_t)kAhead * kLanes * kSize) {
+      Raw<T, kSize> raw[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) load_raw<kStream>(raw[k], z + at + (int64_t)k * kLanes * kSize);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) {
+        float v[kSize];
+        raw[k].get(v);
+#pragma unroll
+        for (int e = 0; e < kSize; ++e) v[e] = empty ? 0.0f : factor * slope(v[e]);
+        store_raw<kStream>(v, out + at + (int64_t)k * kLanes * kSize);
+      }
+    }
+    for (; at < end; at += (int64_t)kLanes * kSize) {
       float v[kSize];
       load_pack(z, at, end, v);
 #pragma unroll
@@ -235,7 +309,7 @@ __global__ __launch_bounds__(kThreads) void k_loss_gradient(T* __restrict__ dz, 
     for (int k = 0; k < count; ++k) {
       const bool same = entries[k].column == column;
       first = first && !(same && k < j);
-      p += same ? entries[k].p : 0.0f;
+      p += same ? entries[k].value : 0.0f;
     }
     if (first) out[column] = (T)(factor * (slope((float)z[column]) - p));
   }
@@ -246,8 +320,10 @@ struct Plan {
   int64_t parts, part;
 };
 
-// Rows of up to 2,048 columns by a wave, wider ones by a workgroup; where there are
-// few of those, in parts of at least 8,192 columns.
+// Rows of up to 2,048 columns, a lane's 4 packs, by a wave, so that no barrier joins
+// them; wider ones by a workgroup (8,192 rows of 32,768 by a wave each: 2 % slower);
+// where there are too few of those for the chip, in parts of at least 8,192 columns, a
+// lane's 4 packs again.
 Plan plan(int64_t rows, int64_t classes) {
   Plan p = {classes <= 2048 ? kWave : kThreads, 1, classes};
   if (p.lanes == kThreads && rows < 1024) {
@@ -283,12 +359,15 @@ int loss(const MgbDistillation& a, void* workspace, hipStream_t stream) {
   const Teacher teacher = teacher_of(a);
   const T* logits = (const T*)a.logits;
   const dim3 grid((uint32_t)((a.rows * p.lanes + kThreads - 1) / kThreads), (uint32_t)p.parts);
-  if (p.lanes == kWave)
-    k_loss<T, kWave><<<grid, kThreads, 0, stream>>>(a.loss, a.lse, partial, logits, teacher, a.rows, a.classes, a.stride, p.part,
-                                                    a.temperature);
-  else
-    k_loss<T, kThreads><<<grid, kThreads, 0, stream>>>(a.loss, a.lse, partial, logits, teacher, a.rows, a.classes, a.stride, p.part,
-                                                       a.temperature);
+  auto launch = [&](auto stream_it, auto lanes) {
+    k_loss<decltype(stream_it)::value, T, decltype(lanes)::value><<<grid, kThreads, 0, stream>>>(
+        a.loss, a.lse, partial, logits, teacher, a.rows, a.classes, a.stride, p.part, a.temperature);
+  };
+  using Wave = std::integral_constant<int, kWave>;
+  using Group = std::integral_constant<int, kThreads>;
+  if (p.lanes == kWave) launch(std::false_type{}, Wave{});
+  else if (a.rows * a.classes * (int64_t)sizeof(T) >= kStreamBytes) launch(std::true_type{}, Group{});
+  else launch(std::false_type{}, Group{});
   if (partial)
     k_loss_join<T><<<(uint32_t)a.rows, kWave, 0, stream>>>(a.loss, a.lse, partial, (int)p.parts, logits, teacher, a.classes,
                                                            a.stride, a.temperature);
@@ -301,12 +380,16 @@ int gradient(const MgbDistillation& a, hipStream_t stream) {
   const Plan p = plan(a.rows, a.classes);
   const dim3 grid((uint32_t)((a.rows * p.lanes + kThreads - 1) / kThreads), (uint32_t)p.parts);
   const uint32_t lds = (uint32_t)(kThreads / p.lanes * a.top * sizeof(Entry));
-  if (p.lanes == kWave)
-    k_loss_gradient<T, kWave><<<grid, kThreads, lds, stream>>>((T*)a.dlogits, a.grad, (const T*)a.logits, a.lse, teacher_of(a), a.rows,
-                                                             a.classes, a.grad_stride, a.stride, p.part, a.temperature);
-  else
-    k_loss_gradient<T, kThreads><<<grid, kThreads, lds, stream>>>((T*)a.dlogits, a.grad, (const T*)a.logits, a.lse, teacher_of(a),
-                                                                a.rows, a.classes, a.grad_stride, a.stride, p.part, a.temperature);
+  auto launch = [&](auto stream_it, auto lanes) {
+    k_loss_gradient<decltype(stream_it)::value, T, decltype(lanes)::value><<<grid, kThreads, lds, stream>>>(
+        (T*)a.dlogits, a.grad, (const T*)a.logits, a.lse, teacher_of(a), a.rows, a.classes, a.grad_stride, a.stride, p.part,
+        a.temperature);
+  };
+  using Wave = std::integral_constant<int, kWave>;
+  using Group = std::integral_constant<int, kThreads>;
+  if (p.lanes == kWave) launch(std::false_type{}, Wave{});
+  else if (a.rows * a.classes * (int64_t)sizeof(T) >= kStreamBytes) launch(std::true_type{}, Group{});
+  else launch(std::false_type{}, Group{});
   MGB_LAUNCH_CHECK("distillation gradient");
   return 0;
 }

@@ -11,13 +11,14 @@ namespace block {
 namespace {
 
 template <typename T>
-struct Gated {
+struct Gated : product::Plainly {
   static constexpr bool kDual = true;
   const Params& p;
-  __device__ __forceinline__ Gated(const Params& params, const product::Job&, uint32_t) : p(params) {}
-  template <int kCount>
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, const float* gate, const float* up) const {
-    if (n >= p.hidden_columns) return;
+  int64_t rows;
+  __device__ __forceinline__ Gated(const Params& params, const product::Job& job, uint32_t) : p(params), rows(job.rows) {}
+  template <int kCount, bool kWhole, typename L>
+  __device__ __forceinline__ void store(int64_t m, int64_t n, const float* gate, const float* up, const L&) const {
+    if (!kWhole && (m >= rows || n >= p.hidden_columns)) return;
     float h[kCount];
 #pragma unroll
     for (int e = 0; e < kCount; ++e) h[e] = activate<sizeof(T) == 4>(gate[e], p.activation) * up[e];
@@ -25,8 +26,8 @@ struct Gated {
     store_inner<T, kCount>(p.hidden, p.hidden_part, m * p.hidden_stride + n, h);
     if (p.kept) {
       float* to = p.kept + m * 2 * p.true_columns;
-      product::store_some<kCount>(to, n, p.true_columns, gate);
-      product::store_some<kCount>(to + p.true_columns, n, p.true_columns, up);
+      product::store_some<kCount, kWhole>(to, n, p.true_columns, gate);
+      product::store_some<kCount, kWhole>(to + p.true_columns, n, p.true_columns, up);
     }
   }
 };
@@ -89,7 +90,7 @@ int forward(const MgbFeedForward& a, Space& space, hipStream_t stream, bool run)
   inner.job[0].left = operand(x, a.rows, dim);
   inner.job[0].right = operands(gate, up, a.hidden, dim);
   inner.job[0].rows = a.rows;
-  inner.job[0].columns = hidden;
+  inner.job[0].columns = a.hidden;  // (tiles end at multiples of 8: they hold the padding too)
   const Size inner_size = choose(inner, true);
 
   Params outer = {};

@@ -15,23 +15,37 @@ constexpr int64_t kTurnRows = 4096;
 
 template <typename T>
 struct Slope {
-  static constexpr bool kDual = false;
+  static constexpr bool kDual = false, kBlocks = false;
+  static constexpr int kDeep = 4;
   const Params& p;
-  __device__ __forceinline__ Slope(const Params& params, const product::Job&, uint32_t) : p(params) {}
+  int64_t rows;
+  __device__ __forceinline__ Slope(const Params& params, const product::Job& job, uint32_t) : p(params), rows(job.rows) {}
   template <int kCount>
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, const float* dh) const {
-    if (n >= p.hidden_columns) return;
-    const float* from = p.kept + m * 2 * p.true_columns;
-    float gate[kCount], up[kCount], dgate[kCount], dup[kCount], hidden[kCount];
-    load_some<kCount>(from, n, p.true_columns, gate);
-    load_some<kCount>(from + p.true_columns, n, p.true_columns, up);
+  struct Loaded {
+    float gate[kCount], up[kCount];
+  };
+  template <int kCount, bool kWhole, typename L>
+  __device__ __forceinline__ void load(L& l, int64_t m, int64_t n) const {
+    const float* from = p.kept + (kWhole || m < rows ? m : rows - 1) * 2 * p.true_columns;
+    if constexpr (kWhole) {
+      __builtin_memcpy(l.gate, from + n, sizeof(l.gate));
+      __builtin_memcpy(l.up, from + p.true_columns + n, sizeof(l.up));
+    } else {
+      load_some<kCount>(from, n, p.true_columns, l.gate);
+      load_some<kCount>(from + p.true_columns, n, p.true_columns, l.up);
+    }
+  }
+  template <int kCount, bool kWhole, typename L>
+  __device__ __forceinline__ void store(int64_t m, int64_t n, const float* dh, const float*, const L& l) const {
+    if (!kWhole && (m >= rows || n >= p.hidden_columns)) return;
+    float dgate[kCount], dup[kCount], hidden[kCount];
 #pragma unroll
     for (int e = 0; e < kCount; ++e) {
       float slope;
-      const float act = activate<sizeof(T) == 4>(gate[e], p.activation, &slope);
-      const bool there = n + e < p.true_columns;  // columns that pad a row are zero whatever dy holds
-      hidden[e] = there ? act * up[e] : 0.0f;
-      dgate[e] = there ? dh[e] * up[e] * slope : 0.0f;
+      const float act = activate<sizeof(T) == 4>(l.gate[e], p.activation, &slope);
+      const bool there = kWhole || n + e < p.true_columns;  // columns that pad a row are zero whatever dy holds
+      hidden[e] = there ? act * l.up[e] : 0.0f;
+      dgate[e] = there ? dh[e] * l.up[e] * slope : 0.0f;
       dup[e] = there ? dh[e] * act : 0.0f;
     }
     const int64_t at = m * p.hidden_stride + n;
@@ -68,7 +82,8 @@ int gradient(const MgbFeedForwardGradient& a, Space& space, hipStream_t stream, 
   LayJobs jobs = {}, turned = {};
   // Matrices whose products go along their columns are transposed first where that
   // costs little: binary32 ones, which are laid out anyhow, and others of many rows
-  // of x (16,384 x 1,024 x 4,096: two products of 322 and 280 us become TBD).
+  // of x (16,384 x 1,024 x 4,096: two products of
+  // 322 and 280 us become 300 and 182, for 18 us of transposing).
   const bool turn_weights = sizeof(T) == 4 || a.rows >= kTurnRows;
   const int64_t dim = padded(a.dim), hidden = padded(a.hidden);
   const bool copy = !lies_well<T>(a.gate, a.hidden, a.dim, a.gate_stride) ||
@@ -111,7 +126,7 @@ int gradient(const MgbFeedForwardGradient& a, Space& space, hipStream_t stream, 
   inner.job[0].left = operand(grad, a.rows, dim);
   inner.job[0].right = turn_weights ? operand(down, a.hidden, dim) : operand(down, hidden, a.dim);
   inner.job[0].rows = a.rows;
-  inner.job[0].columns = hidden;
+  inner.job[0].columns = a.hidden;  // (tiles end at multiples of 8: they hold the padding too)
   const Size inner_size = choose(inner, false);
 
   Params input = {};

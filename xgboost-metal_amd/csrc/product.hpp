@@ -26,7 +26,8 @@
 // chunks permuted.  Whatever lies outside an operand is read as zero by the bounds
 // of its buffer descriptor: rows beyond the last, and the depth's end inside a step.
 //
-// Measured (one MI355X): DESIGN has the cases; 8,192 x 4,096 x 4,096 bfloat16.
+// 8,192 x 4,096 x 4,096 in blocks of 8 bits: 137 us, 2.0 PFLOP/s; the gated pair of
+// 16,384 x 1,024 to 2 x 4,096 in bfloat16: 310 us, 0.89 PFLOP/s with its epilogue.
 #pragma once
 #include <type_traits>
 
@@ -632,38 +633,88 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_product(Params p) {
 
   // ---- what becomes of the sums: a lane has 4 or, of pairs, 8 columns of a row
   const Finish finish(p, job, split);
-  constexpr int kCount = kPairs ? 8 : 4;
+  constexpr int kCount = kPairs ? 8 : 4, kGroups = S::kTilesN * 4 / kCount, kHalves = Finish::kDual ? 1 : 2;
+  constexpr int kItems = 2 * S::kTilesM * kGroups * kHalves, kDeep = Finish::kDeep < kItems ? Finish::kDeep : kItems;
+  const int64_t m0 = row0 + wm * S::kRowsM + lane % 16, n0 = column0 + wn * S::kRowsN + lane / 16 * kCount;
+  auto row_of = [&](int item) {
+    return m0 + item / (S::kTilesM * kGroups * kHalves) * S::kHalfM + item / (kGroups * kHalves) % S::kTilesM * 16;
+  };
+  auto column_of = [&](int item) { return n0 + item / kHalves % kGroups * (4 * kCount) + item % kHalves * S::kHalfN; };
+  if constexpr (Finish::kBlocks) {
+    // Results in 8 bits: a tile's 128 columns are a block.  Each wave's largest values
+    // of its rows meet in LDS.
+    static_assert(Finish::kDual && kPairs && S::kHalfN == 128, "a block a tile");
+    float* const tops = (float*)lds;
+    wait_barrier();
 #pragma unroll
-  for (int x = 0; x < 2; ++x)
+    for (int x = 0; x < 2; ++x)
 #pragma unroll
-    for (int i = 0; i < S::kTilesM; ++i) {
-      const int64_t m = row0 + x * S::kHalfM + wm * S::kRowsM + i * 16 + lane % 16;
-      if (m >= job.rows) continue;
+      for (int i = 0; i < S::kTilesM; ++i) {
+        float top = 0.0f;
 #pragma unroll
-      for (int j = 0; j < S::kTilesN; j += kCount / 4) {
-        const int64_t n = column0 + wn * S::kRowsN + j * 16 + lane / 16 * kCount;
+        for (int j = 0; j < S::kTilesN; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float v = finish.value(sum[x][0][i][j][e], sum[x][1][i][j][e]);
+            sum[x][0][i][j][e] = v;
+            top = fmaxf(top, fabsf(v) < INFINITY ? fabsf(v) : 0.0f);
+          }
+        top = fmaxf(top, __shfl_xor(top, 16, kWave));
+        top = fmaxf(top, __shfl_xor(top, 32, kWave));
+        if (lane < 16) tops[wn * S::kTileM + x * S::kHalfM + wm * S::kRowsM + i * 16 + lane] = top;
+      }
+    wait_loads<0>();
+    wait_barrier();
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int i = 0; i < S::kTilesM; ++i) {
+        const int row = x * S::kHalfM + wm * S::kRowsM + i * 16 + lane % 16;
+        if (row0 + row >= job.rows) continue;
+        float top = 0.0f, v[S::kTilesN * 4];
+#pragma unroll
+        for (int w = 0; w < S::kWavesN; ++w) top = fmaxf(top, tops[w * S::kTileM + row]);
+#pragma unroll
+        for (int e = 0; e < S::kTilesN * 4; ++e) v[e] = sum[x][0][i][e / 4][e % 4];
+        finish.store(row0 + row, n0, tj, v, top, wn == 0 && lane < 16);
+      }
+  } else {
+    auto finish_tile = [&](auto whole) {
+      // What the end reads of memory is on its way kDeep items ahead.
+      typename Finish::template Loaded<kCount> ring[kDeep];
+#pragma unroll
+      for (int item = 0; item < kDeep; ++item)
+        finish.template load<kCount, decltype(whole)::value>(ring[item], row_of(item), column_of(item));
+#pragma unroll
+      for (int item = 0; item < kItems; ++item) {
+        const int x = item / (S::kTilesM * kGroups * kHalves), i = item / (kGroups * kHalves) % S::kTilesM;
+        const int j = item / kHalves % kGroups * (kCount / 4), y = item % kHalves;
         float v[2][kCount];
 #pragma unroll
-        for (int y = 0; y < 2; ++y)
-#pragma unroll
-          for (int e = 0; e < kCount; ++e) v[y][e] = sum[x][y][i][j + e / 4][e % 4];
-        if constexpr (Finish::kDual) {
-          finish.template operator()<kCount>(m, n, v[0], v[1]);
-        } else {
-#pragma unroll
-          for (int y = 0; y < 2; ++y) finish.template operator()<kCount>(m, n + y * S::kHalfN, v[y]);
+        for (int e = 0; e < kCount; ++e) {
+          v[0][e] = sum[x][y][i][j + e / 4][e % 4];
+          if constexpr (Finish::kDual) v[1][e] = sum[x][1][i][j + e / 4][e % 4];
         }
+        finish.template store<kCount, decltype(whole)::value>(row_of(item), column_of(item), v[0], v[1], ring[item % kDeep]);
+        if (item + kDeep < kItems)
+          finish.template load<kCount, decltype(whole)::value>(ring[item % kDeep], row_of(item + kDeep), column_of(item + kDeep));
       }
-    }
+    };
+    if (row0 + S::kTileM <= job.rows && column0 + (Finish::kDual ? S::kHalfN : S::kTileN) <= job.columns)
+      finish_tile(std::true_type{});
+    else
+      finish_tile(std::false_type{});
+  }
 }
 
-// Values of a row, to the type rounded once; those beyond `columns` are not stored.
-template <int kCount, typename T>
+// Values of a row, to the type rounded once; without kWhole those beyond `columns` are
+// not stored.
+template <int kCount, bool kWhole, typename T>
 __device__ __forceinline__ void store_some(T* row, int64_t n, int64_t columns, const float* v) {
   T r[kCount];
 #pragma unroll
   for (int e = 0; e < kCount; ++e) r[e] = (T)v[e];
-  if (n + kCount <= columns) {
+  if (kWhole || n + kCount <= columns) {
     __builtin_memcpy(row + n, r, sizeof(r));
   } else {
 #pragma unroll
@@ -672,29 +723,39 @@ __device__ __forceinline__ void store_some(T* row, int64_t n, int64_t columns, c
   }
 }
 
-template <typename T>
-struct Store {
-  static constexpr bool kDual = false;
-  T* out;
-  int64_t stride, columns;
-  __device__ __forceinline__ Store(const Params&, const Job& job, uint32_t)
-      : out((T*)job.out), stride(job.out_stride), columns(job.columns) {}
+// What ends a tile: store() takes the sums (of a dual form both matrices') of kCount
+// columns of a row from n on, and what load() fetched before.  kWhole: the tile lies
+// within the result.
+struct Plainly {
+  static constexpr bool kDual = false, kBlocks = false;
+  static constexpr int kDeep = 1;
   template <int kCount>
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, const float* v) const {
-    store_some<kCount>(out + m * stride, n, columns, v);
+  struct Loaded {};
+  template <int kCount, bool kWhole, typename L>
+  __device__ __forceinline__ void load(L&, int64_t, int64_t) const {}
+};
+
+template <typename T>
+struct Store : Plainly {
+  T* out;
+  int64_t stride, rows, columns;
+  __device__ __forceinline__ Store(const Params&, const Job& job, uint32_t)
+      : out((T*)job.out), stride(job.out_stride), rows(job.rows), columns(job.columns) {}
+  template <int kCount, bool kWhole, typename L>
+  __device__ __forceinline__ void store(int64_t m, int64_t n, const float* v, const float*, const L&) const {
+    if (kWhole || m < rows) store_some<kCount, kWhole>(out + m * stride, n, columns, v);
   }
 };
 
 // A share of the depth, added up by k_join.
-struct Partial {
-  static constexpr bool kDual = false;
+struct Partial : Plainly {
   float* out;
-  int64_t columns;
+  int64_t rows, columns;
   __device__ __forceinline__ Partial(const Params& p, const Job& job, uint32_t split)
-      : out(p.partials + split * p.partial_size + job.partial), columns(job.columns) {}
-  template <int kCount>
-  __device__ __forceinline__ void operator()(int64_t m, int64_t n, const float* v) const {
-    store_some<kCount>(out + m * columns, n, columns, v);
+      : out(p.partials + split * p.partial_size + job.partial), rows(job.rows), columns(job.columns) {}
+  template <int kCount, bool kWhole, typename L>
+  __device__ __forceinline__ void store(int64_t m, int64_t n, const float* v, const float*, const L&) const {
+    if (kWhole || m < rows) store_some<kCount, kWhole>(out + m * columns, n, columns, v);
   }
 };
 
