@@ -3,18 +3,30 @@
 //
 // A workgroup has 16 rows of w (result columns), its waves a share of the depth
 // each, in units of one or four instructions (32 or 128 values), whose loads are all
-// in flight; the waves' sums meet in LDS.  Operands go from memory to registers in the matrix instruction's
-// layout, whatever their alignment, and become bfloat16 or binary16 there: binary32
-// values three bfloat16 each (six instructions a product), blocks of 8 bits the values
-// they stand for, exactly, and x, where the other operand is blocks, is rounded to
-// blocks on the way (a block is a unit, and lies in the registers of four lanes).
+// in flight; the waves' sums meet in LDS.  Where there are few such workgroups, the 16
+// rows that an instruction takes of w are those of 8 columns in 2 slices of the depth,
+// or of 4 in 4, and x's likewise: of its products those of equal slices count, and
+// twice or four times as many workgroups read.
+//
+// Operands go from memory to registers in the matrix instruction's layout, whatever
+// their alignment, and become bfloat16 or binary16 there: binary32 values three
+// bfloat16 each (six instructions a product), blocks of 8 bits the values they stand
+// for, exactly, and x, where the other operand is blocks, is rounded to blocks on the
+// way (a block is a unit, and lies in the registers of four lanes).
 #pragma once
 #include "feed_forward.hpp"
 
 namespace mgb {
 namespace block {
 
+// Above it tiles: 1,024 x 4,096 in bfloat16, 32 rows 18 us and 33, as tiles, 21 (64:
+// 22); 256 x 1,024: 7 and 12.
 constexpr int kMostFewRows = 32;
+
+// Slices pay where workgroups are few.  1,024 x 4,096 in bfloat16, a row: 7.0 us, whole
+// 11.8; 16 rows: 12.6, whole 15.2; 32 rows: 18.0, whole 20.3.  4,096 x 14,336, four rows:
+// 96 us, whole 77.
+constexpr int64_t kSlicedColumns = 4096, kSlicedDepth = 8192;
 
 struct Few {
   const void* x;
@@ -67,20 +79,18 @@ __device__ __forceinline__ uint2 round_eight(const float* v, float factor) {
   return {(uint32_t)word[0], (uint32_t)word[1]};
 }
 
-// What eight e4m3 values times 2^(scale - 127) are, as bfloat16 (whose steps end at 2^-133).
+// What eight e4m3 values times 2^(scale - 127) are, as bfloat16 (whose steps end at
+// 2^-133); scale 255 is a block of NaN.
 __device__ __forceinline__ product::bf16x8 widen_eight(uint2 bytes, uint32_t scale) {
+  using Pair = __attribute__((ext_vector_type(2))) __bf16;
   const float factor = scale_value(scale);
-  product::bf16x8 v;
+  Pair v[4];
 #pragma unroll
   for (int w = 0; w < 2; ++w) {
-    const int word = (int)(w ? bytes.y : bytes.x);
-    const auto low = __builtin_amdgcn_cvt_pk_f32_fp8(word, false), high = __builtin_amdgcn_cvt_pk_f32_fp8(word, true);
-    v[w * 4] = (__bf16)(low[0] * factor);
-    v[w * 4 + 1] = (__bf16)(low[1] * factor);
-    v[w * 4 + 2] = (__bf16)(high[0] * factor);
-    v[w * 4 + 3] = (__bf16)(high[1] * factor);
+    v[w * 2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w ? bytes.y : bytes.x, factor, false);
+    v[w * 2 + 1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w ? bytes.y : bytes.x, factor, true);
   }
-  return v;
+  return __builtin_bit_cast(product::bf16x8, v);
 }
 
 // A unit of 16 rows: lane l has 8 values of row l % 16 for each of kSteps instructions.
@@ -134,17 +144,43 @@ struct Unit {
   }
 };
 
-// x rounded to blocks: a unit's scale, of the four lanes that hold a row's.
+// x rounded to blocks: a unit's scale, of the four lanes that hold a row's.  Sizes are
+// compared as integers, 16-bit ones two at once; infinities and NaN, the largest of
+// them, are left out where there are any.
 template <class Kind_, int kSteps>
 __device__ __forceinline__ void find_scale(Unit<Kind_, kSteps>& u) {
   if constexpr (std::is_same_v<Kind_, Rounded<typename Kind_::Type>>) {
-    float largest = 0.0f;
+    using T = typename Kind_::Type;
+    using Pair = __attribute__((ext_vector_type(2))) uint16_t;
+    constexpr uint32_t kInfinite = sizeof(T) == 4 ? 0x7f800000u : std::is_same_v<T, _Float16> ? 0x7c00u : 0x7f80u;
+    uint32_t most = 0;
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-      float v[8];
-      u.values(s, v);
+      for (const uint4& r : u.raw)
+        most = max(max(most, max(r.x & 0x7fffffffu, r.y & 0x7fffffffu)), max(r.z & 0x7fffffffu, r.w & 0x7fffffffu));
+    } else {
+      Pair both = {};
 #pragma unroll
-      for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.0f);
+      for (const uint4& r : u.raw)
+#pragma unroll
+        for (const uint32_t word : {r.x, r.y, r.z, r.w})
+          both = __builtin_elementwise_max(both, __builtin_bit_cast(Pair, word & 0x7fff7fffu));
+      most = max((uint32_t)both[0], (uint32_t)both[1]);
+    }
+    float largest;
+    if (__any(most >= kInfinite)) {
+      largest = 0.0f;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        float v[8];
+        u.values(s, v);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) largest = fmaxf(largest, fabsf(v[e]) < INFINITY ? fabsf(v[e]) : 0.0f);
+      }
+    } else if constexpr (sizeof(T) == 4) {
+      largest = __uint_as_float(most);
+    } else {
+      largest = (float)__builtin_bit_cast(T, (uint16_t)most);
     }
     largest = fmaxf(largest, __shfl_xor(largest, 16, kWave));
     largest = fmaxf(largest, __shfl_xor(largest, 32, kWave));
@@ -191,18 +227,21 @@ __device__ __forceinline__ float4v multiply_one(product::int4v w, product::int4v
                                                    __builtin_bit_cast(product::bf16x8, x), sum, 0, 0, 0);
 }
 
-// kTiles of 16 rows of x; kDual: out = act(x w0^T) (x w1^T).
-template <class X, class W, typename Out, int kTiles, bool kDual, int kWaves, int kSteps>
+// kTiles of 16 / kSlices rows of x; kDual: out = act(x w0^T) (x w1^T).
+template <class X, class W, typename Out, int kTiles, int kSlices, bool kDual, int kWaves, int kSteps>
 __global__ __launch_bounds__(kWaves* kWave) void k_few(Few p) {
   constexpr int kMatrices = kDual ? 2 : 1;
   constexpr bool kBlocks = std::is_same_v<W, InBlocks>;
   static_assert(X::kParts == W::kParts, "both in as many parts");
-  __shared__ float4v shared[kWaves][kMatrices][kTiles][kWave];
+  constexpr int kColumns = 16 / kSlices, kRows = 16 / kSlices, kSums = 4 / kSlices;
+  using Sum = __attribute__((ext_vector_type(kSums))) float;
+  __shared__ Sum shared[kWaves][kMatrices][kTiles][kWave];
   using XT = typename X::Type;
   using WT = typename W::Type;
   const int lane = threadIdx.x % kWave, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int quarter = lane / 16;
-  const int64_t column0 = (int64_t)blockIdx.x * 16, column = column0 + lane % 16;
+  const int slice = lane % kSlices;
+  const int64_t column0 = (int64_t)blockIdx.x * kColumns, column = column0 + lane % 16 / kSlices;
   const bool column_there = column < p.columns;
   const WT* w[kMatrices];
   const uint8_t* w_scales[kMatrices];
@@ -216,22 +255,24 @@ __global__ __launch_bounds__(kWaves* kWave) void k_few(Few p) {
   bool row_there[kTiles];
 #pragma unroll
   for (int t = 0; t < kTiles; ++t) {
-    const int64_t row = t * 16 + lane % 16;
+    const int64_t row = t * kRows + lane % 16 / kSlices;
     row_there[t] = row < p.rows;
     x[t] = (const XT*)p.x + (row_there[t] ? row * p.x_stride : 0);
     x_scales[t] = std::is_same_v<X, InBlocks> ? p.x_scales + (row_there[t] ? row * p.x_scale_stride : 0) : nullptr;
   }
   float4v sum[kMatrices][kTiles] = {};
-  const int64_t units = (p.depth + 32 * kSteps - 1) / (32 * kSteps);
+  const int64_t units = (p.depth + 32 * kSteps * kSlices - 1) / (32 * kSteps * kSlices);
   int64_t unit = units * wave / kWaves;
   const int64_t end = units * (wave + 1) / kWaves;
   Unit<W, kSteps> next_w[kMatrices];
   Unit<X, kSteps> next_x[kTiles];
   auto fetch = [&] {
+    const int64_t at = unit * kSlices + slice;
+    const bool within = kSlices == 1 || at * (32 * kSteps) < p.depth;
 #pragma unroll
-    for (int m = 0; m < kMatrices; ++m) next_w[m].load(w[m], w_scales[m], unit, p.depth, column_there, quarter, kBlocks);
+    for (int m = 0; m < kMatrices; ++m) next_w[m].load(w[m], w_scales[m], at, p.depth, column_there && within, quarter, kBlocks);
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) next_x[t].load(x[t], x_scales[t], unit, p.depth, row_there[t], quarter, kBlocks);
+    for (int t = 0; t < kTiles; ++t) next_x[t].load(x[t], x_scales[t], at, p.depth, row_there[t] && within, quarter, kBlocks);
   };
   // The next unit's loads are on their way while one is multiplied, where the
   // registers hold both.
@@ -272,62 +313,76 @@ __global__ __launch_bounds__(kWaves* kWave) void k_few(Few p) {
 #pragma unroll
   for (int m = 0; m < kMatrices; ++m)
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) shared[wave][m][t][lane] = sum[m][t];
+    for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+      for (int e = 0; e < kSums; ++e) shared[wave][m][t][lane][e] = group_sum<kSlices>(sum[m][t][e * kSlices + slice]);
   __syncthreads();
-  // A lane joins four columns of a row.
+  auto finish = [&](int64_t row, int64_t column, float first, float second) {
+    if (row >= p.rows || column >= p.columns) return;
+    if constexpr (kDual) {
+      if (p.kept) {
+        p.kept[row * 2 * p.columns + column] = first;
+        p.kept[(row * 2 + 1) * p.columns + column] = second;
+      }
+      first = activate<sizeof(Out) == 4>(first, p.activation) * second;
+    }
+    ((Out*)p.out)[row * p.columns + column] = (Out)first;
+  };
+  // A lane joins kSums columns of a row.
   for (int at = threadIdx.x; at < kTiles * kWave; at += kWaves * kWave) {
     const int t = at / kWave, l = at % kWave;
-    float4v total[kMatrices];
+    Sum total[kMatrices];
 #pragma unroll
     for (int m = 0; m < kMatrices; ++m) {
       total[m] = shared[0][m][t][l];
 #pragma unroll
       for (int k = 1; k < kWaves; ++k) total[m] += shared[k][m][t][l];
     }
-    const int64_t row = t * 16 + l % 16, first = column0 + l / 16 * 4;
-    if (row >= p.rows) continue;
+    if (l % kSlices != 0) continue;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (first + e >= p.columns) continue;
-      float v = total[0][e];
-      if constexpr (kDual) {
-        if (p.kept) {
-          p.kept[row * 2 * p.columns + first + e] = total[0][e];
-          p.kept[(row * 2 + 1) * p.columns + first + e] = total[kMatrices - 1][e];
-        }
-        v = activate<sizeof(Out) == 4>(v, p.activation) * total[kMatrices - 1][e];
-      }
-      ((Out*)p.out)[row * p.columns + first + e] = (Out)v;
-    }
+    for (int e = 0; e < kSums; ++e)
+      finish(t * kRows + l % 16 / kSlices, column0 + l / 16 * kSums + e, total[0][e], total[kMatrices - 1][e]);
   }
 }
 
 template <class X, class W, typename Out, bool kDual>
 void few_rows(const Few& p, hipStream_t stream) {
-  const uint32_t groups = (uint32_t)((p.columns + 15) / 16);
   // Waves for every unit, up to as many as the registers of their loads allow; units of
   // one instruction where there are fewer of four than waves.
   constexpr int kMost = kDual ? 8 : 16;
   constexpr bool kBlocks = std::is_same_v<W, InBlocks>;
-  auto launch = [&](auto tiles, auto waves, auto steps) {
-    constexpr int kWaves = decltype(waves)::value;
-    k_few<X, W, Out, decltype(tiles)::value, kDual, kWaves, decltype(steps)::value><<<groups, kWaves * kWave, 0, stream>>>(p);
+  auto launch = [&](auto tiles, auto slices, auto waves, auto steps) {
+    constexpr int kWaves = decltype(waves)::value, kSlices = decltype(slices)::value;
+    const uint32_t groups = (uint32_t)((p.columns * kSlices + 15) / 16);
+    k_few<X, W, Out, decltype(tiles)::value, kSlices, kDual, kWaves, decltype(steps)::value><<<groups, kWaves * kWave, 0, stream>>>(p);
   };
-  auto with_tiles = [&](auto tiles) {
+  auto with = [&](auto tiles, auto slices) {
+    using One = std::integral_constant<int, 1>;
     using Four = std::integral_constant<int, 4>;
-    using Most = std::integral_constant<int, kMost>;
+    using Most = std::integral_constant<int, (kBlocks && decltype(slices)::value > 1) ? 8 : kMost>;
+    const int64_t depth = (p.depth + decltype(slices)::value - 1) / decltype(slices)::value;
     if constexpr (kBlocks) {
-      if (p.depth > 512) launch(tiles, Most{}, Four{});
-      else launch(tiles, Four{}, Four{});
+      if (depth > 512) launch(tiles, slices, Most{}, Four{});
+      else launch(tiles, slices, Four{}, Four{});
     } else {
-      using One = std::integral_constant<int, 1>;
-      if (p.depth <= 128) launch(tiles, Four{}, One{});
-      else if (sizeof(typename X::Type) == 4 || p.depth < 128 * kMost) launch(tiles, Most{}, One{});
-      else launch(tiles, Most{}, Four{});
+      if (depth <= 128) launch(tiles, slices, Four{}, One{});
+      else if constexpr (sizeof(typename X::Type) == 4) launch(tiles, slices, Most{}, One{});
+      else if (depth < 128 * kMost) launch(tiles, slices, Most{}, One{});
+      else launch(tiles, slices, Most{}, Four{});
     }
   };
-  if (p.rows <= 16) with_tiles(std::integral_constant<int, 1>{});
-  else with_tiles(std::integral_constant<int, 2>{});
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  using Four = std::integral_constant<int, 4>;
+  if (p.columns <= kSlicedColumns && p.depth <= kSlicedDepth) {
+    if (p.rows <= 4) return with(One{}, Four{});
+    if (p.rows <= 8) return with(One{}, Two{});
+    if constexpr (!kBlocks)
+      if (p.rows <= 16) return with(Two{}, Two{});
+    if constexpr (!kBlocks && sizeof(typename X::Type) == 2) return with(Four{}, Two{});
+  }
+  if (p.rows <= 16) with(One{}, One{});
+  else with(Two{}, One{});
 }
 
 }  // namespace block
