@@ -143,7 +143,7 @@ int multiply(T* out, const MgbBlocks& x, const MgbBlocks& weight, Space& space, 
     p.job[0].left = operand(left, x.rows, p.depth);
     p.job[0].right = operand(right, weight.rows, p.depth);
     const Size size = choose_shares(p, space, false);
-    if (run) store_product<__bf16, T, false, false>(p, size, stream);
+    if (run) store_product<__bf16, __bf16, T, false, false>(p, size, stream);
   } else {
     p.job[0].left = operand8(x);
     p.job[0].right = operand8(weight);
@@ -152,7 +152,7 @@ int multiply(T* out, const MgbBlocks& x, const MgbBlocks& weight, Space& space, 
     p.left_scale_stride = x.scale_stride;
     p.right_scale_stride = weight.scale_stride;
     const Size size = choose_shares(p, space, false, kBlock, product::kScaleSteps);
-    if (run) store_product<product::E4m3, T, false, false>(p, size, stream);
+    if (run) store_product<product::E4m3, uint8_t, T, false, false>(p, size, stream);
   }
   return 0;
 }

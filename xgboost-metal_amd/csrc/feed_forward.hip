@@ -107,8 +107,8 @@ int forward(const MgbFeedForward& a, Space& space, hipStream_t stream, bool run)
   const Size outer_size = choose_shares(outer, space, false);
   if (!run) return 0;
   lay_out<T>(jobs, stream);
-  launch_product<E, false, false, Gated<T>>(inner, inner_size, stream);
-  store_product<E, T, false, false>(outer, outer_size, stream);
+  launch_product<E, T, false, false, Gated<T>>(inner, inner_size, stream);
+  store_product<E, T, T, false, false>(outer, outer_size, stream);
   MGB_LAUNCH_CHECK("feed forward");
   return 0;
 }

@@ -5,7 +5,7 @@
 #include <algorithm>
 #include <vector>
 
-#include "product.hpp"
+#include "product_parts.hpp"
 
 namespace mgb {
 namespace block {
@@ -69,6 +69,7 @@ struct LayJob {
   const void* from;
   char* to;
   int64_t rows, columns, stride, chunks, part;  // stride in elements, chunks of 8 a row of `to`, part in bytes
+  bool turned;
 };
 constexpr int kMostLay = 5;
 struct LayJobs {
@@ -79,10 +80,9 @@ struct LayJobs {
 constexpr int kLayThreads = 256;
 
 template <typename T>
-__global__ __launch_bounds__(kLayThreads) void k_lay_out(LayJobs jobs) {
+__device__ __forceinline__ void lay_straight(const LayJob& job) {
   using E = typename Kind<T>::E;
   constexpr int kParts = Kind<T>::kParts;
-  const LayJob job = jobs.job[blockIdx.y];
   const int64_t all = job.rows * job.chunks, step = (int64_t)gridDim.x * kLayThreads;
   const int64_t step_rows = step / job.chunks, step_chunks = step % job.chunks;
   int64_t at = (int64_t)blockIdx.x * kLayThreads + threadIdx.x, row = at / job.chunks, chunk = at % job.chunks;
@@ -116,11 +116,10 @@ __global__ __launch_bounds__(kLayThreads) void k_lay_out(LayJobs jobs) {
 // The same, transposed: rows of `to` are columns of `from`.
 constexpr int kTurnSide = 64;
 template <typename T>
-__global__ __launch_bounds__(kLayThreads) void k_turn(LayJobs jobs) {
+__device__ __forceinline__ void lay_across(const LayJob& job) {
   using E = typename Kind<T>::E;
   constexpr int kParts = Kind<T>::kParts;
   __shared__ float tile[kTurnSide][kTurnSide + 1];
-  const LayJob job = jobs.job[blockIdx.y];
   const int64_t across = (job.columns + kTurnSide - 1) / kTurnSide, down = (job.rows + kTurnSide - 1) / kTurnSide;
   for (int64_t at = blockIdx.x; at < across * down; at += gridDim.x) {
     const int64_t row0 = at / across * kTurnSide, column0 = at % across * kTurnSide;
@@ -160,6 +159,13 @@ __global__ __launch_bounds__(kLayThreads) void k_turn(LayJobs jobs) {
   }
 }
 
+template <typename T>
+__global__ __launch_bounds__(kLayThreads) void k_lay_out(LayJobs jobs) {
+  const LayJob& job = jobs.job[blockIdx.y];
+  if (job.turned) lay_across<T>(job);
+  else lay_straight<T>(job);
+}
+
 // A matrix as a product takes it.
 struct Laid {
   const char* data;
@@ -179,7 +185,7 @@ Laid lay(Space& space, LayJobs& jobs, const void* data, int64_t rows, int64_t co
   if (!copy) return {(const char*)data, (rows > 1 ? stride : columns) * 2, 0};
   const int64_t width = padded(columns) * 2, part = width * rows;
   char* to = space.take(part * Kind<T>::kParts);
-  jobs.job[jobs.count++] = {data, to, rows, columns, stride, width / 16, part};
+  jobs.job[jobs.count++] = {data, to, rows, columns, stride, width / 16, part, false};
   return {to, width, part};
 }
 
@@ -193,24 +199,20 @@ template <typename T>
 Laid lay_turned(Space& space, LayJobs& jobs, const void* data, int64_t rows, int64_t columns, int64_t stride) {
   const int64_t width = inner_stride(padded(rows)) * 2, part = width * columns;
   char* to = space.take(part * Kind<T>::kParts);
-  jobs.job[jobs.count++] = {data, to, rows, columns, stride, width / 16, part};
+  jobs.job[jobs.count++] = {data, to, rows, columns, stride, width / 16, part, true};
   return {to, width, part};
-}
-
-template <typename T>
-void turn(const LayJobs& jobs, hipStream_t stream) {
-  int64_t most = 0;
-  for (int k = 0; k < jobs.count; ++k)
-    most = std::max(most, ((jobs.job[k].rows + kTurnSide - 1) / kTurnSide) * ((jobs.job[k].columns + kTurnSide - 1) / kTurnSide));
-  if (most > 0) k_turn<T><<<dim3((uint32_t)std::min<int64_t>(most, 4096), jobs.count), kLayThreads, 0, stream>>>(jobs);
 }
 
 template <typename T>
 void lay_out(const LayJobs& jobs, hipStream_t stream) {
   int64_t most = 0;
-  for (int k = 0; k < jobs.count; ++k) most = std::max(most, jobs.job[k].rows * jobs.job[k].chunks);
+  for (int k = 0; k < jobs.count; ++k) {
+    const LayJob& job = jobs.job[k];
+    most = std::max(most, job.turned ? ((job.rows + kTurnSide - 1) / kTurnSide) * ((job.columns + kTurnSide - 1) / kTurnSide)
+                                     : (job.rows * job.chunks + kLayThreads - 1) / kLayThreads);
+  }
   if (most == 0) return;
-  const int64_t groups = std::min<int64_t>((most + kLayThreads - 1) / kLayThreads, 2048);
+  const int64_t groups = std::min<int64_t>(most, 4096);
   k_lay_out<T><<<dim3((uint32_t)groups, jobs.count), kLayThreads, 0, stream>>>(jobs);
 }
 
@@ -231,15 +233,20 @@ inline uint32_t lay_tiles(Params& p, Size size, bool dual) {
   return p.tiles;
 }
 
-inline int64_t steps_of(const Params& p, int values) {
-  return std::max<int64_t>(1, (p.depth + values - 1) / values) * p.pairs * p.sources;
+// Steps of a workgroup that has the whole depth.  Parts' products go by k_product's
+// large tiles, or by k_parts' smaller ones, which have all six in a step of 32.
+inline bool in_parts(const Params& p, Size size) { return p.pairs > 1 && size != kLarge; }
+inline int64_t steps_of(const Params& p, Size size, int values) {
+  const bool parts = in_parts(p, size);
+  if (parts) values = 32;
+  return std::max<int64_t>(1, (p.depth + values - 1) / values) * (parts ? 1 : p.pairs) * p.sources;
 }
 
 // Estimated times, in us, of a workgroup's step and of what comes before and after its
 // steps, with 1, 2, .. workgroups a compute unit (measured with 64 to 1,024 tiles and
-// depths of 512 to 4,096; turned operands' steps take a third longer).  Products of few
-// tiles are short of workgroups, those of many small ones of LDS' rate: the estimate
-// finds sizes and shares between.
+// depths of 512 to 4,096; turned operands' steps take a third longer, of k_parts a
+// twelfth).  Products of few tiles are short of workgroups, those of many small ones of
+// LDS' rate: the estimate finds sizes and shares between.
 struct Rate {
   int most;       // workgroups a compute unit
   float step[4], fixed[4];
@@ -247,15 +254,18 @@ struct Rate {
 constexpr Rate kRates[3] = {{1, {1.42f}, {10.0f}},
                             {2, {0.575f, 0.87f}, {6.4f, 8.8f}},
                             {4, {0.346f, 0.446f, 0.6f, 0.748f}, {4.9f, 5.3f, 6.5f, 7.6f}}};
+constexpr Rate kPartRates[3] = {{}, {1, {1.3f}, {8.0f}}, {2, {0.53f, 0.95f}, {7.5f, 7.5f}}};  // of k_parts
 constexpr int64_t kUnits = 256;  // compute units
 
-inline float estimate(Size size, int64_t workgroups, int64_t steps, bool turned) {
-  const Rate& r = kRates[size];
-  const int64_t each = (workgroups + kUnits - 1) / kUnits;
+// (Each of the 8 chiplets of 32 units has an eighth of the tiles, find_tile's stretch.)
+inline float estimate(const Params& p, Size size, int64_t tiles, int64_t shares, int64_t steps, bool turned) {
+  const Rate& r = in_parts(p, size) ? kPartRates[size] : kRates[size];
+  const float longer = !turned ? 1.0f : in_parts(p, size) ? 1.08f : 1.3f;
+  const int64_t each = ((tiles + 7) / 8 * shares + kUnits / 8 - 1) / (kUnits / 8);
   float time = 0.0f;
   for (int64_t left = each; left > 0;) {  // rounds of r.most, the last of what is left
     const int64_t rounds = left >= r.most ? left / r.most : 1, now = left >= r.most ? r.most : left;
-    time += rounds * (r.fixed[now - 1] + steps * r.step[now - 1] * (turned ? 1.3f : 1.0f));
+    time += rounds * (r.fixed[now - 1] + steps * r.step[now - 1] * longer);
     left -= rounds * now;
   }
   return time;
@@ -266,7 +276,7 @@ inline Size choose(Params& p, bool dual, int values = 64) {
   Size best = kSmall;
   float least = INFINITY;
   for (const Size size : {kLarge, kMedium, kSmall}) {
-    const float time = estimate(size, lay_tiles(p, size, dual), steps_of(p, values), false);
+    const float time = estimate(p, size, lay_tiles(p, size, dual), 1, steps_of(p, size, values), false);
     if (time < least) {
       least = time;
       best = size;
@@ -274,7 +284,7 @@ inline Size choose(Params& p, bool dual, int values = 64) {
   }
   lay_tiles(p, best, dual);
   p.splits = 1;
-  p.first_steps = p.other_steps = (uint32_t)steps_of(p, values);
+  p.first_steps = p.other_steps = (uint32_t)steps_of(p, best, values);
   return best;
 }
 
@@ -283,7 +293,6 @@ inline Size choose(Params& p, bool dual, int values = 64) {
 // or, of large tiles that leave compute units idle, a first one as long as the whole
 // work is to take and shorter ones for the idle units.
 inline Size choose_shares(Params& p, Space& space, bool turned, int values = 64, int64_t most_steps = INT32_MAX) {
-  const int64_t steps = steps_of(p, values);
   Size best = kSmall;
   int64_t best_first = 0, best_other = 0;
   float least = INFINITY;
@@ -295,22 +304,23 @@ inline Size choose_shares(Params& p, Space& space, bool turned, int values = 64,
     best_other = other;
   };
   for (const Size size : {kLarge, kMedium, kSmall}) {
-    const int64_t tiles = lay_tiles(p, size, false);
+    const int64_t tiles = lay_tiles(p, size, false), steps = steps_of(p, size, values);
     const float area = (float)side(size) * side(size) * tiles * 8.0f / 5e6f;  // written and read again, 5 TB/s
     for (int64_t shares = 1; shares <= 64; shares += shares < 8 ? 1 : shares < 16 ? 2 : 8) {
       const int64_t each = (steps + shares - 1) / shares;
       if (shares > 1 && each < 4 && each * (shares - 1) >= steps) break;
-      consider(size, each, each, estimate(size, tiles * shares, each, turned) + (shares > 1 ? 3.0f + area * shares : 0.0f));
+      consider(size, each, each, estimate(p, size, tiles, shares, each, turned) + (shares > 1 ? 3.0f + area * shares : 0.0f));
     }
     if (size != kLarge || tiles <= kUnits / 2 || tiles >= kUnits) continue;
     const int64_t first = (steps * tiles + kUnits - 1) / kUnits, rest = steps - first;
     for (int64_t shares = 1; shares <= 6 && rest >= shares; ++shares) {
       const int64_t other = (rest + shares - 1) / shares, rounds = (tiles * shares + kUnits - tiles - 1) / (kUnits - tiles);
-      const float idle = rounds * estimate(size, 1, other, turned), own = estimate(size, 1, first, turned);
+      const float idle = rounds * estimate(p, size, 1, 1, other, turned), own = estimate(p, size, 1, 1, first, turned);
       consider(size, first, other, std::max(idle, own) + 3.0f + area * (1 + shares));
     }
   }
   lay_tiles(p, best, false);
+  const int64_t steps = steps_of(p, best, values);
   p.first_steps = (uint32_t)std::min(best_first, steps);
   p.other_steps = (uint32_t)best_other;
   p.splits = steps > best_first ? 1 + (uint32_t)((steps - best_first + best_other - 1) / best_other) : 1;
@@ -343,35 +353,39 @@ __global__ __launch_bounds__(256) void k_join(Params p) {
   }
 }
 
-template <typename E, bool kLeftTurned, bool kRightTurned, class Finish>
+// T: the values' type, whose parts k_parts multiplies in smaller tiles.
+template <typename E, typename T, bool kLeftTurned, bool kRightTurned, class Finish>
 void launch_product(const Params& p, Size size, hipStream_t stream) {
   const uint32_t groups = (p.tiles + 7) / 8 * 8 * p.splits;
-  switch (size) {
-    case kLarge:
-      product::k_product<E, kLeftTurned, kRightTurned, product::Large, Finish>
-          <<<groups, product::Large::kThreads, 0, stream>>>(p);
-      break;
-    case kMedium:
-      product::k_product<E, kLeftTurned, kRightTurned, product::Medium, Finish>
-          <<<groups, product::Medium::kThreads, 0, stream>>>(p);
-      break;
-    case kSmall:
-      product::k_product<E, kLeftTurned, kRightTurned, product::Small, Finish>
-          <<<groups, product::Small::kThreads, 0, stream>>>(p);
+  auto launch = [&](auto tile) {
+    using S = decltype(tile);
+    product::k_product<E, kLeftTurned, kRightTurned, S, Finish><<<groups, S::kThreads, 0, stream>>>(p);
+  };
+  if (size == kLarge) return launch(product::Large{});
+  if constexpr (Kind<T>::kParts == 3) {
+    auto parts = [&](auto tile) {
+      using S = decltype(tile);
+      product::k_parts<kLeftTurned, kRightTurned, S, Finish><<<groups, S::kThreads, 0, stream>>>(p);
+    };
+    if (size == kMedium) parts(product::PartMedium{});
+    else parts(product::PartSmall{});
+  } else {
+    if (size == kMedium) launch(product::Medium{});
+    else launch(product::Small{});
   }
 }
 
-// Products whose results are stored as they are, without gaps.
-template <typename E, typename T, bool kLeftTurned, bool kRightTurned>
+// Products whose results are stored as they are, without gaps; Out: their type.
+template <typename E, typename T, typename Out, bool kLeftTurned, bool kRightTurned>
 void store_product(const Params& p, Size size, hipStream_t stream) {
   if (p.splits == 1) {
-    launch_product<E, kLeftTurned, kRightTurned, product::Store<T>>(p, size, stream);
+    launch_product<E, T, kLeftTurned, kRightTurned, product::Store<Out>>(p, size, stream);
     return;
   }
-  launch_product<E, kLeftTurned, kRightTurned, product::Partial>(p, size, stream);
+  launch_product<E, T, kLeftTurned, kRightTurned, product::Partial>(p, size, stream);
   int64_t most = 0;
   for (int j = 0; j < p.jobs; ++j) most = std::max(most, p.job[j].rows * p.job[j].columns);
-  k_join<T><<<dim3((uint32_t)std::min<int64_t>((most + 1023) / 1024, 2048), p.jobs), 256, 0, stream>>>(p);
+  k_join<Out><<<dim3((uint32_t)std::min<int64_t>((most + 1023) / 1024, 2048), p.jobs), 256, 0, stream>>>(p);
 }
 
 // ---- activations -----------------------------------------------------------------

@@ -79,24 +79,24 @@ int gradient(const MgbFeedForwardGradient& a, Space& space, hipStream_t stream, 
     MGB_LAUNCH_CHECK("feed forward gradient");
     return 0;
   }
-  LayJobs jobs = {}, turned = {};
+  LayJobs jobs = {};
   // Matrices whose products go along their columns are transposed first where that
   // costs little: binary32 ones, which are laid out anyhow, and others of many rows
-  // of x (16,384 x 1,024 x 4,096: two products of
-  // 322 and 280 us become 300 and 182, for 18 us of transposing).
+  // of x (16,384 x 1,024 x 4,096: two products of 322 and 280 us become 300 and 182,
+  // for 18 us of transposing).
   const bool turn_weights = sizeof(T) == 4 || a.rows >= kTurnRows;
   const int64_t dim = padded(a.dim), hidden = padded(a.hidden);
   const bool copy = !lies_well<T>(a.gate, a.hidden, a.dim, a.gate_stride) ||
                     !lies_well<T>(a.up, a.hidden, a.dim, a.up_stride) ||
                     (a.hidden > 1 && a.gate_stride != a.up_stride);
   const Laid grad = lay<T>(space, jobs, a.grad, a.rows, a.dim, a.grad_stride);
-  const Laid down = turn_weights ? lay_turned<T>(space, turned, a.down, a.dim, a.hidden, a.down_stride)
+  const Laid down = turn_weights ? lay_turned<T>(space, jobs, a.down, a.dim, a.hidden, a.down_stride)
                                  : lay<T>(space, jobs, a.down, a.dim, a.hidden, a.down_stride);
   Laid x = {}, gate = {}, up = {};
   if (a.dgate || a.dup) x = lay<T>(space, jobs, a.x, a.rows, a.dim, a.x_stride);
   if (a.dx && turn_weights) {
-    gate = lay_turned<T>(space, turned, a.gate, a.hidden, a.dim, a.gate_stride);
-    up = lay_turned<T>(space, turned, a.up, a.hidden, a.dim, a.up_stride);
+    gate = lay_turned<T>(space, jobs, a.gate, a.hidden, a.dim, a.gate_stride);
+    up = lay_turned<T>(space, jobs, a.up, a.hidden, a.dim, a.up_stride);
   } else if (a.dx) {
     gate = lay<T>(space, jobs, a.gate, a.hidden, a.dim, a.gate_stride, copy);
     up = lay<T>(space, jobs, a.up, a.hidden, a.dim, a.up_stride, copy);
@@ -168,15 +168,14 @@ int gradient(const MgbFeedForwardGradient& a, Space& space, hipStream_t stream, 
   }
   if (!run) return 0;
   lay_out<T>(jobs, stream);
-  turn<T>(turned, stream);
   if (turn_weights) {
-    launch_product<E, false, false, Slope<T>>(inner, inner_size, stream);
-    if (a.dx) store_product<E, T, false, false>(input, input_size, stream);
+    launch_product<E, T, false, false, Slope<T>>(inner, inner_size, stream);
+    if (a.dx) store_product<E, T, T, false, false>(input, input_size, stream);
   } else if constexpr (sizeof(T) == 2) {
-    launch_product<E, false, true, Slope<T>>(inner, inner_size, stream);
-    if (a.dx) store_product<E, T, false, true>(input, input_size, stream);
+    launch_product<E, T, false, true, Slope<T>>(inner, inner_size, stream);
+    if (a.dx) store_product<E, T, T, false, true>(input, input_size, stream);
   }
-  if (matrices) store_product<E, T, true, true>(weights, weights_size, stream);
+  if (matrices) store_product<E, T, T, true, true>(weights, weights_size, stream);
   MGB_LAUNCH_CHECK("feed forward gradient");
   return 0;
 }
