@@ -247,7 +247,10 @@ int serve(const MgbBlockFeedForward& a, Space& space, hipStream_t stream, bool r
   p.activation = a.activation;
   p.job[0].rows = a.rows;
   p.job[0].columns = a.hidden;
-  const Size size = choose(p, true, std::is_same_v<T, __bf16> ? kBlock : 64);
+  // In 8 bits for bfloat16 rows, up to the scales that a workgroup holds; wider ones as
+  // those of the other types.
+  const bool in_eight = std::is_same_v<T, __bf16> && a.gate.blocks <= product::kScaleSteps;
+  const Size size = choose(p, true, in_eight ? kBlock : 64);
   const bool rounds = size == kLarge;
   if (rounds) {
     p.hidden = (char*)h.values;
@@ -258,7 +261,7 @@ int serve(const MgbBlockFeedForward& a, Space& space, hipStream_t stream, bool r
     p.hidden_stride = a.hidden;
     p.hidden = space.take(a.rows * a.hidden * sizeof(float));
   }
-  if constexpr (std::is_same_v<T, __bf16>) {
+  if (in_eight) {
     p.job[0].left = operand8(x);
     p.job[0].right = {{(const char*)a.gate.values, (const char*)a.up.values}, {a.gate.stride, a.up.stride}, 0, a.hidden, dim};
     p.left_scales = (const uint8_t*)x.scales;
@@ -326,8 +329,6 @@ int check_serve(const MgbBlockFeedForward* a) {
               "block feed forward: the matrices' sizes do not fit");
   MGB_REQUIRE(a->gate.stride == a->up.stride && a->gate.scale_stride == a->up.scale_stride,
               "block feed forward: gate and up must lie alike");
-  MGB_REQUIRE(a->gate.blocks <= product::kScaleSteps || a->dtype != MGB_BF16,
-              "block feed forward: rows of bfloat16 must be at most 8,192 wide");
   MGB_REQUIRE(a->activation == MGB_SILU || a->activation == MGB_GELU, "block feed forward: activation must be silu or gelu");
   MGB_REQUIRE(a->dtype >= MGB_F32 && a->dtype <= MGB_BF16, "block feed forward: types must be float32, float16 or bfloat16");
   MGB_REQUIRE(a->x_stride < (int64_t(1) << 40) && a->x_stride > -(int64_t(1) << 40), "block feed forward: row stride out of range");
