@@ -146,6 +146,48 @@ def test_training_captured(enc, dtype):
         assert all(torch.equal(a, b) for a, b in zip(grads, want)), seed
 
 
+def test_capture_while_an_eager_graph_lives(enc):
+    """Refused where the leaves' gradients would be added up on the default stream; once
+    the eager results are gone, or were made on another stream, it is captured."""
+    block = enc.FeedForward(24, 40)
+    x = torch.randn(50, 24, device="cuda")
+    leaves = list(block.parameters())
+    values, indices = torch.randn(50, 40, device="cuda").topk(4)
+    logits = torch.randn(50, 40, device="cuda", requires_grad=True)
+
+    def refused(work):
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="default stream"):
+            with torch.cuda.graph(graph):
+                work()
+
+    y = block(x)
+    refused(lambda: block(x))
+    loss = enc.distillation_loss(logits, values, indices)[0]
+    refused(lambda: enc.distillation_loss(logits, values, indices))
+    want = torch.autograd.grad(y.sum(), leaves)
+    del y, loss
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(block(x).sum(), leaves)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(block(x).sum(), leaves)
+    for _ in range(2):
+        for g in got:
+            g.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with torch.no_grad():  # without gradients nothing is held
+        y = block(x)
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            block(x)
+    assert torch.equal(y, enc.feed_forward(x, *(p.detach() for p in leaves)))
+
+
 @pytest.mark.parametrize("dtype", TYPES, ids=NAMES)
 def test_matrices_that_lie_across(enc, dtype):
     """Parameters as transposed views, frozen ones, and a gradient that is one value."""

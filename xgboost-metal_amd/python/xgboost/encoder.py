@@ -9,15 +9,24 @@ operators such an encoder runs on the GPU as hand-written gfx950 kernels:
   tokens;
 - `layer_norm` / `layer_norm_gradient`;
 - `orthogonalize`: a matrix's update by Newton-Schulz products;
+- `feed_forward` / `feed_forward_gradient`: the gated block
+  (act(x gate^T) * (x up^T)) down^T, for training and for single rows;
+- `quantize_blocks`, `block_matmul`, `block_feed_forward`: values in 8 bits with a
+  scale a block of 128, products of them, and the gated block served from them;
+- `distillation_loss` / `distillation_gradient`: logits against a teacher's largest
+  ones, such as the margins of a boosted model per class;
 
-and over them `LeafTokenizer`, the torch modules `Embedding` and `LayerNorm`
-and the optimizer `Muon`.
+and over them `LeafTokenizer`, the torch modules `Embedding`, `LayerNorm`,
+`FeedForward` and `QuantizedFeedForward`, and the optimizer `Muon`.
 
 Tensors are float32, float16 or bfloat16 on a GPU.  The operators run on the
 current stream of the tensors' device, wait for nothing, and keep nothing
 between calls; as with torch's own, a tensor that another stream still writes
 has to be waited for first.  Sums are in 32 bits and rounded once; no result
-depends on the order of atomics.  Derivatives are reverse-mode and of first order;
+depends on the order of atomics.  Calls can be captured in a graph; a backward pass
+only with its forward pass, and while no eager graph of the same leaves that was made
+on the default stream lives (`feed_forward` and `distillation_loss` refuse the capture
+then).  Derivatives are reverse-mode and of first order;
 forward-mode (dual) tensors and traces (torch.jit.trace, make_fx, torch.export)
 raise NotImplementedError.  The module needs torch, which the rest of the
 package does not: import torch before xgboost, so that both use one HIP runtime,
@@ -172,6 +181,19 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5,
     return _without_derivative("orthogonalize", _encoder.orthogonalize, update, steps, coefficients, eps)
 
 
+# What adds up a leaf's gradient runs on the stream of the first graph that holds the
+# leaf, for as long as a graph does.  If that is the default stream, a backward pass that
+# is captured would have it wait for the capture, which ends the process.
+def _leaves_of(result: torch.Tensor) -> None:
+    stream = torch.cuda.current_stream(result.device).cuda_stream
+    for node, _ in result.grad_fn.next_functions:
+        if hasattr(node, "variable"):
+            made_on = node.metadata.setdefault("xgboost.encoder", stream)
+            if made_on == 0 and torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a graph made on the default stream still holds a leaf of this capture: its backward "
+                                   "pass cannot be captured; drop the eager pass's results first, or run it on another stream")
+
+
 # ---- gated feed-forward block ---------------------------------------------------
 
 def feed_forward_gradient(grad: torch.Tensor, x: torch.Tensor, kept: torch.Tensor, gate: torch.Tensor, up: torch.Tensor,
@@ -215,6 +237,7 @@ def feed_forward(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: to
     gives NaN.  Differentiable in x and the matrices through y."""
     if torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in (x, gate, up, down)):
         y, kept = _FeedForward.apply(x, gate, up, down, activation)
+        _leaves_of(y)
         return (y, kept) if keep else y
     return _encoder.feed_forward(x, gate, up, down, activation, keep)
 
@@ -314,7 +337,9 @@ def distillation_loss(logits: torch.Tensor, values: torch.Tensor, indices: torch
     loss 0.  At most 1,024 entries.  Differentiable in logits through the loss; the
     teacher is constant."""
     if torch.is_grad_enabled() and getattr(logits, "requires_grad", False):
-        return _Distillation.apply(logits, values, indices, temperature)
+        loss, lse = _Distillation.apply(logits, values, indices, temperature)
+        _leaves_of(loss)
+        return loss, lse
     return _encoder.distillation_loss(logits, values, indices, temperature)
 
 
