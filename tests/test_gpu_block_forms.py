@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from test_gpu_block import E, NAMES, TYPES, _act, _case, _forward64, _gen, _gradient64, _inner64, _near, _randn
+from test_gpu_block8 import _blocks64
 
 pytestmark = pytest.mark.gpu
 
@@ -35,6 +36,26 @@ def test_few_rows(enc, dim, hidden, dtype):
         assert torch.equal(enc.feed_forward(wide[:rows, 2:2 + dim], gate, up, down), y), rows
         assert torch.equal(enc.feed_forward(x[:1].expand(rows, dim), gate, up, down),
                            enc.feed_forward(x[:1].repeat(rows, 1), gate, up, down)), rows
+
+
+@pytest.mark.parametrize("dtype", TYPES[1:], ids=NAMES[1:])
+@pytest.mark.parametrize("rows,dim,hidden", [(1, 16, 64), (3, 200, 500), (31, 250, 333), (40, 24, 700), (33, 248, 1000), (500, 16, 3000),
+                                             (5000, 8, 40)])
+def test_few_results_are_rounded_once(enc, rows, dim, hidden, dtype, monkeypatch):
+    """Up to 8,192 of them: inner values count as two of the type, off by u^2, and their
+    products are twice as many terms."""
+    import test_gpu_block
+    g = _gen(rows + dim + hidden)
+    x, gate, up, down, grad = _case(g, rows, dim, hidden, dtype)
+    y, kept = enc.feed_forward(x, gate, up, down, keep=True)
+    got = (y, *enc.feed_forward_gradient(grad, x, kept, gate, up, down))
+    with monkeypatch.context() as m:
+        m.setattr(test_gpu_block, "U", {t: u * u for t, u in test_gpu_block.U.items()})
+        wants = (_forward64(x, gate, up, down, "silu"), *_gradient64(grad, x, kept, gate, up, down, "silu"))
+    for name, out, (want, error) in zip(("y", "dx", "dgate", "dup", "ddown"), got, wants):
+        few = rows * dim if name == "y" else min(rows, hidden) * dim
+        if few <= 8192:
+            _near(out, want, 2 * error, name)
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=NAMES)
@@ -71,6 +92,25 @@ def test_rows_beyond_a_workgroups_scales(enc, rows, dtype):
     want = h @ down.double().t()
     # float16 and bfloat16 round the sum, a whole number of 64s, once.
     _near(got, want, want.abs() * 2.0 ** -16 if dtype == torch.bfloat16 else want * 0)
+
+
+@pytest.mark.parametrize("rows,dim,hidden", [(40, 256, 512), (130, 200, 777), (300, 512, 1024)])
+def test_served_few_hidden_values(enc, rows, dim, hidden):
+    """Bfloat16 rows of up to 2 million hidden values are served as the 64-bit form
+    rounds, but for values that lie next to a border to its last bits: the result is off
+    by its own rounding, u / sqrt(3) of its norm, and at most a tenth of that."""
+    g = _gen(rows)
+    x = _randn(g, rows, dim, dtype=torch.bfloat16)
+    gate, up = (enc.quantize_blocks(_randn(g, hidden, dim, scale=dim ** -0.5)) for _ in range(2))
+    down = enc.quantize_blocks(_randn(g, dim, hidden, scale=hidden ** -0.5))
+    v = enc.quantize_blocks(x).dequantize().double()
+    h = _act(v @ gate.dequantize().double().t(), "silu")[0] * (v @ up.dequantize().double().t())
+    values, exponent = _blocks64(h)
+    kept = (values.view(rows, -1, 128) * torch.exp2(exponent)[..., None]).flatten(1)[:, :hidden]
+    want = kept @ down.dequantize().double().t()
+    got = enc.block_feed_forward(x, gate, up, down)
+    rounding = (want.bfloat16().double() - want).norm()
+    assert (got.double() - want).norm() <= 1.1 * rounding
 
 
 def test_scales_at_their_ends(enc):

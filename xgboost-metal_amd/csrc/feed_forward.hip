@@ -10,7 +10,7 @@ namespace mgb {
 namespace block {
 namespace {
 
-template <typename T>
+template <typename T, bool kRest>
 struct Gated : product::Plainly {
   static constexpr bool kDual = true;
   const Params& p;
@@ -23,7 +23,7 @@ struct Gated : product::Plainly {
 #pragma unroll
     for (int e = 0; e < kCount; ++e) h[e] = activate<sizeof(T) == 4>(gate[e], p.activation) * up[e];
     // (Columns that pad hidden's rows are products with zeros.)
-    store_inner<T, kCount>(p.hidden, p.hidden_part, m * p.hidden_stride + n, h);
+    store_inner<T, kRest, kCount>(p.hidden, p.hidden_part, p.hidden_rest, m * p.hidden_stride + n, h);
     if (p.kept) {
       float* to = p.kept + m * 2 * p.true_columns;
       product::store_some<kCount, kWhole>(to, n, p.true_columns, gate);
@@ -35,6 +35,7 @@ struct Gated : product::Plainly {
 template <typename T>
 int forward(const MgbFeedForward& a, Space& space, hipStream_t stream, bool run) {
   using E = typename Kind<T>::E;
+  const bool halves = sizeof(T) == 2 && a.rows * a.dim <= kFewResults;
   if (a.rows <= kMostFewRows) {
     Few f = {};
     f.x = a.x;
@@ -46,7 +47,7 @@ int forward(const MgbFeedForward& a, Space& space, hipStream_t stream, bool run)
     f.rows = a.rows;
     f.columns = a.hidden;
     f.depth = a.dim;
-    f.out = space.take(a.rows * a.hidden * sizeof(T));
+    f.out = space.take(a.rows * a.hidden * (halves ? sizeof(float) : sizeof(T)));
     f.kept = a.kept;
     f.activation = a.activation;
     Few g = {};
@@ -59,8 +60,13 @@ int forward(const MgbFeedForward& a, Space& space, hipStream_t stream, bool run)
     g.depth = a.hidden;
     g.out = a.y;
     if (run) {
-      few_rows<Plain<T>, Plain<T>, T, true>(f, stream);
-      few_rows<Plain<T>, Plain<T>, T, false>(g, stream);
+      if (halves) {
+        few_rows<Plain<T>, Plain<T>, float, true>(f, stream);
+        few_rows<std::conditional_t<sizeof(T) == 2, Halves<T>, Plain<T>>, Plain<T>, T, false>(g, stream);
+      } else {
+        few_rows<Plain<T>, Plain<T>, T, true>(f, stream);
+        few_rows<Plain<T>, Plain<T>, T, false>(g, stream);
+      }
       MGB_LAUNCH_CHECK("feed forward");
     }
     return 0;
@@ -83,7 +89,8 @@ int forward(const MgbFeedForward& a, Space& space, hipStream_t stream, bool run)
   inner.hidden_columns = hidden;
   inner.hidden_stride = inner_stride(hidden);
   inner.hidden_part = a.rows * inner.hidden_stride;
-  inner.hidden = space.take(inner.hidden_part * Kind<T>::kParts * 2);
+  inner.hidden_rest = halves ? inner.hidden_part : 0;
+  inner.hidden = space.take(inner.hidden_part * (halves ? 2 : Kind<T>::kParts) * 2);
   inner.kept = a.kept;
   inner.true_columns = a.hidden;
   inner.activation = a.activation;
@@ -95,11 +102,13 @@ int forward(const MgbFeedForward& a, Space& space, hipStream_t stream, bool run)
 
   Params outer = {};
   outer.jobs = 1;
-  outer.sources = 1;
+  outer.sources = halves ? 2 : 1;
   outer.pairs = Kind<T>::kPairs;
   outer.depth = hidden;
-  outer.job[0].left = operand({inner.hidden, inner.hidden_stride * 2, inner.hidden_part * 2}, a.rows, hidden);
-  outer.job[0].right = operand(down, a.dim, hidden);
+  const Laid middle = {inner.hidden, inner.hidden_stride * 2, inner.hidden_part * 2};
+  outer.job[0].left = operands(middle, {inner.hidden + inner.hidden_rest * 2, middle.stride, 0}, a.rows, hidden);
+  outer.job[0].left.part = middle.part;
+  outer.job[0].right = operands(down, down, a.dim, hidden);
   outer.job[0].out = a.y;
   outer.job[0].out_stride = a.dim;
   outer.job[0].rows = a.rows;
@@ -107,7 +116,12 @@ int forward(const MgbFeedForward& a, Space& space, hipStream_t stream, bool run)
   const Size outer_size = choose_shares(outer, space, false);
   if (!run) return 0;
   lay_out<T>(jobs, stream);
-  launch_product<E, T, false, false, Gated<T>>(inner, inner_size, stream);
+  if constexpr (sizeof(T) == 2) {
+    if (halves) launch_product<E, T, false, false, Gated<T, true>>(inner, inner_size, stream);
+    else launch_product<E, T, false, false, Gated<T, false>>(inner, inner_size, stream);
+  } else {
+    launch_product<E, T, false, false, Gated<T, false>>(inner, inner_size, stream);
+  }
   store_product<E, T, T, false, false>(outer, outer_size, stream);
   MGB_LAUNCH_CHECK("feed forward");
   return 0;

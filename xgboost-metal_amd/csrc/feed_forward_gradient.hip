@@ -13,7 +13,7 @@ namespace {
 
 constexpr int64_t kTurnRows = 4096;
 
-template <typename T>
+template <typename T, bool kRest>
 struct Slope {
   static constexpr bool kDual = false, kBlocks = false;
   static constexpr int kDeep = 4;
@@ -49,9 +49,9 @@ struct Slope {
       dup[e] = there ? dh[e] * act : 0.0f;
     }
     const int64_t at = m * p.hidden_stride + n;
-    store_inner<T, kCount>(p.dgate, p.gradient_part, at, dgate);
-    store_inner<T, kCount>(p.dgate, p.gradient_part, p.gradient_second + at, dup);
-    if (p.hidden) store_inner<T, kCount>(p.hidden, p.hidden_part, at, hidden);
+    store_inner<T, kRest, kCount>(p.dgate, p.gradient_part, p.gradient_rest, at, dgate);
+    store_inner<T, kRest, kCount>(p.dgate, p.gradient_part, p.gradient_rest, p.gradient_second + at, dup);
+    if (p.hidden) store_inner<T, kRest, kCount>(p.hidden, p.hidden_part, p.hidden_rest, at, hidden);
   }
 };
 
@@ -102,6 +102,7 @@ int gradient(const MgbFeedForwardGradient& a, Space& space, hipStream_t stream, 
     up = lay<T>(space, jobs, a.up, a.hidden, a.dim, a.up_stride, copy);
   }
 
+  const bool halves = sizeof(T) == 2 && std::min(a.rows, a.hidden) * a.dim <= kFewResults;
   Params inner = {};
   inner.jobs = 1;
   inner.sources = 1;
@@ -112,12 +113,14 @@ int gradient(const MgbFeedForwardGradient& a, Space& space, hipStream_t stream, 
   inner.hidden_part = a.rows * inner.hidden_stride;
   inner.gradient_second = inner.hidden_part;
   inner.gradient_part = 2 * inner.hidden_part;
-  inner.dgate = space.take(inner.gradient_part * kParts * 2);
+  inner.gradient_rest = halves ? inner.gradient_part : 0;
+  inner.dgate = space.take(inner.gradient_part * (halves ? 2 : kParts) * 2);
   const Laid dgate = {inner.dgate, inner.hidden_stride * 2, inner.gradient_part * 2};
   const Laid dup = {inner.dgate + inner.gradient_second * 2, inner.hidden_stride * 2, inner.gradient_part * 2};
   Laid middle = {};
   if (a.ddown) {
-    inner.hidden = space.take(inner.hidden_part * kParts * 2);
+    inner.hidden_rest = halves ? inner.hidden_part : 0;
+    inner.hidden = space.take(inner.hidden_part * (halves ? 2 : kParts) * 2);
     middle = {inner.hidden, inner.hidden_stride * 2, inner.hidden_part * 2};
   }
   inner.kept = const_cast<float*>(a.kept);
@@ -133,10 +136,11 @@ int gradient(const MgbFeedForwardGradient& a, Space& space, hipStream_t stream, 
   Size input_size = kSmall;
   if (a.dx) {
     input.jobs = 1;
-    input.sources = 2;
+    input.sources = halves ? 4 : 2;
     input.pairs = Kind<T>::kPairs;
     input.depth = hidden;
     input.job[0].left = operands(dgate, dup, a.rows, hidden);
+    for (int k = 0; k < 2; ++k) input.job[0].left.data[2 + k] += inner.gradient_rest * 2;
     input.job[0].right = turn_weights ? operands(gate, up, a.dim, hidden) : operands(gate, up, dim, a.hidden);
     input.job[0].out = a.dx;
     input.job[0].out_stride = a.dim;
@@ -148,31 +152,41 @@ int gradient(const MgbFeedForwardGradient& a, Space& space, hipStream_t stream, 
   Params weights = {};
   Size weights_size = kSmall;
   if (matrices) {
-    weights.sources = 1;
+    weights.sources = halves ? 2 : 1;
     weights.pairs = Kind<T>::kPairs;
     weights.depth = a.rows;
-    auto add = [&](void* out, const Laid& left, int64_t rows, const Laid& right, int64_t columns) {
+    auto add = [&](void* out, const Laid& left, int64_t left_rest, int64_t rows, const Laid& right, int64_t right_rest,
+                   int64_t columns) {
       if (!out) return;
       product::Job& job = weights.job[weights.jobs++];
-      job.left = operand(left, padded(rows), a.rows);
-      job.right = operand(right, padded(columns), a.rows);
+      job.left = operands(left, left, padded(rows), a.rows);
+      job.right = operands(right, right, padded(columns), a.rows);
+      job.left.data[1] += left_rest * 2;
+      job.right.data[1] += right_rest * 2;
       job.out = out;
       job.out_stride = columns;
       job.rows = rows;
       job.columns = columns;
     };
-    add(a.dgate, dgate, a.hidden, x, a.dim);
-    add(a.dup, dup, a.hidden, x, a.dim);
-    add(a.ddown, grad, a.dim, middle, a.hidden);
+    add(a.dgate, dgate, inner.gradient_rest, a.hidden, x, 0, a.dim);
+    add(a.dup, dup, inner.gradient_rest, a.hidden, x, 0, a.dim);
+    add(a.ddown, grad, 0, a.dim, middle, inner.hidden_rest, a.hidden);
     weights_size = choose_shares(weights, space, true);
   }
   if (!run) return 0;
   lay_out<T>(jobs, stream);
+  auto launch_inner = [&](auto turned) {
+    constexpr bool kTurned = decltype(turned)::value;
+    if constexpr (sizeof(T) == 2) {
+      if (halves) return launch_product<E, T, false, kTurned, Slope<T, true>>(inner, inner_size, stream);
+    }
+    launch_product<E, T, false, kTurned, Slope<T, false>>(inner, inner_size, stream);
+  };
   if (turn_weights) {
-    launch_product<E, T, false, false, Slope<T>>(inner, inner_size, stream);
+    launch_inner(std::bool_constant<false>{});
     if (a.dx) store_product<E, T, T, false, false>(input, input_size, stream);
   } else if constexpr (sizeof(T) == 2) {
-    launch_product<E, T, false, true, Slope<T>>(inner, inner_size, stream);
+    launch_inner(std::bool_constant<true>{});
     if (a.dx) store_product<E, T, T, false, true>(input, input_size, stream);
   }
   if (matrices) store_product<E, T, T, true, true>(weights, weights_size, stream);

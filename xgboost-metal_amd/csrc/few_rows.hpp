@@ -12,7 +12,8 @@
 // their alignment, and become bfloat16 or binary16 there: binary32 values three
 // bfloat16 each (six instructions a product), blocks of 8 bits the values they stand
 // for, exactly, and x, where the other operand is blocks, is rounded to blocks on the
-// way (a block is a unit, and lies in the registers of four lanes).
+// way (a block is a unit, and lies in the registers of four lanes).  Binary32 hidden
+// values beside 16-bit matrices are two 16-bit values each.
 #pragma once
 #include "feed_forward.hpp"
 
@@ -45,6 +46,12 @@ template <typename T>
 struct Plain {
   using Type = T;
   static constexpr int kParts = Kind<T>::kParts;
+};
+template <typename T>
+struct Halves {  // binary32, each the sum of two of T
+  using Type = float;
+  using Half = T;
+  static constexpr int kParts = 2;
 };
 struct InBlocks {
   using Type = uint8_t;
@@ -199,6 +206,19 @@ __device__ __forceinline__ void operand_of(const Unit<Kind_, kSteps>& u, int s, 
     u.values(s, v);
     const uint2 bytes = round_eight(v, __uint_as_float((254u - u.scale) << 23));
     out[0] = __builtin_bit_cast(product::int4v, widen_eight(bytes, u.scale));
+  } else if constexpr (Kind_::kParts == 2) {
+    using Eight = __attribute__((ext_vector_type(8))) typename Kind_::Half;
+    float v[8];
+    u.values(s, v);
+    Eight first, second;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      first[e] = (typename Kind_::Half)v[e];
+      const float rest = v[e] - (float)first[e];
+      second[e] = (typename Kind_::Half)(fabsf(rest) < INFINITY ? rest : 0.0f);
+    }
+    out[0] = __builtin_bit_cast(product::int4v, first);
+    out[1] = __builtin_bit_cast(product::int4v, second);
   } else if constexpr (Kind_::kParts == 3) {
     float v[8];
     u.values(s, v);
@@ -232,7 +252,7 @@ template <class X, class W, typename Out, int kTiles, int kSlices, bool kDual, i
 __global__ __launch_bounds__(kWaves* kWave) void k_few(Few p) {
   constexpr int kMatrices = kDual ? 2 : 1;
   constexpr bool kBlocks = std::is_same_v<W, InBlocks>;
-  static_assert(X::kParts == W::kParts, "both in as many parts");
+  static_assert(X::kParts == W::kParts || (X::kParts == 2 && W::kParts == 1), "the products of parts that are made");
   constexpr int kColumns = 16 / kSlices, kRows = 16 / kSlices, kSums = 4 / kSlices;
   using Sum = __attribute__((ext_vector_type(kSums))) float;
   __shared__ Sum shared[kWaves][kMatrices][kTiles][kWave];
@@ -301,11 +321,11 @@ __global__ __launch_bounds__(kWaves* kWave) void k_few(Few p) {
         product::int4v of_x[X::kParts];
         operand_of(this_x[t], s, of_x);
 #pragma unroll
-        for (int pair = 0; pair < (X::kParts == 3 ? Kind<float>::kPairs : 1); ++pair) {
-          const int xp = X::kParts == 3 ? product::left_part(pair) : 0, wp = X::kParts == 3 ? product::right_part(pair) : 0;
+        for (int pair = 0; pair < (X::kParts == 3 ? Kind<float>::kPairs : X::kParts); ++pair) {
+          const int xp = X::kParts == 3 ? product::left_part(pair) : pair, wp = X::kParts == 3 ? product::right_part(pair) : 0;
 #pragma unroll
           for (int m = 0; m < kMatrices; ++m)
-            sum[m][t] = multiply_one<std::is_same_v<X, Plain<_Float16>>>(of_w[m][wp], of_x[xp], sum[m][t]);
+            sum[m][t] = multiply_one<std::is_same_v<W, Plain<_Float16>>>(of_w[m][wp], of_x[xp], sum[m][t]);
         }
       }
     }
@@ -366,7 +386,8 @@ void few_rows(const Few& p, hipStream_t stream) {
       else launch(tiles, slices, Four{}, Four{});
     } else {
       if (depth <= 128) launch(tiles, slices, Four{}, One{});
-      else if constexpr (sizeof(typename X::Type) == 4) launch(tiles, slices, Most{}, One{});
+      else if constexpr (sizeof(typename W::Type) == 4 || (sizeof(typename X::Type) == 4 && decltype(tiles)::value > 1))
+        launch(tiles, slices, Most{}, One{});
       else if (depth < 128 * kMost) launch(tiles, slices, Most{}, One{});
       else launch(tiles, slices, Most{}, Four{});
     }
@@ -379,7 +400,7 @@ void few_rows(const Few& p, hipStream_t stream) {
     if (p.rows <= 8) return with(One{}, Two{});
     if constexpr (!kBlocks)
       if (p.rows <= 16) return with(Two{}, Two{});
-    if constexpr (!kBlocks && sizeof(typename X::Type) == 2) return with(Four{}, Two{});
+    if constexpr (!kBlocks && sizeof(typename W::Type) == 2) return with(Four{}, Two{});
   }
   if (p.rows <= 16) with(One{}, One{});
   else with(Two{}, One{});

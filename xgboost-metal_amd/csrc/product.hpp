@@ -54,10 +54,10 @@ constexpr int kScaleSteps = 64;  // of 8-bit operands, a workgroup's most
 __host__ __device__ constexpr int left_part(int pair) { return (0x201100 >> (4 * pair)) & 15; }
 __host__ __device__ constexpr int right_part(int pair) { return (0x021010 >> (4 * pair)) & 15; }
 
-// One operand: up to two matrices whose products are added (`data[1]` may be null).
+// One operand: up to four matrices whose products are added.
 struct Operand {
-  const char* data[2];
-  int64_t stride[2];   // bytes from row to row as they lie
+  const char* data[4];
+  int64_t stride[4];   // bytes from row to row as they lie
   int64_t part;        // bytes between the parts of binary32 values
   int64_t extent;      // rows (straight), columns (turned) that there are
   int64_t depth;       // values along the depth that there are; straight: whole chunks of 16 bytes
@@ -90,6 +90,7 @@ struct Params {
   char* hidden;              // act(gate) up, in parts
   char* dgate;               // [2][row][stride], in parts: dgate, then dup
   int64_t hidden_stride, hidden_part, gradient_part, gradient_second;  // elements
+  int64_t hidden_rest, gradient_rest;  // to what 16-bit values leave, or 0 if that is dropped
   int64_t hidden_columns;    // whole chunks of 8, the rest zeros
   int64_t true_columns;      // columns of `kept`
   int activation;

@@ -232,7 +232,8 @@ def feed_forward(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: to
     (hidden, dim), down (dim, hidden), all of x's type; `activation` is "silu" or
     "gelu" (by the normal distribution's function).  With `keep` the result is
     (y, kept), kept being x gate^T and x up^T, float32 (..., 2, hidden), which
-    `feed_forward_gradient` reads.  The hidden values are rounded to x's type.
+    `feed_forward_gradient` reads.  The hidden values are rounded to x's type (of up to
+    8,192 results to two values of it each, here as in the gradients).
     Float32 values are multiplied as three bfloat16 each; an infinity among them
     gives NaN.  Differentiable in x and the matrices through y."""
     if torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in (x, gate, up, down)):
@@ -287,9 +288,9 @@ def block_matmul(x: BlockScaled, weight: BlockScaled, *, dtype: torch.dtype = to
 def block_feed_forward(x: torch.Tensor, gate: BlockScaled, up: BlockScaled, down: BlockScaled, *,
                        activation: str = "silu") -> torch.Tensor:
     """`feed_forward` as it is served: the matrices as `quantize_blocks` keeps them, x
-    and the hidden values rounded so in the call.  The products of bfloat16 rows are
-    `block_matmul`'s 16-bit ones; those of float16 and float32 rows, up to the hidden
-    values' rounding, are exact.  Has no derivative: where x requires one, a backward
+    and the hidden values rounded so in the call.  The products of bfloat16 rows, where
+    there are 2^21 hidden values or more, are `block_matmul`'s 16-bit ones; the others',
+    up to the hidden values' rounding, are exact.  Has no derivative: where x requires one, a backward
     pass through the result is an error."""
     gate, up, down = _blocks("gate", gate), _blocks("up", up), _blocks("down", down)
     return _without_derivative("block_feed_forward", _encoder.block_feed_forward, x, gate.values, gate.scales, up.values,
