@@ -522,8 +522,8 @@ int mgb_orthogonalize(void* out, const void* update, int64_t batch, int64_t rows
  * rows of `dim` values, gate and up (hidden, dim), down (dim, hidden), all of
  * dtype; y without gaps.  kept, NULL or (rows, 2, hidden) binary32, gets the
  * rows' x gate^T, then x up^T, for the gradient.  The hidden values are rounded
- * to dtype (as operands of the second product); sums are binary32.  Sides up to
- * 2^20. */
+ * to dtype (as operands of the second product; for up to 8,192 results to two
+ * values of it each); sums are binary32.  Sides up to 2^20. */
 enum { MGB_SILU = 0, MGB_GELU = 1 };
 typedef struct {
   void* y;

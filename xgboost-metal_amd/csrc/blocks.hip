@@ -9,9 +9,9 @@
 //
 // The 8-bit instructions add a few products at a time with about 16 bits (1.5e-5 of
 // the norm for normal values, whatever the depth), which 16-bit results do not show.
-// Binary32 results, and the hidden values of a block in binary32 and binary16 (which
-// are rounded to e4m3 next: what crosses a border there shows), come of the bfloat16
-// instructions, which take e4m3 values with their scales exactly.
+// Binary32 results, and the hidden values of a block in binary32 and binary16, or if
+// they are few (they are rounded to e4m3 next: what crosses a border there shows), come
+// of the bfloat16 instructions, which take e4m3 values with their scales exactly.
 #include "few_rows.hpp"
 
 namespace mgb {
