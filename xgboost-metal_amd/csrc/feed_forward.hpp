@@ -313,7 +313,9 @@ inline Size choose_shares(Params& p, Space& space, bool turned, int values = 64,
   for (const Size size : {kLarge, kMedium, kSmall}) {
     const int64_t tiles = lay_tiles(p, size, false), steps = steps_of(p, size, values);
     const float area = (float)side(size) * side(size) * tiles * 8.0f / 5e6f;  // written and read again, 5 TB/s
-    for (int64_t shares = 1; shares <= 64; shares += shares < 8 ? 1 : shares < 16 ? 2 : 8) {
+    // (64 shares of most_steps need not hold the depth: then as many as do, in eights.)
+    const int64_t most_shares = std::max<int64_t>(64, ((steps + most_steps - 1) / most_steps + 7) / 8 * 8);
+    for (int64_t shares = 1; shares <= most_shares; shares += shares < 8 ? 1 : shares < 16 ? 2 : 8) {
       const int64_t each = (steps + shares - 1) / shares;
       if (shares > 1 && each < 4 && each * (shares - 1) >= steps) break;
       consider(size, each, each, estimate(p, size, tiles, shares, each, turned) + (shares > 1 ? 3.0f + area * shares : 0.0f));
