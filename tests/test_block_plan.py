@@ -28,6 +28,13 @@ def test_every_depth_has_shares(plan):
     assert plan("shares") == ["plans", str(8 * 8192), "wrong", "0"]
 
 
+def test_scales_are_read_within_their_rows(plan):
+    """Shares that begin at any step: the words that hold their scales, no byte behind the
+    last row, and every byte where its lanes look for it."""
+    out = plan("scales")
+    assert int(out[1]) > 1000 and out[2:] == ["wrong", "0"], out
+
+
 @pytest.mark.parametrize("blocks", [4096, 4097, 8192])
 def test_workspaces_of_long_rows(plan, blocks):
     """The entries' own answers for the longest rows that they take."""

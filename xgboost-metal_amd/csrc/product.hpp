@@ -278,35 +278,43 @@ struct Scales {
   static constexpr int kBytes = (kM + kN) * 4;  // a step's
 
   template <int kHalf, int kRows, int kTiles, int kWords, bool kPairs>
-  static __device__ __forceinline__ int place(int row) {  // byte
+  static __host__ __device__ __forceinline__ int place(int row) {  // byte
     const int half = row / kHalf, wave = row % kHalf / kRows, in = row % kRows;
     const int tile = kPairs ? in / 32 * 2 + in / 4 % 2 : in / 16;
     const int lane = kPairs ? in % 32 / 8 * 4 + in % 4 : in % 16;
     const int byte = half * kTiles + tile;
     return ((wave * 16 + lane) * kWords + byte / 4) * 4 + byte % 4;
   }
+  // Words of a row that hold steps begin to end, and one of them, `at` of all the tile's rows'.
+  static __host__ __device__ __forceinline__ int words(uint32_t begin, uint32_t end) {
+    return (int)((end + 3) / 4 - begin / 4);
+  }
+  static __host__ __device__ __forceinline__ void fill_word(char* panel, int at, const Params& p, int64_t row0, int64_t rows,
+                                                            int64_t column0, int64_t columns, bool dual, uint32_t begin,
+                                                            uint32_t end) {
+    const int each = words(begin, end), row = at / each, quad = at % each;
+    const uint8_t* from = nullptr;
+    int to;
+    if (row < S::kTileM) {
+      if (row0 + row < rows) from = p.left_scales + (row0 + row) * p.left_scale_stride;
+      to = place<S::kHalfM, S::kRowsM, S::kTilesM, kWordsM, false>(row);
+    } else {
+      const int r = row - S::kTileM;
+      const int64_t column = column0 + (dual ? r % S::kHalfN : r);
+      if (column < columns) from = p.right_scales[dual ? r / S::kHalfN : 0] + column * p.right_scale_stride;
+      to = kM * 4 + place<S::kHalfN, S::kRowsN, S::kTilesN, kWordsN, paired<false, S>()>(r);
+    }
+    // (Rows are whole words, and shares begin anywhere: the first and the last may have other
+    // shares' steps.)
+    const uint32_t first = (begin / 4 + quad) * 4, word = from ? *(const uint32_t*)(from + first) : 0x7f7f7f7fu;
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e)
+      if (first + e >= begin && first + e < end) panel[(first + e - begin) * kBytes + to] = (char)(word >> (8 * e));
+  }
   static __device__ __forceinline__ void fill(char* panel, const Params& p, int64_t row0, int64_t rows, int64_t column0,
                                               int64_t columns, bool dual, uint32_t begin, uint32_t end) {
-    const int quads = (int)(end - begin + 3) / 4;
-    for (int at = threadIdx.x; at < (S::kTileM + S::kTileN) * quads; at += S::kThreads) {
-      const int row = at / quads, quad = at % quads;
-      const uint8_t* from = nullptr;
-      int to;
-      if (row < S::kTileM) {
-        if (row0 + row < rows) from = p.left_scales + (row0 + row) * p.left_scale_stride;
-        to = place<S::kHalfM, S::kRowsM, S::kTilesM, kWordsM, false>(row);
-      } else {
-        const int r = row - S::kTileM;
-        const int64_t column = column0 + (dual ? r % S::kHalfN : r);
-        if (column < columns) from = p.right_scales[dual ? r / S::kHalfN : 0] + column * p.right_scale_stride;
-        to = kM * 4 + place<S::kHalfN, S::kRowsN, S::kTilesN, kWordsN, paired<false, S>()>(r);
-      }
-      // (Rows are whole words: a word that begins in a row ends in it.)
-      const uint32_t word = from ? *(const uint32_t*)(from + begin + quad * 4) : 0x7f7f7f7fu;
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (quad * 4 + e < (int)(end - begin)) panel[(quad * 4 + e) * kBytes + to] = (char)(word >> (8 * e));
-    }
+    for (int at = threadIdx.x; at < (S::kTileM + S::kTileN) * words(begin, end); at += S::kThreads)
+      fill_word(panel, at, p, row0, rows, column0, columns, dual, begin, end);
   }
 };
 
