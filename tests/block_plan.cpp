@@ -6,6 +6,8 @@
 //   scales   what a workgroup of an 8-bit product keeps of its operands' scales, for every share of
 //            such plans: each row's and column's bytes where its lanes read them.  Behind the last
 //            row lies a page that cannot be read.  Prints how many panels and how many wrong bytes.
+//   ahead    the panel's steps that are read while others are multiplied: the next one's, and none
+//            behind the panel.  Prints how many and how many wrong ones.
 #include <sys/mman.h>
 #include <unistd.h>
 
@@ -139,10 +141,22 @@ int scales() {
   return 0;
 }
 
+int ahead() {
+  long reads = 0, wrong = 0;
+  for (uint32_t steps = 1; steps <= (uint32_t)product::kScaleSteps; ++steps)
+    for (uint32_t step = 0; step < steps; ++step, ++reads) {
+      const uint32_t next = product::Scales<product::Large>::ahead(step, steps);
+      wrong += next >= steps || (step + 1 < steps && next != step + 1);
+    }
+  printf("reads %ld wrong %ld\n", reads, wrong);
+  return 0;
+}
+
 }  // namespace
 
 int main(int count, char** args) {
   if (count == 2 && !strcmp(args[1], "shares")) return shares();
   if (count == 2 && !strcmp(args[1], "scales")) return scales();
+  if (count == 2 && !strcmp(args[1], "ahead")) return ahead();
   return 2;
 }

@@ -35,6 +35,10 @@ def test_scales_are_read_within_their_rows(plan):
     assert int(out[1]) > 1000 and out[2:] == ["wrong", "0"], out
 
 
+def test_scales_are_read_within_the_panel(plan):
+    assert plan("ahead") == ["reads", str(64 * 65 // 2), "wrong", "0"]
+
+
 @pytest.mark.parametrize("blocks", [4096, 4097, 8192])
 def test_workspaces_of_long_rows(plan, blocks):
     """The entries' own answers for the longest rows that they take."""

@@ -285,6 +285,11 @@ struct Scales {
     const int byte = half * kTiles + tile;
     return ((wave * 16 + lane) * kWords + byte / 4) * 4 + byte % 4;
   }
+  // The step whose exponents are read while one of `steps` is multiplied: a panel ends at its
+  // last.
+  static __host__ __device__ __forceinline__ uint32_t ahead(uint32_t step, uint32_t steps) {
+    return step + 1 < steps ? step + 1 : step;
+  }
   // Words of a row that hold steps begin to end, and one of them, `at` of all the tile's rows'.
   static __host__ __device__ __forceinline__ int words(uint32_t begin, uint32_t end) {
     return (int)((end + 3) / 4 - begin / 4);
@@ -569,6 +574,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_product(Params p) {
   };
   using Zero = std::integral_constant<int, 0>;
   using One = std::integral_constant<int, 1>;
+  const uint32_t steps = end > begin ? end - begin : 0;
   auto step = [&](auto stage_constant, uint32_t t) {
     constexpr int kStage = decltype(stage_constant)::value;
     using Now = std::integral_constant<int, kStage>;
@@ -585,7 +591,7 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_product(Params p) {
       fetch_right(1, kStage);
       multiply_quarter(1, 1, other);
       take_right(other, Zero{}, Next{});
-      next_scales = read_scales(t + 1);
+      next_scales = read_scales(Panel::ahead(t, steps));
       fetch_left(1, kStage);
       advance();
       multiply_quarter(1, 0, now);
@@ -629,7 +635,6 @@ __global__ __launch_bounds__(S::kThreads, 2) void k_product(Params p) {
   wait_barrier();
   if constexpr (S::kAlternate)
     if (wave >= S::kWaves / 2) wait_barrier();
-  const uint32_t steps = end > begin ? end - begin : 0;
   for (uint32_t t = 0; t + 2 <= steps; t += 2) {
     step(std::integral_constant<int, 0>{}, t);
     step(std::integral_constant<int, 1>{}, t + 1);
