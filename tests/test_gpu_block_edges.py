@@ -1,0 +1,53 @@
+"""The block, its 8-bit form and distillation at the ends of what they accept
+(xgboost.encoder): more rows than a launch holds, infinities, types that modules are
+cast to.  Tolerances are those of test_gpu_block.py and test_gpu_block8.py."""
+import pytest
+import torch
+
+from test_gpu_block import _gen, _randn
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def enc():
+    from xgboost import encoder
+    return encoder
+
+
+def test_distillation_of_more_rows_than_a_launch_holds(enc):
+    """2^26 rows and a few, 64 lanes each: every part of them as in a call of its own."""
+    rows, classes = (1 << 26) + 5, 10
+    g = _gen(3)
+    logits = torch.empty(rows, classes, device="cuda", dtype=torch.float16).normal_(generator=g)
+    indices = torch.randint(-1, classes, (rows, 2), generator=g, device="cuda", dtype=torch.int32)
+    values = torch.empty(rows, 2, device="cuda", dtype=torch.float16).normal_(generator=g)
+    grad = torch.rand(rows, generator=g, device="cuda")
+    loss, lse = enc.distillation_loss(logits, values, indices, temperature=1.5)
+    d = enc.distillation_gradient(grad, logits, lse, values, indices, temperature=1.5)
+    assert torch.isfinite(loss).all() and torch.isfinite(d).all()
+    for begin in (0, 1 << 24, (1 << 25) - 500, (1 << 26) - 500):
+        part = slice(begin, begin + 1000)
+        want, want_lse = enc.distillation_loss(logits[part], values[part], indices[part], temperature=1.5)
+        assert torch.equal(loss[part], want) and torch.equal(lse[part], want_lse)
+        assert torch.equal(d[part], enc.distillation_gradient(grad[part], logits[part], want_lse, values[part], indices[part],
+                                                              temperature=1.5))
+    # One gradient for all rows, and teachers' rows that are one row.
+    d = enc.distillation_gradient(grad[:1].expand(rows), logits, lse, values[:1].expand(rows, 2), indices[:1].expand(rows, 2))
+    part = slice(rows - 1000, rows)
+    assert torch.equal(d[part], enc.distillation_gradient(grad[:1].expand(1000), logits[part], lse[part],
+                                                          values[:1].expand(1000, 2), indices[:1].expand(1000, 2)))
+
+
+def test_distillation_of_more_wide_rows_than_a_launch_holds(enc):
+    """2^24 rows and a few, 256 lanes each, of one row of logits: the loss at one entry of
+    each row is that of the entry's column."""
+    rows, classes = (1 << 24) + 3, 2100
+    g = _gen(4)
+    row = _randn(g, 1, classes)
+    indices = torch.randint(0, classes, (rows, 1), generator=g, device="cuda", dtype=torch.int32)
+    one = torch.zeros(1, 1, device="cuda")
+    loss, lse = enc.distillation_loss(row.expand(rows, classes), one.expand(rows, 1), indices)
+    each, each_lse = enc.distillation_loss(row.expand(classes, classes), one.expand(classes, 1),
+                                           torch.arange(classes, device="cuda")[:, None])
+    assert torch.equal(loss, each[indices[:, 0].long()]) and (lse == each_lse[0]).all()

@@ -352,45 +352,70 @@ Teacher teacher_of(const MgbDistillation& a) {
   return {a.values, a.indices, a.top, a.value_stride, a.index_stride, a.value_dtype, a.index_bytes};
 }
 
+// A launch holds fewer than 2^32 lanes: very many rows take several.
+constexpr int64_t kLanesAtOnce = int64_t(1) << 31;
+
+// Rows from `first` on, as many as a launch takes.
+MgbDistillation rows_from(const MgbDistillation& a, int64_t first, int64_t most) {
+  auto size = [](int type) { return type == MGB_F32 ? 4 : 2; };
+  auto at = [](auto* from, int64_t bytes) { return from ? (decltype(from))((const char*)from + bytes) : from; };
+  MgbDistillation part = a;
+  part.rows = std::min(a.rows - first, most);
+  part.loss = at(a.loss, first * 4);
+  part.lse = at(a.lse, first * 4);
+  part.dlogits = at(a.dlogits, first * a.classes * size(a.dtype));
+  part.grad = at(a.grad, first * a.grad_stride * 4);
+  part.logits = at(a.logits, first * a.stride * size(a.dtype));
+  part.values = at(a.values, first * a.value_stride * size(a.value_dtype));
+  part.indices = at(a.indices, first * a.index_stride * a.index_bytes);
+  return part;
+}
+
 template <typename T>
 int loss(const MgbDistillation& a, void* workspace, hipStream_t stream) {
   const Plan p = plan(a.rows, a.classes);
-  Running* partial = p.parts > 1 ? (Running*)workspace : nullptr;
-  const Teacher teacher = teacher_of(a);
-  const T* logits = (const T*)a.logits;
-  const dim3 grid((uint32_t)((a.rows * p.lanes + kThreads - 1) / kThreads), (uint32_t)p.parts);
-  auto launch = [&](auto stream_it, auto lanes) {
-    k_loss<decltype(stream_it)::value, T, decltype(lanes)::value><<<grid, kThreads, 0, stream>>>(
-        a.loss, a.lse, partial, logits, teacher, a.rows, a.classes, a.stride, p.part, a.temperature);
-  };
-  using Wave = std::integral_constant<int, kWave>;
-  using Group = std::integral_constant<int, kThreads>;
-  if (p.lanes == kWave) launch(std::false_type{}, Wave{});
-  else if (a.rows * a.classes * (int64_t)sizeof(T) >= kStreamBytes) launch(std::true_type{}, Group{});
-  else launch(std::false_type{}, Group{});
-  if (partial)
-    k_loss_join<T><<<(uint32_t)a.rows, kWave, 0, stream>>>(a.loss, a.lse, partial, (int)p.parts, logits, teacher, a.classes,
-                                                           a.stride, a.temperature);
-  MGB_LAUNCH_CHECK("distillation loss");
+  const bool past_caches = a.rows * a.classes * (int64_t)sizeof(T) >= kStreamBytes;
+  Running* partial = p.parts > 1 ? (Running*)workspace : nullptr;  // (of fewer rows than a launch takes)
+  for (int64_t done = 0; done < a.rows; done += kLanesAtOnce / p.lanes) {
+    const MgbDistillation r = rows_from(a, done, kLanesAtOnce / p.lanes);
+    const dim3 grid((uint32_t)((r.rows * p.lanes + kThreads - 1) / kThreads), (uint32_t)p.parts);
+    auto launch = [&](auto stream_it, auto lanes) {
+      k_loss<decltype(stream_it)::value, T, decltype(lanes)::value><<<grid, kThreads, 0, stream>>>(
+          r.loss, r.lse, partial, (const T*)r.logits, teacher_of(r), r.rows, r.classes, r.stride, p.part, r.temperature);
+    };
+    using Wave = std::integral_constant<int, kWave>;
+    using Group = std::integral_constant<int, kThreads>;
+    if (p.lanes == kWave) launch(std::false_type{}, Wave{});
+    else if (past_caches) launch(std::true_type{}, Group{});
+    else launch(std::false_type{}, Group{});
+    if (partial)
+      k_loss_join<T><<<(uint32_t)r.rows, kWave, 0, stream>>>(r.loss, r.lse, partial, (int)p.parts, (const T*)r.logits,
+                                                             teacher_of(r), r.classes, r.stride, r.temperature);
+    MGB_LAUNCH_CHECK("distillation loss");
+  }
   return 0;
 }
 
 template <typename T>
 int gradient(const MgbDistillation& a, hipStream_t stream) {
   const Plan p = plan(a.rows, a.classes);
-  const dim3 grid((uint32_t)((a.rows * p.lanes + kThreads - 1) / kThreads), (uint32_t)p.parts);
+  const bool past_caches = a.rows * a.classes * (int64_t)sizeof(T) >= kStreamBytes;
   const uint32_t lds = (uint32_t)(kThreads / p.lanes * a.top * sizeof(Entry));
-  auto launch = [&](auto stream_it, auto lanes) {
-    k_loss_gradient<decltype(stream_it)::value, T, decltype(lanes)::value><<<grid, kThreads, lds, stream>>>(
-        (T*)a.dlogits, a.grad, (const T*)a.logits, a.lse, teacher_of(a), a.rows, a.classes, a.grad_stride, a.stride, p.part,
-        a.temperature);
-  };
-  using Wave = std::integral_constant<int, kWave>;
-  using Group = std::integral_constant<int, kThreads>;
-  if (p.lanes == kWave) launch(std::false_type{}, Wave{});
-  else if (a.rows * a.classes * (int64_t)sizeof(T) >= kStreamBytes) launch(std::true_type{}, Group{});
-  else launch(std::false_type{}, Group{});
-  MGB_LAUNCH_CHECK("distillation gradient");
+  for (int64_t done = 0; done < a.rows; done += kLanesAtOnce / p.lanes) {
+    const MgbDistillation r = rows_from(a, done, kLanesAtOnce / p.lanes);
+    const dim3 grid((uint32_t)((r.rows * p.lanes + kThreads - 1) / kThreads), (uint32_t)p.parts);
+    auto launch = [&](auto stream_it, auto lanes) {
+      k_loss_gradient<decltype(stream_it)::value, T, decltype(lanes)::value><<<grid, kThreads, lds, stream>>>(
+          (T*)r.dlogits, r.grad, (const T*)r.logits, r.lse, teacher_of(r), r.rows, r.classes, r.grad_stride, r.stride, p.part,
+          r.temperature);
+    };
+    using Wave = std::integral_constant<int, kWave>;
+    using Group = std::integral_constant<int, kThreads>;
+    if (p.lanes == kWave) launch(std::false_type{}, Wave{});
+    else if (past_caches) launch(std::true_type{}, Group{});
+    else launch(std::false_type{}, Group{});
+    MGB_LAUNCH_CHECK("distillation gradient");
+  }
   return 0;
 }
 
