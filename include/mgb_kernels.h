@@ -523,7 +523,8 @@ int mgb_orthogonalize(void* out, const void* update, int64_t batch, int64_t rows
  * dtype; y without gaps.  kept, NULL or (rows, 2, hidden) binary32, gets the
  * rows' x gate^T, then x up^T, for the gradient.  The hidden values are rounded
  * to dtype (as operands of the second product; for up to 8,192 results to two
- * values of it each); sums are binary32.  Sides up to 2^20. */
+ * values of it each); sums are binary32.  Sides up to 2^20, fewer than
+ * 2^31 - 2,048 rows. */
 enum { MGB_SILU = 0, MGB_GELU = 1 };
 typedef struct {
   void* y;

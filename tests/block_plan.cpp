@@ -8,6 +8,9 @@
 //            row lies a page that cannot be read.  Prints how many panels and how many wrong bytes.
 //   ahead    the panel's steps that are read while others are multiplied: the next one's, and none
 //            behind the panel.  Prints how many and how many wrong ones.
+//   launches products of up to the most rows that the entries take, of widths of one tile (more do
+//            not fit the memory), can be launched: fewer than 2^32 lanes.  Prints how many and how
+//            many wrong ones.
 #include <sys/mman.h>
 #include <unistd.h>
 
@@ -152,11 +155,54 @@ int ahead() {
   return 0;
 }
 
+int launches() {
+  long plans = 0, wrong = 0;
+  auto check = [&](const Params& p, Size size, bool dual) {
+    int threads = size == kLarge ? product::Large::kThreads : size == kMedium ? product::Medium::kThreads : product::Small::kThreads;
+    if (in_parts(p, size)) threads = size == kMedium ? product::PartMedium::kThreads : product::PartSmall::kThreads;
+    const uint64_t m = side(size), n = dual ? m / 2 : m;
+    const uint64_t tiles = (p.job[0].rows + m - 1) / m * ((p.job[0].columns + n - 1) / n);
+    ++plans;
+    wrong += p.tiles != tiles || (tiles + 7) / 8 * 8 * p.splits * threads >= uint64_t(1) << 32;
+  };
+  for (const int64_t rows : {int64_t(1) << 20, int64_t(1) << 28, (int64_t(1) << 29) + 1, (int64_t(1) << 30) - 64, (int64_t(1) << 30) + 1,
+                             kMostRows - 1})
+    for (const int64_t columns : {1, 8, 32, 33, 64, 65, 128})
+      for (const int64_t depth : {8, 64, 512})
+        for (const int pairs : {1, 6})
+          for (const int sources : {1, 2}) {
+            Params p = {};
+            p.jobs = 1;
+            p.sources = sources;
+            p.pairs = pairs;
+            p.depth = depth;
+            p.job[0].rows = rows;
+            p.job[0].columns = columns;
+            Size size = choose(p, true);
+            check(p, size, true);
+            size = choose(p, false);
+            check(p, size, false);
+            Space space = {};
+            for (const bool turned : {false, true}) {
+              size = choose_shares(p, space, turned);
+              check(p, size, false);
+            }
+            if (pairs > 1 || depth % 128) continue;
+            size = choose(p, true, 128);
+            check(p, size, true);
+            size = choose_shares(p, space, false, 128, product::kScaleSteps);
+            check(p, size, false);
+          }
+  printf("plans %ld wrong %ld\n", plans, wrong);
+  return 0;
+}
+
 }  // namespace
 
 int main(int count, char** args) {
   if (count == 2 && !strcmp(args[1], "shares")) return shares();
   if (count == 2 && !strcmp(args[1], "scales")) return scales();
   if (count == 2 && !strcmp(args[1], "ahead")) return ahead();
+  if (count == 2 && !strcmp(args[1], "launches")) return launches();
   return 2;
 }

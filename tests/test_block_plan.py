@@ -39,6 +39,11 @@ def test_scales_are_read_within_the_panel(plan):
     assert plan("ahead") == ["reads", str(64 * 65 // 2), "wrong", "0"]
 
 
+def test_every_number_of_rows_can_be_launched(plan):
+    out = plan("launches")
+    assert int(out[1]) > 2000 and out[2:] == ["wrong", "0"], out
+
+
 @pytest.mark.parametrize("blocks", [4096, 4097, 8192])
 def test_workspaces_of_long_rows(plan, blocks):
     """The entries' own answers for the longest rows that they take."""

@@ -4,7 +4,7 @@ cast to.  Tolerances are those of test_gpu_block.py and test_gpu_block8.py."""
 import pytest
 import torch
 
-from test_gpu_block import _gen, _randn
+from test_gpu_block import _forward64, _gen, _gradient64, _near, _randn
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +51,28 @@ def test_distillation_of_more_wide_rows_than_a_launch_holds(enc):
     each, each_lse = enc.distillation_loss(row.expand(classes, classes), one.expand(classes, 1),
                                            torch.arange(classes, device="cuda")[:, None])
     assert torch.equal(loss, each[indices[:, 0].long()]) and (lse == each_lse[0]).all()
+
+
+def test_block_of_more_rows_than_small_tiles_launch(enc):
+    """2^30 rows and a few of three values: smaller tiles would be 2^32 lanes.  Gradients come
+    of rows at the beginning, where the small tiles would end, and at the end."""
+    rows, dim, hidden = (1 << 30) + 300, 3, 5
+    g = _gen(5)
+    gate, up = (_randn(g, hidden, dim, dtype=torch.bfloat16) for _ in range(2))
+    down = _randn(g, dim, hidden, dtype=torch.bfloat16)
+    x = torch.empty(rows, dim, device="cuda", dtype=torch.bfloat16).normal_(generator=g)
+    y, kept = enc.feed_forward(x, gate, up, down, keep=True)
+    parts = [slice(0, 3000), slice((1 << 29) - 1500, (1 << 29) + 1500), slice((1 << 30) - 3000, (1 << 30)), slice(1 << 30, rows)]
+    for part in parts:
+        _near(y[part], *_forward64(x[part], gate, up, down, "silu"), "y")
+    del y
+    grad = torch.zeros(rows, dim, device="cuda", dtype=torch.bfloat16)
+    for part in parts:
+        grad[part] = _randn(g, part.stop - part.start, dim, dtype=torch.bfloat16)
+    got = enc.feed_forward_gradient(grad, x, kept, gate, up, down)
+    some = [torch.cat([t[part] for part in parts]) for t in (grad, x, kept)]
+    wants = _gradient64(*some, gate, up, down, "silu")
+    dx = torch.cat([got[0][part] for part in parts])
+    for name, out, (want, error) in zip(("dx", "dgate", "dup", "ddown"), (dx, *got[1:]), wants):
+        _near(out, want, error, name)
+    assert not got[0][3000:4000].any()

@@ -305,7 +305,7 @@ int with_type(int dtype, const Call& call) {
 }
 
 int check_blocks(const MgbBlocks& m) {
-  MGB_REQUIRE(m.rows >= 0 && m.rows < kMostRows, "blocks: rows must be below 2^31");
+  MGB_REQUIRE(m.rows >= 0 && m.rows < kMostRows, "blocks: rows must be below 2^31 - 2,048");
   MGB_REQUIRE(m.blocks >= 1 && m.blocks <= kMostSide / kBlock, "blocks: a row must have 1 to 8,192 blocks");
   MGB_REQUIRE(m.stride >= m.blocks * kBlock && m.stride <= kMostSide && m.stride % 16 == 0,
               "blocks: rows of values must be 16-byte multiples apart, at most 2^20");
@@ -327,7 +327,7 @@ int check_matmul(const MgbBlockMatmul* a) {
 int check_serve(const MgbBlockFeedForward* a) {
   MGB_REQUIRE(a, "block feed forward: null pointer");
   if (check_blocks(a->gate) || check_blocks(a->up) || check_blocks(a->down)) return -1;
-  MGB_REQUIRE(a->rows >= 0 && a->rows < kMostRows, "block feed forward: rows must be below 2^31");
+  MGB_REQUIRE(a->rows >= 0 && a->rows < kMostRows, "block feed forward: rows must be below 2^31 - 2,048");
   MGB_REQUIRE(a->dim >= 1 && a->hidden >= 1 && a->dim <= kMostSide && a->hidden <= kMostSide,
               "block feed forward: a matrix' sides must be 1 to 2^20");
   MGB_REQUIRE(a->gate.rows == a->hidden && a->up.rows == a->hidden && a->down.rows == a->dim &&

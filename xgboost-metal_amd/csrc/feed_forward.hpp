@@ -13,7 +13,8 @@ namespace block {
 using product::Params;
 using product::float4v;
 
-constexpr int64_t kMostSide = int64_t(1) << 20, kMostRows = int64_t(1) << 31;
+// (Rows: as many as tiles of 256 by 512 lanes take in a launch, which holds fewer than 2^32.)
+constexpr int64_t kMostSide = int64_t(1) << 20, kMostRows = (int64_t(1) << 31) - 2048;
 
 // The matrix instructions' type for values of T, and the parts that hold one.
 // Binary32 values are three bfloat16, 24 bits (or 2^-134, where bfloat16's steps end),
@@ -278,12 +279,21 @@ inline float estimate(const Params& p, Size size, int64_t tiles, int64_t shares,
   return time;
 }
 
+// Added to the estimates of what no launch holds.  Very many rows of few columns take larger
+// tiles than they would otherwise.
+inline float too_many(const Params& p, Size size, int64_t tiles, int64_t shares) {
+  int64_t lanes = size == kLarge ? product::Large::kThreads : size == kMedium ? product::Medium::kThreads : product::Small::kThreads;
+  if (in_parts(p, size)) lanes = size == kMedium ? product::PartMedium::kThreads : product::PartSmall::kThreads;
+  return (tiles + 7) / 8 * 8 * shares * lanes < int64_t(1) << 32 ? 0.0f : 1e12f;
+}
+
 // The size of the tiles where the depth stays whole.
 inline Size choose(Params& p, bool dual, int values = 64) {
   Size best = kSmall;
   float least = INFINITY;
   for (const Size size : {kLarge, kMedium, kSmall}) {
-    const float time = estimate(p, size, lay_tiles(p, size, dual), 1, steps_of(p, size, values), false);
+    const int64_t tiles = lay_tiles(p, size, dual);
+    const float time = estimate(p, size, tiles, 1, steps_of(p, size, values), false) + too_many(p, size, tiles, 1);
     if (time < least) {
       least = time;
       best = size;
@@ -318,7 +328,8 @@ inline Size choose_shares(Params& p, Space& space, bool turned, int values = 64,
     for (int64_t shares = 1; shares <= most_shares; shares += shares < 8 ? 1 : shares < 16 ? 2 : 8) {
       const int64_t each = (steps + shares - 1) / shares;
       if (shares > 1 && each < 4 && each * (shares - 1) >= steps) break;
-      consider(size, each, each, estimate(p, size, tiles, shares, each, turned) + (shares > 1 ? 3.0f + area * shares : 0.0f));
+      consider(size, each, each, estimate(p, size, tiles, shares, each, turned) + (shares > 1 ? 3.0f + area * shares : 0.0f) +
+                                     too_many(p, size, tiles, shares));
     }
     if (size != kLarge || tiles <= kUnits / 2 || tiles >= kUnits) continue;
     const int64_t first = (steps * tiles + kUnits - 1) / kUnits, rest = steps - first;

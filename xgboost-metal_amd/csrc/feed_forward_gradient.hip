@@ -208,7 +208,7 @@ int with_type(const MgbFeedForwardGradient& a, Space& space, hipStream_t stream,
 
 int check_sizes(const MgbFeedForwardGradient* a) {
   MGB_REQUIRE(a, "feed forward gradient: null pointer");
-  MGB_REQUIRE(a->rows >= 0 && a->rows < kMostRows, "feed forward gradient: rows must be below 2^31");
+  MGB_REQUIRE(a->rows >= 0 && a->rows < kMostRows, "feed forward gradient: rows must be below 2^31 - 2,048");
   MGB_REQUIRE(a->dim >= 1 && a->hidden >= 1 && a->dim <= kMostSide && a->hidden <= kMostSide,
               "feed forward gradient: a matrix' sides must be 1 to 2^20");
   MGB_REQUIRE(a->activation == MGB_SILU || a->activation == MGB_GELU,
