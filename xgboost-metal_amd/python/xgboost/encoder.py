@@ -262,7 +262,16 @@ class BlockScaled(NamedTuple):
 def _blocks(name: str, m: BlockScaled) -> BlockScaled:
     if not isinstance(m, BlockScaled):
         raise TypeError(f"{name} must be a BlockScaled (see quantize_blocks), got {type(m).__name__}")
+    if getattr(m.values, "dtype", None) == torch.float8_e4m3fn:
+        width = m.values.shape[-1] if m.values.dim() else 0
+        if width % 128 == 0 and not 0 <= width - m.dim < 128:
+            raise ValueError(f"{name}'s rows of {width // 128} blocks do not hold {m.dim} values")
     return m
+
+
+def _length(name: str, m: BlockScaled, dim: int) -> None:
+    if m.dim != dim:
+        raise ValueError(f"{name} must have rows of {-(-dim // 128)} blocks that hold {dim} values, holds {m.dim}")
 
 
 def quantize_blocks(x: torch.Tensor) -> BlockScaled:
@@ -293,6 +302,11 @@ def block_feed_forward(x: torch.Tensor, gate: BlockScaled, up: BlockScaled, down
     up to the hidden values' rounding, are exact.  Has no derivative: where x requires one, a backward
     pass through the result is an error."""
     gate, up, down = _blocks("gate", gate), _blocks("up", up), _blocks("down", down)
+    if isinstance(x, torch.Tensor) and x.dim():
+        _length("gate", gate, x.shape[-1])
+        _length("up", up, x.shape[-1])
+    if isinstance(gate.values, torch.Tensor) and gate.values.dim() == 2:
+        _length("down", down, gate.values.shape[0])
     return _without_derivative("block_feed_forward", _encoder.block_feed_forward, x, gate.values, gate.scales, up.values,
                                up.scales, down.values, down.scales, activation)
 
