@@ -478,7 +478,8 @@ class FeedForward(torch.nn.Module):
 
 
 class QuantizedFeedForward(torch.nn.Module):
-    """`block_feed_forward` with a `FeedForward`'s matrices, laid out once."""
+    """`block_feed_forward` with a `FeedForward`'s matrices, laid out once.  Casts of the
+    module (`to`, `half` and the like) leave them in 8 bits."""
 
     def __init__(self, block: FeedForward) -> None:
         super().__init__()
@@ -487,6 +488,15 @@ class QuantizedFeedForward(torch.nn.Module):
             kept = quantize_blocks(getattr(block, name).detach())
             self.register_buffer(name + "_values", kept.values)
             self.register_buffer(name + "_scales", kept.scales)
+
+    def _apply(self, fn: Any, recurse: bool = True) -> "QuantizedFeedForward":
+        # Moved and cast with the module, as bytes: casts are of what is to be in another type.
+        def apply(t: torch.Tensor) -> torch.Tensor:
+            if t.dtype not in (torch.float8_e4m3fn, torch.float8_e8m0fnu):
+                return fn(t)
+            moved = fn(t.view(torch.uint8))
+            return moved.view(t.dtype) if moved.dtype == torch.uint8 else t.to(moved.device)
+        return super()._apply(apply, recurse)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         matrices = (BlockScaled(getattr(self, name + "_values"), getattr(self, name + "_scales"), dim)
