@@ -76,3 +76,21 @@ def test_block_of_more_rows_than_small_tiles_launch(enc):
     for name, out, (want, error) in zip(("dx", "dgate", "dup", "ddown"), (dx, *got[1:]), wants):
         _near(out, want, error, name)
     assert not got[0][3000:4000].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("rows,dim,hidden", [(5, 24, 41), (40, 24, 41), (700, 24, 41), (700, 24, 40), (300, 64, 1003), (5000, 512, 1027)])
+def test_infinities_stay_infinite(enc, rows, dim, hidden, dtype):
+    """An infinity times positive factors, whatever pads the hidden values' rows, and
+    rows beside it as they are without it."""
+    g = _gen(rows + hidden)
+    x, gate, up = (_randn(g, n, dim, dtype=dtype) for n in (rows, hidden, hidden))
+    down = _randn(g, dim, hidden, dtype=dtype)
+    gate[:, 5], up[:, 5] = gate[:, 5].abs() + 0.5, up[:, 5].abs() + 0.5
+    down[7] = down[7].abs() + 0.5
+    want = enc.feed_forward(x, gate, up, down)
+    x[2, 5] = float("inf")
+    got = enc.feed_forward(x, gate, up, down)
+    assert got[2, 7] == float("inf")
+    there = torch.arange(rows, device="cuda") != 2
+    assert torch.equal(got[there], want[there])

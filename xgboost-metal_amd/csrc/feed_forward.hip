@@ -23,8 +23,10 @@ struct Gated : product::Plainly {
     if (!kWhole && (m >= rows || n >= p.hidden_columns)) return;
     float h[kCount];
 #pragma unroll
-    for (int e = 0; e < kCount; ++e) h[e] = activate<sizeof(T) == 4>(gate[e], p.activation) * up[e];
-    // (Columns that pad hidden's rows are products with zeros.)
+    for (int e = 0; e < kCount; ++e) {
+      const bool there = kWhole || n + e < p.true_columns;  // columns that pad a row are zero whatever x holds
+      h[e] = there ? activate<sizeof(T) == 4>(gate[e], p.activation) * up[e] : 0.0f;
+    }
     store_inner<T, kRest, kCount>(p.hidden, p.hidden_part, p.hidden_rest, m * p.hidden_stride + n, h);
     if (p.kept) {
       float* to = p.kept + m * 2 * p.true_columns;
