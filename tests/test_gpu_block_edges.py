@@ -94,3 +94,23 @@ def test_infinities_stay_infinite(enc, rows, dim, hidden, dtype):
     assert got[2, 7] == float("inf")
     there = torch.arange(rows, device="cuda") != 2
     assert torch.equal(got[there], want[there])
+
+
+@pytest.mark.parametrize("classes", [40, 5000])
+def test_teachers_that_are_not_finite(enc, classes):
+    """NaN or +inf among a row's values: its loss and all of its gradient are NaN, the other
+    rows' as they are; in an absent entry they do not count."""
+    g = _gen(classes)
+    logits, values = _randn(g, 6, classes), _randn(g, 6, 3)
+    indices = torch.tensor([[1, 7, 30]], device="cuda").repeat(6, 1)
+    grad = torch.ones(6, device="cuda")
+    bad, at = values.clone(), indices.clone()
+    bad[1, 2], bad[3, 0], bad[4, 1] = float("nan"), float("inf"), float("nan")
+    at[4, 1] = -1
+    loss, lse = enc.distillation_loss(logits, bad, at)
+    d = enc.distillation_gradient(grad, logits, lse, bad, at)
+    want, want_lse = enc.distillation_loss(logits, values, at)
+    want_d = enc.distillation_gradient(grad, logits, want_lse, values, at)
+    spoilt = torch.tensor([False, True, False, True, False, False], device="cuda")
+    assert torch.isnan(loss[spoilt]).all() and torch.isnan(d[spoilt]).all()
+    assert torch.equal(loss[~spoilt], want[~spoilt]) and torch.equal(d[~spoilt], want_d[~spoilt]) and torch.equal(lse, want_lse)

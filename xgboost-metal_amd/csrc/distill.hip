@@ -274,7 +274,9 @@ __global__ __launch_bounds__(kThreads) void k_loss_gradient(T* __restrict__ dz, 
       entries[j] = {there ? e.column : -1, there ? expf((e.value - t.largest) * inverse - log_total) : 0.0f};
     }
     empty = t.sum == 0.0f;
-    factor = grad[row * grad_stride] * temperature;
+    // (Of NaN or an infinity among the teacher's values there are no probabilities: all of the
+    // row's gradient is NaN, as its loss is.)
+    factor = t.sum == t.sum ? grad[row * grad_stride] * temperature : t.sum;
     lse = lses[row];
     constexpr int kAhead = 4;
     int64_t at = begin + (int64_t)lane * kSize;
