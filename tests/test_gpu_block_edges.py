@@ -1,6 +1,8 @@
 """The block, its 8-bit form and distillation at the ends of what they accept
 (xgboost.encoder): more rows than a launch holds, infinities, types that modules are
 cast to.  Tolerances are those of test_gpu_block.py and test_gpu_block8.py."""
+import math
+
 import pytest
 import torch
 
@@ -114,3 +116,34 @@ def test_teachers_that_are_not_finite(enc, classes):
     spoilt = torch.tensor([False, True, False, True, False, False], device="cuda")
     assert torch.isnan(loss[spoilt]).all() and torch.isnan(d[spoilt]).all()
     assert torch.equal(loss[~spoilt], want[~spoilt]) and torch.equal(d[~spoilt], want_d[~spoilt]) and torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("classes", [12, 3000, 40000])
+@pytest.mark.parametrize("offset", [0.0, 3000.0, -3000.0])
+def test_loss_of_logits_far_from_zero(enc, classes, offset):
+    """What all of a row's logits have in common does not count: its loss is off by 2^-23 of
+    the differences' sizes (below 30 / T), of the sum (classes / 64 terms a lane, and 16) and
+    of the entries' products, not of the logits' 12,000 / T."""
+    temperature = 0.25
+    g = _gen(classes)
+    logits = _randn(g, 20, classes) + offset
+    values, indices = (_randn(g, 20, classes) + 50).topk(8, 1)
+    loss, lse = enc.distillation_loss(logits, values, indices, temperature=temperature)
+    log_q = (logits.double() / temperature).log_softmax(1).gather(1, indices)
+    log_p = (values.double() / temperature).log_softmax(1)
+    want = temperature ** 2 * (log_p.exp() * (log_p - log_q)).sum(1)
+    size = temperature ** 2 * (log_p.exp() * (log_p.abs() + log_q.abs() + 1)).sum(1)
+    _near(loss, want, size * (30 / temperature + classes / 64 + 16) * 2.0 ** -23)
+    z = logits.double() / temperature
+    _near(lse, z.logsumexp(1), z.abs().amax(1) * 2.0 ** -23 + (classes / 64 + 32 + 30 / temperature) * 2.0 ** -23)
+
+
+def test_loss_between_the_largest_values(enc):
+    """A difference that passes binary32 before it is divided by the temperature: an entry of
+    probability e^-3 that the logits hold for impossible, T^2 p 2 top / T = 0.38 top."""
+    top = torch.finfo(torch.float32).max
+    logits = torch.tensor([[top, -top, 0.0]], device="cuda")
+    loss, _ = enc.distillation_loss(logits, torch.tensor([[0.0, -12.0]], device="cuda"), torch.tensor([[0, 1]], device="cuda"),
+                                    temperature=4.0)
+    want = 8.0 * top * math.exp(-3.0) / (1.0 + math.exp(-3.0))
+    assert abs(loss.item() / want - 1) < 1e-6

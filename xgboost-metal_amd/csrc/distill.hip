@@ -186,14 +186,17 @@ __device__ __forceinline__ void finish_row(float* loss, float* lses, const T* z,
   const float logit = first.value != -INFINITY ? (float)z[first.column] : 0.0f;
   Running t = teach<kLanes>(teacher, first, row, classes, lane, c);
   join_lanes<kLanes>(r, t, c, shared);
-  const float lse = fmaf(r.largest, inverse, logf(r.sum)), log_total = logf(t.sum);
+  const float log_sum = logf(r.sum), lse = fmaf(r.largest, inverse, log_sum), log_total = logf(t.sum);
   float sum = 0.0f;
   for (int64_t j = lane; j < teacher.count; j += kLanes) {
     const Entry e = j == lane ? first : entry_of(teacher, row, classes, j);
     if (e.value == -INFINITY) continue;
     const float log_p = (e.value - t.largest) * inverse - log_total, p = expf(log_p);
     const float there = j == lane ? logit : (float)z[e.column];
-    if (p != 0.0f) sum = fmaf(p, log_p - (there * inverse - lse), sum);
+    // log q from the row's largest logit: lse, rounded, is as far off as the logits are
+    // from zero.  (Halves: their difference does not overflow.)
+    const float log_q = (0.5f * there - 0.5f * r.largest) * (2.0f * inverse) - log_sum;
+    if (p != 0.0f) sum = fmaf(p, log_p - log_q, sum);
   }
   sum = sum_lanes<kLanes>(sum, (float*)shared);
   if (lane == 0) {
