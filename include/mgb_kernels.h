@@ -552,7 +552,7 @@ int mgb_feed_forward_gradient(const MgbFeedForwardGradient* p, void* workspace, 
  * zeros), `stride` bytes (a multiple of 16) from row to row, and for each block a
  * byte of exponent + 127 of the power of two that its values are times, whole
  * words a row, `scale_stride` bytes from row to row.  Values begin at 16 bytes,
- * scales at 4. */
+ * scales at 4.  Fewer than 2^31 - 2,048 rows. */
 typedef struct {
   void *values, *scales;
   int64_t rows, blocks, stride, scale_stride;
@@ -586,7 +586,8 @@ int mgb_block_feed_forward(const MgbBlockFeedForward* p, void* workspace, size_t
 /* Distillation from a teacher's largest logits: with q = softmax(logits / T) and p the
  * softmax of values / T over a row's `top` (at most 1,024) entries whose index lies
  * in [0, classes), loss = T^2 sum p (log p - log q at the index), 0 for a row
- * without entries; lse = log sum exp(logits / T).  The gradient takes the loss's
+ * without entries, NaN (and all of the gradient) for one with NaN or +inf among
+ * them; lse = log sum exp(logits / T).  The gradient takes the loss's
  * (`grad`, a value a row) and lse: dlogits (rows without gaps) = grad T (q - p). */
 typedef struct {
   float *loss, *lse;

@@ -1,6 +1,7 @@
 """How the encoder's products divide their work (csrc/feed_forward.hpp, csrc/product.hpp),
 on the host: tests/block_plan.cpp goes through the sizes that the entries take."""
 import ctypes
+import shutil
 import subprocess
 from pathlib import Path
 
@@ -13,7 +14,8 @@ ROOT = Path(__file__).resolve().parents[1]
 @pytest.fixture(scope="module")
 def plan(tmp_path_factory):
     out = tmp_path_factory.mktemp("plan") / "block_plan"
-    subprocess.run(["hipcc", "-x", "hip", "--cuda-host-only", "-O1", "-std=c++17", f"-I{ROOT / 'include'}",
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    subprocess.run([hipcc, "-x", "hip", "--cuda-host-only", "-O1", "-std=c++17", f"-I{ROOT / 'include'}",
                     f"-I{ROOT / 'xgboost-metal_amd' / 'csrc'}", "-o", str(out), str(ROOT / "tests" / "block_plan.cpp")],
                    check=True)
 

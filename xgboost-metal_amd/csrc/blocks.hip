@@ -19,7 +19,8 @@ namespace block {
 namespace {
 
 // Hidden values from which on bfloat16 rows go by the 8-bit instructions.  64 rows of
-// 1,024 x 4,096: 35 us exactly, 23 by them; 300 of 512 x 1,024: 23 and 19.
+// 1,024 x 4,096: 35 us exactly, 23 by them, which is what the 16-bit block takes; 300 of
+// 512 x 1,024: 23 and 19.
 constexpr int64_t kManyHidden = int64_t(1) << 21;
 
 constexpr int kBlock = 128, kQuantThreads = 256, kQuantLanes = kBlock / 8;

@@ -7,8 +7,8 @@
 //
 // Bound by memory: the loss reads z once, with the running largest value and sum of a
 // softmax in each lane, 32 bfloat16 values between two changes of it; the gradient
-// reads it once and writes dz.  8,192 rows of 32,768 bfloat16: loss 84 us, 6.4 TB/s of
-// the logits (a plain read reaches 6.2, one past the caches 7.1); gradient 193 us, 5.6
+// reads it once and writes dz.  8,192 rows of 32,768 bfloat16: loss 92 us, 5.8 TB/s of
+// the logits (a plain read reaches 6.2, one past the caches 7.1); gradient 209 us, 5.1
 // TB/s (a large copy 5.0).  Sums are binary32.
 #include <algorithm>
 #include <type_traits>
@@ -21,8 +21,8 @@ namespace {
 constexpr int kThreads = 256;
 constexpr float kLog2e = 1.44269504f, kLowest = -3.40282347e38f;
 // Logits of this many bytes go past the caches, of whose last level this is the size.
-// 8,192 rows of 32,768 in bfloat16 (537 MB): loss 84 us, gradient 193, through the
-// caches 95 and 208; a quarter of them 24 and 51, through the caches 26 and 48.
+// 8,192 rows of 32,768 in bfloat16 (537 MB): loss 92 us, gradient 209, through the
+// caches 98 and 237; a quarter of them 27 and 58, through the caches 28 and 53.
 constexpr int64_t kStreamBytes = 256 << 20;
 constexpr int64_t kMostClasses = int64_t(1) << 31;
 
@@ -242,8 +242,10 @@ __global__ __launch_bounds__(kWave) void k_loss_join(float* __restrict__ loss, f
   finish_row<T, kWave>(loss, lses, z, teacher, first, r, row, classes, lane, temperature, c, nullptr);
 }
 
-// dz of a part of a row: q everywhere, then the teacher's columns once more, by the
-// lane of a column's first entry.  The entries' columns and probabilities lie in LDS.
+// dz of a part of a row: q everywhere (0 where it is below 2^-126), then the teacher's
+// columns once more, by the lane of a column's first entry.  The entries' columns and
+// probabilities lie in LDS, and each is compared with all others: 8,192 rows of 32,768 with
+// 64 entries 207 us, with 256 292, with 1,024 1,427.
 template <bool kStream, typename T, int kLanes>
 __global__ __launch_bounds__(kThreads) void k_loss_gradient(T* __restrict__ dz, const float* __restrict__ grad,
                                                             const T* __restrict__ logits, const float* __restrict__ lses,

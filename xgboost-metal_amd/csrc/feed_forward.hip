@@ -5,7 +5,7 @@
 // which reads them in binary32: rounded to 16 bits they would show in it), the
 // second is y's.  hidden is rounded to x's type once, or where results are few to two
 // values of it (or stays binary32); sums are binary32.  8,192 x 1,024 x 4,096 in binary16:
-// 164 and 84 us, 0.84 and 0.82 PFLOP/s.
+// 132 and 68 us, 1.04 and 1.01 PFLOP/s.
 #include "few_rows.hpp"
 
 namespace mgb {

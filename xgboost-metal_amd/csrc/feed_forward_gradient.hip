@@ -84,7 +84,7 @@ int gradient(const MgbFeedForwardGradient& a, Space& space, hipStream_t stream, 
   LayJobs jobs = {};
   // Matrices whose products go along their columns are transposed first where that
   // costs little: binary32 ones, which are laid out anyhow, and others of many rows
-  // of x (16,384 x 1,024 x 4,096: two products of 322 and 280 us become 300 and 182,
+  // of x (16,384 x 1,024 x 4,096: two products of 322 and 280 us become 303 and 193,
   // for 18 us of transposing).
   const bool turn_weights = sizeof(T) == 4 || a.rows >= kTurnRows;
   const int64_t dim = padded(a.dim), hidden = padded(a.hidden);

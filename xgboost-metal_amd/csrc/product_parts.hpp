@@ -5,8 +5,9 @@
 // one is multiplied, the next is on its way or there, and the third is filled once all
 // waves have left it, which one barrier a step sees to.
 //
-// The gradients of 2,003 x 200 x 777: 83 us, 104 with k_product's tiles of these sizes;
-// those of 2,048 x 1,024 x 4,096 667 us, 206 TFLOP/s (a library's binary32 product 152).
+// The gradients of 2,003 x 200 x 777: 74 us (83, as the parts came, and 104 with k_product's
+// tiles of these sizes); those of 2,048 x 1,024 x 4,096 641 us, 161 TFLOP/s (a library's
+// binary32 product 152).
 // What bounds small ones are the loads to LDS, 64 bytes of a row each, at 21 bytes a
 // cycle and compute unit.
 #pragma once

@@ -233,7 +233,8 @@ def feed_forward(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: to
     "gelu" (by the normal distribution's function).  With `keep` the result is
     (y, kept), kept being x gate^T and x up^T, float32 (..., 2, hidden), which
     `feed_forward_gradient` reads.  The hidden values are rounded to x's type (of up to
-    8,192 results to two values of it each, here as in the gradients).
+    8,192 results to two values of it each, here as in the gradients); those of float16
+    beyond 65,504 become infinite, as do the gradients' inner values.
     Float32 values are multiplied as three bfloat16 each; an infinity among them
     gives NaN.  Differentiable in x and the matrices through y."""
     if torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in (x, gate, up, down)):
@@ -316,7 +317,8 @@ def block_feed_forward(x: torch.Tensor, gate: BlockScaled, up: BlockScaled, down
 def distillation_gradient(grad: torch.Tensor, logits: torch.Tensor, lse: torch.Tensor, values: torch.Tensor,
                           indices: torch.Tensor, *, temperature: float = 1.0) -> torch.Tensor:
     """The logits' gradient from that of `distillation_loss`'s loss (float32, a value a
-    row) and the lse it returned.  Has no derivative itself, like
+    row) and the lse it returned, whose rounding to float32 is in all of a row's
+    softmax: |lse| 2^-24 of it.  Has no derivative itself, like
     `embedding_gradient`."""
     return _without_derivative("distillation_gradient", _encoder.distillation_gradient, grad, logits, lse, values, indices,
                                temperature)
@@ -349,7 +351,8 @@ def distillation_loss(logits: torch.Tensor, values: torch.Tensor, indices: torch
     softmax of values / T over the entries, and log sum exp(logits / T), which
     `distillation_gradient` reads, both float32.  An entry whose index lies outside the
     row, -1 for padding, or whose value is -inf is absent; a row without entries has
-    loss 0.  At most 1,024 entries.  Differentiable in logits through the loss; the
+    loss 0, one with NaN or +inf among its entries NaN, and all of its gradient.  At
+    most 1,024 entries.  Differentiable in logits through the loss; the
     teacher is constant."""
     if torch.is_grad_enabled() and getattr(logits, "requires_grad", False):
         loss, lse = _Distillation.apply(logits, values, indices, temperature)
@@ -478,8 +481,10 @@ class FeedForward(torch.nn.Module):
 
 
 class QuantizedFeedForward(torch.nn.Module):
-    """`block_feed_forward` with a `FeedForward`'s matrices, laid out once.  Casts of the
-    module (`to`, `half` and the like) leave them in 8 bits."""
+    """`block_feed_forward` with a `FeedForward`'s matrices, laid out once: half of a
+    16-bit block's memory.  It takes less time than the block does for float32 rows, and
+    for 16-bit ones where they are thousands and the matrices wide; for fewer more.  Casts of
+    the module (`to`, `half` and the like) leave the matrices in 8 bits."""
 
     def __init__(self, block: FeedForward) -> None:
         super().__init__()
