@@ -147,3 +147,44 @@ def test_loss_between_the_largest_values(enc):
                                     temperature=4.0)
     want = 8.0 * top * math.exp(-3.0) / (1.0 + math.exp(-3.0))
     assert abs(loss.item() / want - 1) < 1e-6
+
+
+def test_capture_while_a_graph_of_torchs_lives(enc):
+    """Refused too where what holds the leaves on the default stream are torch's operators;
+    once their results are gone, it is captured."""
+    block = enc.FeedForward(24, 40)
+    x = torch.randn(50, 24, device="cuda")
+    values, indices = torch.randn(50, 24, device="cuda").topk(4)
+    logits = torch.randn(50, 24, device="cuda", requires_grad=True)
+    leaves = [*block.parameters(), logits]
+
+    def refused(work):
+        with pytest.raises(RuntimeError, match="default stream"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                work()
+
+    held = block.down * 2
+    refused(lambda: block(x))
+    held = logits.exp()
+    refused(lambda: enc.distillation_loss(logits, values, indices))
+    del held
+
+    def step():
+        loss = enc.distillation_loss(block(x) + logits, values, indices)[0] + enc.distillation_loss(logits, values, indices)[0]
+        return torch.autograd.grad(loss.sum(), leaves)
+
+    want = step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(2):
+        for g in got:
+            g.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -6,9 +6,11 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/utils/object_ptr.h>
 
@@ -697,11 +699,35 @@ PyObject* distillation_gradient(PyObject*, PyObject* const* args, Py_ssize_t n) 
   END_HANDLE_TH_ERRORS
 }
 
+// (result of a pass that has a backward pass)
+// What adds up a leaf's gradient runs on the stream of the first graph that holds the
+// leaf, for as long as a graph does, be it of torch's operators.  If that is the default
+// stream, a backward pass that is captured would have it wait for the capture, which ends
+// the process.
+PyObject* check_capture(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  arguments("check_capture", n, 1);
+  const Tensor& result = THPVariable_Unpack(args[0]);
+  const c10::DeviceGuard guard(result.device());
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None && result.grad_fn())
+    for (const torch::autograd::Edge& edge : result.grad_fn()->next_edges()) {
+      const auto* leaf = dynamic_cast<const torch::autograd::AccumulateGrad*>(edge.function.get());
+      if (leaf && leaf->input_metadata(0).stream().id() == 0) {
+        PyErr_SetString(PyExc_RuntimeError,
+                        "a graph made on the default stream still holds a leaf of this capture: its backward pass cannot "
+                        "be captured; drop the eager pass's results first, or run it on another stream");
+        throw python_error();
+      }
+    }
+  Py_RETURN_NONE;
+  END_HANDLE_TH_ERRORS
+}
+
 #define ENTRY(fn) {#fn, (PyCFunction)(void (*)(void))fn, METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {ENTRY(lookup), ENTRY(lookup_gradient), ENTRY(norm), ENTRY(norm_gradient),
                            ENTRY(orthogonalize), ENTRY(feed_forward), ENTRY(feed_forward_gradient),
                            ENTRY(quantize_blocks), ENTRY(block_matmul), ENTRY(block_feed_forward), ENTRY(distillation_loss),
-                           ENTRY(distillation_gradient), {nullptr, nullptr, 0, nullptr}};
+                           ENTRY(distillation_gradient), ENTRY(check_capture), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_encoder", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -181,19 +181,6 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5,
     return _without_derivative("orthogonalize", _encoder.orthogonalize, update, steps, coefficients, eps)
 
 
-# What adds up a leaf's gradient runs on the stream of the first graph that holds the
-# leaf, for as long as a graph does.  If that is the default stream, a backward pass that
-# is captured would have it wait for the capture, which ends the process.
-def _leaves_of(result: torch.Tensor) -> None:
-    stream = torch.cuda.current_stream(result.device).cuda_stream
-    for node, _ in result.grad_fn.next_functions:
-        if hasattr(node, "variable"):
-            made_on = node.metadata.setdefault("xgboost.encoder", stream)
-            if made_on == 0 and torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("a graph made on the default stream still holds a leaf of this capture: its backward "
-                                   "pass cannot be captured; drop the eager pass's results first, or run it on another stream")
-
-
 # ---- gated feed-forward block ---------------------------------------------------
 
 def feed_forward_gradient(grad: torch.Tensor, x: torch.Tensor, kept: torch.Tensor, gate: torch.Tensor, up: torch.Tensor,
@@ -239,7 +226,7 @@ def feed_forward(x: torch.Tensor, gate: torch.Tensor, up: torch.Tensor, down: to
     gives NaN.  Differentiable in x and the matrices through y."""
     if torch.is_grad_enabled() and any(getattr(t, "requires_grad", False) for t in (x, gate, up, down)):
         y, kept = _FeedForward.apply(x, gate, up, down, activation)
-        _leaves_of(y)
+        _encoder.check_capture(y)
         return (y, kept) if keep else y
     return _encoder.feed_forward(x, gate, up, down, activation, keep)
 
@@ -356,7 +343,7 @@ def distillation_loss(logits: torch.Tensor, values: torch.Tensor, indices: torch
     teacher is constant."""
     if torch.is_grad_enabled() and getattr(logits, "requires_grad", False):
         loss, lse = _Distillation.apply(logits, values, indices, temperature)
-        _leaves_of(loss)
+        _encoder.check_capture(loss)
         return loss, lse
     return _encoder.distillation_loss(logits, values, indices, temperature)
 
